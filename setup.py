@@ -34,6 +34,19 @@ sources = sorted(glob.glob(os.path.join(CSRC, "*.cu")) + glob.glob(os.path.join(
 CHECK_SOURCES = sorted(glob.glob(os.path.join(CSRC, "check", "*.cu")) + glob.glob(os.path.join(CSRC, "check", "*.cpp")))
 CHECK_FLAGS = [f for f in NVCC_FLAGS if f != "-DMAMF_BOUNDS_CHECK=1"]
 
+
+
+def cxx_runtime():
+    """The libstdc++ that torch has loaded into this process, as a link argument.  A compiler that finds no shared
+    libstdc++ links its static one instead; the module then mixes two copies, and formatting a number into an error
+    message crashes in the wrong copy's locale instead of raising."""
+    with open("/proc/self/maps") as f:
+        paths = {line.split()[-1] for line in f if "libstdc++.so" in line}
+    return sorted(paths)[:1]
+
+
+LINK_ARGS = cxx_runtime()
+
 setup(
     name="mamformer_b200",
     version="0.1.0",
@@ -44,12 +57,14 @@ setup(
             sources=sources,
             include_dirs=[os.path.join(HERE, CSRC)],
             extra_compile_args={"cxx": ["-O3", "-std=c++17"], "nvcc": NVCC_FLAGS},
+            extra_link_args=LINK_ARGS,
         ),
         CUDAExtension(
             name="mamformer_b200._C_check",
             sources=CHECK_SOURCES,
             include_dirs=[os.path.join(HERE, CSRC)],
             extra_compile_args={"cxx": ["-O3", "-std=c++17"], "nvcc": CHECK_FLAGS},
+            extra_link_args=LINK_ARGS,
         ),
     ],
     cmdclass={"build_ext": BuildExtension.with_options(use_ninja=True)},
