@@ -82,6 +82,20 @@ int64_t flash_tc_bwd_error();
 std::vector<at::Tensor> flash_attn_fwd(at::Tensor q, at::Tensor k, at::Tensor v, int64_t lo, int64_t hi, double scale);
 std::vector<at::Tensor> flash_attn_bwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor out, at::Tensor lse,
                                        at::Tensor dout, int64_t lo, int64_t hi, double scale);
+std::vector<at::Tensor> token_scores_fwd(at::Tensor logits, at::Tensor target, int64_t ignore_index, double temperature,
+                                         int64_t top_k);
+at::Tensor token_scores_bwd(at::Tensor logits, at::Tensor target, int64_t ignore_index, double temperature,
+                            at::Tensor stats, at::Tensor ent, at::Tensor top_id, c10::optional<at::Tensor> g_lp,
+                            c10::optional<at::Tensor> g_ent, c10::optional<at::Tensor> g_top);
+std::vector<at::Tensor> kv_append(at::Tensor k, at::Tensor v, at::Tensor ck, at::Tensor cv, at::Tensor ks, at::Tensor vs,
+                                  at::Tensor table, at::Tensor cu, at::Tensor lens, int64_t max_new,
+                                  c10::optional<at::Tensor> cos, c10::optional<at::Tensor> sin,
+                                  c10::optional<at::Tensor> pos, std::vector<at::Tensor> queries);
+int64_t kv_append_error();
+at::Tensor paged_attention(at::Tensor q1, c10::optional<at::Tensor> q2, c10::optional<at::Tensor> lam, at::Tensor ck,
+                           at::Tensor cv, at::Tensor ks, at::Tensor vs, at::Tensor table, at::Tensor cu, at::Tensor lens,
+                           int64_t max_new, int64_t window, double scale);
+int64_t paged_attention_error();
 void gemm_ag(std::vector<int64_t> a_ptrs, int64_t shard_rows, int64_t lda, int64_t rank, at::Tensor B, bool b_mn,
              at::Tensor D);
 void gemm_rs(at::Tensor A, at::Tensor B, bool b_mn, std::vector<int64_t> d_ptrs, int64_t shard_rows, int64_t ldd,
@@ -145,6 +159,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("flash_tc_bwd_error", &mamf::flash_tc_bwd_error);
   m.def("flash_attn_fwd", &mamf::flash_attn_fwd);
   m.def("flash_attn_bwd", &mamf::flash_attn_bwd);
+  m.def("token_scores_fwd", &mamf::token_scores_fwd);
+  m.def("token_scores_bwd", &mamf::token_scores_bwd);
+  m.def("kv_append", &mamf::kv_append);
+  m.def("kv_append_error", &mamf::kv_append_error);
+  m.def("paged_attention", &mamf::paged_attention);
+  m.def("paged_attention_error", &mamf::paged_attention_error);
   m.def("gemm_ag", &mamf::gemm_ag);
   m.def("gemm_rs", &mamf::gemm_rs);
 }

@@ -44,12 +44,17 @@ class KernelTimeoutError(RuntimeError):
     """A bounded pipeline wait inside the GEMM gave up."""
 
 
+class PagedCacheError(RuntimeError):
+    """A paged-cache kernel met a page, length or position out of range and skipped that access."""
+
+
 class RankFailureError(RuntimeError):
     """Another rank reported a failure or stopped sending heartbeats."""
 
 
 def check_device_status(clear: bool = True) -> None:
-    """Raise if a native kernel recorded a timeout (reads two device words; call between steps)."""
+    """Raise if a native kernel recorded a timeout or a skipped access (reads device words; call between
+    steps)."""
     from mamformer_b200.ops._ext import ext
     C = ext()
     if C is None or not torch.cuda.is_available():
@@ -66,6 +71,8 @@ def check_device_status(clear: bool = True) -> None:
         fn = getattr(C, name, None)
         if fn is not None:
             attn = attn or int(fn())
+    # the paged-cache kernels' words; also cleared by the read itself
+    paged = int(C.kv_append_error()) or int(C.paged_attention_error())
     if comm:
         raise CommTimeoutError(f"cross-GPU barrier timed out waiting for peer {comm - 100}")
     if gemm:
@@ -73,6 +80,12 @@ def check_device_status(clear: bool = True) -> None:
     if attn:
         raise KernelTimeoutError(f"tcgen05 attention kernel reported code {attn} "
                                  "(a pipeline wait timed out, or a checked index was out of range)")
+    if paged == 4:
+        raise KernelTimeoutError("paged attention: a pipeline wait timed out")
+    if paged:
+        what = {1: "a block table entry that is not a page of the pool", 2: "lengths that do not fit the new tokens",
+                3: "a position outside the rotation tables"}.get(paged, f"code {paged}")
+        raise PagedCacheError(f"paged KV cache: {what}")
 
 
 class Heartbeat:

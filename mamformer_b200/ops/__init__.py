@@ -14,7 +14,7 @@ from __future__ import annotations
 
 import math
 import os
-from typing import Optional
+from typing import List, NamedTuple, Optional, Sequence
 
 import torch
 import torch.nn.functional as F
@@ -26,7 +26,8 @@ __all__ = [
     "rms_norm", "rope", "swiglu", "causal_conv1d_silu", "selective_scan", "mamba_inner",
     "linear_diff_attention", "diff_attention", "attention", "head_group_norm", "router_topk",
     "expert_histogram", "moe_routed", "moe_expert_outputs", "linear_cross_entropy",
-    "fused_ce_available", "token_log_probs", "NATIVE", "has_native", "force_reference",
+    "fused_ce_available", "token_log_probs", "token_scores", "TokenScores", "PagedKV", "kv_append", "paged_attention",
+    "NATIVE", "has_native", "force_reference",
 ]
 
 # Native-kernel coverage (op name -> kernel source file).  Filled by ops.native on import.
@@ -201,10 +202,83 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     return ref.linear_cross_entropy(h, weight, labels, ignore_index)
 
 
+class TokenScores(NamedTuple):
+    """Scores of one given token per row of logits, fp32 (ids int64)."""
+    log_probs: torch.Tensor        # (..)
+    entropy: torch.Tensor          # (..)
+    top_log_probs: torch.Tensor    # (.., k)
+    top_ids: torch.Tensor          # (.., k)
+
+
+_SCORE_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def token_scores(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, temperature: float = 1.0,
+                 ignore_index: int = -100) -> TokenScores:
+    """Under p = softmax(logits / temperature): log p of ``targets``, the entropy of p, and the ``top_k`` (at most
+    32) most likely tokens with their log probabilities, ties to the lower id.
+
+    logits (.., V) bf16 / f16 / fp32 (other types run the eager form), targets (..) int64.  Differentiable in all three scores.  Rows whose target is
+    ``ignore_index`` give 0, ids -1 and no gradient, and are not read; a logit of -inf has probability 0; a row of
+    -inf only gives log probabilities of -inf, entropy 0 and no gradient."""
+    if logits.dim() < 1 or targets.shape != logits.shape[:-1]:
+        raise ValueError(f"token_scores: targets {tuple(targets.shape)} for logits {tuple(logits.shape)}")
+    if not temperature > 0:
+        raise ValueError(f"token_scores: temperature must be positive, got {temperature}")
+    if not 0 <= top_k <= min(32, logits.shape[-1]):
+        raise ValueError(f"token_scores: top_k from 0 to {min(32, logits.shape[-1])}, got {top_k}")
+    if _native(logits) and "token_scores" in NATIVE and logits.dtype in _SCORE_TYPES:
+        return TokenScores(*_nat().token_scores(logits, targets, top_k, temperature, ignore_index))
+    return TokenScores(*ref.token_scores(logits, targets, top_k, temperature, ignore_index))
+
+
 def token_log_probs(logits: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
     """log_softmax(logits)[..., target] without materialising the full log-softmax."""
+    if _native(logits) and "token_scores" in NATIVE and logits.dtype in _SCORE_TYPES:
+        return _nat().token_scores(logits, targets, 0, 1.0, -100)[0]
     lf = logits.float()
     return lf.gather(-1, targets.unsqueeze(-1)).squeeze(-1) - torch.logsumexp(lf, dim=-1)
+
+
+class PagedKV(NamedTuple):
+    """One layer's paged 8-bit cache: e4m3 codes and a power-of-two scale per (page, KV head)."""
+    k: torch.Tensor          # (P, G, page, hd) float8_e4m3fn
+    v: torch.Tensor
+    k_scale: torch.Tensor    # (P, G) fp32
+    v_scale: torch.Tensor
+
+
+def kv_append(k: torch.Tensor, v: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
+              kv_lens: torch.Tensor, max_new: int, cos: Optional[torch.Tensor] = None,
+              sin: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+              queries: Sequence[torch.Tensor] = ()) -> List[torch.Tensor]:
+    """Write packed new keys and values (T, G, hd) into the cache's pages, in place; returns the rotated ``queries``.
+
+    Sequence b's new tokens are rows cu_seqlens[b] : cu_seqlens[b + 1] (int32, B + 1) and take the last slots of its
+    kv_lens[b] (int32, the length *with* them); block_table (B, W) int32 gives the page of each block of slots;
+    ``max_new`` is the largest number of new tokens of a sequence.  With ``cos`` / ``sin`` (positions, hd / 2) fp32
+    and ``positions`` (T,) int64, keys and up to two query tensors (T, H, hd) are rotated on the way (halves, as
+    :func:`rope`).  A page that takes new tokens must belong to one sequence only.  On the GPU a page or length out
+    of range is skipped and a position is clamped to the tables, and ``fault.check_device_status`` raises
+    afterwards."""
+    if _native(k) and "kv_append" in NATIVE:
+        return _nat().kv_append(k, v, cache, block_table, cu_seqlens, kv_lens, max_new, cos, sin, positions, queries)
+    return ref.kv_append(k, v, cache, block_table, cu_seqlens, kv_lens, cos, sin, positions, queries)
+
+
+def paged_attention(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
+                    kv_lens: torch.Tensor, max_new: int, q2: Optional[torch.Tensor] = None,
+                    lam: Optional[torch.Tensor] = None, window: int = 0, scale: Optional[float] = None) -> torch.Tensor:
+    """Causal attention of packed queries (T, H, hd) over the paged cache, H / G query heads per KV head -> (T, H, hd).
+
+    Arguments as in :func:`kv_append`, called after it: query i of a sequence's n sees slots up to
+    kv_lens - n + i, with ``window`` > 0 only the last ``window`` of them.  With ``q2`` and ``lam`` (H,) fp32, the
+    differential form (softmax(q k) v - lam softmax(q2 k) v) / (1 - lam + 1e-8).  A query that sees nothing, and
+    rows past cu_seqlens[-1], give 0.  No gradient."""
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    if _native(q) and "paged_attention" in NATIVE:
+        return _nat().paged_attention(q, cache, block_table, cu_seqlens, kv_lens, max_new, q2, lam, window, scale)
+    return ref.paged_attention(q, cache, block_table, cu_seqlens, kv_lens, q2, lam, window, scale)
 
 
 # Register native ops (import has no side effects when the extension is absent).

@@ -411,3 +411,40 @@ def diff_attention(q1, q2, k, v, lam, lo, hi, scale=None):
     o2 = flash_attention(q2, k, v, lo, hi, scale)
     lam4 = lam.view(1, 1, -1, 1).to(o1.dtype)
     return (o1 - lam4 * o2) / (1.0 - lam4 + 1e-8)
+
+
+# ---------------------------------------------------------------------------------------------
+class _TokenScores(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, top_k, temperature, ignore_index):
+        lp, ent, top_lp, top_ids, stats = _C.token_scores_fwd(logits, targets, ignore_index, temperature, top_k)
+        ctx.save_for_backward(logits, targets, stats, ent, top_ids)
+        ctx.args = (ignore_index, temperature)
+        ctx.mark_non_differentiable(top_ids)
+        ctx.set_materialize_grads(False)
+        return lp, ent, top_lp, top_ids
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_lp, g_ent, g_top, _):
+        logits, targets, stats, ent, top_ids = ctx.saved_tensors
+        g = [None if x is None else x.float().contiguous() for x in (g_lp, g_ent, g_top)]
+        return _C.token_scores_bwd(logits, targets, *ctx.args, stats, ent, top_ids, *g), None, None, None, None
+
+
+@_register("token_scores", "csrc/token_scores.cu")
+def token_scores(logits, targets, top_k, temperature, ignore_index):
+    targets = targets.long().contiguous()
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _TokenScores.apply(logits, targets, top_k, temperature, ignore_index)
+    return _C.token_scores_fwd(logits, targets, ignore_index, temperature, top_k)[:4]
+
+
+@_register("kv_append", "csrc/paged_kv.cu")
+def kv_append(k, v, cache, block_table, cu_seqlens, kv_lens, max_new, cos, sin, positions, queries):
+    return _C.kv_append(k, v, *cache, block_table, cu_seqlens, kv_lens, max_new, cos, sin, positions, list(queries))
+
+
+@_register("paged_attention", "csrc/paged_attn.cu")
+def paged_attention(q, cache, block_table, cu_seqlens, kv_lens, max_new, q2, lam, window, scale):
+    return _C.paged_attention(q, q2, lam, *cache, block_table, cu_seqlens, kv_lens, max_new, window, scale)

@@ -356,3 +356,100 @@ def diff_attention_band(q1, q2, k, v, lam, lo, hi, scale=None):
     o2 = attention_band(q2, k, v, lo, hi, scale)
     lam4 = lam.view(1, 1, -1, 1).to(o1.dtype)
     return (o1 - lam4 * o2) / (1.0 - lam4 + 1e-8)
+
+
+# ---------------------------------------------------------------------------------------------
+# token scores, paged 8-bit cache
+# ---------------------------------------------------------------------------------------------
+
+def token_scores(logits, targets, top_k: int, temperature: float, ignore_index: int):
+    """(log_probs, entropy, top_log_probs, top_ids); differentiable through autograd."""
+    x = logits if logits.dtype == torch.float64 else logits.float()
+    V = x.shape[-1]
+    live = (targets != ignore_index) & (targets >= 0) & (targets < V)
+    m = x.detach().amax(-1, keepdim=True)
+    none = m == -math.inf
+    u = torch.where(none, 0.0, x - m) / temperature
+    d = u.clamp(min=-1e30)                            # a logit of -inf adds 0 to both sums
+    e = d.exp()
+    z = e.sum(-1, keepdim=True)
+    lse = z.log()
+    ent = torch.where(none, 0.0, lse - (d * e).sum(-1, keepdim=True) / z)[..., 0]
+    ids = torch.sort(x.detach(), dim=-1, descending=True, stable=True).indices[..., :top_k]
+    pick = torch.cat([targets.clamp(0, V - 1).unsqueeze(-1), ids], -1)
+    lp = torch.where(none, -math.inf, u.gather(-1, pick) - lse)
+    lp = torch.where(live.unsqueeze(-1), lp, 0.0)
+    return lp[..., 0], torch.where(live, ent, 0.0), lp[..., 1:], torch.where(live.unsqueeze(-1), ids, -1)
+
+
+def block_scale(amax: torch.Tensor) -> torch.Tensor:
+    """2^e with the least e for which amax <= 448 * 2^e, e within [-100, 119]."""
+    m, x = torch.frexp(amax)                          # 448 = 0.875 * 2^9, m in [0.5, 1)
+    e = torch.where(amax > 0, torch.where(m > 0.875, x - 8, x - 9), -100).clamp(-100, 119)
+    return torch.ldexp(torch.ones_like(amax), e)
+
+
+def _codes(x: torch.Tensor) -> torch.Tensor:
+    return x.clamp(-448.0, 448.0).to(torch.float8_e4m3fn)
+
+
+def kv_append(k, v, cache, block_table, cu_seqlens, kv_lens, cos, sin, positions, queries):
+    if k.shape != v.shape or k.dim() != 3 or k.shape[1] != cache.k.shape[1] or k.shape[2] != cache.k.shape[3]:
+        raise ValueError(f"kv_append: k {tuple(k.shape)}, v {tuple(v.shape)} for pages {tuple(cache.k.shape)}")
+
+    def turn(x):
+        c, s = cos[positions].unsqueeze(1), sin[positions].unsqueeze(1)
+        a, b = x.float().chunk(2, -1)
+        return torch.cat([a * c - b * s, b * c + a * s], -1)
+
+    page = cache.k.shape[2]
+    cu, lens = cu_seqlens.tolist(), kv_lens.tolist()
+    kf = turn(k) if cos is not None else k.float()
+    for x, codes, scale in ((kf, cache.k, cache.k_scale), (v.float(), cache.v, cache.v_scale)):
+        for b, end in enumerate(lens):
+            t, slot = cu[b], end - (cu[b + 1] - cu[b])
+            while slot < end:
+                p, lo = int(block_table[b, slot // page]), slot % page
+                n = min(page - lo, end - slot)
+                new = x[t:t + n].transpose(0, 1)                                     # (G, n, hd)
+                s = block_scale(torch.where(new.isfinite(), new.abs(), 0.0).amax((1, 2)))
+                if lo:
+                    s = torch.maximum(s, scale[p])
+                    codes[p, :, :lo] = _codes(codes[p, :, :lo].float() * (scale[p] / s)[:, None, None])
+                codes[p, :, lo:lo + n] = _codes(new / s[:, None, None])
+                scale[p] = s
+                t, slot = t + n, slot + n
+    return [turn(q).to(q.dtype) for q in queries]
+
+
+def paged_attention(q, cache, block_table, cu_seqlens, kv_lens, q2, lam, window, scale):
+    page, G = cache.k.shape[2], cache.k.shape[1]
+    if q.dim() != 3 or q.shape[1] % G or q.shape[2] != cache.k.shape[3] or (q2 is None) != (lam is None):
+        raise ValueError(f"paged_attention: q {tuple(q.shape)} for pages {tuple(cache.k.shape)}")
+    acc = torch.float64 if q.dtype == torch.float64 else torch.float32
+    out = torch.zeros_like(q)
+    cu, lens = cu_seqlens.tolist(), kv_lens.tolist()
+    for b, L in enumerate(lens):
+        n = cu[b + 1] - cu[b]
+        if n == 0:
+            continue
+        pages = block_table[b, :(L + page - 1) // page].long()
+
+        def held(codes, s):
+            x = codes.view(torch.uint8)[pages].view(torch.float8_e4m3fn).to(acc) * s[pages][..., None, None].to(acc)
+            return x.transpose(0, 1).reshape(G, -1, x.shape[-1])[:, :L].repeat_interleave(q.shape[1] // G, 0)
+
+        kx, vx = held(cache.k, cache.k_scale), held(cache.v, cache.v_scale)
+        dist = torch.arange(L - n, L, device=q.device)[:, None] - torch.arange(L, device=q.device)
+        hide = (dist < 0) | (dist >= window) if window > 0 else dist < 0
+        maps = []
+        for x in (q,) if q2 is None else (q, q2):
+            s = (x[cu[b]:cu[b + 1]].transpose(0, 1).to(acc) @ kx.transpose(1, 2)) * scale
+            p = torch.softmax(s.masked_fill(hide, -math.inf), -1)
+            maps.append(torch.where(hide.all(-1)[:, None], 0.0, p @ vx if L else p.new_zeros(p.shape[0], n, q.shape[2])))
+        o = maps[0]
+        if q2 is not None:
+            w = lam.view(-1, 1, 1).to(acc)
+            o = (o - w * maps[1]) / (1.0 - w + 1e-8)
+        out[cu[b]:cu[b + 1]] = o.transpose(0, 1).to(q.dtype)
+    return out
