@@ -23,7 +23,7 @@ struct Cache {
   uint8_t *k, *v;
   float *ks, *vs;
   const int *table, *cu, *lens;
-  int P, G, page, W, B, T;
+  int P, G, page, shift, W, B, T;        // page = 1 << shift
 };
 
 struct Layer { at::Tensor k, v, ks, vs, table, cu, lens; };
@@ -47,7 +47,7 @@ inline Cache check_cache(const char* what, const Layer& l, int64_t T, int64_t hd
   TORCH_CHECK(P < (1LL << 31) && G <= 65535 && l.table.size(1) * page < (1LL << 31) && T < (1LL << 31) && B < (1 << 24), what, ": sizes");
   return Cache{(uint8_t*)l.k.data_ptr(), (uint8_t*)l.v.data_ptr(), l.ks.data_ptr<float>(), l.vs.data_ptr<float>(),
                l.table.data_ptr<int>(), l.cu.data_ptr<int>(), l.lens.data_ptr<int>(), (int)P, (int)G, (int)page,
-               (int)l.table.size(1), (int)B, (int)T};
+               page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7, (int)l.table.size(1), (int)B, (int)T};
 }
 
 // A tensor whose rows of adjacent values start on 16-byte boundaries: t itself, or a copy of it.
