@@ -9,26 +9,30 @@
 // ones.  An item that ends in another CTA than it began in leaves partial (m, l, O) in a workspace and a
 // second small kernel joins them in order (results do not depend on timing).
 //
-// A CTA is 4 warps; warp w takes tokens 16 w .. 16 w + 15 of each tile through a ring of its own, filled
-// with 16-byte cp.async, and never waits for the other warps inside an item.  A warp's 16 tokens are the M
-// rows of mma.m16n8k16 (f16 operands, fp32 sums): S^T = K Q^T and O^T = V^T P^T with up to 8 query rows as
-// N, so 8 rows (4 heads of a group x 2 maps) fill the instruction; 16 rows take two.  e4m3 is exact in f16,
-// and the rows of q are scaled by a power of two to [1, 2) first, which f16 holds exactly down to 2^-14 of a
-// row's largest value.  P is rounded to f16 (11 bits; 8 in bf16).  The order of the head's dims in the
-// products is free as long as both sides agree: a lane takes 16 adjacent bytes of K (and of V), so a
-// fragment is loaded with one 16-byte read and no shuffles.
+// A CTA is 4 warps; warp w takes tokens 16 w .. 16 w + 15 of each tile through a ring of its own, filled by
+// TMA (128-byte swizzle, one lane issues), and never waits for the other warps inside an item.  Its 16 tokens
+// are the M rows of mma.m16n8k16 (f16 operands, fp32 sums): S^T = K Q^T and O^T = V^T P^T with up to 8 query
+// rows as N, so 8 rows (4 heads of a group x 2 maps) fill the instruction; 16 rows take two.  e4m3 is exact
+// in f16, and the rows of q are scaled by a power of two to [1, 2) first, which f16 holds exactly down to
+// 2^-14 of a row's largest value.  P is rounded to f16 (11 bits; bf16 would keep 8).  The order of the head's
+// dims in the products is free as long as both sides agree: a lane takes 16 adjacent bytes of K (and of V),
+// so a fragment is one 16-byte read and no shuffles; so is the order of the 8 tokens of a fragment (`token`).
 #include "paged.cuh"
+#include "tc5.cuh"
 
 namespace mamf {
 namespace pa {
 
 using namespace paged;
 
-constexpr int NW = 4, NT = NW * 32;
-constexpr int TILE = 16 * NW;                  // tokens per tile
+constexpr int NW = 4, NT = NW * 32, NJ = 512;
+constexpr int STEP = 16;                       // tokens of a warp per tile
+constexpr int TILE = STEP * NW;                // tokens per tile
+constexpr long long WAIT_CYCLES = 4000000000LL;      // about 2 s
+constexpr float NONE = -1e30f;                 // maximum of no scores: 2^(score - NONE) is never formed, 2^(NONE - m) is 0
 constexpr float LAZY = 8.f;                    // log2 by which a row may outgrow its reference maximum
 
-__device__ int g_err = 0;
+__device__ int g_err = 0, g_wait_err = 0;
 __device__ __forceinline__ void record(int code) { atomicCAS(&g_err, 0, code); }
 
 struct Params {
@@ -43,20 +47,8 @@ struct Params {
   int4* joins;        // [ctas]: the item that ends in this CTA after it began in another one
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ uint32_t su32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+using tc5::ex2;
+using tc5::su32;
 __device__ __forceinline__ uint4 lds16(uint32_t a) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
@@ -67,11 +59,10 @@ __device__ __forceinline__ uint2 lds8(uint32_t a) {
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
   return v;
 }
-// two e4m3 codes -> two f16 values (exact)
-__device__ __forceinline__ uint32_t to_h2(uint32_t two) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)two));
-  return r;
+// four e4m3 codes -> the first two and the last two as f16 (exact)
+__device__ __forceinline__ void to_h4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}\n"
+      : "=r"(lo), "=r"(hi) : "r"(w));
 }
 __device__ __forceinline__ void mma(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -86,6 +77,31 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
 __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ void tma_lines(uint32_t dst, const CUtensorMap* map, uint32_t bar, int line) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+               ::"r"(dst), "l"(map), "r"(bar), "r"(0), "r"(line) : "memory");
+}
+__device__ __forceinline__ bool try_tile(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
+               : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000000u) : "memory");
+  return ok != 0;
+}
+// Waits for the warp's tile, the same answer for all lanes; false after WAIT_CYCLES (recorded), or once
+// another warp of the grid has given up.
+__device__ __forceinline__ bool wait_tile(uint32_t bar, uint32_t parity) {
+  if (__all_sync(0xffffffffu, try_tile(bar, parity))) return true;
+  const long long t0 = clock64();
+  for (uint32_t n = 1;; ++n) {
+    if (__all_sync(0xffffffffu, try_tile(bar, parity))) return true;
+    if ((n & 63u) == 0) {
+      const bool over = clock64() - t0 > WAIT_CYCLES;
+      if (over) atomicCAS(&g_wait_err, 0, (int)ERR_WAIT);
+      if (__any_sync(0xffffffffu, over || *((volatile int*)&g_wait_err) != 0)) return false;
+    }
+  }
 }
 
 // One row tile of one KV head of one sequence.
@@ -114,12 +130,13 @@ __device__ __forceinline__ bool set_sequence(const Params& p, Item& it, int b) {
   if (it.n <= 0 || it.t0 < 0 || it.t0 + it.n > p.c.T) return false;
   it.rows = it.n * p.rep * p.maps;
   it.g = it.rt = 0;
+  if (ROWS == 8 && it.rows > ROWS) record(ERR_LENGTH);          // more new tokens than max_new
   set_range<ROWS>(p, it);
   return true;
 }
 template <int ROWS>
 __device__ __forceinline__ void next_item(const Params& p, Item& it) {
-  if ((it.rt + 1) * ROWS < it.rows) { ++it.rt; set_range<ROWS>(p, it); return; }
+  if (ROWS > 8 && (it.rt + 1) * ROWS < it.rows) { ++it.rt; set_range<ROWS>(p, it); return; }
   if (it.g + 1 < p.c.G) { ++it.g; it.rt = 0; set_range<ROWS>(p, it); return; }
   int b = it.b + 1;
   while (b < p.c.B && !set_sequence<ROWS>(p, it, b)) ++b;
@@ -130,27 +147,35 @@ __device__ __forceinline__ int64_t tiles_of(const Params& p, int b) {
   Item it;
   if (!set_sequence<ROWS>(p, it, b)) return 0;
   int64_t n = 0;
-  for (it.rt = 0; it.rt * ROWS < it.rows; ++it.rt) {
-    set_range<ROWS>(p, it);
-    n += it.nt;
-  }
+  if constexpr (ROWS == 8) n = it.nt;                           // 8 rows are all there can be
+  else
+    for (; it.rt * ROWS < it.rows; ++it.rt) {
+      set_range<ROWS>(p, it);
+      n += it.nt;
+    }
   return n * p.c.G;
 }
 
-template <int HD, int NR> constexpr int stage_bytes() { return 2 * 16 * HD + 16; }
-template <int HD, int NR> constexpr int merge_floats() { return NW * 8 * NR * (HD + 4) + 2 * NW * 8 * NR; }
-constexpr int STAGES = 3;
-template <int HD, int NR> constexpr int smem_bytes() { return NW * STAGES * stage_bytes<HD, NR>() + 4 * merge_floats<HD, NR>(); }
-
-// byte offset of 16-byte chunk c of token row r in a 16-token slice, arranged so that the 8 lanes of each
-// phase of a 16-byte read (K: rows 2x, chunks of 4 lanes; V: rows 0, 2, 4, 6, two chunks) hit all banks once
-template <int HD> __device__ __forceinline__ int k_at(int r, int c) {
-  if (HD == 128) return r * 128 + ((c ^ ((r & 1) << 2)) << 4);
-  return (r >> 1) * 128 + ((((r & 1) * 4 + c) ^ (2 * ((r >> 1) & 3))) << 4);
+template <int HD> constexpr int stage_bytes() { return 2 * STEP * HD; }
+constexpr int ST = 3;                          // tiles of a warp's ring
+// resident CTAs per SM: the latency of a warp's chain (products, exponentials, products) is hidden by other
+// warps, so registers are held to 128 for 8 rows
+template <int NR> constexpr int residents() { return NR == 1 ? 4 : 2; }
+template <int HD, int NR> constexpr int merge_words() { return NR * (HD / 4 + 4); }      // of a lane
+template <int HD, int NR> constexpr int smem_bytes() {
+  return 1024 + NW * ST * stage_bytes<HD>() + 32 * 4 * merge_words<HD, NR>();
 }
-template <int HD> __device__ __forceinline__ int v_at(int r, int c) {
-  if (HD == 128) return r * 128 + ((c ^ (((r >> 1) & 3) << 1)) << 4);
-  return k_at<HD>(r, c);
+
+// The token of row r (0..7) of a fragment, and where TMA's 128-byte swizzle puts 16-byte chunk c of token n
+// (0..15) of a slice: chunk index xor line & 7, a line being one token of 128 dims or two of 64.  The orders
+// make the lanes of each phase of a shared-memory read hit every bank once: for K two rows r = 2 i, 2 i + 1 at
+// four chunks, for V the rows 2 i (then 2 i + 1) of four i at two chunks.
+template <int HD> __device__ __forceinline__ int token(int r) {
+  return HD == 128 ? (int)(0x36147250u >> (4 * r) & 7) : (int)(0x65742130u >> (4 * r) & 7);
+}
+template <int HD> __device__ __forceinline__ int chunk_at(int n, int c) {
+  if (HD == 128) return n * 128 + ((c ^ (n & 7)) << 4);
+  return (n >> 1) * 128 + ((((n & 1) * 4 + c) ^ (n >> 1 & 7)) << 4);
 }
 
 template <typename T> __device__ __forceinline__ void q_row16(const T* q, float* f) {
@@ -163,12 +188,15 @@ template <typename T> __device__ __forceinline__ void q_row16(const T* q, float*
 }
 
 template <typename T, int HD, int NR>
-__global__ void __launch_bounds__(NT) split_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(NT, residents<NR>()) split_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap map_k,
+                                                      const __grid_constant__ CUtensorMap map_v) {
   constexpr int ROWS = 8 * NR;
   constexpr int KC = HD / 64;                    // 16-byte reads of a K row per lane
   constexpr int MT = HD / 16;                    // 16-dim tiles of O^T
-  constexpr int SB = stage_bytes<HD, NR>();
-  extern __shared__ __align__(16) uint8_t smem[];
+  constexpr int SB = stage_bytes<HD>();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t bars[NW][ST];
   __shared__ int64_t s_pre[NT / 32];
   __shared__ int64_t s_begin;
   __shared__ int s_b;
@@ -228,55 +256,77 @@ __global__ void __launch_bounds__(NT) split_kernel(const __grid_constant__ Param
   int64_t start = s_begin;                          // list position of the item's first tile
   while (first >= start + it.nt) { start += it.nt; next_item<ROWS>(p, it); }
 
-  // ---- ring: the issue side runs STAGES - 1 tiles ahead ----
-  const uint32_t ring = su32(smem) + w * STAGES * SB;
+  // ---- ring: the issue side runs ST - 1 tiles ahead ----
+  const uint32_t ring = su32(smem) + w * ST * SB, bar = su32(bars[w]);
+  if (lane < ST) tc5::bar_init(&bars[w][lane], 1);
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  __syncwarp();
   Item is = it;
-  int is_tile = (int)(first - start);
-  int64_t issued = first;
-  auto page_of = [&](const Item& x, int tile) {
-    const int slot = (x.k0 + tile) * TILE + w * 16;
-    if (slot >= x.hi || slot + 16 <= x.lo) return -2;              // nothing to see in this slice
-    const int j = slot >> c.shift;
-    const int pg = j < c.W ? c.table[(int64_t)x.b * c.W + j] : -1;
-    return (pg < 0 || pg >= c.P) ? -1 : pg;
+  int to_issue = (int)(last - first), issued = 0, waited = 0;
+  int is_left = it.nt - (int)(first - start);                        // tiles of the item still to be looked up
+  int is_slot = (it.k0 + (int)(first - start)) * TILE + w * STEP;     // the warp's first token of the tile
+  const int* is_table = c.table + (int64_t)is.b * c.W;
+  // the page of the warp's 16 tokens of a tile: -2 nothing to see there, -1 not a page of the pool
+  int pg;
+  auto look_up = [&]() {
+    pg = -2;
+    if (is_slot < is.hi && is_slot + STEP > is.lo) {
+      const int j = is_slot >> c.shift;
+      pg = j < c.W ? is_table[j] : -1;
+    }
   };
-  int pg_next = page_of(is, is_tile);
-  uint32_t live_bits = 0;                                           // which ring slots hold a slice
-  auto issue = [&](int stage) {
-    live_bits &= ~(1u << stage);
-    if (issued < last) {
-      if (pg_next >= 0) {
-        const int slot = (is.k0 + is_tile) * TILE + w * 16;
-        const int64_t blk = (int64_t)pg_next * c.G + is.g;
-        const int64_t off = (blk * c.page + (slot & (c.page - 1))) * HD;
-        const uint32_t dst = ring + stage * SB;
+  look_up();
+  // scales of the tiles in flight, newest last; a K scale of 0 marks tokens that are not there
+  float ksr[ST], vsr[ST];
+  bool ok = true;
+  auto issue = [&](uint32_t stage_at, uint32_t bar_at) {
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) {
-          const int idx = i * 32 + lane, r = idx / (HD / 16), cc = idx % (HD / 16);
-          cp16(dst + k_at<HD>(r, cc), c.k + off + idx * 16);
-          cp16(dst + 16 * HD + v_at<HD>(r, cc), c.v + off + idx * 16);
-        }
-        if (lane < 2) cp4(dst + 32 * HD + lane * 4, (lane ? c.vs : c.ks) + blk);
-        live_bits |= 1u << stage;
-      } else if (pg_next == -1 && lane == 0) record(ERR_PAGE);
-      if (++issued < last) {
-        if (++is_tile == is.nt) { next_item<ROWS>(p, is); is_tile = 0; }
-        pg_next = page_of(is, is_tile);
+    for (int i = 0; i + 1 < ST; ++i) { ksr[i] = ksr[i + 1]; vsr[i] = vsr[i + 1]; }
+    ksr[ST - 1] = vsr[ST - 1] = 0.f;
+    if (to_issue <= 0) return;
+    ++issued;
+    const bool there = (unsigned)pg < (unsigned)c.P;
+    const int blk = pg * c.G + is.g;
+    if (there) {
+      ksr[ST - 1] = c.ks[blk];
+      vsr[ST - 1] = c.vs[blk];
+    }
+    if (lane == 0) {
+      if (there) {
+        const int token = (blk << c.shift) + (is_slot & (c.page - 1)), line = HD == 128 ? token : token >> 1;
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar_at), "r"(SB) : "memory");
+        tma_lines(stage_at, &map_k, bar_at, line);
+        tma_lines(stage_at + STEP * HD, &map_v, bar_at, line);
+      } else {
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar_at) : "memory");
+        if (pg != -2) record(ERR_PAGE);
       }
     }
-    cp_commit();
+    if (--to_issue > 0) {
+      is_slot += TILE;
+      if (--is_left == 0) {
+        next_item<ROWS>(p, is);
+        is_left = is.nt;
+        is_slot = is.k0 * TILE + w * STEP;
+        is_table = c.table + (int64_t)is.b * c.W;
+      }
+      look_up();
+    }
   };
 #pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) issue(s);
+  for (int s = 0; s < ST - 1; ++s) issue(ring + s * SB, bar + s * 8);
 
   // ---- state of the current item ----
   uint32_t qf[NR][KC * 4][2];
   float rs[NR][2];                        // score factor of rows 2 t4, 2 t4 + 1
   int lim[NR][2], low[NR][2];             // slots (low, lim] that the row sees
+  int all_lo = 0, all_hi = 0;             // slots [all_lo, all_hi] that every row sees
   float m[NR][2], l[NR][2], o[NR][MT][4];
   float vref = 0.f;
   auto load_rows = [&]() {
-    const int per = p.rep * p.maps;
+    const int per = p.rep * p.maps, at0 = it.len - it.n;
+    all_hi = min(it.len - 1, at0 + it.rt * ROWS / per);
+    all_lo = p.window > 0 ? at0 + min(it.n - 1, (it.rt * ROWS + ROWS - 1) / per) - p.window + 1 : 0;
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
       const int r = it.rt * ROWS + nr * 8 + g8;
@@ -320,7 +370,7 @@ __global__ void __launch_bounds__(NT) split_kernel(const __grid_constant__ Param
         // rows past the last one are rows of zeros that see everything: they ask for no mask and are not written
         lim[nr][x] = rr < it.rows ? min(it.len - 1, it.len - it.n + rr / per) : 0x7fffffff;
         low[nr][x] = rr < it.rows && p.window > 0 ? it.len - it.n + rr / per - p.window : -1;
-        m[nr][x] = -INFINITY;
+        m[nr][x] = NONE;
         l[nr][x] = 0.f;
       }
 #pragma unroll
@@ -331,64 +381,72 @@ __global__ void __launch_bounds__(NT) split_kernel(const __grid_constant__ Param
     vref = 0.f;
   };
 
-  auto compute = [&](int stage, int slot0) {
-    const uint32_t kb = ring + stage * SB, vb = kb + 16 * HD;
-    float s[NR][4];
+  // rows of this lane in the fragments: token tk (K) and tv[0], tv[1] (V), and the same + 8, which is
+  // 8 lines (or 4, with bit 2 of the chunk flipped) further on; 64 dims on is bit 2 of the chunk
+  const int tk = token<HD>(g8), tv[2] = {token<HD>(2 * t4), token<HD>(2 * t4 + 1)};
+  const uint32_t k_off = chunk_at<HD>(tk, t4);
+  const uint32_t v_off[2] = {(uint32_t)chunk_at<HD>(tv[0], HD == 128 ? g8 : g8 >> 1) + (HD == 128 ? 0 : (g8 & 1) * 8),
+                             (uint32_t)chunk_at<HD>(tv[1], HD == 128 ? g8 : g8 >> 1) + (HD == 128 ? 0 : (g8 & 1) * 8)};
+  auto plus8 = [](uint32_t a) { return HD == 128 ? a + 1024 : (a + 512) ^ 64; };
+  auto scores = [&](uint32_t kb, float ks, int slot0, float (&s)[NR][4]) {
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
       for (int x = 0; x < 4; ++x) s[nr][x] = 0.f;
-    // S^T: lane (g8, t4) holds token rows g8 and g8 + 8, dims 64 cc + 16 t4 .. + 15
+    // S^T: tokens tk and tk + 8, dims 64 cc + 16 t4 .. + 15
 #pragma unroll
     for (int cc = 0; cc < KC; ++cc) {
-      const uint4 a = lds16(kb + k_at<HD>(g8, cc * 4 + t4)), b = lds16(kb + k_at<HD>(g8 + 8, cc * 4 + t4));
+      const uint32_t at = (kb + k_off) ^ (cc * 64);
+      const uint4 a = lds16(at), b = lds16(plus8(at));
       const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t a0 = to_h2(aw[i]), a2 = to_h2(aw[i] >> 16), a1 = to_h2(bw[i]), a3 = to_h2(bw[i] >> 16);
+        uint32_t a0, a1, a2, a3;
+        to_h4(aw[i], a0, a2);
+        to_h4(bw[i], a1, a3);
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) mma(s[nr], a0, a1, a2, a3, qf[nr][cc * 4 + i][0], qf[nr][cc * 4 + i][1]);
       }
     }
-    float ks, vs;
-    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(ks), "=f"(vs) : "r"(kb + 32 * HD));
-    bool grow = false, all = true;
-#pragma unroll
-    for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-      for (int x = 0; x < 2; ++x) all = all && slot0 + 15 <= lim[nr][x] && slot0 > low[nr][x];
-    all = __all_sync(0xffffffffu, all);
+    const bool all = slot0 + STEP - 1 <= all_hi && slot0 >= all_lo;
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         s[nr][x] *= rs[nr][x & 1] * ks;
         if (!all) {
-          const int slot = slot0 + g8 + (x >> 1) * 8;
+          const int slot = slot0 + tk + (x >> 1) * 8;
           if (slot > lim[nr][x & 1] || slot <= low[nr][x & 1]) s[nr][x] = -INFINITY;
         }
-        grow = grow || s[nr][x] > m[nr][x & 1] + LAZY;
       }
-    if (__any_sync(0xffffffffu, grow)) {
+  };
+  auto raise = [&](float (&s)[NR][4]) {
+    bool grow = false;
 #pragma unroll
-      for (int nr = 0; nr < NR; ++nr)
+    for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          float mx = fmaxf(s[nr][x], s[nr][x + 2]);
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          mx = fmaxf(mx, m[nr][x]);
-          const float f = m[nr][x] == -INFINITY ? 0.f : ex2(m[nr][x] - mx);
-          if (mx > m[nr][x]) {
-            m[nr][x] = mx;
-            l[nr][x] *= f;
+      for (int x = 0; x < 2; ++x) grow = grow || fmaxf(s[nr][x], s[nr][x + 2]) > m[nr][x] + LAZY;
+    if (!__any_sync(0xffffffffu, grow)) return;
 #pragma unroll
-            for (int j = 0; j < MT; ++j) { o[nr][j][x] *= f; o[nr][j][x + 2] *= f; }
-          }
+    for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        float mx = fmaxf(s[nr][x], s[nr][x + 2]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        if (mx > m[nr][x]) {
+          const float f = ex2(m[nr][x] - mx);
+          m[nr][x] = mx;
+          l[nr][x] *= f;
+#pragma unroll
+          for (int j = 0; j < MT; ++j) { o[nr][j][x] *= f; o[nr][j][x + 2] *= f; }
         }
-    }
-    // O is in units of vref; a block whose scale is within 2^6 of it goes in through P (at most 2^14)
+      }
+  };
+  // P V of one tile.  O is in units of vref; a block whose scale is within 2^6 of it goes in through P (at
+  // most 2^14 then), a larger or smaller one changes vref, and one below 2^-60 of it is below O's last bit.
+  auto values = [&](uint32_t vb, float vs, int slot0, float (&s)[NR][4]) {
     float ratio = 1.f;
     if (vs != vref) {
       if (vref == 0.f) vref = vs;
@@ -401,7 +459,9 @@ __global__ void __launch_bounds__(NT) split_kernel(const __grid_constant__ Param
 #pragma unroll
             for (int x = 0; x < 4; ++x) o[nr][j][x] *= f;
         vref = vs;
-      } else ratio = vs / vref;
+      } else if (vs > vref * 8.6736174e-19f) {
+        ratio = __uint_as_float(__float_as_uint(vs) - __float_as_uint(vref) + (127u << 23));      // powers of two
+      } else ratio = 0.f;
     }
     uint32_t pf[NR][2];
 #pragma unroll
@@ -409,38 +469,40 @@ __global__ void __launch_bounds__(NT) split_kernel(const __grid_constant__ Param
       float e[4];
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const float mm = m[nr][x & 1];
-        e[x] = ex2(s[nr][x] - (mm == -INFINITY ? 0.f : mm));
+        e[x] = ex2(s[nr][x] - m[nr][x & 1]);
         l[nr][x & 1] += e[x];
       }
       pf[nr][0] = transposed(pack_h2(e[0] * ratio, e[1] * ratio));
       pf[nr][1] = transposed(pack_h2(e[2] * ratio, e[3] * ratio));
     }
-    // O^T: lane (g8, t4) holds tokens 2 t4, 2 t4 + 1 and the same + 8, dims HD / 8 * g8 ..
+    // O^T: tokens tv[0], tv[1] and the same + 8, dims HD / 8 * g8 ..
     uint32_t vw[4][HD / 32];
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      const int r = 2 * t4 + (x & 1) + (x >> 1) * 8;
+      const uint32_t at = x < 2 ? vb + v_off[x] : plus8(vb + v_off[x - 2]);
       if (HD == 128) {
-        const uint4 v = lds16(vb + v_at<HD>(r, g8));
+        const uint4 v = lds16(at);
         vw[x][0] = v.x; vw[x][1] = v.y; vw[x][HD / 32 - 2] = v.z; vw[x][HD / 32 - 1] = v.w;
       } else {
-        const uint2 v = lds8(vb + v_at<HD>(r, g8 >> 1) + (g8 & 1) * 8);
+        const uint2 v = lds8(at);
         vw[x][0] = v.x; vw[x][1] = v.y;
       }
-      if (slot0 + 16 > it.hi) {                        // codes past the end may be anything, NaN included
-        if (slot0 + r >= it.hi) {
+    }
+    if (slot0 + 16 > it.hi) {                          // codes past the end may be anything, NaN included
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (slot0 + tv[x & 1] + (x >> 1) * 8 >= it.hi) {
 #pragma unroll
           for (int i = 0; i < HD / 32; ++i) vw[x][i] = 0;
         }
-      }
     }
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i) {
-      const uint32_t x0 = __byte_perm(vw[0][i], vw[1][i], 0x5140), x1 = __byte_perm(vw[0][i], vw[1][i], 0x7362);
-      const uint32_t y0 = __byte_perm(vw[2][i], vw[3][i], 0x5140), y1 = __byte_perm(vw[2][i], vw[3][i], 0x7362);
-      const uint32_t a0 = to_h2(x0), a1 = to_h2(x0 >> 16), a2 = to_h2(y0), a3 = to_h2(y0 >> 16);
-      const uint32_t b0 = to_h2(x1), b1 = to_h2(x1 >> 16), b2 = to_h2(y1), b3 = to_h2(y1 >> 16);
+      uint32_t a0, a1, a2, a3, b0, b1, b2, b3;
+      to_h4(__byte_perm(vw[0][i], vw[1][i], 0x5140), a0, a1);
+      to_h4(__byte_perm(vw[2][i], vw[3][i], 0x5140), a2, a3);
+      to_h4(__byte_perm(vw[0][i], vw[1][i], 0x7362), b0, b1);
+      to_h4(__byte_perm(vw[2][i], vw[3][i], 0x7362), b2, b3);
 #pragma unroll
       for (int nr = 0; nr < NR; ++nr) {
         mma(o[nr][2 * i], a0, a1, a2, a3, pf[nr][0], pf[nr][1]);          // dims HD / 8 g8 + 4 i, + 1
@@ -449,104 +511,145 @@ __global__ void __launch_bounds__(NT) split_kernel(const __grid_constant__ Param
     }
   };
 
-  float* mo = reinterpret_cast<float*>(smem + NW * STAGES * SB);        // [NW][ROWS][HD + 4]
-  float* ml = mo + NW * ROWS * (HD + 4);                                 // [NW][ROWS][2]
+  // Warps 3, 2, 1 pass their joined state on through shared memory, lane by lane; warp 0 writes the result.
+  float* merge = reinterpret_cast<float*>(smem + NW * ST * SB) + lane;
   auto finish = [&](int64_t item_start, bool ends) {
-    // sums over the lanes that share a row, then this warp's rows to shared memory
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        float v = l[nr][x];
-        v += __shfl_xor_sync(0xffffffffu, v, 4);
-        v += __shfl_xor_sync(0xffffffffu, v, 8);
-        v += __shfl_xor_sync(0xffffffffu, v, 16);
-        const int r = nr * 8 + 2 * t4 + x;
-        if (g8 == 0) { ml[(w * ROWS + r) * 2] = m[nr][x]; ml[(w * ROWS + r) * 2 + 1] = v; }
-        float* dst = mo + (w * ROWS + r) * (HD + 4) + g8 * (HD / 8);
+      for (int j = 0; j < MT; ++j)
 #pragma unroll
-        for (int j = 0; j < MT; ++j) {
-          // tile j holds dims 2 j, 2 j + 1 of the lane's HD / 8
-          *reinterpret_cast<float2*>(dst + 2 * j) = make_float2(o[nr][j][x] * vref, o[nr][j][x + 2] * vref);
+        for (int x = 0; x < 4; ++x) o[nr][j][x] *= vref;
+#pragma unroll 1
+    for (int turn = NW - 1; turn >= 0; --turn) {
+      if (w == turn && turn < NW - 1) {
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float mm = merge[(nr * 4 + x) * 32], M = fmaxf(m[nr][x], mm);
+            const float a = ex2(m[nr][x] - M), b = ex2(mm - M);
+            m[nr][x] = M;
+            l[nr][x] = fmaf(l[nr][x], a, merge[(nr * 4 + 2 + x) * 32] * b);
+#pragma unroll
+            for (int j = 0; j < MT; ++j)
+#pragma unroll
+              for (int z = x; z < 4; z += 2) o[nr][j][z] = fmaf(o[nr][j][z], a, merge[(NR * 4 + (nr * MT + j) * 4 + z) * 32] * b);
+          }
+      }
+      if (w == turn && turn > 0) {
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) { merge[(nr * 4 + x) * 32] = m[nr][x]; merge[(nr * 4 + 2 + x) * 32] = l[nr][x]; }
+#pragma unroll
+          for (int j = 0; j < MT; ++j)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) merge[(NR * 4 + (nr * MT + j) * 4 + x) * 32] = o[nr][j][x];
         }
       }
-    __syncthreads();
-    const bool whole = ends && item_start >= first;
-    float* part = p.part + ((int64_t)blockIdx.x * 2 + (item_start > first ? 1 : 0)) * ROWS * (HD + 2);
-    const int per = p.rep * p.maps;
-    for (int i = tid; i < ROWS / p.maps * (HD / 4); i += NT) {
-      const int rr = i / (HD / 4) * p.maps, d = i % (HD / 4) * 4;      // first map's row
-      if (it.rt * ROWS + rr >= it.rows) continue;
-      float4 res = make_float4(0.f, 0.f, 0.f, 0.f);
-      const int row = it.rt * ROWS + rr, tok = it.t0 + row / per, h = it.g * p.rep + row % per / p.maps;
-      for (int map = 0; map < p.maps; ++map) {
-        const int r = rr + map;
-        float M = -INFINITY;
-#pragma unroll
-        for (int x = 0; x < NW; ++x) M = fmaxf(M, ml[(x * ROWS + r) * 2]);
-        float L = 0.f;
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int x = 0; x < NW; ++x) {
-          const float mm = ml[(x * ROWS + r) * 2];
-          const float f = mm == -INFINITY ? 0.f : ex2(mm - M);
-          const float4 v = *reinterpret_cast<const float4*>(mo + (x * ROWS + r) * (HD + 4) + d);
-          L = fmaf(f, ml[(x * ROWS + r) * 2 + 1], L);
-          a.x = fmaf(f, v.x, a.x); a.y = fmaf(f, v.y, a.y); a.z = fmaf(f, v.z, a.z); a.w = fmaf(f, v.w, a.w);
-        }
-        if (whole) {
-          const float lam = p.maps == 2 ? p.lam[h] : 0.f;
-          float f = L == 0.f ? 0.f : 1.f / L;
-          if (p.maps == 2) f *= (map ? -lam : 1.f) / (1.f - lam + 1e-8f);
-          res.x = fmaf(a.x, f, res.x); res.y = fmaf(a.y, f, res.y); res.z = fmaf(a.z, f, res.z); res.w = fmaf(a.w, f, res.w);
-        } else {
-          float2* dst = reinterpret_cast<float2*>(part + r * (HD + 2) + d);
-          dst[0] = make_float2(a.x, a.y);
-          dst[1] = make_float2(a.z, a.w);
-          if (d == 0) *reinterpret_cast<float2*>(part + r * (HD + 2) + HD) = make_float2(M, L);
-        }
-      }
-      if (whole) {
-        T* out = (T*)p.out + ((int64_t)tok * p.H + h) * HD + d;
-        union { T v[4]; uint2 raw; } u;
-        u.v[0] = from_f<T>(res.x); u.v[1] = from_f<T>(res.y); u.v[2] = from_f<T>(res.z); u.v[3] = from_f<T>(res.w);
-        *reinterpret_cast<uint2*>(out) = u.raw;
-      }
+      if (turn > 0) __syncthreads();
     }
-    if (ends && !whole && tid == 0)
-      {
-      const int64_t c0 = item_start / share;       // CTA and place of the item's first part
-      p.joins[blockIdx.x] = make_int4(it.b, it.g, it.rt, (int)(2 * c0 + (item_start > c0 * share ? 1 : 0)));
+    if (w == 0) {
+      const bool whole = ends && item_start >= first;
+      float* part = p.part + ((int64_t)blockIdx.x * 2 + (item_start > first ? 1 : 0)) * ROWS * (HD + 2);
+      const int per = p.rep * p.maps;
+#pragma unroll
+      for (int nr = 0; nr < NR; ++nr) {
+        float f0[2];                                     // 1 / sum over the row's lanes
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float M = m[nr][x];
+          float L = l[nr][x];
+          L += __shfl_xor_sync(0xffffffffu, L, 4);
+          L += __shfl_xor_sync(0xffffffffu, L, 8);
+          L += __shfl_xor_sync(0xffffffffu, L, 16);
+          f0[x] = L == 0.f ? 0.f : 1.f / L;
+          const int r = nr * 8 + 2 * t4 + x;
+          if (!whole) {
+            float* dst = part + r * (HD + 2);
+#pragma unroll
+            for (int j = 0; j < MT; ++j)
+              *reinterpret_cast<float2*>(dst + g8 * (HD / 8) + 2 * j) = make_float2(o[nr][j][x], o[nr][j][x + 2]);
+            if (g8 == 0) *reinterpret_cast<float2*>(dst + HD) = make_float2(M, L);
+          }
+        }
+        if (!whole) continue;
+        // rows 2 t4 and 2 t4 + 1 are two heads, or the two maps of one
+        const int row = it.rt * ROWS + nr * 8 + 2 * t4;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (row + x >= it.rows || (x == 1 && p.maps == 2)) continue;
+          const int tok = it.t0 + (row + x) / per, h = it.g * p.rep + (row + x) % per / p.maps;
+          float wa = f0[x], wb = 0.f;
+          if (p.maps == 2) {
+            const float lam = p.lam[h], den = 1.f / (1.f - lam + 1e-8f);
+            wa *= den;
+            wb = -lam * den * f0[1];
+          }
+          T* out = (T*)p.out + ((int64_t)tok * p.H + h) * HD + g8 * (HD / 8);
+#pragma unroll
+          for (int j = 0; j < MT; j += 4) {
+            Vec16<T> v;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float a0 = o[nr][j + k][x] * wa, a1 = o[nr][j + k][x + 2] * wa;
+              v.v[2 * k] = from_f<T>(p.maps == 2 ? fmaf(o[nr][j + k][1], wb, a0) : a0);
+              v.v[2 * k + 1] = from_f<T>(p.maps == 2 ? fmaf(o[nr][j + k][3], wb, a1) : a1);
+            }
+            st16(out + 2 * j, v);
+          }
+        }
+      }
+      if (ends && !whole && lane == 0) {
+        const int64_t c0 = item_start / share;       // CTA and place of the item's first part
+        p.joins[blockIdx.x] = make_int4(it.b, it.g, it.rt, (int)(2 * c0 + (item_start > c0 * share ? 1 : 0)));
+      }
     }
     __syncthreads();
   };
 
   load_rows();
-  int tile = (int)(first - start);
-  int stage = 0;
-  for (int64_t pos = first; pos < last; ++pos) {
-    issue((stage + STAGES - 1) % STAGES);
-    cp_wait<STAGES - 1>();
-    __syncwarp();
-    if (live_bits >> stage & 1) compute(stage, (it.k0 + tile) * TILE + w * 16);
-    __syncwarp();                                  // the slice is read before its slot is filled again
-    stage = (stage + 1) % STAGES;
-    if (++tile == it.nt || pos + 1 == last) {
-      finish(start, tile == it.nt);
-      if (pos + 1 < last) {
+  int tiles = it.nt - (int)(first - start);                           // of the item, still to be done
+  int slot0 = (it.k0 + (int)(first - start)) * TILE + w * STEP;
+  uint32_t here = ring, bar_here = bar, phase = 0, there = ring + (ST - 1) * SB, bar_there = bar + (ST - 1) * 8;
+  for (int left = (int)(last - first); left > 0; --left) {
+    if (ok) {
+      issue(there, bar_there);
+      ok = wait_tile(bar_here, phase);
+      waited += ok;
+    }
+    if (ok && ksr[0] != 0.f) {
+      float s[NR][4];
+      scores(here, ksr[0], slot0, s);
+      raise(s);
+      values(here + STEP * HD, vsr[0], slot0, s);
+    }
+    __syncwarp();                                  // the tile is read before its place is filled again
+    there = here;
+    bar_there = bar_here;
+    here += SB;
+    bar_here += 8;
+    if (here == ring + ST * SB) { here = ring; bar_here = bar; phase ^= 1; }
+    slot0 += TILE;
+    if (--tiles == 0 || left == 1) {
+      finish(start, tiles == 0);
+      if (left > 1) {
         start += it.nt;
         next_item<ROWS>(p, it);
-        tile = 0;
+        tiles = it.nt;
+        slot0 = it.k0 * TILE + w * STEP;
         load_rows();
       }
     }
   }
-  cp_wait<0>();
+  // after a wait that ran out: no copy may still be under way into this CTA's memory
+  for (; waited < issued; ++waited) tc5::bar_wait(&bars[w][waited % ST], (uint32_t)(waited / ST & 1), ERR_WAIT, &g_wait_err, WAIT_CYCLES);
 }
 
 // Joins the parts of an item that ran over several CTAs: block = the CTA in which it ended.
 template <typename T, int HD, int NR>
-__global__ void __launch_bounds__(NT) join_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(NJ) join_kernel(const __grid_constant__ Params p) {
   constexpr int ROWS = 8 * NR;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 j = p.joins[blockIdx.x];
@@ -555,50 +658,83 @@ __global__ void __launch_bounds__(NT) join_kernel(const __grid_constant__ Params
   set_sequence<ROWS>(p, it, j.x);
   it.g = j.y;
   it.rt = j.z;
-  const int c0 = j.w >> 1, c1 = blockIdx.x, per = p.rep * p.maps;
-  for (int i = threadIdx.x; i < ROWS / p.maps * (HD / 2); i += NT) {
-    const int rr = i / (HD / 2) * p.maps, d = i % (HD / 2) * 2;
-    const int row = it.rt * ROWS + rr;
-    if (row >= it.rows) continue;
-    float2 res = make_float2(0.f, 0.f);
-    const int tok = it.t0 + row / per, h = it.g * p.rep + row % per / p.maps;
-    for (int map = 0; map < p.maps; ++map) {
-      float M = -INFINITY, L = 0.f;
-      float2 a = make_float2(0.f, 0.f);
-      for (int cta = c0; cta <= c1; ++cta) {
-        const int slot = cta == c0 ? (j.w & 1) : 0;
-        const float* part = p.part + (((int64_t)cta * 2 + slot) * ROWS + rr + map) * (HD + 2);
-        const float2 v = *reinterpret_cast<const float2*>(part + d), s = *reinterpret_cast<const float2*>(part + HD);
-        if (s.x == -INFINITY && s.y == 0.f) continue;
-        const float mn = fmaxf(M, s.x), f = M == -INFINITY ? 0.f : ex2(M - mn), e = ex2(s.x - mn);
-        a.x = a.x * f + v.x * e;
-        a.y = a.y * f + v.y * e;
-        L = L * f + s.y * e;
-        M = mn;
+  const int c0 = j.w >> 1, parts = blockIdx.x - c0 + 1, per = p.rep * p.maps;
+  auto part = [&](int i, int r) {
+    return p.part + (((int64_t)(c0 + i) * 2 + (i == 0 ? j.w & 1 : 0)) * ROWS + r) * (HD + 2);
+  };
+  // a group of warps takes a row: the parts' common maximum, then each warp's share of the parts' sums and
+  // values; the two maps of a head are neighbouring rows
+  constexpr int GR = NJ / 32 / ROWS, D = HD / 32;
+  __shared__ float vals[GR][ROWS][HD], sums[GR][ROWS];
+  const int lane = threadIdx.x & 31, r = (threadIdx.x >> 5) % ROWS, gr = (threadIdx.x >> 5) / ROWS;
+  if (it.rt * ROWS + r < it.rows) {
+    float M = NONE;
+    for (int i = lane; i < parts; i += 32) M = fmaxf(M, part(i, r)[HD]);
+    M = warp_max(M);
+    float L = 0.f, a[D] = {};
+#pragma unroll 8
+    for (int i = gr; i < parts; i += GR) {
+      const float* x = part(i, r);
+      const float f = ex2(x[HD] - M);
+      L = fmaf(f, x[HD + 1], L);
+#pragma unroll
+      for (int d = 0; d < D; d += 2) {
+        const float2 v = *reinterpret_cast<const float2*>(x + lane * D + d);
+        a[d] = fmaf(f, v.x, a[d]);
+        a[d + 1] = fmaf(f, v.y, a[d + 1]);
       }
-      const float lam = p.maps == 2 ? p.lam[h] : 0.f;
-      float f = L == 0.f ? 0.f : 1.f / L;
-      if (p.maps == 2) f *= (map ? -lam : 1.f) / (1.f - lam + 1e-8f);
-      res.x = fmaf(a.x, f, res.x);
-      res.y = fmaf(a.y, f, res.y);
     }
-    T* out = (T*)p.out + ((int64_t)tok * p.H + h) * HD + d;
-    out[0] = from_f<T>(res.x);
-    out[1] = from_f<T>(res.y);
+#pragma unroll
+    for (int d = 0; d < D; ++d) vals[gr][r][lane * D + d] = a[d];
+    if (lane == 0) sums[gr][r] = L;
+  }
+  __syncthreads();
+  auto value = [&](int row, int d) {
+    float x = 0.f, L = 0.f;
+#pragma unroll
+    for (int i = 0; i < GR; ++i) { x += vals[i][row][d]; L += sums[i][row]; }
+    return L == 0.f ? 0.f : x / L;
+  };
+  for (int i = threadIdx.x; i < ROWS / p.maps * HD; i += NJ) {
+    const int rr = i / HD * p.maps, d = i % HD, row = it.rt * ROWS + rr;
+    if (row >= it.rows) continue;
+    const int tok = it.t0 + row / per, h = it.g * p.rep + row % per / p.maps;
+    float x = value(rr, d);
+    if (p.maps == 2) x = (x - p.lam[h] * value(rr + 1, d)) / (1.f - p.lam[h] + 1e-8f);
+    ((T*)p.out)[((int64_t)tok * p.H + h) * HD + d] = from_f<T>(x);
   }
 }
 
+// All tokens of a cache tensor as lines of 128 bytes, a box of 16 tokens (they are adjacent in their page).
+static CUtensorMap lines_map(const uint8_t* base, int64_t tokens, int hd) {
+  CUtensorMap m;
+  cuuint64_t gd[2] = {128, (cuuint64_t)(tokens * hd / 128)};
+  cuuint64_t gs[1] = {128};
+  cuuint32_t bx[2] = {128u, (cuuint32_t)(16 * hd / 128)}, es[2] = {1, 1};
+  const CUresult r = tc5_encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(base), gd, gs, bx, es,
+                                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "paged_attention: cuTensorMapEncodeTiled failed: ", (int)r);
+  return m;
+}
+
 template <typename T, int HD, int NR>
-void launch_split(Params& p) {
+void launch_split(const Params& p, const CUtensorMap& mk, const CUtensorMap& mv) {
   auto fn = split_kernel<T, HD, NR>;
   constexpr int SMEM = smem_bytes<HD, NR>();
-  MAMF_CUDA_CHECK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
-  fn<<<p.ctas, NT, SMEM, stream()>>>(p);
+  static bool set[64] = {};                              // by device; the attribute stays
+  int dev = 0;
+  MAMF_CUDA_CHECK(cudaGetDevice(&dev));
+  if (dev >= 64 || !set[dev]) {
+    MAMF_CUDA_CHECK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+    if (dev < 64) set[dev] = true;
+  }
+  fn<<<p.ctas, NT, SMEM, stream()>>>(p, mk, mv);
   MAMF_LAUNCH_CHECK();
   if (p.ctas == 1) return;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(p.ctas);
-  cfg.blockDim = dim3(NT);
+  cfg.blockDim = dim3(NJ);
   cfg.stream = stream();
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -648,28 +784,31 @@ at::Tensor paged_attention(at::Tensor q1, c10::optional<at::Tensor> q2, c10::opt
   const int nr = std::max<int64_t>(1, max_new) * p.rep * p.maps > 8 ? 2 : 1, rows = 8 * nr;
   const int64_t row_tiles = (std::max<int64_t>(1, std::min(max_new, T)) * p.rep * p.maps + rows - 1) / rows;
   const int64_t most = std::max<int64_t>(1, (int64_t)p.c.B * p.c.G * row_tiles * std::max<int64_t>(1, ((int64_t)p.c.W * p.c.page + TILE - 1) / TILE));
-  p.ctas = (int)std::min<int64_t>(most, 3 * num_sms());
+  p.ctas = (int)std::min<int64_t>(most, (nr == 1 ? residents<1>() : residents<2>()) * num_sms());
   const int64_t part = (int64_t)p.ctas * 2 * rows * (hd + 2);
   at::Tensor ws = at::empty({part + 4 * p.ctas}, q1.options().dtype(at::kFloat));
   p.joins = reinterpret_cast<int4*>(ws.data_ptr<float>());
   p.part = ws.data_ptr<float>() + 4 * p.ctas;
+  TORCH_CHECK(p.c.P >= 1, "paged_attention: a pool without pages");
+  TORCH_CHECK((int64_t)p.c.P * p.c.G * p.c.page * hd / 128 < (1LL << 31), "paged_attention: a pool of over 256 GB");
+  const int64_t tokens = (int64_t)p.c.P * p.c.G * p.c.page;
+  const CUtensorMap mk = lines_map(p.c.k, tokens, (int)hd), mv = lines_map(p.c.v, tokens, (int)hd);
   auto go = [&](auto t) {
     using E = decltype(t);
-    if (hd == 128) { if (nr == 1) launch_split<E, 128, 1>(p); else launch_split<E, 128, 2>(p); }
-    else { if (nr == 1) launch_split<E, 64, 1>(p); else launch_split<E, 64, 2>(p); }
+    if (hd == 128) { if (nr == 1) launch_split<E, 128, 1>(p, mk, mv); else launch_split<E, 128, 2>(p, mk, mv); }
+    else { if (nr == 1) launch_split<E, 64, 1>(p, mk, mv); else launch_split<E, 64, 2>(p, mk, mv); }
   };
   if (q1.scalar_type() == at::kBFloat16) go(__nv_bfloat16()); else go(__half());
   return out;
 }
 
 int64_t paged_attention_error() {
-  int v = 0;
+  int v = 0, w = 0, z = 0;
   MAMF_CUDA_CHECK(cudaMemcpyFromSymbol(&v, pa::g_err, sizeof(int)));
-  if (v) {
-    int z = 0;
-    MAMF_CUDA_CHECK(cudaMemcpyToSymbol(pa::g_err, &z, sizeof(int)));
-  }
-  return v;
+  MAMF_CUDA_CHECK(cudaMemcpyFromSymbol(&w, pa::g_wait_err, sizeof(int)));
+  if (v) MAMF_CUDA_CHECK(cudaMemcpyToSymbol(pa::g_err, &z, sizeof(int)));
+  if (w) MAMF_CUDA_CHECK(cudaMemcpyToSymbol(pa::g_wait_err, &z, sizeof(int)));
+  return w ? w : v;
 }
 
 }  // namespace mamf

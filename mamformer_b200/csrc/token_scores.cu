@@ -13,7 +13,7 @@
 // Rows whose target is `ignore_index` (or outside the vocabulary) are not read: results 0, ids -1.
 #include "common.cuh"
 
-#include <cooperative_groups.h>
+#include <type_traits>
 
 namespace mamf {
 namespace ts {
@@ -84,18 +84,99 @@ struct FwdParams {
   float inv_t;
 };
 
-// One CTA per row.
+// ---- two fp32 values per instruction ----
+__device__ __forceinline__ uint64_t pk(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpk(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// maximum of a 16-byte vector, NaN if one is in it
+__device__ __forceinline__ float vec_max(const Vec16<float>& v) { return max_nan(max_nan(v.v[0], v.v[1]), max_nan(v.v[2], v.v[3])); }
+__device__ __forceinline__ float vec_max(const Vec16<__nv_bfloat16>& v) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v.raw);
+  const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+  return max_nan(__bfloat162float(m.x), __bfloat162float(m.y));
+}
+__device__ __forceinline__ float vec_max(const Vec16<__half>& v) {
+  const __half2* h = reinterpret_cast<const __half2*>(&v.raw);
+  const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+  return max_nan(__half2float(m.x), __half2float(m.y));
+}
+
+// Raises a thread's running maximum to cm and scales its sums to it.
+__device__ __forceinline__ void raise(Stat& st, float cm, float k2) {
+  if (cm <= st.m || st.m != st.m) return;                 // a NaN maximum stays, and so do its sums
+  if (st.m != -INFINITY) {
+    const float d = max_nan(st.m - cm, DMIN), f = ex2(d * k2);
+    st.s1 = fmaf(d, st.s0, st.s1) * f;
+    st.s0 *= f;
+  }
+  st.m = cm;
+}
 template <typename T>
-__global__ void __launch_bounds__(NT) scores_fwd_kernel(const T* __restrict__ logits, FwdParams p) {
+__device__ __forceinline__ void add_vec(const Vec16<T>& v, float m, float k2, uint64_t& s0, uint64_t& s1) {
   constexpr int VEC = 16 / sizeof(T);
-  __shared__ Stat sm_stat[NT / 32];
-  __shared__ Stat sm_all;
-  __shared__ uint64_t sm_key[NT / 32];
-  __shared__ uint64_t sm_top[MAXK];
-  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-  const int64_t row = blockIdx.x;
+  const uint64_t nm = pk(-m, -m), kk = pk(k2, k2);
+#pragma unroll
+  for (int j = 0; j < VEC; j += 2) {
+    float a, b;
+    unpk(add2(pk(to_f(v.v[j]), to_f(v.v[j + 1])), nm), a, b);
+    const uint64_t d = pk(max_nan(a, DMIN), max_nan(b, DMIN));
+    unpk(mul2(d, kk), a, b);
+    const uint64_t e = pk(ex2(a), ex2(b));
+    s0 = add2(s0, e);
+    s1 = fma2(d, e, s1);
+  }
+}
+
+template <int CL> __device__ __forceinline__ int cluster_rank() {
+  if (CL == 1) return 0;
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return (int)r;
+}
+template <int CL> __device__ __forceinline__ void cluster_sync() {
+  if (CL > 1) asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+}
+// the same variable of CTA `rank` of the cluster
+template <typename V> __device__ __forceinline__ V* in_cta(V* p, int rank) {
+  uint64_t r;
+  asm volatile("mapa.u64 %0, %1, %2;" : "=l"(r) : "l"(p), "r"(rank));
+  return reinterpret_cast<V*>(r);
+}
+
+// A row for each cluster of CL CTAs (CL = 1 where there are enough rows to fill the GPU): one pass with a
+// running maximum per thread.  The alternatives come from the maxima: at least k threads hold an element no
+// smaller than the k-th largest of the threads' maxima, so only threads whose maximum reaches that bound can
+// hold an alternative, and only their elements (about k / NT of the row) are read again, by all threads.
+template <typename T, int CL>
+__global__ void __launch_bounds__(NT, 2) scores_fwd_kernel(const T* __restrict__ logits, const __grid_constant__ FwdParams p) {
+  constexpr int VEC = 16 / sizeof(T), U = 4;
+  __shared__ Stat sm_stat[NT / 32], sm_cta;
+  __shared__ uint64_t sm_key[NT / 32], sm_top[MAXK], sm_cand[CAP];
+  __shared__ int sm_hot[NT], sm_nh, sm_n;
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, rank = cluster_rank<CL>();
+  const int64_t row = blockIdx.x / CL;
   const int64_t tgt = p.target[row];
   if (tgt == p.ignore || tgt < 0 || tgt >= p.V) {
+    if (rank > 0) return;
     if (tid == 0) {
       p.lp[row] = 0.f; p.ent[row] = 0.f;
       p.stats[2 * row] = -INFINITY; p.stats[2 * row + 1] = 0.f;
@@ -105,43 +186,56 @@ __global__ void __launch_bounds__(NT) scores_fwd_kernel(const T* __restrict__ lo
   }
   const T* x = logits + p.rows.at(row);
   const float k2 = p.inv_t * LOG2E;
-  // elements before the first 16-byte boundary and after the last full vector are taken one by one
+  // elements before the first 16-byte boundary and after the last full vector are taken one by one by CTA 0
   const int head = min(p.V, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
-  const int nv = (p.V - head) / VEC;
-  const int rem = p.V - nv * VEC;
+  const int nv = (p.V - head) / VEC, rem = rank == 0 ? p.V - nv * VEC : 0;
   const T* xv = x + head;
+  const int g0 = rank * NT + tid;
+  auto rem_at = [&](int i) { return i < head ? i : nv * VEC + i; };
 
   Stat st{-INFINITY, 0.f, 0.f};
-  auto add = [&](const float* v, int n) {
-    float cm = v[0];
-    for (int i = 1; i < n; ++i) cm = max_nan(cm, v[i]);
-    if (!(cm <= st.m) && st.m == st.m) {
-      Stat b{cm, 0.f, 0.f};
-      if (st.m != -INFINITY) {
-        const float d = max_nan(st.m - cm, DMIN), f = ex2(d * k2);
-        b.s1 = fmaf(d, st.s0, st.s1) * f;
-        b.s0 = st.s0 * f;
-      }
-      st = b;
-    }
-    if (st.m == -INFINITY) return;
-    for (int i = 0; i < n; ++i) {
-      const float d = max_nan(v[i] - st.m, DMIN), e = ex2(d * k2);
+  int i = g0;
+  for (; i + (U - 1) * CL * NT < nv; i += U * CL * NT) {
+    Vec16<T> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = ld16(xv + (int64_t)(i + u * CL * NT) * VEC);
+    float cm = vec_max(v[0]);
+#pragma unroll
+    for (int u = 1; u < U; ++u) cm = max_nan(cm, vec_max(v[u]));
+    raise(st, cm, k2);
+    if (st.m == -INFINITY) continue;
+    uint64_t s0 = pk(st.s0, 0.f), s1 = pk(st.s1, 0.f);
+#pragma unroll
+    for (int u = 0; u < U; ++u) add_vec(v[u], st.m, k2, s0, s1);
+    float a, b;
+    unpk(s0, a, b);
+    st.s0 = a + b;
+    unpk(s1, a, b);
+    st.s1 = a + b;
+  }
+  for (; i < nv; i += CL * NT) {
+    const Vec16<T> v = ld16(xv + (int64_t)i * VEC);
+    raise(st, vec_max(v), k2);
+    if (st.m == -INFINITY) continue;
+    uint64_t s0 = pk(st.s0, 0.f), s1 = pk(st.s1, 0.f);
+    add_vec(v, st.m, k2, s0, s1);
+    float a, b;
+    unpk(s0, a, b);
+    st.s0 = a + b;
+    unpk(s1, a, b);
+    st.s1 = a + b;
+  }
+  if (tid < rem) {
+    const float f = to_f(x[rem_at(tid)]);
+    raise(st, f, k2);
+    if (st.m != -INFINITY) {
+      const float d = max_nan(f - st.m, DMIN), e = ex2(d * k2);
       st.s0 += e;
       st.s1 = fmaf(d, e, st.s1);
     }
-  };
-  for (int i = tid; i < nv; i += NT) {
-    const Vec16<T> v = ld16(xv + (int64_t)i * VEC);
-    float f[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) f[j] = to_f(v.v[j]);
-    add(f, VEC);
   }
-  if (tid < rem) {
-    const float f = to_f(x[tid < head ? tid : nv * VEC + tid]);
-    add(&f, 1);
-  }
+  const uint32_t mine = (g0 < nv || tid < rem) ? order(st.m) : 0u;     // 0: a thread without elements
+
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     Stat b{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s0, o),
@@ -149,40 +243,113 @@ __global__ void __launch_bounds__(NT) scores_fwd_kernel(const T* __restrict__ lo
     merge(st, b, k2);
   }
   if (lane == 0) sm_stat[wid] = st;
+  if (tid == 0) { sm_nh = 0; sm_n = 0; }
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < NT / 32; ++w) merge(st, sm_stat[w], k2);
-    const bool none = st.m == -INFINITY;
-    const float ls = none ? 0.f : logf(st.s0);
-    p.lp[row] = none ? -INFINITY : (to_f(x[tgt]) - st.m) * p.inv_t - ls;
-    p.ent[row] = none ? 0.f : ls - st.s1 * p.inv_t / st.s0;
-    p.stats[2 * row] = st.m;
-    p.stats[2 * row + 1] = ls;
-    sm_all = Stat{st.m, ls, 0.f};
-  }
-  // k rounds: the largest element below the last one taken
-  uint64_t last = ~0ull;
-  for (int r = 0; r < p.k; ++r) {
-    uint64_t best = 0;
-    for (int i = tid; i < p.V; i += NT) {
-      const uint64_t k = key_of(to_f(x[i]), (uint32_t)i);
-      if (k < last && k > best) best = k;
+  if (wid == 0) {
+    st = lane < NT / 32 ? sm_stat[lane] : Stat{-INFINITY, 0.f, 0.f};
+#pragma unroll
+    for (int o = NT / 64; o > 0; o >>= 1) {
+      Stat b{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s0, o),
+             __shfl_xor_sync(0xffffffffu, st.s1, o)};
+      merge(st, b, k2);
     }
-    best = warp_max_u64(best);
+    if (lane == 0) sm_cta = st;
+  }
+
+  if (p.k > 0) {
+    // the largest bound that at least k threads reach; values of the 16-bit types differ in the upper bits only
+    uint32_t bound = 0;
+    constexpr uint32_t LOW = std::is_same<T, float>::value ? 1u : std::is_same<T, __half>::value ? 1u << 13 : 1u << 16;
+    for (uint32_t bit = 1u << 31; bit >= LOW; bit >>= 1)
+      if (__syncthreads_count(mine >= (bound | bit)) >= p.k) bound |= bit;
+    if (mine >= bound && mine) sm_hot[atomicAdd(&sm_nh, 1)] = tid;
     __syncthreads();
-    if (lane == 0) sm_key[wid] = best;
+    const int per = (nv + CL * NT - 1) / (CL * NT), items = sm_nh * per;
+    auto offer = [&](float f, int idx) {
+      if (order(f) < bound) return;
+      const int at = atomicAdd(&sm_n, 1);
+      if (at < CAP) sm_cand[at] = key_of(f, (uint32_t)idx);
+    };
+    for (int it = tid; it < items; it += NT) {
+      const int v = rank * NT + sm_hot[it / per] + it % per * (CL * NT);
+      if (v >= nv) continue;
+      const Vec16<T> w = ld16(xv + (int64_t)v * VEC);
+      if (order(vec_max(w)) < bound) continue;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) offer(to_f(w.v[e]), head + v * VEC + e);
+    }
+    if (tid < rem) offer(to_f(x[rem_at(tid)]), rem_at(tid));
     __syncthreads();
-    best = 0;
-    for (int w = 0; w < NT / 32; ++w) best = sm_key[w] > best ? sm_key[w] : best;
-    if (tid == 0) sm_top[r] = best;
-    last = best;
+    const int n = sm_n;
+    if (tid < p.k) sm_top[tid] = 0;
+    __syncthreads();
+    if (n <= CAP) {
+      for (int c = tid; c < n; c += NT) {
+        const uint64_t me = sm_cand[c];
+        int above = 0;
+        for (int d = 0; d < n && above < p.k; ++d) above += sm_cand[d] > me;
+        if (above < p.k) sm_top[above] = me;
+      }
+    } else {
+      // more equal elements than fit: the largest key below the last one taken, k times
+      uint64_t last = ~0ull;
+      for (int r = 0; r < p.k; ++r) {
+        uint64_t best = 0;
+        auto look = [&](float f, int idx) {
+          const uint64_t k = key_of(f, (uint32_t)idx);
+          if (k < last && k > best) best = k;
+        };
+        for (int v = g0; v < nv; v += CL * NT) {
+          const Vec16<T> w = ld16(xv + (int64_t)v * VEC);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) look(to_f(w.v[e]), head + v * VEC + e);
+        }
+        if (tid < rem) look(to_f(x[rem_at(tid)]), rem_at(tid));
+        best = warp_max_u64(best);
+        __syncthreads();
+        if (lane == 0) sm_key[wid] = best;
+        __syncthreads();
+        for (int w = 0; w < NT / 32; ++w) best = sm_key[w] > best ? sm_key[w] : best;
+        if (tid == 0) sm_top[r] = best;
+        last = best;
+      }
+    }
   }
   __syncthreads();
-  if (tid < p.k) {
-    const uint32_t id = key_index(sm_top[tid]);
-    p.top_id[row * p.k + tid] = id;
-    p.top_lp[row * p.k + tid] = sm_all.m == -INFINITY ? -INFINITY : (to_f(x[id]) - sm_all.m) * p.inv_t - sm_all.s0;
+  cluster_sync<CL>();
+  if (rank == 0) {
+    // every thread joins the CTAs' sums: it costs less than passing them on
+    Stat all = sm_cta;
+    for (int r = 1; r < CL; ++r) merge(all, *in_cta(&sm_cta, r), k2);
+    const bool none = all.m == -INFINITY;
+    const float ls = none ? 0.f : logf(all.s0);
+    auto log_p = [&](float f) { return none ? -INFINITY : (f - all.m) * p.inv_t - ls; };
+    if (tid == 0) {
+      p.lp[row] = log_p(to_f(x[tgt]));
+      p.ent[row] = none ? 0.f : ls - all.s1 * p.inv_t / all.s0;
+      p.stats[2 * row] = all.m;
+      p.stats[2 * row + 1] = ls;
+    }
+    auto write = [&](int at, uint64_t key) {
+      const uint32_t id = key_index(key);
+      p.top_id[row * p.k + at] = id;
+      p.top_lp[row * p.k + at] = log_p(to_f(x[id]));
+    };
+    if (CL == 1) {
+      if (tid < p.k) write(tid, sm_top[tid]);
+    } else {
+      // CL lists of k, each key in one of them: its rank among all of them
+      for (int c = tid; c < CL * p.k; c += NT) sm_cand[c] = *in_cta(&sm_top[c % p.k], c / p.k);
+      __syncthreads();
+      for (int c = tid; c < CL * p.k; c += NT) {
+        const uint64_t me = sm_cand[c];
+        int above = 0;
+        for (int d = 0; d < CL * p.k && above < p.k; ++d) above += sm_cand[d] > me;
+        if (above < p.k && me) write(above, me);
+      }
+    }
   }
+  cluster_sync<CL>();
 }
 
 struct BwdParams {
@@ -279,9 +446,30 @@ static int64_t check(const at::Tensor& logits, const at::Tensor& target, double 
   TORCH_CHECK(V >= 1 && V < (1LL << 31) - SEG, "token_scores: vocabulary of ", V);
   const int64_t R = logits.numel() / V;
   TORCH_CHECK(target.numel() == R, "token_scores: one target per row (", R, " rows, ", target.numel(), " targets)");
-  TORCH_CHECK(R < (1LL << 31), "token_scores: at most 2^31 - 1 rows");
+  TORCH_CHECK(R < (1LL << 28), "token_scores: at most 2^28 rows");
   TORCH_CHECK(top_k >= 0 && top_k <= std::min<int64_t>(MAXK, V), "token_scores: top_k from 0 to ", std::min<int64_t>(MAXK, V), ", got ", top_k);
   return R;
+}
+
+// CTAs per row: as many (up to 8) as keep all of them resident (two per SM) with 16 KB of the row or more each
+static int cluster_of(int64_t R, int64_t row_bytes) {
+  int cl = 1;
+  while (cl < 8 && R * cl * 2 <= 2 * num_sms() && row_bytes >= 16384 * cl * 2) cl *= 2;
+  return cl;
+}
+template <typename T, int CL>
+void launch_fwd(const T* x, const FwdParams& p, int64_t R) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(R * CL));
+  cfg.blockDim = dim3(NT);
+  cfg.stream = stream();
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CL;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = CL > 1 ? 1 : 0;
+  MAMF_CUDA_CHECK(cudaLaunchKernelEx(&cfg, scores_fwd_kernel<T, CL>, x, p));
 }
 
 }  // namespace ts
@@ -304,9 +492,13 @@ std::vector<at::Tensor> token_scores_fwd(at::Tensor logits, at::Tensor target, i
                 top_lp.data_ptr<float>(), stats.data_ptr<float>(), top_id.data_ptr<int64_t>(), ignore_index,
                 (int)logits.size(-1), (int)top_k, (float)(1.0 / temperature)};
     MAMF_DISPATCH_FLOAT_BF16(logits.scalar_type(), "token_scores", [&] {
-      scores_fwd_kernel<scalar_t><<<(unsigned)R, NT, 0, stream()>>>((const scalar_t*)logits.data_ptr(), p);
+      const scalar_t* x = (const scalar_t*)logits.data_ptr();
+      const int cl = cluster_of(R, p.V * (int64_t)sizeof(scalar_t));
+      if (cl == 8) launch_fwd<scalar_t, 8>(x, p, R);
+      else if (cl == 4) launch_fwd<scalar_t, 4>(x, p, R);
+      else if (cl == 2) launch_fwd<scalar_t, 2>(x, p, R);
+      else launch_fwd<scalar_t, 1>(x, p, R);
     });
-    MAMF_LAUNCH_CHECK();
   }
   return {lp, ent, top_lp, top_id, stats};
 }
