@@ -18,7 +18,6 @@
 namespace mamf {
 namespace ts {
 
-constexpr int NT = 512;
 constexpr int MAXK = 32;          // alternatives per row
 constexpr int CAP = 1024;         // candidates kept in shared memory for the selection
 constexpr float DMIN = -1e30f;
@@ -63,6 +62,10 @@ __device__ __forceinline__ uint32_t order(float x) {
 }
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t idx) {
   return ((uint64_t)order(x) << 32) | (0xFFFFFFFFu - idx);
+}
+__device__ __forceinline__ float key_value(uint64_t k) {          // NaN for the NaN key, +0 for both zeros
+  const uint32_t o = (uint32_t)(k >> 32);
+  return __uint_as_float((o & 0x80000000u) ? o & 0x7FFFFFFFu : ~o);
 }
 __device__ __forceinline__ uint32_t key_index(uint64_t k) { return 0xFFFFFFFFu - (uint32_t)k; }
 __device__ __forceinline__ uint64_t warp_max_u64(uint64_t v) {
@@ -166,11 +169,12 @@ template <typename V> __device__ __forceinline__ V* in_cta(V* p, int rank) {
 // running maximum per thread.  The alternatives come from the maxima: at least k threads hold an element no
 // smaller than the k-th largest of the threads' maxima, so only threads whose maximum reaches that bound can
 // hold an alternative, and only their elements (about k / NT of the row) are read again, by all threads.
-template <typename T, int CL>
-__global__ void __launch_bounds__(NT, 2) scores_fwd_kernel(const T* __restrict__ logits, const __grid_constant__ FwdParams p) {
+template <typename T, int CL, int NT>
+__global__ void __launch_bounds__(NT, NT == 512 ? 3 : 5) scores_fwd_kernel(const T* __restrict__ logits, const __grid_constant__ FwdParams p) {
   constexpr int VEC = 16 / sizeof(T), U = 4;
   __shared__ Stat sm_stat[NT / 32], sm_cta;
   __shared__ uint64_t sm_key[NT / 32], sm_top[MAXK], sm_cand[CAP];
+  __shared__ uint32_t sm_lo[NT / 32], sm_hi[NT / 32];
   __shared__ int sm_hot[NT], sm_nh, sm_n;
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, rank = cluster_rank<CL>();
   const int64_t row = blockIdx.x / CL;
@@ -190,6 +194,7 @@ __global__ void __launch_bounds__(NT, 2) scores_fwd_kernel(const T* __restrict__
   const int head = min(p.V, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
   const int nv = (p.V - head) / VEC, rem = rank == 0 ? p.V - nv * VEC : 0;
   const T* xv = x + head;
+  const float x_tgt = rank == 0 && tid == 0 ? to_f(x[tgt]) : 0.f;
   const int g0 = rank * NT + tid;
   auto rem_at = [&](int i) { return i < head ? i : nv * VEC + i; };
 
@@ -243,6 +248,10 @@ __global__ void __launch_bounds__(NT, 2) scores_fwd_kernel(const T* __restrict__
     merge(st, b, k2);
   }
   if (lane == 0) sm_stat[wid] = st;
+  if (p.k > 0) {
+    const uint32_t lo = __reduce_min_sync(0xffffffffu, mine), hi = __reduce_max_sync(0xffffffffu, mine);
+    if (lane == 0) { sm_lo[wid] = lo; sm_hi[wid] = hi; }
+  }
   if (tid == 0) { sm_nh = 0; sm_n = 0; }
   __syncthreads();
   if (wid == 0) {
@@ -257,11 +266,19 @@ __global__ void __launch_bounds__(NT, 2) scores_fwd_kernel(const T* __restrict__
   }
 
   if (p.k > 0) {
-    // the largest bound that at least k threads reach; values of the 16-bit types differ in the upper bits only
-    uint32_t bound = 0;
+    // A bound that at least k threads reach: bits that all maxima share, then one bit at a time, until few
+    // more than k threads reach it.  Values of the 16-bit types differ in the upper bits only.
+    uint32_t lo = ~0u, hi = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) { lo = min(lo, sm_lo[w]); hi = max(hi, sm_hi[w]); }
     constexpr uint32_t LOW = std::is_same<T, float>::value ? 1u : std::is_same<T, __half>::value ? 1u << 13 : 1u << 16;
-    for (uint32_t bit = 1u << 31; bit >= LOW; bit >>= 1)
-      if (__syncthreads_count(mine >= (bound | bit)) >= p.k) bound |= bit;
+    uint32_t bit = lo == hi ? 0u : 0x80000000u >> __clz(lo ^ hi);
+    uint32_t bound = bit ? lo & ~(2 * bit - 1) : lo & ~(LOW - 1);
+    for (; bit >= LOW; bit >>= 1) {
+      const int n = __syncthreads_count(mine >= (bound | bit));
+      if (n >= p.k) bound |= bit;
+      if (n >= p.k && n <= p.k + 4) break;
+    }
     if (mine >= bound && mine) sm_hot[atomicAdd(&sm_nh, 1)] = tid;
     __syncthreads();
     const int per = (nv + CL * NT - 1) / (CL * NT), items = sm_nh * per;
@@ -270,13 +287,21 @@ __global__ void __launch_bounds__(NT, 2) scores_fwd_kernel(const T* __restrict__
       const int at = atomicAdd(&sm_n, 1);
       if (at < CAP) sm_cand[at] = key_of(f, (uint32_t)idx);
     };
-    for (int it = tid; it < items; it += NT) {
-      const int v = rank * NT + sm_hot[it / per] + it % per * (CL * NT);
-      if (v >= nv) continue;
-      const Vec16<T> w = ld16(xv + (int64_t)v * VEC);
-      if (order(vec_max(w)) < bound) continue;
+    for (int it = tid; it < items; it += 4 * NT) {
+      Vec16<T> w[4];
+      int at[4];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) offer(to_f(w.v[e]), head + v * VEC + e);
+      for (int u = 0; u < 4; ++u) {
+        const int i = it + u * NT;
+        at[u] = i < items ? rank * NT + sm_hot[i / per] + i % per * (CL * NT) : nv;
+        if (at[u] < nv) w[u] = ld16(xv + (int64_t)at[u] * VEC);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (at[u] >= nv || order(vec_max(w[u])) < bound) continue;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) offer(to_f(w[u].v[e]), head + at[u] * VEC + e);
+      }
     }
     if (tid < rem) offer(to_f(x[rem_at(tid)]), rem_at(tid));
     __syncthreads();
@@ -325,15 +350,14 @@ __global__ void __launch_bounds__(NT, 2) scores_fwd_kernel(const T* __restrict__
     const float ls = none ? 0.f : logf(all.s0);
     auto log_p = [&](float f) { return none ? -INFINITY : (f - all.m) * p.inv_t - ls; };
     if (tid == 0) {
-      p.lp[row] = log_p(to_f(x[tgt]));
+      p.lp[row] = log_p(x_tgt);
       p.ent[row] = none ? 0.f : ls - all.s1 * p.inv_t / all.s0;
       p.stats[2 * row] = all.m;
       p.stats[2 * row + 1] = ls;
     }
     auto write = [&](int at, uint64_t key) {
-      const uint32_t id = key_index(key);
-      p.top_id[row * p.k + at] = id;
-      p.top_lp[row * p.k + at] = log_p(to_f(x[id]));
+      p.top_id[row * p.k + at] = key_index(key);
+      p.top_lp[row * p.k + at] = log_p(key_value(key));
     };
     if (CL == 1) {
       if (tid < p.k) write(tid, sm_top[tid]);
@@ -363,21 +387,34 @@ struct BwdParams {
   float inv_t;
 };
 
-constexpr int SEG = 16384;               // elements of a row per CTA
+constexpr int NB = 256, BU = 4;          // threads, 16-byte vectors of a thread: a CTA's share of a row is in flight at once
+template <typename T> constexpr int seg() { return NB * BU * (16 / (int)sizeof(T)); }
 
 // dx_j = p_j (a log p_j + b) with a = -gH / T, b = -(sum g + gH H) / T; the target's and the
 // alternatives' elements get their own g on top, written after the rest of the segment.
 template <typename T>
-__global__ void __launch_bounds__(NT) scores_bwd_kernel(const T* __restrict__ logits, T* __restrict__ out, BwdParams p) {
+__global__ void __launch_bounds__(NB, 6) scores_bwd_kernel(const T* __restrict__ logits, T* __restrict__ out,
+                                                           const __grid_constant__ BwdParams p) {
   constexpr int VEC = 16 / sizeof(T);
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x;
-  const int c0 = blockIdx.y * SEG, c1 = min(p.V, c0 + SEG);
+  const int c0 = blockIdx.y * seg<T>(), c1 = min(p.V, c0 + seg<T>());
   const T* x = logits + p.rows.at(row);
   T* y = out + row * p.V;
   const int64_t tgt = p.target[row];
   const float m = p.stats[2 * row], ls = p.stats[2 * row + 1];
   const bool dead = tgt == p.ignore || tgt < 0 || tgt >= p.V || m == -INFINITY;
+  // vectors where input and output share their place in a 16-byte line, single elements at the ends
+  const bool vec = ((reinterpret_cast<uintptr_t>(x + c0) ^ reinterpret_cast<uintptr_t>(y + c0)) & 15) == 0;
+  const int head = vec ? min(c1 - c0, (int)(((16 - (reinterpret_cast<uintptr_t>(y + c0) & 15)) & 15) / sizeof(T))) : 0;
+  const int nv = vec ? (c1 - c0 - head) / VEC : 0;
+  const int rem = c1 - c0 - nv * VEC;
+  Vec16<T> v[BU];
+#pragma unroll
+  for (int u = 0; u < BU; ++u) {
+    v[u].raw = make_uint4(0, 0, 0, 0);
+    if (!dead && u * NB + tid < nv) v[u] = ld16(x + c0 + head + (int64_t)(u * NB + tid) * VEC);
+  }
   float G = 0.f, a = 0.f, b = 0.f;
   if (!dead) {
     const float gh = p.g_ent ? p.g_ent[row] : 0.f;
@@ -403,22 +440,25 @@ __global__ void __launch_bounds__(NT) scores_bwd_kernel(const T* __restrict__ lo
     if (col < c0 || col >= c1) col = -1;
     else fix = grad(to_f(x[col])) + own * p.inv_t;
   }
-  const bool vec = ((reinterpret_cast<uintptr_t>(x + c0) ^ reinterpret_cast<uintptr_t>(y + c0)) & 15) == 0;
-  const int head = vec ? min(c1 - c0, (int)(((16 - (reinterpret_cast<uintptr_t>(y + c0) & 15)) & 15) / sizeof(T))) : 0;
-  const int nv = vec ? (c1 - c0 - head) / VEC : 0;
-  const int rem = c1 - c0 - nv * VEC;
-  for (int i = tid; i < nv; i += NT) {
-    const int64_t o = c0 + head + (int64_t)i * VEC;
-    Vec16<T> v;
-    if (dead) v.raw = make_uint4(0, 0, 0, 0);
-    else {
-      v = ld16(x + o);
+  const uint64_t nm = pk(-m, -m), it2 = pk(p.inv_t, p.inv_t), nl = pk(-ls, -ls), a2 = pk(a, a), b2 = pk(b, b), l2 = pk(LOG2E, LOG2E);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) v.v[j] = from_f<T>(grad(to_f(v.v[j])));
+  for (int u = 0; u < BU; ++u) {
+    if (u * NB + tid >= nv) break;
+    if (!dead) {
+#pragma unroll
+      for (int j = 0; j < VEC; j += 2) {
+        float f0, f1;
+        unpk(fma2(add2(pk(to_f(v[u].v[j]), to_f(v[u].v[j + 1])), nm), it2, nl), f0, f1);
+        const uint64_t lp = pk(max_nan(f0, DMIN), max_nan(f1, DMIN));
+        unpk(mul2(lp, l2), f0, f1);
+        unpk(mul2(pk(ex2(f0), ex2(f1)), fma2(a2, lp, b2)), f0, f1);
+        v[u].v[j] = from_f<T>(f0);
+        v[u].v[j + 1] = from_f<T>(f1);
+      }
     }
-    st16(y + o, v);
+    st16(y + c0 + head + (int64_t)(u * NB + tid) * VEC, v[u]);
   }
-  for (int i = tid; i < rem; i += NT) {
+  for (int i = tid; i < rem; i += NB) {
     const int c = c0 + (i < head ? i : nv * VEC + i);
     y[c] = from_f<T>(dead ? 0.f : grad(to_f(x[c])));
   }
@@ -443,7 +483,7 @@ static int64_t check(const at::Tensor& logits, const at::Tensor& target, double 
               "token_scores: logits and targets on one GPU");
   TORCH_CHECK(target.scalar_type() == at::kLong && target.is_contiguous(), "token_scores: contiguous int64 targets");
   const int64_t V = logits.size(-1);
-  TORCH_CHECK(V >= 1 && V < (1LL << 31) - SEG, "token_scores: vocabulary of ", V);
+  TORCH_CHECK(V >= 1 && V < (1LL << 30), "token_scores: vocabulary of ", V);
   const int64_t R = logits.numel() / V;
   TORCH_CHECK(target.numel() == R, "token_scores: one target per row (", R, " rows, ", target.numel(), " targets)");
   TORCH_CHECK(R < (1LL << 28), "token_scores: at most 2^28 rows");
@@ -451,13 +491,13 @@ static int64_t check(const at::Tensor& logits, const at::Tensor& target, double 
   return R;
 }
 
-// CTAs per row: as many (up to 8) as keep all of them resident (two per SM) with 16 KB of the row or more each
+// CTAs per row: 8, 4 or 2 where that many per row stay resident at one per SM and each has 16 KB of the row
 static int cluster_of(int64_t R, int64_t row_bytes) {
   int cl = 1;
-  while (cl < 8 && R * cl * 2 <= 2 * num_sms() && row_bytes >= 16384 * cl * 2) cl *= 2;
+  while (cl < 8 && R * cl * 2 <= num_sms() && row_bytes >= 32768 * cl) cl *= 2;
   return cl;
 }
-template <typename T, int CL>
+template <typename T, int CL, int NT>
 void launch_fwd(const T* x, const FwdParams& p, int64_t R) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(R * CL));
@@ -469,7 +509,19 @@ void launch_fwd(const T* x, const FwdParams& p, int64_t R) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = CL > 1 ? 1 : 0;
-  MAMF_CUDA_CHECK(cudaLaunchKernelEx(&cfg, scores_fwd_kernel<T, CL>, x, p));
+  MAMF_CUDA_CHECK(cudaLaunchKernelEx(&cfg, scores_fwd_kernel<T, CL, NT>, x, p));
+}
+// 512 threads have a row done sooner; 256 waste less at its end, which counts once every SM has several rows
+// (3686 x 128000 bf16: 160 us, with 512 174), unless the search for many alternatives is most of that (k = 20:
+// 229 us, with 512 209).
+template <typename T>
+void launch_fwd(const T* x, const FwdParams& p, int64_t R) {
+  const int cl = cluster_of(R, p.V * (int64_t)sizeof(T));
+  if (cl == 8) launch_fwd<T, 8, 512>(x, p, R);
+  else if (cl == 4) launch_fwd<T, 4, 512>(x, p, R);
+  else if (cl == 2) launch_fwd<T, 2, 512>(x, p, R);
+  else if (R < 3 * num_sms() || p.k > 8) launch_fwd<T, 1, 512>(x, p, R);
+  else launch_fwd<T, 1, 256>(x, p, R);
 }
 
 }  // namespace ts
@@ -492,12 +544,7 @@ std::vector<at::Tensor> token_scores_fwd(at::Tensor logits, at::Tensor target, i
                 top_lp.data_ptr<float>(), stats.data_ptr<float>(), top_id.data_ptr<int64_t>(), ignore_index,
                 (int)logits.size(-1), (int)top_k, (float)(1.0 / temperature)};
     MAMF_DISPATCH_FLOAT_BF16(logits.scalar_type(), "token_scores", [&] {
-      const scalar_t* x = (const scalar_t*)logits.data_ptr();
-      const int cl = cluster_of(R, p.V * (int64_t)sizeof(scalar_t));
-      if (cl == 8) launch_fwd<scalar_t, 8>(x, p, R);
-      else if (cl == 4) launch_fwd<scalar_t, 4>(x, p, R);
-      else if (cl == 2) launch_fwd<scalar_t, 2>(x, p, R);
-      else launch_fwd<scalar_t, 1>(x, p, R);
+      launch_fwd<scalar_t>((const scalar_t*)logits.data_ptr(), p, R);
     });
   }
   return {lp, ent, top_lp, top_id, stats};
@@ -525,8 +572,8 @@ at::Tensor token_scores_bwd(at::Tensor logits, at::Tensor target, int64_t ignore
               top_id.data_ptr<int64_t>(), ptr(g_lp, R), ptr(g_ent, R), ptr(g_top, R * k), ignore_index,
               (int)logits.size(-1), (int)k, (float)(1.0 / temperature)};
   MAMF_DISPATCH_FLOAT_BF16(logits.scalar_type(), "token_scores", [&] {
-    dim3 grid((unsigned)R, (unsigned)((p.V + SEG - 1) / SEG));
-    scores_bwd_kernel<scalar_t><<<grid, NT, 0, stream()>>>((const scalar_t*)logits.data_ptr(), (scalar_t*)out.data_ptr(), p);
+    dim3 grid((unsigned)R, (unsigned)((p.V + seg<scalar_t>() - 1) / seg<scalar_t>()));
+    scores_bwd_kernel<scalar_t><<<grid, NB, 0, stream()>>>((const scalar_t*)logits.data_ptr(), (scalar_t*)out.data_ptr(), p);
   });
   MAMF_LAUNCH_CHECK();
   return out;
