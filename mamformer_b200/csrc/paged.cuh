@@ -50,6 +50,23 @@ inline Cache check_cache(const char* what, const Layer& l, int64_t T, int64_t hd
                page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7, (int)l.table.size(1), (int)B, (int)T};
 }
 
+// What both attention kernels are given.
+struct Attn {
+  Cache c;
+  const void *q1, *q2;                 // packed queries (T, H, hd); q2 null: one map
+  void* out;                           // (T, H, hd), contiguous
+  const float* lam;
+  int64_t st1, sh1, st2, sh2;          // token and head strides of q1, q2 in elements
+  int H, rep, maps, window;            // rep = H / G query heads per KV head
+  int few;                             // sequences of up to this many rows (n * rep * maps) are the split kernel's
+  float scale_log2;
+};
+
+// csrc/paged_attn_tc.cu: sequences of more than `few` rows (of any number where few is 0, and then rows past
+// the last sequence are cleared too)
+void paged_chunk_attention(const Attn& p, int hd, bool bf16);
+int paged_chunk_error();
+
 // A tensor whose rows of adjacent values start on 16-byte boundaries: t itself, or a copy of it.
 inline at::Tensor rows16(const at::Tensor& t) {
   const int64_t n = 16 / t.element_size();

@@ -30,19 +30,14 @@ constexpr int STEP = 16;                       // tokens of a warp per tile
 constexpr int TILE = STEP * NW;                // tokens per tile
 constexpr long long WAIT_CYCLES = 4000000000LL;      // about 2 s
 constexpr float NONE = -1e30f;                 // maximum of no scores: 2^(score - NONE) is never formed, 2^(NONE - m) is 0
+constexpr int FEW = 64;                        // rows of a sequence and KV head above which the chunk kernel takes over
 constexpr float LAZY = 8.f;                    // log2 by which a row may outgrow its reference maximum
 
 __device__ int g_err = 0, g_wait_err = 0;
 __device__ __forceinline__ void record(int code) { atomicCAS(&g_err, 0, code); }
 
-struct Params {
-  Cache c;
-  const void *q1, *q2;
-  void* out;
-  const float* lam;
-  int64_t st1, sh1, st2, sh2;
-  int H, rep, maps, window, ctas;
-  float scale_log2;
+struct Params : Attn {
+  int ctas;
   float* part;        // [ctas][2][rows][HD + 2]: O (not divided), m, l
   int4* joins;        // [ctas]: the item that ends in this CTA after it began in another one
 };
@@ -129,8 +124,11 @@ __device__ __forceinline__ bool set_sequence(const Params& p, Item& it, int b) {
   it.len = p.c.lens[b];
   if (it.n <= 0 || it.t0 < 0 || it.t0 + it.n > p.c.T) return false;
   it.rows = it.n * p.rep * p.maps;
+  if (it.rows > p.few) {
+    if (p.few != FEW) record(ERR_LENGTH);                       // more new tokens than max_new
+    return false;
+  }
   it.g = it.rt = 0;
-  if (ROWS == 8 && it.rows > ROWS) record(ERR_LENGTH);          // more new tokens than max_new
   set_range<ROWS>(p, it);
   return true;
 }
@@ -774,22 +772,30 @@ at::Tensor paged_attention(at::Tensor q1, c10::optional<at::Tensor> q2, c10::opt
   }
   at::Tensor out = at::empty({T, H, hd}, q1.options());
   if (T == 0) return out;
+  TORCH_CHECK(p.c.P >= 1, "paged_attention: a pool without pages");
   p.out = out.data_ptr();
   p.H = (int)H;
   p.window = (int)std::min<int64_t>(window, 1LL << 30);
   p.scale_log2 = (float)(scale * 1.4426950408889634);
   p.rep = (int)(H / p.c.G);
   p.maps = p.q2 ? 2 : 1;
-  // one query row tile holds 8 rows, or 16 where some sequence can have more than 8
-  const int nr = std::max<int64_t>(1, max_new) * p.rep * p.maps > 8 ? 2 : 1, rows = 8 * nr;
-  const int64_t row_tiles = (std::max<int64_t>(1, std::min(max_new, T)) * p.rep * p.maps + rows - 1) / rows;
+  TORCH_CHECK(T * H < (1LL << 31), "paged_attention: sizes");
+  // Sequences of up to FEW rows go to the split kernel, longer runs of tokens to the chunk kernel; where all
+  // have the same number of tokens one of them does everything.
+  const int64_t most_rows = std::max<int64_t>(1, std::min(max_new, T)) * p.rep * p.maps;
+  const bool chunks = most_rows > FEW, alone = chunks && T == p.c.B * max_new;
+  p.few = chunks ? (alone ? 0 : FEW) : (int)most_rows;
+  if (chunks) paged_chunk_attention(p, (int)hd, q1.scalar_type() == at::kBFloat16);
+  if (alone) return out;
+  // one query row tile holds 8 rows, or 16 where a sequence can have more than 8
+  const int nr = p.few > 8 ? 2 : 1, rows = 8 * nr;
+  const int64_t row_tiles = (p.few + rows - 1) / rows;
   const int64_t most = std::max<int64_t>(1, (int64_t)p.c.B * p.c.G * row_tiles * std::max<int64_t>(1, ((int64_t)p.c.W * p.c.page + TILE - 1) / TILE));
   p.ctas = (int)std::min<int64_t>(most, (nr == 1 ? residents<1>() : residents<2>()) * num_sms());
   const int64_t part = (int64_t)p.ctas * 2 * rows * (hd + 2);
   at::Tensor ws = at::empty({part + 4 * p.ctas}, q1.options().dtype(at::kFloat));
   p.joins = reinterpret_cast<int4*>(ws.data_ptr<float>());
   p.part = ws.data_ptr<float>() + 4 * p.ctas;
-  TORCH_CHECK(p.c.P >= 1, "paged_attention: a pool without pages");
   TORCH_CHECK((int64_t)p.c.P * p.c.G * p.c.page * hd / 128 < (1LL << 31), "paged_attention: a pool of over 256 GB");
   const int64_t tokens = (int64_t)p.c.P * p.c.G * p.c.page;
   const CUtensorMap mk = lines_map(p.c.k, tokens, (int)hd), mv = lines_map(p.c.v, tokens, (int)hd);
@@ -808,7 +814,8 @@ int64_t paged_attention_error() {
   MAMF_CUDA_CHECK(cudaMemcpyFromSymbol(&w, pa::g_wait_err, sizeof(int)));
   if (v) MAMF_CUDA_CHECK(cudaMemcpyToSymbol(pa::g_err, &z, sizeof(int)));
   if (w) MAMF_CUDA_CHECK(cudaMemcpyToSymbol(pa::g_wait_err, &z, sizeof(int)));
-  return w ? w : v;
+  const int t = paged::paged_chunk_error();
+  return w ? w : v ? v : t;
 }
 
 }  // namespace mamf

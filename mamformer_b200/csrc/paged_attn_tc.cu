@@ -1,0 +1,428 @@
+// Attention over the paged 8-bit cache (layout in paged.cuh) for many query rows per KV head: chunks of a
+// prompt.  The products run on the 5th-generation tensor cores; every key tile is read once per CTA.
+//
+// A CTA holds two streams of 128 query rows of one KV head that share its keys and values:
+//   differential: the two maps of the same rows;   single softmax: two neighbouring tiles of rows.
+// A row is (token, head of the group), so short runs of tokens still fill a tile.  13 warps:
+//   warps 0-3, 4-7  softmax of stream A, B (thread = row = TMEM lane): write the row of q to shared memory
+//                   as f16, scaled by a power of two to [1, 2); then S from TMEM, P as packed f16 back over it
+//   warps 8-11      keys and values: 64-token tiles, 16 bytes per load, through registers one tile ahead,
+//                   e4m3 -> f16 (exact) into a ring of 128-byte-swizzled tiles; codes past the end become 0
+//   warp 12         TMEM allocation, MMA issue: S = Q K^T (M 128, N 64), O += P V (N = head size, P in TMEM)
+// The blocks' scales are powers of two and stay out of the products: a key's goes into the factor of its
+// score, a value's (relative to a reference that O is kept in) into the exponent of its weight, so a 16-token
+// group costs four multiplications per row.  Online softmax with lazy rescaling as in flash_tc.cu.  Every
+// wait is bounded; a wait that runs out records a code, and the CTA winds down.
+#include "paged.cuh"
+#include "tc5.cuh"
+
+namespace mamf {
+namespace ptc {
+
+using namespace paged;
+using namespace tc5;
+
+constexpr int BM = 128, BN = 64, ST = 4, NT = 416;
+constexpr long long WAIT_CYCLES = 4000000000LL;        // about 2 s
+constexpr float LAZY = 8.f, NONE = -1e30f;
+
+__device__ int g_err = 0, g_wait_err = 0;
+
+template <int HD> constexpr int q_bytes() { return BM * HD * 2; }
+template <int HD> constexpr int k_bytes() { return BN * HD * 2; }
+// the epilogue's exchange rows (fp32) lie over Q and the ring
+template <int HD> constexpr int smem_bytes() { return 1024 + 2 * q_bytes<HD>() + 2 * ST * k_bytes<HD>(); }
+
+using Params = Attn;
+
+__device__ __forceinline__ bool wait(uint64_t* b, uint32_t parity) { return bar_wait(b, parity, ERR_WAIT, &g_wait_err, WAIT_CYCLES); }
+// kind::f16, f16 x f16 -> fp32, A K-major
+__host__ __device__ constexpr uint32_t idesc(int n, bool b_mn) {
+  return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+}
+__device__ __forceinline__ uint32_t h2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void to_h4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}\n"
+      : "=r"(lo), "=r"(hi) : "r"(w));
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Params p) {
+  constexpr int QB = q_bytes<HD>(), KB = k_bytes<HD>();
+  constexpr int O_COL = 256;                       // TMEM: S_A[2], S_B[2] of 64 columns, then O_A, O_B of HD
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t q_full, kv_full[ST], kv_empty[ST], s_full[4], p_full[4], o_done[4], ex_full;
+  __shared__ float sc_k[ST][4], sc_v[ST][4];       // scales of the tile's 16-token groups, 0: not there
+  __shared__ uint32_t tmem_slot;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Cache& c = p.c;
+
+  if (p.few == 0) {                                // rows past the last sequence
+    const int64_t end = (int64_t)max(0, c.cu[c.B]) * p.H * HD, all = (int64_t)c.T * p.H * HD;
+    for (int64_t i = end + (int64_t)blockIdx.x * NT + threadIdx.x; i < all; i += (int64_t)gridDim.x * NT)
+      ((T*)p.out)[i] = from_f<T>(0.f);
+  }
+  // ---- the CTA's rows ----
+  const int rows = p.maps == 2 ? BM : 2 * BM;      // (token, head) pairs per CTA
+  const int g = blockIdx.x % c.G;
+  const int u = (gridDim.x - 1 - blockIdx.x) / c.G;        // later rows, which see more, first
+  // unit numbers of sequence b start at cu[b] rep / rows + b: it has ceil(n rep / rows) tiles or less
+  int b = 0;
+  {
+    int hi = c.B - 1;
+    while (b < hi) {
+      const int mid = (b + hi + 1) >> 1;
+      if ((int64_t)c.cu[mid] * p.rep / rows + mid <= u) b = mid; else hi = mid - 1;
+    }
+  }
+  const int t0 = c.cu[b], n = c.cu[b + 1] - t0, len = c.lens[b];
+  const int64_t tile64 = u - ((int64_t)t0 * p.rep / rows + b);
+  if (n <= 0 || t0 < 0 || t0 + n > c.T || (int64_t)n * p.rep * p.maps <= p.few || tile64 * rows >= (int64_t)n * p.rep) return;
+  const int r0 = (int)tile64 * rows, total = n * p.rep;    // first row of the tile, rows of the sequence
+  const int at0 = len - n;                                 // slot of token 0
+  const int i0 = r0 / p.rep, i1 = min(n - 1, (r0 + rows - 1) / p.rep);
+  const int key_hi = max(0, min(len, at0 + i1 + 1));
+  const int key_lo = p.window > 0 ? max(0, at0 + i0 - p.window + 1) : 0;
+  const int kt0 = key_lo / BN;
+  const int ntile = key_hi > key_lo ? (key_hi + BN - 1) / BN - kt0 : 0;
+
+  if (threadIdx.x == 0) {
+    bar_init(&q_full, 256);
+    bar_init(&ex_full, 128);
+    for (int s = 0; s < ST; ++s) { bar_init(&kv_full[s], 4); bar_init(&kv_empty[s], 1); }
+    for (int i = 0; i < 4; ++i) { bar_init(&s_full[i], 1); bar_init(&p_full[i], 128); bar_init(&o_done[i], 1); }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&tmem_slot)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_slot;
+  uint8_t* ring = sm + 2 * QB;
+
+  if (warp >= 8 && warp < 12) {
+    // ------------------------------- keys and values -------------------------------
+    constexpr int CR = HD / 16, N = BN * CR / 128;          // 16-byte chunks of a token, chunks per thread
+    const int ct = threadIdx.x - 256;
+    // chunk i of the thread: token (i * 128 + ct) / CR, dims 16 * (ct % CR) ..
+    uint4 kx[N], vx[N];
+    float ks = 0.f, vs = 0.f;                                // of group lane (lanes 0-3)
+    auto look_up = [&](int j) {
+      const int slot = (kt0 + j) * BN + (lane & 3) * 16;
+      if (j >= ntile || slot >= key_hi) return -2;
+      const int w = slot >> c.shift;
+      const int pg = w < c.W ? c.table[(int64_t)b * c.W + w] : -1;
+      return (unsigned)pg < (unsigned)c.P ? pg : -1;
+    };
+    auto load = [&](int j, int pg) {
+      const int slot = (kt0 + j) * BN;
+      const int64_t blk = (int64_t)pg * c.G + g;
+      ks = vs = 0.f;
+      if (pg >= 0) { ks = c.ks[blk]; vs = c.vs[blk]; }
+      else if (pg == -1 && ct < 4) atomicCAS(&g_err, 0, (int)ERR_PAGE);
+      const int64_t mine = pg >= 0 ? (blk << c.shift) + ((slot + (lane & 3) * 16) & (c.page - 1)) : -1;    // first token
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int r = (i * 128 + ct) / CR;
+        const int64_t first = __shfl_sync(0xffffffffu, mine, r >> 4);
+        kx[i] = vx[i] = make_uint4(0, 0, 0, 0);
+        if (first >= 0 && slot + r < key_hi) {               // codes past the end may be anything, NaN included
+          const int64_t off = (first + (r & 15)) * HD + (ct % CR) * 16;
+          kx[i] = *reinterpret_cast<const uint4*>(c.k + off);
+          vx[i] = *reinterpret_cast<const uint4*>(c.v + off);
+        }
+      }
+    };
+    auto store = [&](uint8_t* tile, const uint4& x, int r) {
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+      uint4 lo, hi;
+      to_h4(w[0], lo.x, lo.y);
+      to_h4(w[1], lo.z, lo.w);
+      to_h4(w[2], hi.x, hi.y);
+      to_h4(w[3], hi.z, hi.w);
+      const int cc = ct % CR;
+      uint8_t* row = tile + (cc >> 2) * (BN * 128) + r * 128;
+      const int c0 = ((cc & 3) * 2) ^ (r & 7), c1 = c0 ^ 1;
+      // the lanes of the second 64 dims store their halves the other way round: the banks of both differ
+      if (cc & 4) {
+        *reinterpret_cast<uint4*>(row + c1 * 16) = hi;
+        *reinterpret_cast<uint4*>(row + c0 * 16) = lo;
+      } else {
+        *reinterpret_cast<uint4*>(row + c0 * 16) = lo;
+        *reinterpret_cast<uint4*>(row + c1 * 16) = hi;
+      }
+    };
+    if (ntile > 0) load(0, look_up(0));
+    int next = look_up(1);                                   // the page of group lane % 4 of the tile to load next
+    bool ok = true;
+    for (int j = 0; j < ntile; ++j) {
+      const int st = j % ST;
+      if (j >= ST) ok = __all_sync(0xffffffffu, wait(&kv_empty[st], (uint32_t)((j / ST - 1) & 1)));
+      if (!ok) break;
+      uint8_t* kt = ring + st * 2 * KB;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int r = (i * 128 + ct) / CR;
+        store(kt, kx[i], r);
+        store(kt + KB, vx[i], r);
+      }
+      if (ct < 4) { sc_k[st][ct] = ks; sc_v[st][ct] = vs; }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) bar_arrive(&kv_full[st]);
+      if (j + 1 < ntile) {
+        const int pg = next;
+        next = look_up(j + 2);
+        load(j + 1, pg);
+      }
+    }
+  } else if (warp == 12) {
+    // ------------------------------- MMA issue -------------------------------
+    if (lane == 0 && ntile > 0) {
+      bool ok = wait(&q_full, 0);
+      fence_after();
+      constexpr uint32_t ID_QK = idesc(BN, false), ID_PV = idesc(HD, true);
+      auto issue_qk = [&](int j) -> bool {
+        const int st = j % ST, buf = j & 1;
+        // the S buffer last held P(j - 2), read by the O += P V that this thread issued before
+        if (!wait(&kv_full[st], (uint32_t)((j / ST) & 1))) return false;
+        fence_after();
+        const uint32_t kb = su32(ring + st * 2 * KB);
+        for (int s = 0; s < 2; ++s) {
+          const uint32_t qb = su32(sm + s * QB);
+          const uint32_t d = tmem + (uint32_t)(s * 128 + buf * 64);
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k)
+            mma_ss(d, sdesc(qb + (k >> 2) * (BM * 128) + (k & 3) * 32, 16, 1024), sdesc(kb + (k >> 2) * (BN * 128) + (k & 3) * 32, 16, 1024),
+                   ID_QK, k > 0 ? 1u : 0u);
+          commit(&s_full[s * 2 + buf]);
+        }
+        return true;
+      };
+      if (ok) ok = issue_qk(0);
+      for (int j = 0; j < ntile && ok; ++j) {
+        if (j + 1 < ntile && !issue_qk(j + 1)) { ok = false; break; }
+        const int st = j % ST, buf = j & 1;
+        const uint32_t vb = su32(ring + st * 2 * KB + KB);
+        for (int s = 0; s < 2 && ok; ++s) {
+          if (!wait(&p_full[s * 2 + buf], (uint32_t)((j >> 1) & 1))) { ok = false; break; }
+          fence_after();
+          const uint32_t pa = tmem + (uint32_t)(s * 128 + buf * 64);
+          const uint32_t d = tmem + (uint32_t)(O_COL + s * HD);
+#pragma unroll
+          for (int k = 0; k < BN / 16; ++k)
+            mma_ts(d, pa + (uint32_t)(k * 8), sdesc(vb + k * 2048, BN * 128, 1024), ID_PV, (j > 0 || k > 0) ? 1u : 0u);
+          commit(&o_done[s * 2 + buf]);
+        }
+        if (ok) commit(&kv_empty[st]);
+      }
+    }
+  } else if (warp < 8) {
+    // ------------------------------- softmax -------------------------------
+    const int s = warp >> 2, r = (warp & 3) * 32 + lane;    // stream, row in its tile = TMEM lane
+    const int row = r0 + r + (p.maps == 1 ? s * BM : 0);
+    const bool row_ok = row < total;
+    const int i = row / p.rep, h = g * p.rep + row % p.rep;
+    const int at = at0 + i;
+    const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    float rs = 0.f;
+    {
+      const bool second = p.maps == 2 && s == 1;
+      const T* q = second ? (const T*)p.q2 + (int64_t)(t0 + i) * p.st2 + (int64_t)h * p.sh2
+                          : (const T*)p.q1 + (int64_t)(t0 + i) * p.st1 + (int64_t)h * p.sh1;
+      Vec16<T> x[HD / 8];
+      float mx = 0.f;
+#pragma unroll
+      for (int k = 0; k < HD / 8; ++k) {
+        x[k].raw = make_uint4(0, 0, 0, 0);
+        if (row_ok) x[k] = ld16(q + 8 * k);
+      }
+#pragma unroll
+      for (int k = 0; k < HD / 8; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fabsf(to_f(x[k].v[j])));
+      int e = (int)(__float_as_uint(mx) >> 23) - 127;       // rows of zeros and rows with infinities stay as they are
+      if (e == -127 || e == 128) e = 0;
+      e = max(-126, min(126, e));
+      const float down = pow2(-e);
+      rs = p.scale_log2 * pow2(e);
+      uint8_t* qrow = sm + s * QB + r * 128;
+#pragma unroll
+      for (int k = 0; k < HD / 8; ++k) {
+        uint4 v;
+        v.x = h2(to_f(x[k].v[0]) * down, to_f(x[k].v[1]) * down);
+        v.y = h2(to_f(x[k].v[2]) * down, to_f(x[k].v[3]) * down);
+        v.z = h2(to_f(x[k].v[4]) * down, to_f(x[k].v[5]) * down);
+        v.w = h2(to_f(x[k].v[6]) * down, to_f(x[k].v[7]) * down);
+        *reinterpret_cast<uint4*>(qrow + (k >> 3) * (BM * 128) + (((k & 7) ^ (r & 7)) << 4)) = v;
+      }
+      fence_async_smem();
+      bar_arrive(&q_full);
+    }
+    // slots [lo, hi] that the row sees; rows past the last one (zeros) see everything and are not written
+    const int hi = row_ok ? min(len - 1, at) : 0x7fffffff, lo = row_ok && p.window > 0 ? at - p.window + 1 : 0;
+    float m = NONE, l = 0.f, vref = 0.f;
+    bool ok = true;
+    for (int j = 0; j < ntile && ok; ++j) {
+      const int buf = j & 1, st = j % ST;
+      ok = __all_sync(0xffffffffu, wait(&kv_full[st], (uint32_t)((j / ST) & 1)) && wait(&s_full[s * 2 + buf], (uint32_t)((j >> 1) & 1)));
+      if (!ok) break;
+      fence_after();
+      float sv[BN];
+      tld64(tl + (uint32_t)(s * 128 + buf * 64), sv);
+      float f[4], vg[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) { f[k] = sc_k[st][k]; vg[k] = sc_v[st][k]; }
+      const int kbase = (kt0 + j) * BN;
+      const bool there = f[0] != 0.f && f[1] != 0.f && f[2] != 0.f && f[3] != 0.f;
+      if (__any_sync(0xffffffffu, !(there && kbase >= lo && kbase + BN - 1 <= hi))) {
+#pragma unroll
+        for (int k = 0; k < BN; ++k) {
+          const int key = kbase + k;
+          sv[k] = (key >= lo && key <= hi && f[k >> 4] != 0.f) ? sv[k] : -INFINITY;
+        }
+        // a masked group's factor: -inf stays -inf
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[k] = f[k] != 0.f ? f[k] : 1.f;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float a = sv[16 * k], a2 = sv[16 * k + 1], a3 = sv[16 * k + 2], a4 = sv[16 * k + 3];
+#pragma unroll
+        for (int q = 4; q < 16; q += 4) {
+          a = fmaxf(a, sv[16 * k + q]);
+          a2 = fmaxf(a2, sv[16 * k + q + 1]);
+          a3 = fmaxf(a3, sv[16 * k + q + 2]);
+          a4 = fmaxf(a4, sv[16 * k + q + 3]);
+        }
+        f[k] *= rs;
+        mx = fmaxf(mx, fmaxf(fmaxf(a, a2), fmaxf(a3, a4)) * f[k]);
+      }
+      // the reference that O's values are in: the tile's largest value scale, once that is 2^6 away from it
+      const float vmax = fmaxf(fmaxf(vg[0], vg[1]), fmaxf(vg[2], vg[3]));
+      float fo = 1.f;
+      if (vmax > 0.f) {
+        if (vref == 0.f) vref = vmax;
+        else if (vmax > vref * 64.f || (vmax < vref * 0.015625f && vmax > vref * 8.6736174e-19f)) {
+          fo = vref / vmax;
+          vref = vmax;
+        }
+      }
+      const bool grow = mx > m + LAZY;
+      if (grow) {
+        const float g2 = ex2(m - mx);                       // 0 for the first key of a row
+        l *= g2;
+        fo *= g2;
+        m = mx;
+      }
+      if (j > 0 && __any_sync(0xffffffffu, fo != 1.f)) {
+        ok = __all_sync(0xffffffffu, wait(&o_done[s * 2 + ((j - 1) & 1)], (uint32_t)(((j - 1) >> 1) & 1)));
+        if (!ok) break;
+        fence_after();
+#pragma unroll 1
+        for (int cc = 0; cc < HD; cc += 32) {
+          float o[32];
+          tld32(tl + (uint32_t)(O_COL + s * HD + cc), o);
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] *= fo;
+          tst32(tl + (uint32_t)(O_COL + s * HD + cc), o);
+        }
+      }
+      float pk[BN / 2];                                     // P as f16 pairs, bit patterns in fp32 registers
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        // weights of group k are 2^e times P, e the exponent of its value scale over vref (at most 6)
+        const int e = vg[k] > 0.f ? max(-100, ((int)__float_as_uint(vg[k]) - (int)__float_as_uint(vref)) >> 23) : 0;
+        const float neg = (float)e - m;
+        float a = 0.f, a2 = 0.f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const float e0 = ex2(fmaf(sv[16 * k + 2 * q], f[k], neg)), e1 = ex2(fmaf(sv[16 * k + 2 * q + 1], f[k], neg));
+          a += e0;
+          a2 += e1;
+          pk[8 * k + q] = __uint_as_float(h2(e0, e1));
+        }
+        l = fmaf(a + a2, pow2(-e), l);
+      }
+      tst32(tl + (uint32_t)(s * 128 + buf * 64), pk);       // over this row's S, which is in registers
+      fence_before();
+      bar_arrive(&p_full[s * 2 + buf]);
+    }
+    // ---- result ----
+    if (ok && ntile > 0) {
+      ok = __all_sync(0xffffffffu, wait(&o_done[s * 2 + ((ntile - 1) & 1)], (uint32_t)(((ntile - 1) >> 1) & 1)));
+      fence_after();
+    }
+    const float inv = l == 0.f ? 0.f : vref / l;
+    float lam = 0.f, den = 1.f;
+    if (p.maps == 2 && row_ok) { lam = p.lam[h]; den = 1.f / (1.f - lam + 1e-8f); }
+    float* xrow = reinterpret_cast<float*>(sm) + r * (HD + 4);        // stream B's row; Q and the ring are free now
+    if (p.maps == 2 && s == 0) ok = __all_sync(0xffffffffu, ok && wait(&ex_full, 0));
+    T* out = (T*)p.out + ((int64_t)(t0 + i) * p.H + h) * HD;
+#pragma unroll 1
+    for (int cc = 0; cc < HD && ok; cc += 32) {
+      float o[32];
+      if (ntile > 0) tld32(tl + (uint32_t)(O_COL + s * HD + cc), o);
+#pragma unroll
+      for (int k = 0; k < 32; ++k) o[k] = ntile > 0 ? o[k] * inv : 0.f;
+      if (p.maps == 2 && s == 1) {
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(xrow + cc + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+      } else if (row_ok) {
+#pragma unroll
+        for (int k = 0; k < 32; k += 8) {
+          Vec16<T> v;
+#pragma unroll
+          for (int q = 0; q < 8; ++q) v.v[q] = from_f<T>(p.maps == 2 ? (o[k + q] - lam * xrow[cc + k + q]) * den : o[k + q]);
+          st16(out + cc + k, v);
+        }
+      }
+    }
+    if (p.maps == 2 && s == 1) bar_arrive(&ex_full);
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+template <typename T, int HD>
+void launch(const Params& p) {
+  auto fn = chunk_kernel<T, HD>;
+  MAMF_CUDA_CHECK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<HD>()));
+  const int64_t rows = p.maps == 2 ? BM : 2 * BM;
+  const int64_t units = ((int64_t)p.c.T * p.rep / rows + p.c.B) * p.c.G;
+  TORCH_CHECK(units < (1LL << 31), "paged_attention: sizes");
+  fn<<<(unsigned)units, NT, smem_bytes<HD>(), stream()>>>(p);
+  MAMF_LAUNCH_CHECK();
+}
+
+}  // namespace ptc
+
+namespace paged {
+void paged_chunk_attention(const Attn& p, int hd, bool bf16) {
+  if (bf16) { if (hd == 128) ptc::launch<__nv_bfloat16, 128>(p); else ptc::launch<__nv_bfloat16, 64>(p); }
+  else { if (hd == 128) ptc::launch<__half, 128>(p); else ptc::launch<__half, 64>(p); }
+}
+int paged_chunk_error() {
+  int v = 0, w = 0, z = 0;
+  MAMF_CUDA_CHECK(cudaMemcpyFromSymbol(&v, ptc::g_err, sizeof(int)));
+  MAMF_CUDA_CHECK(cudaMemcpyFromSymbol(&w, ptc::g_wait_err, sizeof(int)));
+  if (v) MAMF_CUDA_CHECK(cudaMemcpyToSymbol(ptc::g_err, &z, sizeof(int)));
+  if (w) MAMF_CUDA_CHECK(cudaMemcpyToSymbol(ptc::g_wait_err, &z, sizeof(int)));
+  return w ? w : v;
+}
+}  // namespace paged
+
+}  // namespace mamf
