@@ -32,7 +32,8 @@ struct Params {
   Cache c;
   Src k, v, q[2];
   void* qo[2];
-  const float *cos, *sin;                            // (n_pos, hd / 2), null: no rotation
+  const float *cos, *sin;                            // (n_pos, hd / 2) with row stride rot, null: no rotation
+  int64_t rot;
   const int64_t* pos;                                // (T)
   int n_pos, H, units, per_seq, kv_blocks, nq;
 };
@@ -64,8 +65,12 @@ template <int HD>
 __device__ __forceinline__ void rotate8(const Params& p, int t, int d, float* a, float* b) {
   int64_t pos = p.pos[t];
   if (pos < 0 || pos >= p.n_pos) { record(ERR_POSITION); pos = pos < 0 ? 0 : p.n_pos - 1; }
-  const float* c = p.cos + pos * (HD / 2) + d;
-  const float* s = p.sin + pos * (HD / 2) + d;
+  float c[8], s[8];
+#pragma unroll
+  for (int i = 0; i < 8; i += 4) {
+    *reinterpret_cast<float4*>(c + i) = *reinterpret_cast<const float4*>(p.cos + pos * p.rot + d + i);
+    *reinterpret_cast<float4*>(s + i) = *reinterpret_cast<const float4*>(p.sin + pos * p.rot + d + i);
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float x = a[i], y = b[i], cv = c[i], sv = s[i];
@@ -241,14 +246,18 @@ std::vector<at::Tensor> kv_append(at::Tensor k, at::Tensor v, at::Tensor ck, at:
   TORCH_CHECK(queries.size() <= 2, "kv_append: at most two query tensors");
   if (cos.has_value()) {
     TORCH_CHECK(sin.has_value() && pos.has_value(), "kv_append: cos, sin and positions go together");
-    for (const at::Tensor* t : {&*cos, &*sin})
-      TORCH_CHECK(t->is_cuda() && t->device() == k.device() && t->scalar_type() == at::kFloat && t->is_contiguous() && t->dim() == 2 &&
+    for (at::Tensor* t : {&*cos, &*sin}) {
+      TORCH_CHECK(t->is_cuda() && t->device() == k.device() && t->scalar_type() == at::kFloat && t->dim() == 2 &&
                   t->size(1) == hd / 2 && t->size(0) == cos->size(0) && t->size(0) >= 1, "kv_append: fp32 cos and sin (positions, hd / 2)");
+      if (t->stride(1) != 1 || t->stride(0) % 4 != 0 || !aligned16(t->data_ptr())) *t = t->clone(at::MemoryFormat::Contiguous);
+    }
+    if (cos->stride(0) != sin->stride(0)) { cos = cos->contiguous(); sin = sin->contiguous(); }
     TORCH_CHECK(pos->is_cuda() && pos->device() == k.device() && pos->scalar_type() == at::kLong && pos->is_contiguous() &&
                 pos->numel() == T, "kv_append: int64 position of each token");
     TORCH_CHECK(cos->size(0) < (1LL << 31), "kv_append: table length");
     p.cos = cos->data_ptr<float>(); p.sin = sin->data_ptr<float>(); p.pos = pos->data_ptr<int64_t>();
     p.n_pos = (int)cos->size(0);
+    p.rot = cos->stride(0);
   } else {
     TORCH_CHECK(queries.empty(), "kv_append: queries are only passed to be rotated");
   }

@@ -8,7 +8,7 @@ Reference: ``scripts/train_grpo.py`` (``GRPOPromptDataset`` 99-152, ``collate_pr
    ``(r - mean_g r) / (std_g r + 1e-8)``;
 3. policy and frozen reference mean log-probs over the response tokens (optionally the S-GRPO
    random subset, the same subset for both);
-4. loss ``-mean(A * logp) + beta * mean(logp_ref - logp)``; gradient accumulation, clipping and
+4. loss ``-mean(A * logp) + beta * mean(logp_ref - logp)``, less ``entropy_beta`` times the mean token entropy; gradient accumulation, clipping and
    the mixed-precision AdamW of the pre-training engine.
 
 Deviation: the S-GRPO mask is placed on the response positions of the shifted label axis (the
@@ -40,7 +40,9 @@ class GRPOConfig:
     gen_temperature: float = 0.8
     gen_top_k: int = 50
     gen_top_p: float = 0.95
+    gen_kv_cache: str = "dense"            # "paged": 8-bit pages and the paged attention kernels for rollouts
     kl_beta: float = 0.04
+    entropy_beta: float = 0.0              # weight of the policy's mean token entropy, which is rewarded
     learning_rate: float = 1e-6
     weight_decay: float = 0.0
     max_grad_norm: float = 1.0
@@ -150,7 +152,7 @@ class GRPOTrainer:
         outs = []
         for t in rollout_temperatures(c.gen_temperature, c.group_size):
             g = self.policy.generate(prompt_ids, max_new_tokens=c.gen_max_tokens, temperature=t, top_k=c.gen_top_k,
-                                     top_p=c.gen_top_p)
+                                     top_p=c.gen_top_p, kv_cache=c.gen_kv_cache)
             outs.append(g[:, prompt_ids.shape[1]:])
         self.policy.train()
         return outs
@@ -218,13 +220,22 @@ class GRPOTrainer:
         sb = c.sub_batch_size or N
         pol = torch.zeros(N, device=self.device)
         ref = torch.zeros(N, device=self.device)
+        ent = torch.zeros(N, device=self.device)
         for s in range(0, N, sb):
             e = min(N, s + sb)
             tm = tmask[s:e] if tmask is not None else None
-            pol[s:e] = self.policy.get_log_probs(ids[s:e], labels=labels[s:e], token_mask=tm).float()
+            if c.entropy_beta:
+                sc = self.policy.get_token_scores(ids[s:e], labels=labels[s:e], token_mask=tm)
+                w = self.policy._score_weights(labels[s:e], tm)
+                pol[s:e], ent[s:e] = ((x.float() * w).sum(1) / w.sum(1).clamp(min=1) for x in (sc.log_probs, sc.entropy))
+            else:
+                pol[s:e] = self.policy.get_log_probs(ids[s:e], labels=labels[s:e], token_mask=tm).float()
             with torch.no_grad():
                 ref[s:e] = self.reference.get_log_probs(ids[s:e], labels=labels[s:e], token_mask=tm).float()
         loss, metrics = compute_grpo_loss(pol.view(B, -1), ref.view(B, -1), adv, c.kl_beta)
+        if c.entropy_beta:
+            metrics["entropy"] = ent.detach().mean()
+            loss = loss - c.entropy_beta * ent.mean()
         if self.global_step % c.grad_accum == 0:
             self.optimizer.zero_grad()
         (loss / c.grad_accum).backward()

@@ -9,6 +9,9 @@ Window semantics: the reference's sliding-window mask keeps keys with
 ``0 <= key - query < W`` and, for this module, *replaces* the causal mask
 (``attention.py:157-166, 193-216``), i.e. each query sees itself and the following W-1 keys.
 ``window_mode='reference'`` (default) reproduces that; ``'causal'`` uses ``0 <= q - k < W``.
+
+A ``cache`` of the form ``{"paged": PagedLayer}`` (:mod:`mamformer_b200.paged_cache`) keeps K / V in 8-bit pages and
+attends to all of them causally.
 """
 
 from __future__ import annotations
@@ -53,6 +56,12 @@ class GroupedQueryAttention(nn.Module):
         v = self.v_proj(x).view(B, S, self.n_kv_heads, self.head_dim)
         offset = kwargs.get("rope_offset", 0)
         cos, sin = self.rope(S, x.device, offset)
+        if use_cache and cache is not None and "paged" in cache:
+            if attention_mask is not None:
+                raise ValueError("the paged cache attends causally and takes no attention_mask")
+            out = cache["paged"].attend(q, k, v, cos[0, 0, :, : self.head_dim // 2], sin[0, 0, :, : self.head_dim // 2],
+                                        window=self.sliding_window)
+            return self.o_proj(out.reshape(B, S, -1)), cache
         q = ops.rope(q, cos[0, 0, :, : self.head_dim // 2], sin[0, 0, :, : self.head_dim // 2])
         k = ops.rope(k, cos[0, 0, :, : self.head_dim // 2], sin[0, 0, :, : self.head_dim // 2])
         if use_cache and cache is not None:

@@ -95,13 +95,20 @@ class DifferentialStateAttention(nn.Module):
         k, v = k.view(B, S, G, hd), v.view(B, S, G, hd)
         cos, sin = self.rope(S, x.device, rope_offset)
         c, s = cos[0, 0, :, : hd // 2], sin[0, 0, :, : hd // 2]
-        q1, q2, k = ops.rope(q1, c, s), ops.rope(q2, c, s), ops.rope(k, c, s)
-        if use_cache and cache is not None:
-            k = torch.cat([cache["k"], k], dim=1)
-            v = torch.cat([cache["v"], v], dim=1)
-        new_cache = {"k": k, "v": v} if use_cache else None
-        out = ops.diff_attention(q1, q2, k, v, _lambda(self.lambda_raw), window=self.sliding_window,
-                                 window_mode=self.window_mode, attention_mask=attention_mask)
+        if use_cache and cache is not None and "paged" in cache:
+            if attention_mask is not None:
+                raise ValueError("the paged cache attends causally and takes no attention_mask")
+            new_cache = cache
+            out = cache["paged"].attend(q1, k, v, c, s, q2=q2, lam=_lambda(self.lambda_raw).float(),
+                                        window=self.sliding_window)
+        else:
+            q1, q2, k = ops.rope(q1, c, s), ops.rope(q2, c, s), ops.rope(k, c, s)
+            if use_cache and cache is not None:
+                k = torch.cat([cache["k"], k], dim=1)
+                v = torch.cat([cache["v"], v], dim=1)
+            new_cache = {"k": k, "v": v} if use_cache else None
+            out = ops.diff_attention(q1, q2, k, v, _lambda(self.lambda_raw), window=self.sliding_window,
+                                     window_mode=self.window_mode, attention_mask=attention_mask)
         flat = out.reshape(B, S, -1)
         normed = ops.head_group_norm(flat, H, self.group_norm.weight, self.group_norm.bias,
                                      self.group_norm.eps)

@@ -10,7 +10,8 @@ Reference: ``mamformer/layers/kda_diff.py``.
   Decode keeps the O(1) state ``S (B,H,K,hd)``, ``z (B,H,K,1)``.
 * ``FullDiffAttention`` (``kda_diff.py:639-898``): MLA-style ``k = k_expand(k_compress(x))``,
   same for v, injection, RoPE, two softmaxes with a causal (finfo.min) mask, differential
-  combine, GroupNorm, o_proj.  The KV cache holds the expanded k, v.
+  combine, GroupNorm, o_proj.  The KV cache holds the expanded k, v: bf16 tensors, or 8-bit pages
+  (``{"attn_type": "full", "paged": PagedLayer}``, :mod:`mamformer_b200.paged_cache`).
 * ``DynamicInterleaveGate`` (``kda_diff.py:905-958``): ``sigmoid(MLP(h_states))``.
 * ``KDADiffAttention`` (``kda_diff.py:965-1170``): full attention iff the mean gate > 0.5 when
   h_states is present and dynamic mode is on (a host sync, as in the reference), else iff
@@ -229,6 +230,12 @@ class FullDiffAttention(_DiffHeadNormMixin, nn.Module):
         k, v = k.view(B, S, G, hd), v.view(B, S, G, hd)
         cos, sin = self.rope(S, x.device, rope_offset)
         c, s = cos[0, 0, :, : hd // 2], sin[0, 0, :, : hd // 2]
+        if use_cache and cache is not None and "paged" in cache:
+            if attention_mask is not None:
+                raise ValueError("the paged cache attends causally and takes no attention_mask")
+            out = cache["paged"].attend(q1, k, v, c, s, q2=q2, lam=_lambda(self.lambda_raw).float(),
+                                        window=self.sliding_window)
+            return self._norm_and_project(out), cache
         q1, q2, k = ops.rope(q1, c, s), ops.rope(q2, c, s), ops.rope(k, c, s)
         if use_cache and cache is not None and cache.get("attn_type") == "full":
             k = torch.cat([cache["k"], k], dim=1)

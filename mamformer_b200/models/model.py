@@ -405,9 +405,16 @@ class MamformerForCausalLM(GenerationMixin, nn.Module):
                  temperature: Optional[float] = None, top_k: Optional[int] = None,
                  top_p: Optional[float] = None, eos_token_id: Optional[int] = None,
                  pad_token_id: Optional[int] = None,
-                 thinking_config: Optional[object] = None) -> Union[torch.Tensor, dict]:
+                 thinking_config: Optional[object] = None, kv_cache: str = "dense") -> Union[torch.Tensor, dict]:
+        """Sample up to ``max_new_tokens`` per row.  ``kv_cache="paged"`` keeps the full-attention layers' K / V in
+        8-bit pages (:class:`mamformer_b200.paged_cache.PagedKVCache`) instead of growing tensors, and attends with
+        the paged kernels."""
+        if kv_cache not in ("dense", "paged"):
+            raise ValueError(f"kv_cache must be 'dense' or 'paged', got {kv_cache!r}")
         if (thinking_config is not None and getattr(thinking_config, "enabled", False)
                 and getattr(thinking_config, "is_active", False)):
+            if kv_cache != "dense":
+                raise ValueError("thinking-mode generation copies its cache between paths: kv_cache='dense' only")
             self._ensure_thinking_tokens()
             return self._generate_with_thinking(input_ids, max_new_tokens, temperature, top_k,
                                                 top_p, eos_token_id, pad_token_id, thinking_config)
@@ -416,12 +423,18 @@ class MamformerForCausalLM(GenerationMixin, nn.Module):
         rep = self.config.generation.repetition_penalty
         B = input_ids.shape[0]
         generated = input_ids.clone()
-        cache = None
+        cache = paged = None
+        if kv_cache == "paged":
+            from mamformer_b200.paged_cache import PagedKVCache
+            paged = PagedKVCache.for_model(self, B, input_ids.shape[1] + max_new_tokens)
         alive = torch.ones(B, dtype=torch.bool, device=input_ids.device)
         for _ in range(max_new_tokens):
             if not bool(alive.any()):
                 break
             cur = generated if cache is None else generated[:, -1:]
+            if paged is not None:
+                paged.extend(cur.shape[1])
+                cache = paged.layer_caches() if cache is None else cache
             out = self.forward(cur, use_cache=True, cache=cache, return_logits=True)
             logits = out["logits"][:, -1, :].float()
             cache = out.get("cache")
@@ -563,16 +576,34 @@ class MamformerForCausalLM(GenerationMixin, nn.Module):
         """Per-token log p(input_ids[t+1] | <= t); with labels, the mean over response tokens
         (labels != -100, optionally AND token_mask) per sequence."""
         out = self.forward(input_ids, attention_mask=attention_mask, use_cache=False, return_logits=True)
-        logits = out["logits"][:, :-1, :]
-        tgt = input_ids[:, 1:]
-        tok_lp = ops.token_log_probs(logits, tgt.clamp(min=0))
-        tok_lp = tok_lp.masked_fill(tgt == -100, 0.0)
-        if labels is None:
+        mask = None if labels is None else self._score_weights(labels, token_mask)
+        tok_lp = ops.token_log_probs(out["logits"], self._score_targets(input_ids, mask))[:, :-1]
+        if mask is None:
             return tok_lp
-        mask = (labels[:, 1:] != -100).float()
-        if token_mask is not None:
-            mask = mask * token_mask.float()
         return (tok_lp * mask).sum(1) / mask.sum(1).clamp(min=1)
+
+    @staticmethod
+    def _score_weights(labels: torch.Tensor, token_mask: Optional[torch.Tensor]) -> torch.Tensor:
+        mask = (labels[:, 1:] != -100).float()
+        return mask if token_mask is None else mask * token_mask.float()
+
+    @staticmethod
+    def _score_targets(input_ids: torch.Tensor, mask: Optional[torch.Tensor]) -> torch.Tensor:
+        """(B, S) targets of whole logits: the next token, -100 (not scored) where the mask is 0 and in the last row.
+        The logits go in whole so that their gradient needs no copy."""
+        tgt = input_ids[:, 1:] if mask is None else input_ids[:, 1:].masked_fill(mask == 0, -100)
+        return F.pad(tgt, (0, 1), value=-100)
+
+    def get_token_scores(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None,
+                         attention_mask: Optional[torch.Tensor] = None, token_mask: Optional[torch.Tensor] = None,
+                         top_k: int = 0, temperature: float = 1.0) -> "ops.TokenScores":
+        """Scores (B, S - 1, ..) of input_ids[t + 1] given <= t: log probability, entropy, ``top_k`` alternatives, all
+        differentiable.  Positions without a label (with labels), outside ``token_mask`` or with target -100 are not
+        scored: 0, ids -1."""
+        logits = self.forward(input_ids, attention_mask=attention_mask, use_cache=False, return_logits=True)["logits"]
+        tgt = self._score_targets(input_ids, None if labels is None else self._score_weights(labels, token_mask))
+        s = ops.token_scores(logits, tgt, top_k=top_k, temperature=temperature)
+        return ops.TokenScores(*(x[:, :-1] for x in s))
 
     # -- info ------------------------------------------------------------------------------
     def num_parameters(self) -> int:

@@ -233,11 +233,12 @@ def token_scores(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, te
 
 
 def token_log_probs(logits: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
-    """log_softmax(logits)[..., target] without materialising the full log-softmax."""
+    """log_softmax(logits)[..., target] without materialising the full log-softmax; 0 where the target is -100."""
     if _native(logits) and "token_scores" in NATIVE and logits.dtype in _SCORE_TYPES:
         return _nat().token_scores(logits, targets, 0, 1.0, -100)[0]
     lf = logits.float()
-    return lf.gather(-1, targets.unsqueeze(-1)).squeeze(-1) - torch.logsumexp(lf, dim=-1)
+    lp = lf.gather(-1, targets.masked_fill(targets == -100, 0).unsqueeze(-1)).squeeze(-1) - torch.logsumexp(lf, dim=-1)
+    return lp.masked_fill(targets == -100, 0.0)
 
 
 class PagedKV(NamedTuple):
@@ -246,6 +247,11 @@ class PagedKV(NamedTuple):
     v: torch.Tensor
     k_scale: torch.Tensor    # (P, G) fp32
     v_scale: torch.Tensor
+
+
+def _no_gradient(what: str, *tensors: torch.Tensor) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
 
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -260,7 +266,8 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, cache: PagedKV, block_table: tor
     and ``positions`` (T,) int64, keys and up to two query tensors (T, H, hd) are rotated on the way (halves, as
     :func:`rope`).  A page that takes new tokens must belong to one sequence only.  On the GPU a page or length out
     of range is skipped and a position is clamped to the tables, and ``fault.check_device_status`` raises
-    afterwards."""
+    afterwards.  No gradient."""
+    _no_gradient("kv_append", k, v, *queries)
     if _native(k) and "kv_append" in NATIVE:
         return _nat().kv_append(k, v, cache, block_table, cu_seqlens, kv_lens, max_new, cos, sin, positions, queries)
     return ref.kv_append(k, v, cache, block_table, cu_seqlens, kv_lens, cos, sin, positions, queries)
@@ -275,6 +282,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, 
     kv_lens - n + i, with ``window`` > 0 only the last ``window`` of them.  With ``q2`` and ``lam`` (H,) fp32, the
     differential form (softmax(q k) v - lam softmax(q2 k) v) / (1 - lam + 1e-8).  A query that sees nothing, and
     rows past cu_seqlens[-1], give 0.  No gradient."""
+    _no_gradient("paged_attention", q, *(x for x in (q2, lam) if x is not None))
     scale = q.shape[-1] ** -0.5 if scale is None else scale
     if _native(q) and "paged_attention" in NATIVE:
         return _nat().paged_attention(q, cache, block_table, cu_seqlens, kv_lens, max_new, q2, lam, window, scale)

@@ -375,7 +375,8 @@ def token_scores(logits, targets, top_k: int, temperature: float, ignore_index: 
     z = e.sum(-1, keepdim=True)
     lse = z.log()
     ent = torch.where(none, 0.0, lse - (d * e).sum(-1, keepdim=True) / z)[..., 0]
-    ids = torch.sort(x.detach(), dim=-1, descending=True, stable=True).indices[..., :top_k]
+    ids = torch.sort(x.detach(), dim=-1, descending=True, stable=True).indices[..., :top_k] if top_k else \
+        torch.empty(*x.shape[:-1], 0, dtype=torch.long, device=x.device)
     pick = torch.cat([targets.clamp(0, V - 1).unsqueeze(-1), ids], -1)
     lp = torch.where(none, -math.inf, u.gather(-1, pick) - lse)
     lp = torch.where(live.unsqueeze(-1), lp, 0.0)

@@ -30,6 +30,8 @@ def build_parser():
     p.add_argument("--summary_budget", type=int, default=0)
     p.add_argument("--show_thinking", action="store_true")
     p.add_argument("--bf16", action="store_true")
+    p.add_argument("--kv_cache", default="dense", choices=("dense", "paged"),
+                   help="paged: keys and values in 8-bit pages (sampling only)")
     p.add_argument("--seed", type=int, default=42, help="seeds the weights of a model built without a checkpoint "
                                                          "and the sampling")
     return p
@@ -53,7 +55,7 @@ def generate_text(model, tok, prompt, args):
                                  eos_token_id=tok.eos_token_id)
     else:
         seq = model.generate(ids, max_new_tokens=args.max_new_tokens, temperature=args.temperature,
-                             top_k=args.top_k, top_p=args.top_p, eos_token_id=tok.eos_token_id)
+                             top_k=args.top_k, top_p=args.top_p, eos_token_id=tok.eos_token_id, kv_cache=args.kv_cache)
     return tok.decode(seq[0, ids.shape[1]:].tolist(), skip_special_tokens=not args.show_thinking)
 
 

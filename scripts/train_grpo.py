@@ -26,6 +26,9 @@ def build_parser():
     p.add_argument("--gen_temperature", type=float, default=1.0)
     p.add_argument("--gen_top_p", type=float, default=0.95)
     p.add_argument("--gen_top_k", type=int, default=50)
+    p.add_argument("--gen_kv_cache", default="dense", choices=("dense", "paged"),
+                   help="paged: rollouts keep keys and values in 8-bit pages")
+    p.add_argument("--entropy_beta", type=float, default=0.0, help="weight of the policy's token entropy in the loss")
     p.add_argument("--batch_size", type=int, default=4)
     p.add_argument("--gradient_accumulation_steps", type=int, default=1)
     p.add_argument("--learning_rate", type=float, default=1e-6)
@@ -71,7 +74,7 @@ def main(argv=None):
     tok = MamformerTokenizer()
     gcfg = GRPOConfig(group_size=args.group_size, gen_max_tokens=args.gen_max_tokens,
                       gen_temperature=args.gen_temperature, gen_top_k=args.gen_top_k, gen_top_p=args.gen_top_p,
-                      kl_beta=args.kl_beta, learning_rate=args.learning_rate, weight_decay=args.weight_decay,
+                      gen_kv_cache=args.gen_kv_cache, entropy_beta=args.entropy_beta, kl_beta=args.kl_beta, learning_rate=args.learning_rate, weight_decay=args.weight_decay,
                       max_grad_norm=args.max_grad_norm, grad_accum=args.gradient_accumulation_steps,
                       sub_batch_size=args.sub_batch_size or None, warmup_steps=args.warmup_steps,
                       max_steps=args.max_steps,
