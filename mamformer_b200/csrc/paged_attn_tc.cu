@@ -3,16 +3,17 @@
 //
 // A CTA holds two streams of 128 query rows of one KV head that share its keys and values:
 //   differential: the two maps of the same rows;   single softmax: two neighbouring tiles of rows.
-// A row is (token, head of the group), so short runs of tokens still fill a tile.  13 warps:
+// A row is (token, head of the group), so short runs of tokens still fill a tile.  11 warps:
 //   warps 0-3, 4-7  softmax of stream A, B (thread = row = TMEM lane): write the row of q to shared memory
 //                   as f16, scaled by a power of two to [1, 2); then S from TMEM, P as packed f16 back over it
-//   warps 8-11      keys and values: 64-token tiles, 16 bytes per load, through registers one tile ahead,
+//   warps 8-9       keys and values: 64-token tiles, 16 bytes per load, through registers one tile ahead,
 //                   e4m3 -> f16 (exact) into a ring of 128-byte-swizzled tiles; codes past the end become 0
-//   warp 12         TMEM allocation, MMA issue: S = Q K^T (M 128, N 64), O += P V (N = head size, P in TMEM)
+//   warp 10         TMEM allocation, MMA issue: S = Q K^T (M 128, N 64), O += P V (N = head size, P in TMEM)
 // The blocks' scales are powers of two and stay out of the products: a key's goes into the factor of its
 // score, a value's (relative to a reference that O is kept in) into the exponent of its weight, so a 16-token
 // group costs four multiplications per row.  Online softmax with lazy rescaling as in flash_tc.cu.  Every
 // wait is bounded; a wait that runs out records a code, and the CTA winds down.
+#include "f32x2.cuh"
 #include "paged.cuh"
 #include "tc5.cuh"
 
@@ -22,7 +23,7 @@ namespace ptc {
 using namespace paged;
 using namespace tc5;
 
-constexpr int BM = 128, BN = 64, ST = 4, NT = 416;
+constexpr int BM = 128, BN = 64, ST = 4, NC = 64, NT = 256 + NC + 32;       // NC converting threads
 constexpr long long WAIT_CYCLES = 4000000000LL;        // about 2 s
 constexpr float LAZY = 8.f, NONE = -1e30f;
 
@@ -50,6 +51,15 @@ __device__ __forceinline__ void to_h4(uint32_t w, uint32_t& lo, uint32_t& hi) {
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
+// What the softmax needs to know of a tile's four 16-token groups.
+struct __align__(16) Groups {
+  float k[4];          // scale of the keys, 0: the group is not there
+  float e[4];          // weights enter P V as 2^e times themselves: e is the exponent of the value scale over vref
+  float c[4];          // 2^-e
+  float vref, fo;      // the scale that O's values are in, and what it takes O there from the tile before
+  int all;             // all four groups are there
+};
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Params p) {
   constexpr int QB = q_bytes<HD>(), KB = k_bytes<HD>();
@@ -57,7 +67,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t q_full, kv_full[ST], kv_empty[ST], s_full[4], p_full[4], o_done[4], ex_full;
-  __shared__ float sc_k[ST][4], sc_v[ST][4];       // scales of the tile's 16-token groups, 0: not there
+  __shared__ Groups groups[ST];
   __shared__ uint32_t tmem_slot;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Cache& c = p.c;
@@ -94,11 +104,11 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
   if (threadIdx.x == 0) {
     bar_init(&q_full, 256);
     bar_init(&ex_full, 128);
-    for (int s = 0; s < ST; ++s) { bar_init(&kv_full[s], 4); bar_init(&kv_empty[s], 1); }
+    for (int s = 0; s < ST; ++s) { bar_init(&kv_full[s], NC / 32); bar_init(&kv_empty[s], 1); }
     for (int i = 0; i < 4; ++i) { bar_init(&s_full[i], 1); bar_init(&p_full[i], 128); bar_init(&o_done[i], 1); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 12) {
+  if (warp == 8 + NC / 32) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&tmem_slot)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -108,14 +118,14 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
   const uint32_t tmem = tmem_slot;
   uint8_t* ring = sm + 2 * QB;
 
-  if (warp >= 8 && warp < 12) {
+  if (warp >= 8 && warp < 8 + NC / 32) {
     // ------------------------------- keys and values -------------------------------
-    constexpr int CR = HD / 16, N = BN * CR / 128;          // 16-byte chunks of a token, chunks per thread
-    const int ct = threadIdx.x - 256;
-    // chunk i of the thread: token (i * 128 + ct) / CR, dims 16 * (ct % CR) ..
-    uint4 kx[N], vx[N];
-    float ks = 0.f, vs = 0.f;                                // of group lane (lanes 0-3)
-    auto look_up = [&](int j) {
+    constexpr int CR = HD / 16, N = BN * CR / NC;           // 16-byte chunks of a token, chunks per thread
+    constexpr int RS = NC / CR;                              // rows between a thread's chunks: 8 or 16
+    const int ct = threadIdx.x - 256, r0c = ct / CR, cc = ct % CR;
+    uint4 kx[N], vx[N];                                      // chunk i: token i RS + r0c, dims 16 cc ..
+    float ks = 0.f, vs = 0.f, vref = 0.f, fo = 1.f;          // ks, vs: of group lane % 4
+    auto look_up = [&](int j) {                              // the page of group lane % 4 of tile j
       const int slot = (kt0 + j) * BN + (lane & 3) * 16;
       if (j >= ntile || slot >= key_hi) return -2;
       const int w = slot >> c.shift;
@@ -128,53 +138,66 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
       ks = vs = 0.f;
       if (pg >= 0) { ks = c.ks[blk]; vs = c.vs[blk]; }
       else if (pg == -1 && ct < 4) atomicCAS(&g_err, 0, (int)ERR_PAGE);
-      const int64_t mine = pg >= 0 ? (blk << c.shift) + ((slot + (lane & 3) * 16) & (c.page - 1)) : -1;    // first token
+      // byte offset of the group's first token, -1: not there
+      const int64_t mine = pg >= 0 ? ((blk << c.shift) + ((slot + (lane & 3) * 16) & (c.page - 1))) * HD : -1;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int r = (i * 128 + ct) / CR;
-        const int64_t first = __shfl_sync(0xffffffffu, mine, r >> 4);
-        kx[i] = vx[i] = make_uint4(0, 0, 0, 0);
-        if (first >= 0 && slot + r < key_hi) {               // codes past the end may be anything, NaN included
-          const int64_t off = (first + (r & 15)) * HD + (ct % CR) * 16;
-          kx[i] = *reinterpret_cast<const uint4*>(c.k + off);
-          vx[i] = *reinterpret_cast<const uint4*>(c.v + off);
+      for (int q = 0; q < 4; ++q) {
+        const int64_t off = __shfl_sync(0xffffffffu, mine, q) + r0c * HD + cc * 16;
+        const bool there = __shfl_sync(0xffffffffu, pg, q) >= 0;
+#pragma unroll
+        for (int i = q * 16 / RS; i < (q + 1) * 16 / RS; ++i) {
+          kx[i] = vx[i] = make_uint4(0, 0, 0, 0);
+          if (there && slot + i * RS + r0c < key_hi) {       // codes past the end may be anything, NaN included
+            kx[i] = *reinterpret_cast<const uint4*>(c.k + off + (i * RS - q * 16) * HD);
+            vx[i] = *reinterpret_cast<const uint4*>(c.v + off + (i * RS - q * 16) * HD);
+          }
         }
       }
     };
-    auto store = [&](uint8_t* tile, const uint4& x, int r) {
-      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    // place of chunk 0's two 16-byte halves; row i RS + r0c has the same place in its 8 rows of 128 bytes.
+    // The lanes of the second 64 dims store their halves the other way round: the banks of both differ.
+    const int c0 = ((cc & 3) * 2) ^ (r0c & 7), swap = cc >> 2 & 1;
+    uint8_t* const at = ring + (cc >> 2) * (BN * 128) + r0c * 128;
+    const int first = (c0 ^ swap) * 16, second = (c0 ^ swap ^ 1) * 16;
+    auto store = [&](uint8_t* row, const uint4& x) {
       uint4 lo, hi;
-      to_h4(w[0], lo.x, lo.y);
-      to_h4(w[1], lo.z, lo.w);
-      to_h4(w[2], hi.x, hi.y);
-      to_h4(w[3], hi.z, hi.w);
-      const int cc = ct % CR;
-      uint8_t* row = tile + (cc >> 2) * (BN * 128) + r * 128;
-      const int c0 = ((cc & 3) * 2) ^ (r & 7), c1 = c0 ^ 1;
-      // the lanes of the second 64 dims store their halves the other way round: the banks of both differ
-      if (cc & 4) {
-        *reinterpret_cast<uint4*>(row + c1 * 16) = hi;
-        *reinterpret_cast<uint4*>(row + c0 * 16) = lo;
-      } else {
-        *reinterpret_cast<uint4*>(row + c0 * 16) = lo;
-        *reinterpret_cast<uint4*>(row + c1 * 16) = hi;
-      }
+      to_h4(x.x, lo.x, lo.y);
+      to_h4(x.y, lo.z, lo.w);
+      to_h4(x.z, hi.x, hi.y);
+      to_h4(x.w, hi.z, hi.w);
+      *reinterpret_cast<uint4*>(row + first) = swap ? hi : lo;
+      *reinterpret_cast<uint4*>(row + second) = swap ? lo : hi;
     };
     if (ntile > 0) load(0, look_up(0));
-    int next = look_up(1);                                   // the page of group lane % 4 of the tile to load next
+    int next = look_up(1);
     bool ok = true;
     for (int j = 0; j < ntile; ++j) {
       const int st = j % ST;
       if (j >= ST) ok = __all_sync(0xffffffffu, wait(&kv_empty[st], (uint32_t)((j / ST - 1) & 1)));
       if (!ok) break;
-      uint8_t* kt = ring + st * 2 * KB;
+      // the reference for O's values: the tile's largest value scale, once that is 2^6 away from it.  Scales
+      // below 2^-60 of it add nothing to O.
+      float vmax = fmaxf(vs, __shfl_xor_sync(0xffffffffu, vs, 1));
+      vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 2));
+      fo = 1.f;
+      if (vref == 0.f) vref = vmax;
+      else if (vmax > vref * 64.f || (vmax < vref * 0.015625f && vmax > vref * 8.6736174e-19f)) {
+        fo = vref / vmax;
+        vref = vmax;
+      }
+      const bool all = __all_sync(0xffffffffu, ks != 0.f);
+      if (ct < 4) {
+        const int e = vs > 0.f ? max(-100, ((int)__float_as_uint(vs) - (int)__float_as_uint(vref)) >> 23) : 0;
+        groups[st].k[ct] = ks;
+        groups[st].e[ct] = (float)e;
+        groups[st].c[ct] = pow2(-e);
+        if (ct == 0) { groups[st].vref = vref; groups[st].fo = fo; groups[st].all = all; }
+      }
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int r = (i * 128 + ct) / CR;
-        store(kt, kx[i], r);
-        store(kt + KB, vx[i], r);
+        store(at + st * 2 * KB + i * RS * 128, kx[i]);
+        store(at + st * 2 * KB + KB + i * RS * 128, vx[i]);
       }
-      if (ct < 4) { sc_k[st][ct] = ks; sc_v[st][ct] = vs; }
       fence_async_smem();
       __syncwarp();
       if (lane == 0) bar_arrive(&kv_full[st]);
@@ -184,7 +207,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
         load(j + 1, pg);
       }
     }
-  } else if (warp == 12) {
+  } else if (warp == 8 + NC / 32) {
     // ------------------------------- MMA issue -------------------------------
     if (lane == 0 && ntile > 0) {
       bool ok = wait(&q_full, 0);
@@ -269,7 +292,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
     }
     // slots [lo, hi] that the row sees; rows past the last one (zeros) see everything and are not written
     const int hi = row_ok ? min(len - 1, at) : 0x7fffffff, lo = row_ok && p.window > 0 ? at - p.window + 1 : 0;
-    float m = NONE, l = 0.f, vref = 0.f;
+    float m = NONE, l = 0.f;
     bool ok = true;
     for (int j = 0; j < ntile && ok; ++j) {
       const int buf = j & 1, st = j % ST;
@@ -278,12 +301,11 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
       fence_after();
       float sv[BN];
       tld64(tl + (uint32_t)(s * 128 + buf * 64), sv);
-      float f[4], vg[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) { f[k] = sc_k[st][k]; vg[k] = sc_v[st][k]; }
+      const Groups& gr = groups[st];
+      float f[4];
+      *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(gr.k);
       const int kbase = (kt0 + j) * BN;
-      const bool there = f[0] != 0.f && f[1] != 0.f && f[2] != 0.f && f[3] != 0.f;
-      if (__any_sync(0xffffffffu, !(there && kbase >= lo && kbase + BN - 1 <= hi))) {
+      if (__any_sync(0xffffffffu, !(gr.all && kbase >= lo && kbase + BN - 1 <= hi))) {
 #pragma unroll
         for (int k = 0; k < BN; ++k) {
           const int key = kbase + k;
@@ -296,29 +318,14 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
       float mx = -INFINITY;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        float a = sv[16 * k], a2 = sv[16 * k + 1], a3 = sv[16 * k + 2], a4 = sv[16 * k + 3];
+        float a[4];
 #pragma unroll
-        for (int q = 4; q < 16; q += 4) {
-          a = fmaxf(a, sv[16 * k + q]);
-          a2 = fmaxf(a2, sv[16 * k + q + 1]);
-          a3 = fmaxf(a3, sv[16 * k + q + 2]);
-          a4 = fmaxf(a4, sv[16 * k + q + 3]);
-        }
+        for (int q = 0; q < 4; ++q) a[q] = fmaxf(fmaxf(sv[16 * k + q], sv[16 * k + 4 + q]), fmaxf(sv[16 * k + 8 + q], sv[16 * k + 12 + q]));
         f[k] *= rs;
-        mx = fmaxf(mx, fmaxf(fmaxf(a, a2), fmaxf(a3, a4)) * f[k]);
+        mx = fmaxf(mx, fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])) * f[k]);
       }
-      // the reference that O's values are in: the tile's largest value scale, once that is 2^6 away from it
-      const float vmax = fmaxf(fmaxf(vg[0], vg[1]), fmaxf(vg[2], vg[3]));
-      float fo = 1.f;
-      if (vmax > 0.f) {
-        if (vref == 0.f) vref = vmax;
-        else if (vmax > vref * 64.f || (vmax < vref * 0.015625f && vmax > vref * 8.6736174e-19f)) {
-          fo = vref / vmax;
-          vref = vmax;
-        }
-      }
-      const bool grow = mx > m + LAZY;
-      if (grow) {
+      float fo = gr.fo;
+      if (mx > m + LAZY) {
         const float g2 = ex2(m - mx);                       // 0 for the first key of a row
         l *= g2;
         fo *= g2;
@@ -337,23 +344,26 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
           tst32(tl + (uint32_t)(O_COL + s * HD + cc), o);
         }
       }
-      float pk[BN / 2];                                     // P as f16 pairs, bit patterns in fp32 registers
+      float pk_[BN / 2];                                    // P as f16 pairs, bit patterns in fp32 registers
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        // weights of group k are 2^e times P, e the exponent of its value scale over vref (at most 6)
-        const int e = vg[k] > 0.f ? max(-100, ((int)__float_as_uint(vg[k]) - (int)__float_as_uint(vref)) >> 23) : 0;
-        const float neg = (float)e - m;
-        float a = 0.f, a2 = 0.f;
+        const float neg = gr.e[k] - m;
+        const uint64_t ff = pk(f[k], f[k]), nn = pk(neg, neg);
+        uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-          const float e0 = ex2(fmaf(sv[16 * k + 2 * q], f[k], neg)), e1 = ex2(fmaf(sv[16 * k + 2 * q + 1], f[k], neg));
-          a += e0;
-          a2 += e1;
-          pk[8 * k + q] = __uint_as_float(h2(e0, e1));
+          float e0, e1;
+          unpk(fma2(pk(sv[16 * k + 2 * q], sv[16 * k + 2 * q + 1]), ff, nn), e0, e1);
+          e0 = ex2(e0);
+          e1 = ex2(e1);
+          sum[q & 1] = add2(sum[q & 1], pk(e0, e1));
+          pk_[8 * k + q] = __uint_as_float(h2(e0, e1));
         }
-        l = fmaf(a + a2, pow2(-e), l);
+        float a, a2;
+        unpk(add2(sum[0], sum[1]), a, a2);
+        l = fmaf(a + a2, gr.c[k], l);
       }
-      tst32(tl + (uint32_t)(s * 128 + buf * 64), pk);       // over this row's S, which is in registers
+      tst32(tl + (uint32_t)(s * 128 + buf * 64), pk_);      // over this row's S, which is in registers
       fence_before();
       bar_arrive(&p_full[s * 2 + buf]);
     }
@@ -362,7 +372,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
       ok = __all_sync(0xffffffffu, wait(&o_done[s * 2 + ((ntile - 1) & 1)], (uint32_t)(((ntile - 1) >> 1) & 1)));
       fence_after();
     }
-    const float inv = l == 0.f ? 0.f : vref / l;
+    const float inv = l == 0.f ? 0.f : groups[(ntile - 1) % ST].vref / l;        // l is 0 where there is no tile
     float lam = 0.f, den = 1.f;
     if (p.maps == 2 && row_ok) { lam = p.lam[h]; den = 1.f / (1.f - lam + 1e-8f); }
     float* xrow = reinterpret_cast<float*>(sm) + r * (HD + 4);        // stream B's row; Q and the ring are free now
@@ -391,7 +401,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
   }
   fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 8 + NC / 32) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
   }

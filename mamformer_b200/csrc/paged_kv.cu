@@ -13,7 +13,9 @@
 //
 // One CTA owns one (sequence, page, KV head) of K or of V: it reads the page's new tokens once, keeps them
 // in registers, reduces their maximum, and writes the codes; no other CTA touches that block, so there are
-// no atomics.  Pages that take new tokens must belong to one sequence only.  Further CTAs rotate the queries.
+// no atomics.  Where no sequence has more than one new token, 8 lanes (4 for 64 dims) do that instead of a CTA:
+// a step of 200 sequences and 8 heads is then one wave of CTAs.  Pages that take new tokens must belong to one
+// sequence only.  Further CTAs rotate the queries in the same launch.
 #include "paged.cuh"
 
 namespace mamf {
@@ -35,7 +37,7 @@ struct Params {
   const float *cos, *sin;                            // (n_pos, hd / 2) with row stride rot, null: no rotation
   int64_t rot;
   const int64_t* pos;                                // (T)
-  int n_pos, H, units, per_seq, kv_blocks, nq;
+  int n_pos, H, units, per_seq, max_new, nq;
 };
 
 // 8 consecutive values of a token's head as floats
@@ -59,23 +61,28 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const float* 
   }
 }
 
-// (a, b) -> (a cos - b sin, b cos + a sin).  Separate roundings, as elementwise operations have them, so
-// that a value on the edge between two codes goes the same way.
+// cos and sin of 8 dims at token t's position
+struct Turn { float c[8], s[8]; };
 template <int HD>
-__device__ __forceinline__ void rotate8(const Params& p, int t, int d, float* a, float* b) {
+__device__ __forceinline__ Turn turn_of(const Params& p, int t, int d) {
   int64_t pos = p.pos[t];
   if (pos < 0 || pos >= p.n_pos) { record(ERR_POSITION); pos = pos < 0 ? 0 : p.n_pos - 1; }
-  float c[8], s[8];
+  Turn r;
 #pragma unroll
   for (int i = 0; i < 8; i += 4) {
-    *reinterpret_cast<float4*>(c + i) = *reinterpret_cast<const float4*>(p.cos + pos * p.rot + d + i);
-    *reinterpret_cast<float4*>(s + i) = *reinterpret_cast<const float4*>(p.sin + pos * p.rot + d + i);
+    *reinterpret_cast<float4*>(r.c + i) = *reinterpret_cast<const float4*>(p.cos + pos * p.rot + d + i);
+    *reinterpret_cast<float4*>(r.s + i) = *reinterpret_cast<const float4*>(p.sin + pos * p.rot + d + i);
   }
+  return r;
+}
+// (a, b) -> (a cos - b sin, b cos + a sin).  Separate roundings, as elementwise operations have them, so
+// that a value on the edge between two codes goes the same way.
+__device__ __forceinline__ void rotate8(const Turn& r, float* a, float* b) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float x = a[i], y = b[i], cv = c[i], sv = s[i];
-    a[i] = __fsub_rn(__fmul_rn(x, cv), __fmul_rn(y, sv));
-    b[i] = __fadd_rn(__fmul_rn(y, cv), __fmul_rn(x, sv));
+    const float x = a[i], y = b[i];
+    a[i] = __fsub_rn(__fmul_rn(x, r.c[i]), __fmul_rn(y, r.s[i]));
+    b[i] = __fadd_rn(__fmul_rn(y, r.c[i]), __fmul_rn(x, r.s[i]));
   }
 }
 
@@ -89,6 +96,41 @@ __device__ __forceinline__ float block_scale(float amax) {
 }
 __device__ __forceinline__ float inverse_pow2(float s) {          // s = 2^e, |e| <= 126
   return __uint_as_float((254u << 23) - __float_as_uint(s));
+}
+
+// The codes of a block's first `tokens` tokens, times f (a power of two below 1).
+template <int HD>
+__device__ __forceinline__ void rescale(uint8_t* codes, int tokens, float f, int first, int step) {
+  for (int i = first; i < tokens * HD / 16; i += step) {
+    union { uint4 raw; uint16_t c2[8]; } w;
+    w.raw = *reinterpret_cast<const uint4*>(codes + i * 16);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float2 v = dec2(w.c2[e]);
+      w.c2[e] = enc2(v.x * f, v.y * f);
+    }
+    *reinterpret_cast<uint4*>(codes + i * 16) = w.raw;
+  }
+}
+// 16 values of a token (8 of each half, from dim d) as codes
+template <int HD>
+__device__ __forceinline__ void put_codes(uint8_t* token, int d, const float* x, float inv) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    union { uint16_t c2[4]; uint2 raw; } w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w.c2[e] = enc2(x[8 * h + 2 * e] * inv, x[8 * h + 2 * e + 1] * inv);
+    *reinterpret_cast<uint2*>(token + h * (HD / 2) + d) = w.raw;
+  }
+}
+// the largest of m and |x|; NaN and infinities do not count
+__device__ __forceinline__ float finite_max(const float* x, float m) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const float a = fabsf(x[e]);
+    m = fmaxf(m, a < INFINITY ? a : 0.f);
+  }
+  return m;
 }
 
 template <typename T, int HD, int NP>
@@ -115,9 +157,9 @@ __device__ __forceinline__ void append_block(const Params& p) {
   const int t0 = c.cu[b], n = c.cu[b + 1] - t0, end = c.lens[b], start = end - n;
   if (n <= 0) return;
   const int pages = (end - 1) / c.page - start / c.page + 1;
-  if (start < 0 || t0 < 0 || t0 + n > c.T || (p.per_seq > 0 && j == 0 && pages > p.per_seq)) {
+  if (start < 0 || t0 < 0 || t0 + n > c.T || n > p.max_new) {
     if (tid == 0) record(ERR_LENGTH);
-    if (start < 0 || t0 < 0 || t0 + n > c.T) return;
+    return;
   }
   if (j >= pages) return;
   const int jp = start / c.page + j;
@@ -139,12 +181,8 @@ __device__ __forceinline__ void append_block(const Params& p) {
       const int t = t0 + jp * c.page + slot - start;
       load8(in + (int64_t)t * src.st + d, x[i]);
       load8(in + (int64_t)t * src.st + HD / 2 + d, x[i] + 8);
-      if (!is_v && p.cos) rotate8<HD>(p, t, d, x[i], x[i] + 8);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float m = fabsf(x[i][e]);
-        amax = fmaxf(amax, m < INFINITY ? m : 0.f);        // NaN and infinities do not set the scale
-      }
+      if (!is_v && p.cos) rotate8(turn_of<HD>(p, t, d), x[i], x[i] + 8);
+      amax = finite_max(x[i], amax);
     }
   }
   __shared__ float sm_max[NT / 32];
@@ -158,65 +196,130 @@ __device__ __forceinline__ void append_block(const Params& p) {
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
     const int slot = lo + i * TPP + tid / TPT;
-    if (slot < hi) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        union { uint16_t c2[4]; uint2 raw; } w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w.c2[e] = enc2(x[i][8 * h + 2 * e] * inv, x[i][8 * h + 2 * e + 1] * inv);
-        *reinterpret_cast<uint2*>(out + slot * HD + h * (HD / 2) + d) = w.raw;
-      }
-    }
+    if (slot < hi) put_codes<HD>(out + slot * HD, d, x[i], inv);
   }
-  if (lo > 0 && had != s) {
-    const float f = had * inv;
-    for (int i = tid; i < lo * HD / 16; i += NT) {
-      union { uint4 raw; uint16_t c2[8]; } w;
-      w.raw = *reinterpret_cast<const uint4*>(out + i * 16);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float2 v = dec2(w.c2[e]);
-        w.c2[e] = enc2(v.x * f, v.y * f);
-      }
-      *reinterpret_cast<uint4*>(out + i * 16) = w.raw;
-    }
-  }
+  if (lo > 0 && had != s) rescale<HD>(out, lo, had * inv, tid, NT);
   __syncthreads();                              // every thread has read the old scale
   if (tid == 0 && had != s) *scale = s;
 }
 
+// One token per CTA at a time; a thread takes the same 16 dims of its heads in every tensor.  The rows are
+// requested before the position, whose load the tables' loads wait for.
 template <typename T, int HD>
-__device__ __forceinline__ void rotate_queries(const Params& p, int64_t block, int64_t blocks) {
+__device__ __forceinline__ void rotate_queries(const Params& p, int block, int blocks) {
   constexpr int TPT = HD / 16;
-  const int64_t per = (int64_t)p.c.T * p.H * TPT, total = per * p.nq;
-  for (int64_t i = block * NT + threadIdx.x; i < total; i += blocks * NT) {
-    const int which = i >= per;
-    const int64_t r = i - which * per;
-    const int d = (int)(r % TPT) * 8, h = (int)(r / TPT % p.H), t = (int)(r / TPT / p.H);
-    const T* in = (const T*)p.q[which].p + (int64_t)t * p.q[which].st + (int64_t)h * p.q[which].sh;
-    T* out = (T*)p.qo[which] + ((int64_t)t * p.H + h) * HD;
-    float x[16];
-    load8(in + d, x);
-    load8(in + HD / 2 + d, x + 8);
-    rotate8<HD>(p, t, d, x, x + 8);
-    store8(out + d, x);
-    store8(out + HD / 2 + d, x + 8);
-  }
+  const int d = (threadIdx.x % TPT) * 8;
+  for (int t = block; t < p.c.T; t += blocks)
+    for (int h = threadIdx.x / TPT; h < p.H; h += NT / TPT) {
+      constexpr int N = 16 / sizeof(T), L = 16 / N;
+      Vec16<T> raw[2][L];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (i >= p.nq) break;
+        const T* in = (const T*)p.q[i].p + (int64_t)t * p.q[i].st + (int64_t)h * p.q[i].sh + d;
+#pragma unroll
+        for (int l = 0; l < L; ++l) raw[i][l] = ld16(in + (l < L / 2 ? 0 : HD / 2) + l % (L / 2) * N);
+      }
+      const Turn turn = turn_of<HD>(p, t, d);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (i >= p.nq) break;
+        float x[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = to_f(raw[i][e / N].v[e % N]);
+        rotate8(turn, x, x + 8);
+        T* out = (T*)p.qo[i] + ((int64_t)t * p.H + h) * HD + d;
+        store8(out, x);
+        store8(out + HD / 2, x + 8);
+      }
+    }
 }
 
 template <typename T, int HD, int NP>
-__global__ void __launch_bounds__(NT) append_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(NT, NP == 1 ? 4 : NP == 2 ? 3 : 2) append_kernel(const __grid_constant__ Params p) {
   if ((int)blockIdx.x < p.units) append_block<T, HD, NP>(p);
   else {
-    const int64_t qb = gridDim.x - p.units, layer = blockIdx.y + (int64_t)gridDim.y * blockIdx.z;
+    const int qb = gridDim.x - p.units, layer = blockIdx.y + gridDim.y * blockIdx.z;
     rotate_queries<T, HD>(p, (blockIdx.x - p.units) + qb * layer, qb * gridDim.y * gridDim.z);
   }
 }
 
+// One new token per sequence at most; a group of TPT lanes does one token of K or V.
 template <typename T, int HD>
-void launch(const Params& p, dim3 grid) {
-  const int np = std::max(1, p.c.page * HD / (NT * 16));
-  if (np == 1) append_kernel<T, HD, 1><<<grid, NT, 0, stream()>>>(p);
+__global__ void __launch_bounds__(NT, 4) append_one_kernel(const __grid_constant__ Params p) {
+  constexpr int TPT = HD / 16;
+  if ((int)blockIdx.x >= p.units) {
+    rotate_queries<T, HD>(p, blockIdx.x - p.units, gridDim.x - p.units);
+    return;
+  }
+  const Cache& c = p.c;
+  const int sub = threadIdx.x % TPT, d = sub * 8;
+  const int64_t item = ((int64_t)blockIdx.x * NT + threadIdx.x) / TPT;
+  const bool is_v = item & 1;
+  const int g = (int)(item / 2 % c.G), t = (int)(item / 2 / c.G);
+  bool ok = t < c.T;
+  int b = -1, slot = 0, pg = -1;
+  if (ok) {
+    // the usual step: every sequence has one token
+    b = t < c.B && c.cu[t] == t && c.cu[t + 1] == t + 1 ? t : sequence_of(c.cu, c.B, t);
+    ok = b >= 0;
+  }
+  if (ok) {
+    const int n = c.cu[b + 1] - c.cu[b];
+    slot = c.lens[b] - 1;
+    ok = n == 1 && slot >= 0;
+    if (!ok && sub == 0) record(ERR_LENGTH);
+  }
+  if (ok) {
+    const int j = slot >> c.shift;
+    pg = j < c.W ? c.table[(int64_t)b * c.W + j] : -1;
+    ok = pg >= 0 && pg < c.P;
+    if (!ok && sub == 0) record(ERR_PAGE);
+  }
+  const int lo = slot & (c.page - 1);
+  const int64_t blk = ok ? (int64_t)pg * c.G + g : 0;
+  uint8_t* out = (is_v ? c.v : c.k) + blk * c.page * HD;
+  float* scale = (is_v ? c.vs : c.ks) + blk;
+  float x[16], had = 0.f;
+  if (ok) {
+    const Src src = is_v ? p.v : p.k;
+    const T* in = (const T*)src.p + (int64_t)t * src.st + (int64_t)g * src.sh + d;
+    load8(in, x);
+    load8(in + HD / 2, x + 8);
+    if (lo > 0) had = *scale;
+    if (!is_v && p.cos) rotate8(turn_of<HD>(p, t, d), x, x + 8);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = 0.f;
+  }
+  float amax = finite_max(x, 0.f);
+#pragma unroll
+  for (int o = TPT / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  __syncwarp();                                 // the group's lanes have read the old scale
+  if (!ok) return;
+  const float s = fmaxf(block_scale(amax), had), inv = inverse_pow2(s);
+  put_codes<HD>(out + lo * HD, d, x, inv);
+  if (lo > 0 && had != s) rescale<HD>(out, lo, had * inv, sub, TPT);
+  if (sub == 0 && had != s) *scale = s;
+}
+
+template <typename T, int HD>
+void launch(Params& p) {
+  const int64_t qblocks = p.nq ? std::min<int64_t>(p.c.T, 1 << 16) : 0;
+  if (p.max_new <= 1) {
+    p.units = (int)(((int64_t)p.c.T * p.c.G * 2 * (HD / 16) + NT - 1) / NT);
+    append_one_kernel<T, HD><<<(unsigned)(p.units + qblocks), NT, 0, stream()>>>(p);
+    return;
+  }
+  // units: (sequence, page) pairs that can take new tokens; the smaller of the two ways to number them
+  const int64_t per_seq = ((int64_t)p.max_new + p.c.page - 2) / p.c.page + 1;
+  const int64_t even = per_seq * p.c.B, packed = p.c.T / p.c.page + 2LL * p.c.B;
+  p.per_seq = even <= packed ? (int)per_seq : 0;
+  p.units = (int)std::min(even, packed);
+  const dim3 grid((unsigned)(p.units + (qblocks + 2 * p.c.G - 1) / (2 * p.c.G)), (unsigned)p.c.G, 2u);
+  // passes over a page's new tokens, which each thread holds 16 values of
+  const int np = (int)(((int64_t)std::min(p.max_new, p.c.page) * HD + NT * 16 - 1) / (NT * 16));
+  if (np <= 1) append_kernel<T, HD, 1><<<grid, NT, 0, stream()>>>(p);
   else if (np == 2) append_kernel<T, HD, 2><<<grid, NT, 0, stream()>>>(p);
   else append_kernel<T, HD, 4><<<grid, NT, 0, stream()>>>(p);
 }
@@ -272,22 +375,10 @@ std::vector<at::Tensor> kv_append(at::Tensor k, at::Tensor v, at::Tensor ck, at:
   p.nq = (int)queries.size();
   for (int i = 0; i < p.nq; ++i) { p.q[i] = src(queries[i]); p.qo[i] = outs[i].data_ptr(); }
   p.H = p.nq ? (int)queries[0].size(1) : 0;
-  // units: (sequence, page) pairs that can take new tokens; the smaller of the two ways to number them
-  const int64_t per_seq = max_new == 0 ? 0 : (max_new + p.c.page - 2) / p.c.page + 1;
-  const int64_t even = per_seq * p.c.B, packed = T / p.c.page + 2LL * p.c.B;
-  if (max_new <= 1 ? true : even <= packed) {
-    p.per_seq = max_new <= 1 ? 1 : (int)per_seq;
-    p.units = max_new <= 1 ? p.c.B : (int)even;
-  } else {
-    p.per_seq = 0;
-    p.units = (int)packed;
-  }
-  const int64_t items = T * p.H * (hd / 16) * p.nq;
-  const int64_t qblocks = std::min<int64_t>((items + NT - 1) / NT, 8 * num_sms());
-  const int64_t qx = (qblocks + 2 * p.c.G - 1) / (2 * p.c.G);
-  dim3 grid((unsigned)(p.units + qx), (unsigned)p.c.G, 2u);
+  p.max_new = (int)std::min<int64_t>(max_new, T);
+  TORCH_CHECK(T * p.c.G * 2 < (1LL << 31), "kv_append: sizes");
   MAMF_DISPATCH_FLOAT_BF16(k.scalar_type(), "kv_append", [&] {
-    if (hd == 128) launch<scalar_t, 128>(p, grid); else launch<scalar_t, 64>(p, grid);
+    if (hd == 128) launch<scalar_t, 128>(p); else launch<scalar_t, 64>(p);
   });
   MAMF_LAUNCH_CHECK();
   return outs;

@@ -12,6 +12,7 @@
 // its log probabilities are -inf, its entropy and gradient 0.  NaN and +inf make the row NaN.
 // Rows whose target is `ignore_index` (or outside the vocabulary) are not read: results 0, ids -1.
 #include "common.cuh"
+#include "f32x2.cuh"
 
 #include <type_traits>
 
@@ -86,29 +87,6 @@ struct FwdParams {
   int V, k;
   float inv_t;
 };
-
-// ---- two fp32 values per instruction ----
-__device__ __forceinline__ uint64_t pk(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void unpk(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 
 // maximum of a 16-byte vector, NaN if one is in it
 __device__ __forceinline__ float vec_max(const Vec16<float>& v) { return max_nan(max_nan(v.v[0], v.v[1]), max_nan(v.v[2], v.v[3])); }
