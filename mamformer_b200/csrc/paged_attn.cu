@@ -39,7 +39,8 @@ __device__ __forceinline__ void record(int code) { atomicCAS(&g_err, 0, code); }
 struct Params : Attn {
   int ctas;
   float* part;        // [ctas][2][rows][HD + 2]: O (not divided), m, l
-  int4* joins;        // [ctas]: the item that ends in this CTA after it began in another one
+  int4* joins;        // [ctas]: {t0, rows, g | rt << 16, 2 c0 + place} of the item that ends in this CTA after it
+                      // began in CTA c0 (its part there is in `place`), or {-1, ..}
 };
 
 using tc5::ex2;
@@ -157,8 +158,8 @@ __device__ __forceinline__ int64_t tiles_of(const Params& p, int b) {
 template <int HD> constexpr int stage_bytes() { return 2 * STEP * HD; }
 constexpr int ST = 3;                          // tiles of a warp's ring
 // resident CTAs per SM: the latency of a warp's chain (products, exponentials, products) is hidden by other
-// warps, so registers are held to 128 for 8 rows
-template <int NR> constexpr int residents() { return NR == 1 ? 4 : 2; }
+// warps, so there are as many as the registers of a row tile allow without spills (128, 168 or 255)
+template <int HD, int NR> constexpr int residents() { return NR == 1 ? 4 : HD == 64 ? 3 : 2; }
 template <int HD, int NR> constexpr int merge_words() { return NR * (HD / 4 + 4); }      // of a lane
 template <int HD, int NR> constexpr int smem_bytes() {
   return 1024 + NW * ST * stage_bytes<HD>() + 32 * 4 * merge_words<HD, NR>();
@@ -186,7 +187,7 @@ template <typename T> __device__ __forceinline__ void q_row16(const T* q, float*
 }
 
 template <typename T, int HD, int NR>
-__global__ void __launch_bounds__(NT, residents<NR>()) split_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap map_k,
+__global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap map_k,
                                                       const __grid_constant__ CUtensorMap map_v) {
   constexpr int ROWS = 8 * NR;
   constexpr int KC = HD / 64;                    // 16-byte reads of a K row per lane
@@ -601,7 +602,7 @@ __global__ void __launch_bounds__(NT, residents<NR>()) split_kernel(const __grid
       }
       if (ends && !whole && lane == 0) {
         const int64_t c0 = item_start / share;       // CTA and place of the item's first part
-        p.joins[blockIdx.x] = make_int4(it.b, it.g, it.rt, (int)(2 * c0 + (item_start > c0 * share ? 1 : 0)));
+        p.joins[blockIdx.x] = make_int4(it.t0, it.rows, it.g | it.rt << 16, (int)(2 * c0 + (item_start > c0 * share ? 1 : 0)));
       }
     }
     __syncthreads();
@@ -652,51 +653,51 @@ __global__ void __launch_bounds__(NJ) join_kernel(const __grid_constant__ Params
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 j = p.joins[blockIdx.x];
   if (j.x < 0) return;
-  Item it;
-  set_sequence<ROWS>(p, it, j.x);
-  it.g = j.y;
-  it.rt = j.z;
+  const int t0 = j.x, row0 = (j.z >> 16) * ROWS, n_rows = min(ROWS, j.y - row0), g = j.z & 0xffff;
   const int c0 = j.w >> 1, parts = blockIdx.x - c0 + 1, per = p.rep * p.maps;
-  auto part = [&](int i, int r) {
-    return p.part + (((int64_t)(c0 + i) * 2 + (i == 0 ? j.w & 1 : 0)) * ROWS + r) * (HD + 2);
-  };
-  // a group of warps takes a row: the parts' common maximum, then each warp's share of the parts' sums and
-  // values; the two maps of a head are neighbouring rows
-  constexpr int GR = NJ / 32 / ROWS, D = HD / 32;
-  __shared__ float vals[GR][ROWS][HD], sums[GR][ROWS];
-  const int lane = threadIdx.x & 31, r = (threadIdx.x >> 5) % ROWS, gr = (threadIdx.x >> 5) / ROWS;
-  if (it.rt * ROWS + r < it.rows) {
-    float M = NONE;
-    for (int i = lane; i < parts; i += 32) M = fmaxf(M, part(i, r)[HD]);
-    M = warp_max(M);
-    float L = 0.f, a[D] = {};
+  // the warps share the rows, and a row's warps its parts, each under a running maximum; the two maps of a head
+  // are neighbouring rows
+  constexpr int W = NJ / 32, D = HD / 32;
+  __shared__ float vals[W][HD];
+  __shared__ float2 sums[W];                           // {maximum, sum}
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, r = w % n_rows, gr = w / n_rows, groups = W / n_rows;
+  if (gr < groups) {
+    float M = NONE, L = 0.f, a[D] = {};
 #pragma unroll 8
-    for (int i = gr; i < parts; i += GR) {
-      const float* x = part(i, r);
-      const float f = ex2(x[HD] - M);
-      L = fmaf(f, x[HD + 1], L);
+    for (int i = gr; i < parts; i += groups) {
+      const float* x = p.part + (((int64_t)(c0 + i) * 2 + (i == 0 ? j.w & 1 : 0)) * ROWS + r) * (HD + 2);
+      const float2 ml = *reinterpret_cast<const float2*>(x + HD);
+      float2 v[D / 2];
 #pragma unroll
-      for (int d = 0; d < D; d += 2) {
-        const float2 v = *reinterpret_cast<const float2*>(x + lane * D + d);
-        a[d] = fmaf(f, v.x, a[d]);
-        a[d + 1] = fmaf(f, v.y, a[d + 1]);
+      for (int d = 0; d < D / 2; ++d) v[d] = *reinterpret_cast<const float2*>(x + lane * D + 2 * d);
+      const float mn = fmaxf(M, ml.x), f = ex2(M - mn), e = ex2(ml.x - mn);
+      M = mn;
+      L = fmaf(L, f, ml.y * e);
+#pragma unroll
+      for (int d = 0; d < D / 2; ++d) {
+        a[2 * d] = fmaf(a[2 * d], f, v[d].x * e);
+        a[2 * d + 1] = fmaf(a[2 * d + 1], f, v[d].y * e);
       }
     }
 #pragma unroll
-    for (int d = 0; d < D; ++d) vals[gr][r][lane * D + d] = a[d];
-    if (lane == 0) sums[gr][r] = L;
+    for (int d = 0; d < D; ++d) vals[w][lane * D + d] = a[d];
+    if (lane == 0) sums[w] = make_float2(M, L);
   }
   __syncthreads();
   auto value = [&](int row, int d) {
-    float x = 0.f, L = 0.f;
-#pragma unroll
-    for (int i = 0; i < GR; ++i) { x += vals[i][row][d]; L += sums[i][row]; }
+    float M = NONE, L = 0.f, x = 0.f;
+    for (int i = row; i < groups * n_rows; i += n_rows) M = fmaxf(M, sums[i].x);
+    for (int i = row; i < groups * n_rows; i += n_rows) {
+      const float e = ex2(sums[i].x - M);
+      x = fmaf(vals[i][d], e, x);
+      L = fmaf(sums[i].y, e, L);
+    }
     return L == 0.f ? 0.f : x / L;
   };
   for (int i = threadIdx.x; i < ROWS / p.maps * HD; i += NJ) {
-    const int rr = i / HD * p.maps, d = i % HD, row = it.rt * ROWS + rr;
-    if (row >= it.rows) continue;
-    const int tok = it.t0 + row / per, h = it.g * p.rep + row % per / p.maps;
+    const int rr = i / HD * p.maps, d = i % HD;
+    if (rr >= n_rows) continue;
+    const int row = row0 + rr, tok = t0 + row / per, h = g * p.rep + row % per / p.maps;
     float x = value(rr, d);
     if (p.maps == 2) x = (x - p.lam[h] * value(rr + 1, d)) / (1.f - p.lam[h] + 1e-8f);
     ((T*)p.out)[((int64_t)tok * p.H + h) * HD + d] = from_f<T>(x);
@@ -791,7 +792,7 @@ at::Tensor paged_attention(at::Tensor q1, c10::optional<at::Tensor> q2, c10::opt
   const int nr = p.few > 8 ? 2 : 1, rows = 8 * nr;
   const int64_t row_tiles = (p.few + rows - 1) / rows;
   const int64_t most = std::max<int64_t>(1, (int64_t)p.c.B * p.c.G * row_tiles * std::max<int64_t>(1, ((int64_t)p.c.W * p.c.page + TILE - 1) / TILE));
-  p.ctas = (int)std::min<int64_t>(most, (nr == 1 ? residents<1>() : residents<2>()) * num_sms());
+  p.ctas = (int)std::min<int64_t>(most, (nr == 1 ? residents<128, 1>() : hd == 64 ? residents<64, 2>() : residents<128, 2>()) * num_sms());
   const int64_t part = (int64_t)p.ctas * 2 * rows * (hd + 2);
   at::Tensor ws = at::empty({part + 4 * p.ctas}, q1.options().dtype(at::kFloat));
   p.joins = reinterpret_cast<int4*>(ws.data_ptr<float>());
