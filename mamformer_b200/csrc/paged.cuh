@@ -59,6 +59,7 @@ struct Attn {
   int64_t st1, sh1, st2, sh2;          // token and head strides of q1, q2 in elements
   int H, rep, maps, window;            // rep = H / G query heads per KV head
   int few;                             // sequences of up to this many rows (n * rep * maps) are the split kernel's
+  bool chunked;                        // the chunk kernel takes the others
   float scale_log2;
 };
 

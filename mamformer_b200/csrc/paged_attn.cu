@@ -126,7 +126,7 @@ __device__ __forceinline__ bool set_sequence(const Params& p, Item& it, int b) {
   if (it.n <= 0 || it.t0 < 0 || it.t0 + it.n > p.c.T) return false;
   it.rows = it.n * p.rep * p.maps;
   if (it.rows > p.few) {
-    if (p.few != FEW) record(ERR_LENGTH);                       // more new tokens than max_new
+    if (!p.chunked) record(ERR_LENGTH);                         // more new tokens than max_new
     return false;
   }
   it.g = it.rt = 0;
@@ -784,9 +784,10 @@ at::Tensor paged_attention(at::Tensor q1, c10::optional<at::Tensor> q2, c10::opt
   // Sequences of up to FEW rows go to the split kernel, longer runs of tokens to the chunk kernel; where all
   // have the same number of tokens one of them does everything.
   const int64_t most_rows = std::max<int64_t>(1, std::min(max_new, T)) * p.rep * p.maps;
-  const bool chunks = most_rows > FEW, alone = chunks && T == p.c.B * max_new;
-  p.few = chunks ? (alone ? 0 : FEW) : (int)most_rows;
-  if (chunks) paged_chunk_attention(p, (int)hd, q1.scalar_type() == at::kBFloat16);
+  p.chunked = most_rows > FEW && p.c.B > 0;
+  const bool alone = p.chunked && T == p.c.B * max_new;
+  p.few = alone ? 0 : (int)std::min<int64_t>(most_rows, FEW);
+  if (p.chunked) paged_chunk_attention(p, (int)hd, q1.scalar_type() == at::kBFloat16);
   if (alone) return out;
   // one query row tile holds 8 rows, or 16 where a sequence can have more than 8
   const int nr = p.few > 8 ? 2 : 1, rows = 8 * nr;
@@ -797,7 +798,7 @@ at::Tensor paged_attention(at::Tensor q1, c10::optional<at::Tensor> q2, c10::opt
   at::Tensor ws = at::empty({part + 4 * p.ctas}, q1.options().dtype(at::kFloat));
   p.joins = reinterpret_cast<int4*>(ws.data_ptr<float>());
   p.part = ws.data_ptr<float>() + 4 * p.ctas;
-  TORCH_CHECK((int64_t)p.c.P * p.c.G * p.c.page * hd / 128 < (1LL << 31), "paged_attention: a pool of over 256 GB");
+  TORCH_CHECK((int64_t)p.c.P * p.c.G * p.c.page < (1LL << 31), "paged_attention: a pool of 2^31 tokens and heads or more");
   const int64_t tokens = (int64_t)p.c.P * p.c.G * p.c.page;
   const CUtensorMap mk = lines_map(p.c.k, tokens, (int)hd), mv = lines_map(p.c.v, tokens, (int)hd);
   auto go = [&](auto t) {

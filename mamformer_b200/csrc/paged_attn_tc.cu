@@ -11,7 +11,8 @@
 //   warp 10         TMEM allocation, MMA issue: S = Q K^T (M 128, N 64), O += P V (N = head size, P in TMEM)
 // The blocks' scales are powers of two and stay out of the products: a key's goes into the factor of its
 // score, a value's (relative to a reference that O is kept in) into the exponent of its weight, so a 16-token
-// group costs four multiplications per row.  Online softmax with lazy rescaling as in flash_tc.cu.  Every
+// group costs four multiplications per row.  Where there are fewer tiles than SMs, several CTAs share a tile's
+// keys and a second kernel joins them.  Online softmax with lazy rescaling as in flash_tc.cu.  Every
 // wait is bounded; a wait that runs out records a code, and the CTA winds down.
 #include "f32x2.cuh"
 #include "paged.cuh"
@@ -34,7 +35,10 @@ template <int HD> constexpr int k_bytes() { return BN * HD * 2; }
 // the epilogue's exchange rows (fp32) lie over Q and the ring
 template <int HD> constexpr int smem_bytes() { return 1024 + 2 * q_bytes<HD>() + 2 * ST * k_bytes<HD>(); }
 
-using Params = Attn;
+struct Params : Attn {
+  int splits;          // CTAs that share a tile's keys; with more than one they leave parts for the join kernel:
+  float* part;         // [unit * G + head][split][stream][BM][HD + 2]: O (not divided), m, l
+};
 
 __device__ __forceinline__ bool wait(uint64_t* b, uint32_t parity) { return bar_wait(b, parity, ERR_WAIT, &g_wait_err, WAIT_CYCLES); }
 // kind::f16, f16 x f16 -> fp32, A K-major
@@ -74,8 +78,9 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
 
   if (p.few == 0) {                                // rows past the last sequence
     const int64_t end = (int64_t)max(0, c.cu[c.B]) * p.H * HD, all = (int64_t)c.T * p.H * HD;
-    for (int64_t i = end + (int64_t)blockIdx.x * NT + threadIdx.x; i < all; i += (int64_t)gridDim.x * NT)
-      ((T*)p.out)[i] = from_f<T>(0.f);
+    if (blockIdx.y == 0)
+      for (int64_t i = end + (int64_t)blockIdx.x * NT + threadIdx.x; i < all; i += (int64_t)gridDim.x * NT)
+        ((T*)p.out)[i] = from_f<T>(0.f);
   }
   // ---- the CTA's rows ----
   const int rows = p.maps == 2 ? BM : 2 * BM;      // (token, head) pairs per CTA
@@ -98,8 +103,13 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
   const int i0 = r0 / p.rep, i1 = min(n - 1, (r0 + rows - 1) / p.rep);
   const int key_hi = max(0, min(len, at0 + i1 + 1));
   const int key_lo = p.window > 0 ? max(0, at0 + i0 - p.window + 1) : 0;
-  const int kt0 = key_lo / BN;
-  const int ntile = key_hi > key_lo ? (key_hi + BN - 1) / BN - kt0 : 0;
+  int kt0 = key_lo / BN;
+  int ntile = key_hi > key_lo ? (key_hi + BN - 1) / BN - kt0 : 0;
+  if (p.splits > 1) {                              // this CTA's share of the key tiles
+    const int share = (ntile + p.splits - 1) / p.splits, first = min(ntile, (int)blockIdx.y * share);
+    kt0 += first;
+    ntile = min(share, ntile - first);
+  }
 
   if (threadIdx.x == 0) {
     bar_init(&q_full, 256);
@@ -372,11 +382,26 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
       ok = __all_sync(0xffffffffu, wait(&o_done[s * 2 + ((ntile - 1) & 1)], (uint32_t)(((ntile - 1) >> 1) & 1)));
       fence_after();
     }
-    const float inv = l == 0.f ? 0.f : groups[(ntile - 1) % ST].vref / l;        // l is 0 where there is no tile
+    const float vref = ntile > 0 ? groups[(ntile - 1) % ST].vref : 0.f;
+    if (p.splits > 1) {
+      float* dst = p.part + ((((int64_t)blockIdx.x * p.splits + blockIdx.y) * 2 + s) * BM + r) * (HD + 2);
+      // a part that a wait's end has cut short is written as no part at all
+      *reinterpret_cast<float2*>(dst + HD) = ok ? make_float2(m, l) : make_float2(NONE, 0.f);
+#pragma unroll 1
+      for (int cc = 0; cc < HD; cc += 32) {
+        float o[32];
+        if (ntile > 0 && ok) tld32(tl + (uint32_t)(O_COL + s * HD + cc), o);
+#pragma unroll
+        for (int k = 0; k < 32; k += 2)
+          *reinterpret_cast<float2*>(dst + cc + k) = ntile > 0 && ok ? make_float2(o[k] * vref, o[k + 1] * vref) : make_float2(0.f, 0.f);
+      }
+      ok = false;                                  // nothing more to write
+    }
+    const float inv = l == 0.f ? 0.f : vref / l;
     float lam = 0.f, den = 1.f;
     if (p.maps == 2 && row_ok) { lam = p.lam[h]; den = 1.f / (1.f - lam + 1e-8f); }
     float* xrow = reinterpret_cast<float*>(sm) + r * (HD + 4);        // stream B's row; Q and the ring are free now
-    if (p.maps == 2 && s == 0) ok = __all_sync(0xffffffffu, ok && wait(&ex_full, 0));
+    if (p.maps == 2 && s == 0 && p.splits == 1) ok = __all_sync(0xffffffffu, ok && wait(&ex_full, 0));
     T* out = (T*)p.out + ((int64_t)(t0 + i) * p.H + h) * HD;
 #pragma unroll 1
     for (int cc = 0; cc < HD && ok; cc += 32) {
@@ -407,15 +432,78 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
   }
 }
 
+// Joins the parts of a row, a warp each: its maps, their splits in order.
 template <typename T, int HD>
-void launch(const Params& p) {
+__global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__ Params p, int units) {
+  constexpr int D = HD / 32;
+  const Cache& c = p.c;
+  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (item >= (int64_t)c.T * p.H) return;
+  const int t = (int)(item / p.H), h = (int)(item % p.H), g = h / p.rep;
+  const int b = sequence_of(c.cu, c.B, t);
+  if (b < 0) return;
+  const int t0 = c.cu[b], n = c.cu[b + 1] - t0;
+  if (t0 < 0 || t0 + n > c.T || (int64_t)n * p.rep * p.maps <= p.few) return;
+  const int rows = p.maps == 2 ? BM : 2 * BM, row = (t - t0) * p.rep + h % p.rep;
+  const int u = (int)((int64_t)t0 * p.rep / rows + b) + row / rows;
+  const int64_t unit = (int64_t)(units - 1 - u) * c.G + g;
+  float res[D] = {};
+  for (int map = 0; map < p.maps; ++map) {
+    const int s = p.maps == 2 ? map : row % rows / BM;
+    const float* x = p.part + ((unit * p.splits * 2 + s) * BM + row % BM) * (HD + 2);
+    const int64_t step = (int64_t)2 * BM * (HD + 2);
+    float M = NONE, L = 0.f, a[D] = {};
+#pragma unroll 4
+    for (int i = 0; i < p.splits; ++i, x += step) {
+      const float2 ml = *reinterpret_cast<const float2*>(x + HD);
+      float2 v[D / 2];
+#pragma unroll
+      for (int d = 0; d < D / 2; ++d) v[d] = *reinterpret_cast<const float2*>(x + lane * D + 2 * d);
+      const float mn = fmaxf(M, ml.x), f = ex2(M - mn), e = ex2(ml.x - mn);
+      M = mn;
+      L = fmaf(L, f, ml.y * e);
+#pragma unroll
+      for (int d = 0; d < D / 2; ++d) {
+        a[2 * d] = fmaf(a[2 * d], f, v[d].x * e);
+        a[2 * d + 1] = fmaf(a[2 * d + 1], f, v[d].y * e);
+      }
+    }
+    float w = L == 0.f ? 0.f : 1.f / L;
+    if (p.maps == 2) w *= (map ? -p.lam[h] : 1.f) / (1.f - p.lam[h] + 1e-8f);
+#pragma unroll
+    for (int d = 0; d < D; ++d) res[d] = fmaf(a[d], w, res[d]);
+  }
+  T* out = (T*)p.out + item * HD + lane * D;
+#pragma unroll
+  for (int d = 0; d < D; ++d) out[d] = from_f<T>(res[d]);
+}
+
+template <typename T, int HD>
+void launch(const Attn& attn) {
   auto fn = chunk_kernel<T, HD>;
+  Params p;
+  static_cast<Attn&>(p) = attn;
   MAMF_CUDA_CHECK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<HD>()));
   const int64_t rows = p.maps == 2 ? BM : 2 * BM;
   const int64_t units = ((int64_t)p.c.T * p.rep / rows + p.c.B) * p.c.G;
   TORCH_CHECK(units < (1LL << 31), "paged_attention: sizes");
-  fn<<<(unsigned)units, NT, smem_bytes<HD>(), stream()>>>(p);
+  // One CTA runs per SM.  Where the tiles leave SMs idle, several CTAs share the keys of a tile, each at least 8
+  // key tiles of the longest sequence that the block table has room for.
+  const int64_t longest = ((int64_t)p.c.W * p.c.page + BN - 1) / BN;
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({num_sms() / units, longest / 8, 32}));
+  at::Tensor ws;
+  p.part = nullptr;
+  if (p.splits > 1) {
+    ws = at::empty({units * p.splits * 2 * BM * (HD + 2)}, at::TensorOptions().dtype(at::kFloat).device(at::kCUDA));
+    p.part = ws.data_ptr<float>();
+  }
+  fn<<<dim3((unsigned)units, (unsigned)p.splits), NT, smem_bytes<HD>(), stream()>>>(p);
   MAMF_LAUNCH_CHECK();
+  if (p.splits > 1) {
+    chunk_join_kernel<T, HD><<<(unsigned)(((int64_t)p.c.T * p.H + 7) / 8), 256, 0, stream()>>>(p, (int)(units / p.c.G));
+    MAMF_LAUNCH_CHECK();
+  }
 }
 
 }  // namespace ptc

@@ -318,6 +318,10 @@ def test_no_sequences_and_padding_rows(dev):
     got = ops.paged_attention(q, cache, table, offsets([2, 1], dev), i32([30, 5], dev), 2)
     want, tol = plain_attention(q[:3], cache, table, [2, 1], [30, 5])
     assert (got[3:] == 0).all() and ((got[:3].double() - want).abs() <= tol + ROUND[torch.bfloat16] * want.abs()).all()
+    many = rand((90, 4, 64), torch.bfloat16, dev, 2)
+    for tb, c, n, ln in ((table[:0], [0], 0, []), (table[:0], [0], 90, []), (table[:1], [0, 80], 80, [30]), (table[:1], [0, 2], 2, [30])):
+        got = ops.paged_attention(many, cache, tb, i32(c, dev), i32(ln, dev), n)
+        assert (got[c[-1]:] == 0).all() and got.isfinite().all()
     none = ops.paged_attention(q[:0], cache, table[:0], i32([0], dev), i32([], dev), 0)
     assert none.shape == (0, 4, 64)
     assert ops.kv_append(q[:0, :2], q[:0, :2], cache, table[:0], i32([0], dev), i32([], dev), 0) == []
@@ -416,3 +420,13 @@ def test_refusals():
                      ((k, k), {"cos": cos, "sin": sin, "positions": pos, "queries": [q.float()]})]:
         with pytest.raises((RuntimeError, ValueError)):
             ops.kv_append(*args, *ok, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [(4, 2), (8, 1)])
+@pytest.mark.parametrize("diff", [False, True])
+@pytest.mark.parametrize("new,lens,window", [([70], [5000], 0), ([33, 40], [4000, 61], 0), ([300], [3000], 700),
+                                             ([20, 0, 90], [2100, 7, 90], 0), ([64], [64], 0)])
+def test_few_tiles_share_their_keys(heads, diff, new, lens, window):
+    check_attention("cuda", torch.bfloat16, 128, 64, *heads, new, lens, diff, window)
+    check_attention("cuda", torch.float16, 64, 16, *heads, new, lens, diff, window)
