@@ -250,6 +250,52 @@ def case_groupnorm(B=4, S=4096, H=32, hd=128, backward=False):
     return (lambda: _C.head_groupnorm_bwd(x, H, w, mr, dy)), 0.0, 3 * x.numel() * 2
 
 
+def _paged(B, new, lens, H, G, hd, page, diff):
+    """A filled cache of B equal sequences with `new` queries each: (cache, table, cu, lens, q, q2, lam)."""
+    from mamformer_b200 import ops
+    W = -(-lens // page)
+    P = B * W
+    code = lambda: torch.randint(0, 0x50, (P, G, page, hd), device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn)  # noqa: E731
+    cache = ops.PagedKV(code(), code(), torch.full((P, G), 2.0 ** -5, device="cuda"), torch.full((P, G), 2.0 ** -5, device="cuda"))
+    table = torch.randperm(P, device="cuda").to(torch.int32).view(B, W)
+    cu = torch.arange(B + 1, device="cuda", dtype=torch.int32) * new
+    ln = torch.full((B,), lens, device="cuda", dtype=torch.int32)
+    q, q2 = (torch.randn(B * new, H, hd, device="cuda").bfloat16() for _ in range(2))
+    return cache, table, cu, ln, q, (q2 if diff else None), (torch.full((H,), 0.5, device="cuda") if diff else None)
+
+
+def case_paged_attention(B=64, new=1, lens=4096, H=32, G=8, hd=128, page=64):
+    """Differential attention over the paged 8-bit cache: a decode step, or (new > 1) a chunk of a prompt."""
+    from mamformer_b200 import ops
+    cache, table, cu, ln, q, q2, lam = _paged(B, new, lens, H, G, hd, page, True)
+    pairs = B * sum(lens - new + i + 1 for i in range(new))
+    return ((lambda: ops.paged_attention(q, cache, table, cu, ln, new, q2=q2, lam=lam)), 8.0 * pairs * H * hd,
+            B * lens * G * hd * 2 + 3 * q.numel() * 2)
+
+
+def case_kv_append(B=16, new=1024, H=32, G=8, hd=128, page=64):
+    """Appending prompts of 1024 tokens with the rotation of K and two query tensors."""
+    from mamformer_b200 import ops
+    cache, table, cu, ln, q, q2, _ = _paged(B, new, new, H, G, hd, page, True)
+    k, v = (torch.randn(B * new, G, hd, device="cuda").bfloat16() for _ in range(2))
+    ang = torch.arange(new, device="cuda")[:, None] * torch.rand(hd // 2, device="cuda")[None]
+    cos, sin, pos = ang.cos(), ang.sin(), torch.arange(new, device="cuda").repeat(B)
+    return ((lambda: ops.kv_append(k, v, cache, table, cu, ln, new, cos, sin, pos, [q, q2])), 0.0,
+            2 * k.numel() * 3 + 4 * q.numel() * 2)
+
+
+def case_token_scores(R=4096, V=128000, k=0, backward=False):
+    """Log probability and entropy of given tokens; backward: their gradient."""
+    from mamformer_b200.ops.native import _C
+    x = torch.randn(R, V, device="cuda").bfloat16()
+    t = torch.randint(0, V, (R,), device="cuda")
+    if not backward:
+        return (lambda: _C.token_scores_fwd(x, t, -100, 1.0, k)), 0.0, x.numel() * 2
+    _, ent, _, ids, stats = _C.token_scores_fwd(x, t, -100, 1.0, 0)
+    g = torch.randn(R, device="cuda")
+    return (lambda: _C.token_scores_bwd(x, t, -100, 1.0, stats, ent, ids, g, g, None)), 0.0, x.numel() * 4
+
+
 CASES = {"gemm": case_gemm, "grouped": case_grouped, "wgrad": case_wgrad, "scan": case_scan,
          "scan_bwd": lambda: case_scan(backward=True), "linear_attn": case_linear_attn,
          "linear_attn_bwd": lambda: case_linear_attn(backward=True), "ce": case_ce, "moe": case_moe,
@@ -260,7 +306,10 @@ CASES = {"gemm": case_gemm, "grouped": case_grouped, "wgrad": case_wgrad, "scan"
          "rmsnorm": case_rmsnorm, "rmsnorm_bwd": lambda: case_rmsnorm(backward=True),
          "swiglu": case_swiglu, "swiglu_bwd": lambda: case_swiglu(backward=True), "rope": case_rope,
          "conv": case_conv, "conv_bwd": lambda: case_conv(backward=True), "groupnorm": case_groupnorm,
-         "groupnorm_bwd": lambda: case_groupnorm(backward=True)}
+         "groupnorm_bwd": lambda: case_groupnorm(backward=True), "kv_append": case_kv_append,
+         "paged_decode": case_paged_attention, "paged_chunk": lambda: case_paged_attention(4, 1024, 8192),
+         "token_scores": case_token_scores, "token_scores_top": lambda: case_token_scores(k=20),
+         "token_scores_bwd": lambda: case_token_scores(backward=True)}
 
 
 def run(op: str, iters: int = 20, once: bool = False) -> dict:
