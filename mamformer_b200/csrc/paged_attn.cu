@@ -17,6 +17,9 @@
 // 2^-14 of a row's largest value.  P is rounded to f16 (11 bits; bf16 would keep 8).  The order of the head's
 // dims in the products is free as long as both sides agree: a lane takes 16 adjacent bytes of K (and of V),
 // so a fragment is one 16-byte read and no shuffles; so is the order of the 8 tokens of a fragment (`token`).
+//
+// 64 sequences of 300 to 8191 slots, 32 / 8 heads of 128, two maps (566 MB): 125 us, 4.5 TB/s, of which 8 us
+// are the start and 6 the join; with the arithmetic left out 105 us.  One token on 131000 slots: 62 us.
 #include "paged.cuh"
 #include "tc5.cuh"
 

@@ -430,3 +430,30 @@ def test_refusals():
 def test_few_tiles_share_their_keys(heads, diff, new, lens, window):
     check_attention("cuda", torch.bfloat16, 128, 64, *heads, new, lens, diff, window)
     check_attention("cuda", torch.float16, 64, 16, *heads, new, lens, diff, window)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 40])
+def test_pages_past_32_bits_of_offset(new):
+    """The same sequences in a small pool and at the end of one of over 2^32 bytes: the same codes and results."""
+    G, page, hd, H, P = 8, 64, 128, 16, 66500
+    lens, news = [200, 130], [new, new]
+    assert P * G * page * hd > 1 << 32
+    small = pool(8, G, page, hd, "cuda")
+    big = ops.PagedKV(*(torch.zeros(P, G, page, hd, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in range(2)),
+                      *(torch.ones(P, G, device="cuda") for _ in range(2)))
+    table = torch.tensor([[3, 0, 6, 1], [2, 7, 5, -1]], dtype=torch.int32, device="cuda")
+    far = torch.where(table >= 0, table + P - 8, table)
+    k, v = rand((330, G, hd), torch.bfloat16, "cuda", 1), rand((330, G, hd), torch.bfloat16, "cuda", 2)
+    q, q2 = rand((2 * new, H, hd), torch.bfloat16, "cuda", 3), rand((2 * new, H, hd), torch.bfloat16, "cuda", 4)
+    lam = torch.full((H,), 0.3, device="cuda")
+    got = []
+    for cache, t in ((small, table), (big, far)):
+        ops.kv_append(k, v, cache, t, offsets(lens, "cuda"), i32(lens, "cuda"), 200)
+        got.append(ops.paged_attention(q, cache, t, offsets(news, "cuda"), i32(lens, "cuda"), new, q2=q2, lam=lam))
+    assert torch.equal(got[0], got[1]) and got[0].isfinite().all()
+    want, tol = plain_attention(q, small, table, news, lens, q2, lam)
+    assert ((got[0].double() - want).abs() <= tol + ROUND[torch.bfloat16] * want.abs()).all()
+    for b in range(2):
+        for x, y in zip(held(small, table, lens, b), held(big, far, lens, b)):
+            assert torch.equal(x, y)
