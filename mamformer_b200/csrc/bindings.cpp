@@ -83,7 +83,7 @@ std::vector<at::Tensor> flash_attn_fwd(at::Tensor q, at::Tensor k, at::Tensor v,
 std::vector<at::Tensor> flash_attn_bwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor out, at::Tensor lse,
                                        at::Tensor dout, int64_t lo, int64_t hi, double scale);
 std::vector<at::Tensor> token_scores_fwd(at::Tensor logits, at::Tensor target, int64_t ignore_index, double temperature,
-                                         int64_t top_k);
+                                         int64_t top_k, bool want_stats);
 at::Tensor token_scores_bwd(at::Tensor logits, at::Tensor target, int64_t ignore_index, double temperature,
                             at::Tensor stats, at::Tensor ent, at::Tensor top_id, c10::optional<at::Tensor> g_lp,
                             c10::optional<at::Tensor> g_ent, c10::optional<at::Tensor> g_top);
@@ -159,7 +159,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("flash_tc_bwd_error", &mamf::flash_tc_bwd_error);
   m.def("flash_attn_fwd", &mamf::flash_attn_fwd);
   m.def("flash_attn_bwd", &mamf::flash_attn_bwd);
-  m.def("token_scores_fwd", &mamf::token_scores_fwd);
+  m.def("token_scores_fwd", &mamf::token_scores_fwd, py::arg("logits"), py::arg("target"), py::arg("ignore_index"),
+        py::arg("temperature"), py::arg("top_k"), py::arg("want_stats") = true);
   m.def("token_scores_bwd", &mamf::token_scores_bwd);
   m.def("kv_append", &mamf::kv_append);
   m.def("kv_append_error", &mamf::kv_append_error);

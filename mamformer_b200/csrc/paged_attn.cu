@@ -33,7 +33,10 @@ constexpr int STEP = 16;                       // tokens of a warp per tile
 constexpr int TILE = STEP * NW;                // tokens per tile
 constexpr long long WAIT_CYCLES = 4000000000LL;      // about 2 s
 constexpr float NONE = -1e30f;                 // maximum of no scores: 2^(score - NONE) is never formed, 2^(NONE - m) is 0
-constexpr int FEW = 64;                        // rows of a sequence and KV head above which the chunk kernel takes over
+// Rows of a sequence and KV head above which the chunk kernel takes over.  This kernel and the chunk kernel, 16
+// sequences of 2000-6000 slots, 32 / 8 heads, two maps: 24 rows 89 and 157 us, 32 rows 90 and 158, 64 rows 160 and
+// 158; one map, 8 sequences of 8000, 16 / 4 heads: 32 rows 55 and 78, 64 rows 83 and 94.
+constexpr int FEW = 64;
 constexpr float LAZY = 8.f;                    // log2 by which a row may outgrow its reference maximum
 
 __device__ int g_err = 0, g_wait_err = 0;

@@ -51,9 +51,15 @@ def _native(t: torch.Tensor) -> bool:
     return True
 
 
+_NATIVE_MODULE = None
+
+
 def _nat():
-    from mamformer_b200.ops import native
-    return native
+    global _NATIVE_MODULE
+    if _NATIVE_MODULE is None:
+        from mamformer_b200.ops import native
+        _NATIVE_MODULE = native
+    return _NATIVE_MODULE
 
 
 # ---------------------------------------------------------------------------------------------
@@ -221,12 +227,13 @@ def token_scores(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, te
     logits (.., V) bf16 / f16 / fp32 (other types run the eager form), targets (..) int64.  Differentiable in all three scores.  Rows whose target is
     ``ignore_index`` give 0, ids -1 and no gradient, and are not read; a logit of -inf has probability 0; a row of
     -inf only gives log probabilities of -inf, entropy 0 and no gradient."""
-    if logits.dim() < 1 or targets.shape != logits.shape[:-1]:
-        raise ValueError(f"token_scores: targets {tuple(targets.shape)} for logits {tuple(logits.shape)}")
+    shape = logits.shape
+    if len(shape) < 1 or targets.shape != shape[:-1]:
+        raise ValueError(f"token_scores: targets {tuple(targets.shape)} for logits {tuple(shape)}")
     if not temperature > 0:
         raise ValueError(f"token_scores: temperature must be positive, got {temperature}")
-    if not 0 <= top_k <= min(32, logits.shape[-1]):
-        raise ValueError(f"token_scores: top_k from 0 to {min(32, logits.shape[-1])}, got {top_k}")
+    if not (0 <= top_k <= 32 and top_k <= shape[-1]):
+        raise ValueError(f"token_scores: top_k from 0 to {min(32, shape[-1])}, got {top_k}")
     if _native(logits) and "token_scores" in NATIVE and logits.dtype in _SCORE_TYPES:
         return TokenScores(*_nat().token_scores(logits, targets, top_k, temperature, ignore_index))
     return TokenScores(*ref.token_scores(logits, targets, top_k, temperature, ignore_index))
@@ -250,8 +257,10 @@ class PagedKV(NamedTuple):
 
 
 def _no_gradient(what: str, *tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
 
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -282,7 +291,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, 
     kv_lens - n + i, with ``window`` > 0 only the last ``window`` of them.  With ``q2`` and ``lam`` (H,) fp32, the
     differential form (softmax(q k) v - lam softmax(q2 k) v) / (1 - lam + 1e-8).  A query that sees nothing, and
     rows past cu_seqlens[-1], give 0.  No gradient."""
-    _no_gradient("paged_attention", q, *(x for x in (q2, lam) if x is not None))
+    _no_gradient("paged_attention", q) if q2 is None or lam is None else _no_gradient("paged_attention", q, q2, lam)
     scale = q.shape[-1] ** -0.5 if scale is None else scale
     if _native(q) and "paged_attention" in NATIVE:
         return _nat().paged_attention(q, cache, block_table, cu_seqlens, kv_lens, max_new, q2, lam, window, scale)

@@ -434,15 +434,16 @@ class _TokenScores(torch.autograd.Function):
 
 @_register("token_scores", "csrc/token_scores.cu")
 def token_scores(logits, targets, top_k, temperature, ignore_index):
-    targets = targets.long().contiguous()
+    if targets.dtype != torch.int64 or not targets.is_contiguous():
+        targets = targets.long().contiguous()
     if logits.requires_grad and torch.is_grad_enabled():
         return _TokenScores.apply(logits, targets, top_k, temperature, ignore_index)
-    return _C.token_scores_fwd(logits, targets, ignore_index, temperature, top_k)[:4]
+    return _C.token_scores_fwd(logits, targets, ignore_index, temperature, top_k, False)
 
 
 @_register("kv_append", "csrc/paged_kv.cu")
 def kv_append(k, v, cache, block_table, cu_seqlens, kv_lens, max_new, cos, sin, positions, queries):
-    return _C.kv_append(k, v, *cache, block_table, cu_seqlens, kv_lens, max_new, cos, sin, positions, list(queries))
+    return _C.kv_append(k, v, *cache, block_table, cu_seqlens, kv_lens, max_new, cos, sin, positions, queries)
 
 
 @_register("paged_attention", "csrc/paged_attn.cu")
