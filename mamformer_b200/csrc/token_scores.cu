@@ -563,4 +563,54 @@ at::Tensor token_scores_bwd(at::Tensor logits, at::Tensor target, int64_t ignore
   return out;
 }
 
+// The operator with its gradient, as a node of torch's graph without Python in it (a small vocabulary's pass is
+// mostly that otherwise).
+namespace ts {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// The gradient as a node of its own, so that a graph may be kept; differentiating it again is refused.
+struct ScoresGrad : torch::autograd::Function<ScoresGrad> {
+  static at::Tensor forward(AutogradContext*, at::Tensor logits, at::Tensor target, at::Tensor stats, at::Tensor ent,
+                            at::Tensor top_id, c10::optional<at::Tensor> g_lp, c10::optional<at::Tensor> g_ent,
+                            c10::optional<at::Tensor> g_top, int64_t ignore_index, double temperature) {
+    return token_scores_bwd(logits, target, ignore_index, temperature, stats, ent, top_id, g_lp, g_ent, g_top);
+  }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK(false, "token_scores has no second derivative");
+  }
+};
+
+struct Scores : torch::autograd::Function<Scores> {
+  static variable_list forward(AutogradContext* ctx, at::Tensor logits, at::Tensor target, int64_t ignore_index,
+                               double temperature, int64_t top_k) {
+    auto r = token_scores_fwd(logits, target, ignore_index, temperature, top_k, true);
+    ctx->save_for_backward({logits, target, r[4], r[1], r[3]});
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->saved_data["temperature"] = temperature;
+    ctx->mark_non_differentiable({r[3]});
+    ctx->set_materialize_grads(false);
+    r.pop_back();
+    return r;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto v = ctx->get_saved_variables();
+    auto plain = [](const at::Tensor& t) {
+      return t.defined() ? c10::optional<at::Tensor>(t.to(at::kFloat).contiguous()) : c10::nullopt;
+    };
+    return {ScoresGrad::apply(v[0], v[1], v[2], v[3], v[4], plain(g[0]), plain(g[1]), plain(g[2]),
+                              ctx->saved_data["ignore_index"].toInt(), ctx->saved_data["temperature"].toDouble()),
+            at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+}  // namespace ts
+
+// -> log_probs, entropy, top_log_probs, top_ids, differentiable in logits
+std::vector<at::Tensor> token_scores(at::Tensor logits, at::Tensor target, int64_t ignore_index, double temperature,
+                                     int64_t top_k) {
+  return ts::Scores::apply(logits, target, ignore_index, temperature, top_k);
+}
+
 }  // namespace mamf

@@ -414,30 +414,12 @@ def diff_attention(q1, q2, k, v, lam, lo, hi, scale=None):
 
 
 # ---------------------------------------------------------------------------------------------
-class _TokenScores(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, targets, top_k, temperature, ignore_index):
-        lp, ent, top_lp, top_ids, stats = _C.token_scores_fwd(logits, targets, ignore_index, temperature, top_k)
-        ctx.save_for_backward(logits, targets, stats, ent, top_ids)
-        ctx.args = (ignore_index, temperature)
-        ctx.mark_non_differentiable(top_ids)
-        ctx.set_materialize_grads(False)
-        return lp, ent, top_lp, top_ids
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_lp, g_ent, g_top, _):
-        logits, targets, stats, ent, top_ids = ctx.saved_tensors
-        g = [None if x is None else x.float().contiguous() for x in (g_lp, g_ent, g_top)]
-        return _C.token_scores_bwd(logits, targets, *ctx.args, stats, ent, top_ids, *g), None, None, None, None
-
-
 @_register("token_scores", "csrc/token_scores.cu")
 def token_scores(logits, targets, top_k, temperature, ignore_index):
     if targets.dtype != torch.int64 or not targets.is_contiguous():
         targets = targets.long().contiguous()
     if logits.requires_grad and torch.is_grad_enabled():
-        return _TokenScores.apply(logits, targets, top_k, temperature, ignore_index)
+        return _C.token_scores(logits, targets, ignore_index, temperature, top_k)
     return _C.token_scores_fwd(logits, targets, ignore_index, temperature, top_k, False)
 
 

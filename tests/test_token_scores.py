@@ -265,3 +265,17 @@ def test_another_stream_and_repeatability():
 def test_token_log_probs_unchanged_for_other_types(dev):
     x, t = logits((3, 77), torch.float64, dev, 6), torch.tensor([0, 5, 76], device=dev)
     close(ops.token_log_probs(x, t), plain(x, t, 0, 1.0)[0], 1e-5)
+
+
+@pytest.mark.gpu
+def test_kept_graph_and_second_derivative():
+    """A graph may be kept and its first gradient used; the gradient itself is not differentiable."""
+    x = logits((3, 40), torch.float32, "cuda", 3).requires_grad_(True)
+    t = torch.tensor([1, 2, 3], device="cuda")
+    s = ops.token_scores(x, t)
+    a, = torch.autograd.grad(s.log_probs.sum(), x, retain_graph=True)
+    b, = torch.autograd.grad(s.log_probs.sum(), x, create_graph=True)
+    assert torch.equal(a, b) and b.requires_grad
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(b.sum(), x)
+    assert not s.top_ids.requires_grad and not ops.token_scores(x.detach(), t).log_probs.requires_grad
