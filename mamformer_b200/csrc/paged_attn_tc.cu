@@ -405,6 +405,16 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
       fence_after();
     }
     const float vref = ntile > 0 ? groups[(ntile - 1) % ST].vref : 0.f;
+    T* out = (T*)p.out + ((int64_t)(t0 + i) * p.H + h) * HD;
+    if (ntile == 0 && p.splits == 1) {
+      // No row sees a key.  The exchange below is ordered after the stores of q by the wait for O, which there is
+      // none of here, so the rows are written without it.
+      Vec16<T> zero;
+      zero.raw = make_uint4(0, 0, 0, 0);
+      if (row_ok && (p.maps == 1 || s == 0))
+        for (int k = 0; k < HD; k += 8) st16(out + k, zero);
+      ok = false;
+    }
     if (p.splits > 1) {
       float* dst = p.part + ((((int64_t)blockIdx.x * p.splits + blockIdx.y) * 2 + s) * BM + r) * (HD + 2);
       // a part that a wait's end has cut short is written as no part at all
@@ -424,13 +434,12 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
     if (p.maps == 2 && row_ok) { lam = p.lam[h]; den = 1.f / (1.f - lam + 1e-8f); }
     float* xrow = reinterpret_cast<float*>(sm) + r * (HD + 4);        // stream B's row; Q and the ring are free now
     if (p.maps == 2 && s == 0 && p.splits == 1) ok = __all_sync(0xffffffffu, ok && wait(&ex_full, 0));
-    T* out = (T*)p.out + ((int64_t)(t0 + i) * p.H + h) * HD;
 #pragma unroll 1
     for (int cc = 0; cc < HD && ok; cc += 32) {
       float o[32];
-      if (ntile > 0) tld32(tl + (uint32_t)(O_COL + s * HD + cc), o);
+      tld32(tl + (uint32_t)(O_COL + s * HD + cc), o);
 #pragma unroll
-      for (int k = 0; k < 32; ++k) o[k] = ntile > 0 ? o[k] * inv : 0.f;
+      for (int k = 0; k < 32; ++k) o[k] *= inv;
       if (p.maps == 2 && s == 1) {
 #pragma unroll
         for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(xrow + cc + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);

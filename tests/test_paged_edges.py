@@ -1,0 +1,88 @@
+"""ops.kv_append and ops.paged_attention where they can go wrong: rows and tiles that see nothing, factors of any sign,
+pages whose values differ by many orders of magnitude, pages given back below a window, what the device reports and when.
+
+Tolerances of an attention row, from the values that this row sees: each weight is rounded once to 11 bits (2^-11 of its
+share) and fp32 sums add less than 2^-14 of the shares; a weight whose share is far below the largest one's is held to
+2^-24 of that instead, for each key and up to 448 times the scale of its block, which is at most twice the block's
+largest value."""
+
+import math
+
+import pytest
+import torch
+
+from mamformer_b200 import ops
+from test_paged_cache import DEVICES, ROUND, held, i32, offsets, pool, rand, tables
+
+
+def plain(q, cache, table, new, lens, q2=None, lam=None, window=0, scale=None):
+    """The definition in 64 bits, and each row's tolerance.  Only what some row of a sequence sees is read."""
+    H, hd = q.shape[1:]
+    G, page = cache.k.shape[1:3]
+    scale = hd ** -0.5 if scale is None else scale
+    out, tol, at = torch.zeros_like(q, dtype=torch.float64), torch.zeros_like(q, dtype=torch.float64), 0
+    for b, (n, L) in enumerate(zip(new, lens)):
+        if n and L:
+            k, v = (x.repeat_interleave(H // G, 0) for x in held(cache, table, lens, b))
+            pages = table[b, :-(-L // page)].long()
+            top = (cache.v_scale[pages].double() * 448).T.repeat_interleave(page, 1)[:, :L].repeat_interleave(H // G, 0)
+            i, j = torch.arange(L - n, L, device=q.device)[:, None], torch.arange(L, device=q.device)
+            see = (j <= i) & (j > i - window) if window else j <= i
+            used = see.any(0)
+            k, v = k.masked_fill(~used[:, None], 0.0), v.masked_fill(~used[:, None], 0.0)
+            maps, tols = [], []
+            for x in (q,) if q2 is None else (q, q2):
+                s = x[at:at + n].double().transpose(0, 1) @ k.transpose(1, 2) * scale
+                p = torch.softmax(s.masked_fill(~see, -math.inf), -1).nan_to_num(0.0)
+                maps.append(p @ v)
+                tols.append((2.0 ** -11 + 2.0 ** -14) * (p @ v.abs()) + L * 2.0 ** -24 * (p * top[:, None]).amax(-1, keepdim=True))
+            o, t = maps[0], tols[0]
+            if q2 is not None:
+                w = lam.double()[:, None, None]
+                o, t = (maps[0] - w * maps[1]) / (1 - w + 1e-8), (tols[0] + w * tols[1]) / (1 - w)
+            out[at:at + n], tol[at:at + n] = o.transpose(0, 1), t.transpose(0, 1)
+        at += n
+    return out, tol
+
+
+def close(got, want, tol):
+    tol = tol + ROUND[got.dtype] * want.abs()
+    bad = ~((got.double() - want).abs() <= tol)
+    assert not bad.any(), ((got.double() - want).abs() / tol)[bad].max()
+
+
+def pair(q, diff):
+    """The second map's arguments."""
+    return {"q2": q.flip(0), "lam": torch.linspace(0.1, 0.8, q.shape[1], device=q.device)} if diff else {}
+
+
+def filled(lens, page, G, hd, dev, gain=None, seed=0):
+    """A cache of unit normals, values of slot j times gain[j // page]."""
+    table, P = tables(lens, page, dev, seed)
+    cache = pool(P, G, page, hd, dev)
+    T = sum(lens)
+    k, v = rand((T, G, hd), torch.float32, dev, seed + 1), rand((T, G, hd), torch.float32, dev, seed + 2)
+    if gain is not None:
+        slot = torch.cat([torch.arange(n) for n in lens]) // page
+        v = v * torch.tensor(gain, device=dev)[slot.to(dev) % len(gain), None, None]
+    ops.kv_append(k, v, cache, table, offsets(lens, dev), i32(lens, dev), max(lens))
+    return cache, table
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("diff", [False, True])
+@pytest.mark.parametrize("new,lens", [([300], [10]), ([280, 90], [0, 90]), ([520, 300], [1, 3])])
+def test_tiles_that_see_nothing_give_zero(dev, hd, diff, new, lens):
+    """Lengths so short that whole tiles of rows have no key at all."""
+    cache, table = filled([max(n, 1) for n in lens], 16, 1, hd, dev)
+    q = rand((sum(new), 2, hd), torch.bfloat16, dev, 1)
+    kw = pair(q, diff)
+    want, tol = plain(q, cache, table, new, lens, **kw)
+    for _ in range(1 if dev == "cpu" else 20):
+        got = ops.paged_attention(q, cache, table, offsets(new, dev), i32(lens, dev), max(new), **kw)
+        at = 0
+        for n, L in zip(new, lens):
+            assert (got[at:at + n - L] == 0).all()
+            at += n
+        close(got, want, tol)
