@@ -98,6 +98,7 @@ at::Tensor paged_attention(at::Tensor q1, c10::optional<at::Tensor> q2, c10::opt
                            at::Tensor cv, at::Tensor ks, at::Tensor vs, at::Tensor table, at::Tensor cu, at::Tensor lens,
                            int64_t max_new, int64_t window, double scale);
 int64_t paged_attention_error();
+int64_t paged_attention_wait_limit(int64_t cycles);
 void gemm_ag(std::vector<int64_t> a_ptrs, int64_t shard_rows, int64_t lda, int64_t rank, at::Tensor B, bool b_mn,
              at::Tensor D);
 void gemm_rs(at::Tensor A, at::Tensor B, bool b_mn, std::vector<int64_t> d_ptrs, int64_t shard_rows, int64_t ldd,
@@ -169,6 +170,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv_append_error", &mamf::kv_append_error);
   m.def("paged_attention", &mamf::paged_attention);
   m.def("paged_attention_error", &mamf::paged_attention_error);
+  m.def("paged_attention_wait_limit", &mamf::paged_attention_wait_limit);
   m.def("gemm_ag", &mamf::gemm_ag);
   m.def("gemm_rs", &mamf::gemm_rs);
 }

@@ -31,7 +31,6 @@ using namespace paged;
 constexpr int NW = 4, NT = NW * 32, NJ = 512;
 constexpr int STEP = 16;                       // tokens of a warp per tile
 constexpr int TILE = STEP * NW;                // tokens per tile
-constexpr long long WAIT_CYCLES = 4000000000LL;      // about 2 s
 constexpr float NONE = -1e30f;                 // maximum of no scores: 2^(score - NONE) is never formed, 2^(NONE - m) is 0
 // Rows of a sequence and KV head above which the chunk kernel takes over.  This kernel and the chunk kernel, 16
 // sequences of 2000-6000 slots, 32 / 8 heads, two maps: 24 rows 89 and 157 us, 32 rows 90 and 158, 64 rows 160 and
@@ -91,19 +90,24 @@ __device__ __forceinline__ bool try_tile(uint32_t bar, uint32_t parity) {
                : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000000u) : "memory");
   return ok != 0;
 }
-// Waits for the warp's tile, the same answer for all lanes; false after WAIT_CYCLES (recorded), or once
+// Waits for the warp's tile, the same answer for all lanes; false after `limit` cycles (recorded), or once
 // another warp of the grid has given up.
-__device__ __forceinline__ bool wait_tile(uint32_t bar, uint32_t parity) {
-  if (__all_sync(0xffffffffu, try_tile(bar, parity))) return true;
+__device__ __forceinline__ bool wait_tile(uint32_t bar, uint32_t parity, long long limit) {
+  if (limit >= 0 && __all_sync(0xffffffffu, try_tile(bar, parity))) return true;
   const long long t0 = clock64();
   for (uint32_t n = 1;; ++n) {
-    if (__all_sync(0xffffffffu, try_tile(bar, parity))) return true;
+    if (limit >= 0 && __all_sync(0xffffffffu, try_tile(bar, parity))) return true;
     if ((n & 63u) == 0) {
-      const bool over = clock64() - t0 > WAIT_CYCLES;
+      const bool over = clock64() - t0 > limit;
       if (over) atomicCAS(&g_wait_err, 0, (int)ERR_WAIT);
       if (__any_sync(0xffffffffu, over || *((volatile int*)&g_wait_err) != 0)) return false;
     }
   }
+}
+// Waits for a copy whose result nobody needs, whatever has been recorded: a CTA's memory may be another's once it ends.
+__device__ __forceinline__ void drain_tile(uint32_t bar, uint32_t parity) {
+  const long long t0 = clock64();
+  while (!try_tile(bar, parity) && clock64() - t0 <= WAIT_CYCLES) {}
 }
 
 // One row tile of one KV head of one sequence.
@@ -621,7 +625,7 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
   for (int left = (int)(last - first); left > 0; --left) {
     if (ok) {
       issue(there, bar_there);
-      ok = wait_tile(bar_here, phase);
+      ok = wait_tile(bar_here, phase, p.wait);
       waited += ok;
     }
     if (ok && ksr[0] != 0.f) {
@@ -648,8 +652,8 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
       }
     }
   }
-  // after a wait that ran out: no copy may still be under way into this CTA's memory
-  for (; waited < issued; ++waited) tc5::bar_wait(&bars[w][waited % ST], (uint32_t)(waited / ST & 1), ERR_WAIT, &g_wait_err, WAIT_CYCLES);
+  // after a wait that ran out: the copies that are still under way into this CTA's memory
+  for (; waited < issued; ++waited) drain_tile(bar + waited % ST * 8, (uint32_t)(waited / ST & 1));
 }
 
 // Joins the parts of an item that ran over several CTAs: block = the CTA in which it ended.
@@ -751,6 +755,16 @@ void launch_split(const Params& p, const CUtensorMap& mk, const CUtensorMap& mv)
 
 }  // namespace pa
 
+static long long g_wait_limit = paged::WAIT_CYCLES;
+
+// Sets the cycles after which the waits of later calls give up (negative: at once), for tests of what follows;
+// returns the number before.
+int64_t paged_attention_wait_limit(int64_t cycles) {
+  const int64_t had = g_wait_limit;
+  g_wait_limit = cycles;
+  return had;
+}
+
 // q1, q2 (T, H, hd) bf16 or f16 packed queries -> (T, H, hd)
 at::Tensor paged_attention(at::Tensor q1, c10::optional<at::Tensor> q2, c10::optional<at::Tensor> lam, at::Tensor ck,
                            at::Tensor cv, at::Tensor ks, at::Tensor vs, at::Tensor table, at::Tensor cu, at::Tensor lens,
@@ -784,6 +798,7 @@ at::Tensor paged_attention(at::Tensor q1, c10::optional<at::Tensor> q2, c10::opt
   p.H = (int)H;
   p.window = (int)std::min<int64_t>(window, 1LL << 30);
   p.scale_log2 = (float)(scale * 1.4426950408889634);
+  p.wait = g_wait_limit;
   p.rep = (int)(H / p.c.G);
   p.maps = p.q2 ? 2 : 1;
   TORCH_CHECK(T * H < (1LL << 31), "paged_attention: sizes");

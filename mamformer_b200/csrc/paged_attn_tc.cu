@@ -30,7 +30,6 @@ using namespace paged;
 using namespace tc5;
 
 constexpr int BM = 128, BN = 64, ST = 4, NC = 64, NT = 256 + NC + 32;       // NC converting threads
-constexpr long long WAIT_CYCLES = 4000000000LL;        // about 2 s
 constexpr float LAZY = 8.f, NONE = -1e30f;
 
 __device__ int g_err = 0, g_wait_err = 0;
@@ -52,14 +51,14 @@ __device__ __forceinline__ bool try_once(uint64_t* b, uint32_t parity) {
                : "=r"(ok) : "r"(su32(b)), "r"(parity) : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ bool wait(uint64_t* b, uint32_t parity) {
-  if (try_once(b, parity)) return true;
+__device__ __forceinline__ bool wait(uint64_t* b, uint32_t parity, long long limit) {
+  if (limit >= 0 && try_once(b, parity)) return true;
   const long long t0 = clock64();
   for (uint32_t n = 1;; ++n) {
-    if (try_once(b, parity)) return true;
+    if (limit >= 0 && try_once(b, parity)) return true;
     if ((n & 1023u) == 0) {
       if (*((volatile int*)&g_wait_err) != 0) return false;
-      if (clock64() - t0 > WAIT_CYCLES) { atomicCAS(&g_wait_err, 0, (int)ERR_WAIT); return false; }
+      if (clock64() - t0 > limit) { atomicCAS(&g_wait_err, 0, (int)ERR_WAIT); return false; }
     }
   }
 }
@@ -92,7 +91,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
   constexpr int O_COL = 256;                       // TMEM: S_A[2], S_B[2] of 64 columns, then O_A, O_B of HD
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t q_full, kv_full[ST], kv_empty[ST], s_full[4], p_full[4], o_done[4], ex_full;
+  __shared__ uint64_t q_full, kv_full[ST], kv_empty[ST], s_full[4], p_full[4], o_done[4], ex_full, idle;
   __shared__ Groups groups[ST];
   __shared__ uint32_t tmem_slot;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -136,6 +135,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
   if (threadIdx.x == 0) {
     bar_init(&q_full, 256);
     bar_init(&ex_full, 128);
+    bar_init(&idle, 1);
     for (int s = 0; s < ST; ++s) { bar_init(&kv_full[s], NC / 32); bar_init(&kv_empty[s], 1); }
     for (int i = 0; i < 4; ++i) { bar_init(&s_full[i], 1); bar_init(&p_full[i], 128); bar_init(&o_done[i], 1); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
     bool ok = true;
     for (int j = 0; j < ntile; ++j) {
       const int st = j % ST;
-      if (j >= ST) ok = __all_sync(0xffffffffu, wait(&kv_empty[st], (uint32_t)((j / ST - 1) & 1)));
+      if (j >= ST) ok = __all_sync(0xffffffffu, wait(&kv_empty[st], (uint32_t)((j / ST - 1) & 1), p.wait));
       if (!ok) break;
       // the reference for O's values: the tile's largest value scale, once that is 2^6 away from it.  Scales
       // below 2^-60 of it add nothing to O.
@@ -242,13 +242,13 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
   } else if (warp == 8 + NC / 32) {
     // ------------------------------- MMA issue -------------------------------
     if (lane == 0 && ntile > 0) {
-      bool ok = wait(&q_full, 0);
+      bool ok = wait(&q_full, 0, p.wait);
       fence_after();
       constexpr uint32_t ID_QK = idesc(BN, false), ID_PV = idesc(HD, true);
       auto issue_qk = [&](int j) -> bool {
         const int st = j % ST, buf = j & 1;
         // the S buffer last held P(j - 2), read by the O += P V that this thread issued before
-        if (!wait(&kv_full[st], (uint32_t)((j / ST) & 1))) return false;
+        if (!wait(&kv_full[st], (uint32_t)((j / ST) & 1), p.wait)) return false;
         fence_after();
         const uint32_t kb = su32(ring + st * 2 * KB);
         for (int s = 0; s < 2; ++s) {
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
         const int st = j % ST, buf = j & 1;
         const uint32_t vb = su32(ring + st * 2 * KB + KB);
         for (int s = 0; s < 2 && ok; ++s) {
-          if (!wait(&p_full[s * 2 + buf], (uint32_t)((j >> 1) & 1))) { ok = false; break; }
+          if (!wait(&p_full[s * 2 + buf], (uint32_t)((j >> 1) & 1), p.wait)) { ok = false; break; }
           fence_after();
           const uint32_t pa = tmem + (uint32_t)(s * 128 + buf * 64);
           const uint32_t d = tmem + (uint32_t)(O_COL + s * HD);
@@ -279,6 +279,10 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
         }
         if (ok) commit(&kv_empty[st]);
       }
+      // products under way read shared memory and write TMEM, both of which go when the CTA ends: where a wait has run
+      // out, nobody else waits for them
+      commit(&idle);
+      for (const long long t = clock64(); !try_once(&idle, 0) && clock64() - t <= WAIT_CYCLES;) {}
     }
   } else if (warp < 8) {
     // ------------------------------- softmax -------------------------------
@@ -328,7 +332,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
     bool ok = true;
     for (int j = 0; j < ntile && ok; ++j) {
       const int buf = j & 1, st = j % ST;
-      ok = __all_sync(0xffffffffu, wait(&kv_full[st], (uint32_t)((j / ST) & 1)) && wait(&s_full[s * 2 + buf], (uint32_t)((j >> 1) & 1)));
+      ok = __all_sync(0xffffffffu, wait(&kv_full[st], (uint32_t)((j / ST) & 1), p.wait) && wait(&s_full[s * 2 + buf], (uint32_t)((j >> 1) & 1), p.wait));
       if (!ok) break;
       fence_after();
       float sv[BN];
@@ -364,7 +368,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
         m = mx;
       }
       if (j > 0 && __any_sync(0xffffffffu, fo != 1.f)) {
-        ok = __all_sync(0xffffffffu, wait(&o_done[s * 2 + ((j - 1) & 1)], (uint32_t)(((j - 1) >> 1) & 1)));
+        ok = __all_sync(0xffffffffu, wait(&o_done[s * 2 + ((j - 1) & 1)], (uint32_t)(((j - 1) >> 1) & 1), p.wait));
         if (!ok) break;
         fence_after();
 #pragma unroll 1
@@ -401,7 +405,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
     }
     // ---- result ----
     if (ok && ntile > 0) {
-      ok = __all_sync(0xffffffffu, wait(&o_done[s * 2 + ((ntile - 1) & 1)], (uint32_t)(((ntile - 1) >> 1) & 1)));
+      ok = __all_sync(0xffffffffu, wait(&o_done[s * 2 + ((ntile - 1) & 1)], (uint32_t)(((ntile - 1) >> 1) & 1), p.wait));
       fence_after();
     }
     const float vref = ntile > 0 ? groups[(ntile - 1) % ST].vref : 0.f;
@@ -433,7 +437,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
     float lam = 0.f, den = 1.f;
     if (p.maps == 2 && row_ok) { lam = p.lam[h]; den = 1.f / (1.f - lam + 1e-8f); }
     float* xrow = reinterpret_cast<float*>(sm) + r * (HD + 4);        // stream B's row; Q and the ring are free now
-    if (p.maps == 2 && s == 0 && p.splits == 1) ok = __all_sync(0xffffffffu, ok && wait(&ex_full, 0));
+    if (p.maps == 2 && s == 0 && p.splits == 1) ok = __all_sync(0xffffffffu, ok && wait(&ex_full, 0, p.wait));
 #pragma unroll 1
     for (int cc = 0; cc < HD && ok; cc += 32) {
       float o[32];

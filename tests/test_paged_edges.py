@@ -86,3 +86,28 @@ def test_tiles_that_see_nothing_give_zero(dev, hd, diff, new, lens):
             assert (got[at:at + n - L] == 0).all()
             at += n
         close(got, want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("diff", [False, True])
+@pytest.mark.parametrize("new,lens", [([1, 2], [5000, 70]), ([200], [900]), ([90, 1], [2000, 300])])
+def test_waits_that_run_out_are_reported_and_wound_down(diff, new, lens):
+    """Waits that give up at once: copies and products are then still under way when the kernel winds down."""
+    from mamformer_b200.fault import KernelTimeoutError, check_device_status
+    from mamformer_b200.ops._ext import require_native
+    C = require_native()
+    cache, table = filled(lens, 64, 2, 128, "cuda")
+    q = rand((sum(new), 4, 128), torch.bfloat16, "cuda", 3)
+    kw = pair(q, diff)
+    run = lambda: ops.paged_attention(q, cache, table, offsets(new, "cuda"), i32(lens, "cuda"), max(new), **kw)  # noqa: E731
+    check_device_status()
+    had = C.paged_attention_wait_limit(-1)
+    try:
+        run()
+        torch.cuda.synchronize()
+    finally:
+        C.paged_attention_wait_limit(had)
+    with pytest.raises(KernelTimeoutError):
+        check_device_status()
+    close(run(), *plain(q, cache, table, new, lens, **kw))
+    check_device_status()
