@@ -64,8 +64,9 @@ struct Attn {
   long long wait;                      // cycles after which a wait gives up; negative: at once, without a look
 };
 
-// Cycles of a wait, about 2 s; paged_attention_wait_limit() sets another number for the waits that a test lets run out.
-constexpr long long WAIT_CYCLES = 4000000000LL;
+// Cycles of a wait, about 0.25 s, where the longest takes microseconds; paged_attention_wait_limit() sets another number
+// for the waits that a test lets run out.
+constexpr long long WAIT_CYCLES = 500000000LL;
 
 // csrc/paged_attn_tc.cu: sequences of more than `few` rows (of any number where few is 0, and then rows past
 // the last sequence are cleared too)

@@ -90,8 +90,9 @@ __device__ __forceinline__ bool try_tile(uint32_t bar, uint32_t parity) {
                : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000000u) : "memory");
   return ok != 0;
 }
-// Waits for the warp's tile, the same answer for all lanes; false after `limit` cycles (recorded), or once
-// another warp of the grid has given up.
+// Waits for the warp's tile, the same answer for all lanes; false after `limit` cycles (recorded).  The record is only
+// written: what another warp, or an earlier call, has recorded ends no wait of this one, and a CTA that gives up ends
+// after one limit for each of its warps' waits at the same time.
 __device__ __forceinline__ bool wait_tile(uint32_t bar, uint32_t parity, long long limit) {
   if (limit >= 0 && __all_sync(0xffffffffu, try_tile(bar, parity))) return true;
   const long long t0 = clock64();
@@ -100,7 +101,7 @@ __device__ __forceinline__ bool wait_tile(uint32_t bar, uint32_t parity, long lo
     if ((n & 63u) == 0) {
       const bool over = clock64() - t0 > limit;
       if (over) atomicCAS(&g_wait_err, 0, (int)ERR_WAIT);
-      if (__any_sync(0xffffffffu, over || *((volatile int*)&g_wait_err) != 0)) return false;
+      if (__any_sync(0xffffffffu, over)) return false;
     }
   }
 }

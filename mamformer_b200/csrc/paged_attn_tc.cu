@@ -44,7 +44,9 @@ struct Params : Attn {
   float* part;         // [unit * G + head][split][stream][BM][HD + 2]: O (not divided), m, l
 };
 
-// As tc5::bar_wait, without its suspend-time hint: the hand-offs of a tile are short (1.72 ms against 1.77).
+// As tc5::bar_wait, without its suspend-time hint: the hand-offs of a tile are short (1.72 ms against 1.77).  The error
+// word is only written here: a wait that ran out in another CTA, or in an earlier call, ends no wait of this one.  After
+// one that ran out a role waits for nothing more, so a CTA ends within a few limits.
 __device__ __forceinline__ bool try_once(uint64_t* b, uint32_t parity) {
   uint32_t ok;
   asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
@@ -56,9 +58,9 @@ __device__ __forceinline__ bool wait(uint64_t* b, uint32_t parity, long long lim
   const long long t0 = clock64();
   for (uint32_t n = 1;; ++n) {
     if (limit >= 0 && try_once(b, parity)) return true;
-    if ((n & 1023u) == 0) {
-      if (*((volatile int*)&g_wait_err) != 0) return false;
-      if (clock64() - t0 > limit) { atomicCAS(&g_wait_err, 0, (int)ERR_WAIT); return false; }
+    if ((n & 1023u) == 0 && clock64() - t0 > limit) {
+      atomicCAS(&g_wait_err, 0, (int)ERR_WAIT);
+      return false;
     }
   }
 }

@@ -111,3 +111,29 @@ def test_waits_that_run_out_are_reported_and_wound_down(diff, new, lens):
         check_device_status()
     close(run(), *plain(q, cache, table, new, lens, **kw))
     check_device_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,lens", [([1, 2], [60000, 70]), ([200], [9000])])
+def test_a_wait_that_ran_out_is_over_with_its_call(new, lens):
+    """Nobody has read the error yet: the calls after it wait as they would have."""
+    from mamformer_b200.fault import KernelTimeoutError, check_device_status
+    from mamformer_b200.ops._ext import require_native
+    C = require_native()
+    cache, table = filled(lens, 64, 2, 128, "cuda")
+    q = rand((sum(new), 4, 128), torch.bfloat16, "cuda", 3)
+    run = lambda: ops.paged_attention(q, cache, table, offsets(new, "cuda"), i32(lens, "cuda"), max(new))  # noqa: E731
+    check_device_status()
+    want = run()
+    had = C.paged_attention_wait_limit(-1)
+    try:
+        run()
+        torch.cuda.synchronize()
+    finally:
+        C.paged_attention_wait_limit(had)
+    for _ in range(50):
+        assert torch.equal(run(), want)
+    with pytest.raises(KernelTimeoutError):
+        check_device_status()
+    assert torch.equal(run(), want)
+    check_device_status()
