@@ -90,9 +90,9 @@ __device__ __forceinline__ uint16_t enc2(float a, float b) {
 }
 
 // The sequence that packed token t belongs to: the last b with cu[b] <= t (an empty sequence never
-// is), or -1 past the last one.
+// is), or -1 before the first and past the last one.
 __device__ __forceinline__ int sequence_of(const int* cu, int B, int t) {
-  if (B == 0 || t >= cu[B]) return -1;
+  if (B == 0 || t < cu[0] || t >= cu[B]) return -1;
   int lo = 0, hi = B - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;

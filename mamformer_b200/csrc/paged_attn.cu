@@ -252,12 +252,13 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
   }
   __syncthreads();
   if (tid == 0) p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
-  // rows past the last sequence
+  // rows before the first and past the last sequence
   {
-    const int end = c.B > 0 ? max(0, c.cu[c.B]) : 0;
-    const int64_t n = (int64_t)max(0, c.T - end) * p.H * HD;
-    for (int64_t i = (int64_t)blockIdx.x * NT + tid; i < n; i += (int64_t)gridDim.x * NT)
-      ((T*)p.out)[(int64_t)end * p.H * HD + i] = from_f<T>(0.f);
+    const int64_t row = (int64_t)p.H * HD;
+    const int64_t front = c.B > 0 ? min(max(0, c.cu[0]), c.T) * row : 0, end = c.B > 0 ? max(0, c.cu[c.B]) * row : 0;
+    for (int64_t i = (int64_t)blockIdx.x * NT + tid; i < front; i += (int64_t)gridDim.x * NT) ((T*)p.out)[i] = from_f<T>(0.f);
+    for (int64_t i = end + (int64_t)blockIdx.x * NT + tid; i < c.T * row; i += (int64_t)gridDim.x * NT)
+      ((T*)p.out)[i] = from_f<T>(0.f);
   }
   if (first >= last) return;
 

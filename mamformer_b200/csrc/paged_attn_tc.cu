@@ -99,11 +99,11 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Cache& c = p.c;
 
-  if (p.few == 0) {                                // rows past the last sequence
-    const int64_t end = (int64_t)max(0, c.cu[c.B]) * p.H * HD, all = (int64_t)c.T * p.H * HD;
-    if (blockIdx.y == 0)
-      for (int64_t i = end + (int64_t)blockIdx.x * NT + threadIdx.x; i < all; i += (int64_t)gridDim.x * NT)
-        ((T*)p.out)[i] = from_f<T>(0.f);
+  if (p.few == 0 && blockIdx.y == 0) {             // rows before the first and past the last sequence
+    const int64_t row = (int64_t)p.H * HD, first = min(max(0, c.cu[0]), c.T) * row, end = max(0, c.cu[c.B]) * row;
+    for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < first; i += (int64_t)gridDim.x * NT) ((T*)p.out)[i] = from_f<T>(0.f);
+    for (int64_t i = end + (int64_t)blockIdx.x * NT + threadIdx.x; i < c.T * row; i += (int64_t)gridDim.x * NT)
+      ((T*)p.out)[i] = from_f<T>(0.f);
   }
   // ---- the CTA's rows ----
   const int rows = p.maps == 2 ? BM : 2 * BM;      // (token, head) pairs per CTA
@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
   }
   const int t0 = c.cu[b], n = c.cu[b + 1] - t0, len = c.lens[b];
   const int64_t tile64 = u - ((int64_t)t0 * p.rep / rows + b);
-  if (n <= 0 || t0 < 0 || t0 + n > c.T || (int64_t)n * p.rep * p.maps <= p.few || tile64 * rows >= (int64_t)n * p.rep) return;
+  if (n <= 0 || t0 < 0 || t0 + n > c.T || (int64_t)n * p.rep * p.maps <= p.few || tile64 < 0 || tile64 * rows >= (int64_t)n * p.rep) return;
   const int r0 = (int)tile64 * rows, total = n * p.rep;    // first row of the tile, rows of the sequence
   const int at0 = len - n;                                 // slot of token 0
   const int i0 = r0 / p.rep, i1 = min(n - 1, (r0 + rows - 1) / p.rep);

@@ -165,7 +165,7 @@ __device__ __forceinline__ void append_block(const Params& p) {
     if (tid == 0) record(ERR_LENGTH);
     return;
   }
-  if (j >= pages) return;
+  if (j < 0 || j >= pages) return;             // below the first unit where the offsets do not start at 0
   const int jp = start / c.page + j;
   const int pg = jp < c.W ? c.table[(int64_t)b * c.W + jp] : -1;
   if (pg < 0 || pg >= c.P) { if (tid == 0) record(ERR_PAGE); return; }

@@ -137,3 +137,31 @@ def test_a_wait_that_ran_out_is_over_with_its_call(new, lens):
         check_device_status()
     assert torch.equal(run(), want)
     check_device_status()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("first", [1, 40, 1000])
+@pytest.mark.parametrize("new,lens", [([1, 1], [40, 20]), ([60, 3], [90, 3]), ([1, 90], [17, 400])])
+def test_offsets_that_do_not_start_at_zero(dev, first, new, lens):
+    """Rows before the first sequence belong to nobody: they are not appended, and their queries give 0."""
+    table, P = tables(lens, 16, dev)
+    G, hd, H, T = 2, 64, 4, sum(new)
+    k, v = rand((T, G, hd), torch.bfloat16, dev, 1), rand((T, G, hd), torch.bfloat16, dev, 2)
+    front = rand((first, G, hd), torch.bfloat16, dev, 5) * 100.0
+    q = rand((first + T, H, hd), torch.bfloat16, dev, 3)
+    caches = pool(P, G, 16, hd, dev), pool(P, G, 16, hd, dev)
+    for c in caches:
+        kx, vx = rand((sum(lens), G, hd), torch.bfloat16, dev, 6), rand((sum(lens), G, hd), torch.bfloat16, dev, 7)
+        ops.kv_append(kx, vx, c, table, offsets(lens, dev), i32(lens, dev), max(lens))
+    cu = offsets(new, dev)
+    ops.kv_append(k, v, caches[0], table, cu, i32(lens, dev), max(new))
+    ops.kv_append(torch.cat([front, k]), torch.cat([front, v]), caches[1], table, cu + first, i32(lens, dev), max(new))
+    for a, b in zip(*caches):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    for diff in (False, True):
+        kw, kw0 = pair(q, diff), pair(q[first:], diff)
+        if diff:
+            kw0["q2"] = kw["q2"][first:]
+        got = ops.paged_attention(q, caches[0], table, cu + first, i32(lens, dev), max(new), **kw)
+        assert (got[:first] == 0).all()
+        close(got[first:], *plain(q[first:], caches[0], table, new, lens, **kw0))
