@@ -133,13 +133,10 @@ __device__ __forceinline__ bool set_sequence(const Params& p, Item& it, int b) {
   it.b = b;
   it.t0 = p.c.cu[b];
   it.n = p.c.cu[b + 1] - it.t0;
-  it.len = p.c.lens[b];
-  if (it.n <= 0 || it.t0 < 0 || it.t0 + it.n > p.c.T) return false;
+  if (it.n <= 0) return false;
   it.rows = it.n * p.rep * p.maps;
-  if (it.rows > p.few) {
-    if (!p.chunked) record(ERR_LENGTH);                         // more new tokens than max_new
-    return false;
-  }
+  if (it.rows > p.few) return false;                            // the chunk kernel's, or too_many
+  it.len = cached_length(p.c, b, &g_err);
   it.g = it.rt = 0;
   set_range<ROWS>(p, it);
   return true;
@@ -164,6 +161,11 @@ __device__ __forceinline__ int64_t tiles_of(const Params& p, int b) {
       n += it.nt;
     }
   return n * p.c.G;
+}
+
+// More new tokens than the caller's max_new, by which this kernel was left to do it all.
+__device__ __forceinline__ bool too_many(const Params& p, int b) {
+  return !p.chunked && (int64_t)(p.c.cu[b + 1] - p.c.cu[b]) * p.rep * p.maps > p.few;
 }
 
 template <int HD> constexpr int stage_bytes() { return 2 * STEP * HD; }
@@ -209,7 +211,7 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
   __shared__ uint64_t bars[NW][ST];
   __shared__ int64_t s_pre[NT / 32];
   __shared__ int64_t s_begin;
-  __shared__ int s_b;
+  __shared__ int s_b, s_cut;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g8 = lane >> 2, t4 = lane & 3;
   const Cache& c = p.c;
   asm volatile("griddepcontrol.launch_dependents;");      // the join kernel waits for this grid's end by itself
@@ -217,9 +219,13 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
   // ---- this CTA's share [first, last) of the list of tiles ----
   const int chunk = (c.B + NT - 1) / NT;
   int64_t mine = 0;
+  bool odd = false;
   for (int i = 0; i < chunk; ++i) {
     const int b = tid * chunk + i;
-    if (b < c.B) mine += tiles_of<ROWS>(p, b);
+    if (b < c.B) {
+      odd = odd || !in_order(c, b) || too_many(p, b);
+      mine += tiles_of<ROWS>(p, b);
+    }
   }
   int64_t incl = mine;
 #pragma unroll
@@ -228,8 +234,23 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
     if (lane >= o) incl += v;
   }
   if (lane == 31) s_pre[w] = incl;
-  if (tid == 0) s_b = -1;
-  __syncthreads();
+  if (tid == 0) { s_b = -1; s_cut = 0; }
+  if (__syncthreads_or(odd)) {
+    // sequences of too many tokens are left out and get zeros; offsets that are not in order give nothing but zeros
+    bool broken = false;
+    for (int b = tid; b < c.B; b += NT) broken = broken || !in_order(c, b);
+    broken = __syncthreads_or(broken);
+    if (tid == 0) record(ERR_LENGTH);
+    for (int t = blockIdx.x; t < c.T; t += gridDim.x) {
+      const int b = broken ? -1 : sequence_of(c.cu, c.B, t);
+      if (broken || (b >= 0 && too_many(p, b)))
+        for (int i = tid; i < p.H * HD; i += NT) ((T*)p.out)[(int64_t)t * p.H * HD + i] = from_f<T>(0.f);
+    }
+    if (broken) {
+      if (tid == 0) p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
+      return;
+    }
+  }
   int64_t total = 0, before = 0;
 #pragma unroll
   for (int i = 0; i < NW; ++i) {
@@ -562,7 +583,7 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
       if (turn > 0) __syncthreads();
     }
     if (w == 0) {
-      const bool whole = ends && item_start >= first;
+      const bool whole = ends && item_start >= first, cut = *(volatile int*)&s_cut != 0;
       float* part = p.part + ((int64_t)blockIdx.x * 2 + (item_start > first ? 1 : 0)) * ROWS * (HD + 2);
       const int per = p.rep * p.maps;
 #pragma unroll
@@ -575,7 +596,8 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
           L += __shfl_xor_sync(0xffffffffu, L, 4);
           L += __shfl_xor_sync(0xffffffffu, L, 8);
           L += __shfl_xor_sync(0xffffffffu, L, 16);
-          f0[x] = L == 0.f ? 0.f : 1.f / L;
+          if (cut) L = -1.f;                             // in a part: the join writes zeros
+          f0[x] = cut || L == 0.f ? 0.f : 1.f / L;
           const int r = nr * 8 + 2 * t4 + x;
           if (!whole) {
             float* dst = part + r * (HD + 2);
@@ -629,6 +651,7 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
       issue(there, bar_there);
       ok = wait_tile(bar_here, phase, p.wait);
       waited += ok;
+      if (!ok) s_cut = 1;                          // this item's rows and the next ones' are zeros
     }
     if (ok && ksr[0] != 0.f) {
       float s[NR][4];
@@ -675,6 +698,7 @@ __global__ void __launch_bounds__(NJ) join_kernel(const __grid_constant__ Params
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, r = w % n_rows, gr = w / n_rows, groups = W / n_rows;
   if (gr < groups) {
     float M = NONE, L = 0.f, a[D] = {};
+    bool cut = false;
 #pragma unroll 8
     for (int i = gr; i < parts; i += groups) {
       const float* x = p.part + (((int64_t)(c0 + i) * 2 + (i == 0 ? j.w & 1 : 0)) * ROWS + r) * (HD + 2);
@@ -684,6 +708,7 @@ __global__ void __launch_bounds__(NJ) join_kernel(const __grid_constant__ Params
       for (int d = 0; d < D / 2; ++d) v[d] = *reinterpret_cast<const float2*>(x + lane * D + 2 * d);
       const float mn = fmaxf(M, ml.x), f = ex2(M - mn), e = ex2(ml.x - mn);
       M = mn;
+      cut = cut || ml.y < 0.f;
       L = fmaf(L, f, ml.y * e);
 #pragma unroll
       for (int d = 0; d < D / 2; ++d) {
@@ -693,18 +718,22 @@ __global__ void __launch_bounds__(NJ) join_kernel(const __grid_constant__ Params
     }
 #pragma unroll
     for (int d = 0; d < D; ++d) vals[w][lane * D + d] = a[d];
-    if (lane == 0) sums[w] = make_float2(M, L);
+    if (lane == 0) sums[w] = make_float2(M, cut ? -1.f : L);
   }
   __syncthreads();
   auto value = [&](int row, int d) {
     float M = NONE, L = 0.f, x = 0.f;
-    for (int i = row; i < groups * n_rows; i += n_rows) M = fmaxf(M, sums[i].x);
+    bool cut = false;                                // a part that a wait's end has cut short
+    for (int i = row; i < groups * n_rows; i += n_rows) {
+      M = fmaxf(M, sums[i].x);
+      cut = cut || sums[i].y < 0.f;
+    }
     for (int i = row; i < groups * n_rows; i += n_rows) {
       const float e = ex2(sums[i].x - M);
       x = fmaf(vals[i][d], e, x);
       L = fmaf(sums[i].y, e, L);
     }
-    return L == 0.f ? 0.f : x / L;
+    return cut || L == 0.f ? 0.f : x / L;
   };
   for (int i = threadIdx.x; i < ROWS / p.maps * HD; i += NJ) {
     const int rr = i / HD * p.maps, d = i % HD;

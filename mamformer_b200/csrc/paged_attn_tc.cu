@@ -96,14 +96,23 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
   __shared__ uint64_t q_full, kv_full[ST], kv_empty[ST], s_full[4], p_full[4], o_done[4], ex_full, idle;
   __shared__ Groups groups[ST];
   __shared__ uint32_t tmem_slot;
+  __shared__ int cut;                              // a wait of the second map ran out
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Cache& c = p.c;
 
-  if (p.few == 0 && blockIdx.y == 0) {             // rows before the first and past the last sequence
+  if (p.few == 0 && blockIdx.y == 0) {             // no other kernel runs: rows before the first and past the last sequence
     const int64_t row = (int64_t)p.H * HD, first = min(max(0, c.cu[0]), c.T) * row, end = max(0, c.cu[c.B]) * row;
     for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < first; i += (int64_t)gridDim.x * NT) ((T*)p.out)[i] = from_f<T>(0.f);
     for (int64_t i = end + (int64_t)blockIdx.x * NT + threadIdx.x; i < c.T * row; i += (int64_t)gridDim.x * NT)
       ((T*)p.out)[i] = from_f<T>(0.f);
+    if (blockIdx.x == gridDim.x - 1) {             // one CTA, of rows that see little, looks at all offsets
+      bool odd = false;
+      for (int i = threadIdx.x; i < c.B; i += NT) odd = odd || !in_order(c, i);
+      if (__syncthreads_or(odd)) {                 // no unit may have some rows: none of the call's results count
+        if (threadIdx.x == 0) atomicCAS(&g_err, 0, (int)ERR_LENGTH);
+        for (int64_t i = threadIdx.x; i < c.T * row; i += NT) ((T*)p.out)[i] = from_f<T>(0.f);
+      }
+    }
   }
   // ---- the CTA's rows ----
   const int rows = p.maps == 2 ? BM : 2 * BM;      // (token, head) pairs per CTA
@@ -118,9 +127,9 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
       if ((int64_t)c.cu[mid] * p.rep / rows + mid <= u) b = mid; else hi = mid - 1;
     }
   }
-  const int t0 = c.cu[b], n = c.cu[b + 1] - t0, len = c.lens[b];
+  const int t0 = c.cu[b], n = c.cu[b + 1] - t0, len = cached_length(c, b, &g_err);
   const int64_t tile64 = u - ((int64_t)t0 * p.rep / rows + b);
-  if (n <= 0 || t0 < 0 || t0 + n > c.T || (int64_t)n * p.rep * p.maps <= p.few || tile64 < 0 || tile64 * rows >= (int64_t)n * p.rep) return;
+  if (!in_order(c, b) || (int64_t)n * p.rep * p.maps <= p.few || tile64 < 0 || tile64 * rows >= (int64_t)n * p.rep) return;
   const int r0 = (int)tile64 * rows, total = n * p.rep;    // first row of the tile, rows of the sequence
   const int at0 = len - n;                                 // slot of token 0
   const int i0 = r0 / p.rep, i1 = min(n - 1, (r0 + rows - 1) / p.rep);
@@ -138,6 +147,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
     bar_init(&q_full, 256);
     bar_init(&ex_full, 128);
     bar_init(&idle, 1);
+    cut = 0;
     for (int s = 0; s < ST; ++s) { bar_init(&kv_full[s], NC / 32); bar_init(&kv_empty[s], 1); }
     for (int i = 0; i < 4; ++i) { bar_init(&s_full[i], 1); bar_init(&p_full[i], 128); bar_init(&o_done[i], 1); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -412,19 +422,24 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
     }
     const float vref = ntile > 0 ? groups[(ntile - 1) % ST].vref : 0.f;
     T* out = (T*)p.out + ((int64_t)(t0 + i) * p.H + h) * HD;
-    if (ntile == 0 && p.splits == 1) {
-      // No row sees a key.  The exchange below is ordered after the stores of q by the wait for O, which there is
-      // none of here, so the rows are written without it.
-      Vec16<T> zero;
-      zero.raw = make_uint4(0, 0, 0, 0);
-      if (row_ok && (p.maps == 1 || s == 0))
-        for (int k = 0; k < HD; k += 8) st16(out + k, zero);
-      ok = false;
+    if (p.splits == 1) {
+      // Rows of zeros: no row sees a key, and then there is no wait for O either, which orders the exchange below after
+      // the stores of q; or a wait has run out, in this warp or in the other map's.
+      bool zeros = !ok || ntile == 0;
+      if (p.maps == 2 && s == 1 && !ok) cut = 1;
+      if (p.maps == 2 && s == 0 && !zeros) zeros = !__all_sync(0xffffffffu, wait(&ex_full, 0, p.wait)) || *(volatile int*)&cut != 0;
+      if (zeros) {
+        Vec16<T> zero;
+        zero.raw = make_uint4(0, 0, 0, 0);
+        if (row_ok && (p.maps == 1 || s == 0))
+          for (int k = 0; k < HD; k += 8) st16(out + k, zero);
+        ok = false;
+      }
     }
     if (p.splits > 1) {
       float* dst = p.part + ((((int64_t)blockIdx.x * p.splits + blockIdx.y) * 2 + s) * BM + r) * (HD + 2);
-      // a part that a wait's end has cut short is written as no part at all
-      *reinterpret_cast<float2*>(dst + HD) = ok ? make_float2(m, l) : make_float2(NONE, 0.f);
+      // a wait that ran out: a negative sum, at which the join writes zeros
+      *reinterpret_cast<float2*>(dst + HD) = ok ? make_float2(m, l) : make_float2(NONE, -1.f);
 #pragma unroll 1
       for (int cc = 0; cc < HD; cc += 32) {
         float o[32];
@@ -439,7 +454,6 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
     float lam = 0.f, den = 1.f;
     if (p.maps == 2 && row_ok) { lam = p.lam[h]; den = 1.f / (1.f - lam + 1e-8f); }
     float* xrow = reinterpret_cast<float*>(sm) + r * (HD + 4);        // stream B's row; Q and the ring are free now
-    if (p.maps == 2 && s == 0 && p.splits == 1) ok = __all_sync(0xffffffffu, ok && wait(&ex_full, 0, p.wait));
 #pragma unroll 1
     for (int cc = 0; cc < HD && ok; cc += 32) {
       float o[32];
@@ -481,7 +495,7 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__
   const int b = sequence_of(c.cu, c.B, t);
   if (b < 0) return;
   const int t0 = c.cu[b], n = c.cu[b + 1] - t0;
-  if (t0 < 0 || t0 + n > c.T || (int64_t)n * p.rep * p.maps <= p.few) return;
+  if (!in_order(c, b) || (int64_t)n * p.rep * p.maps <= p.few) return;
   const int rows = p.maps == 2 ? BM : 2 * BM, row = (t - t0) * p.rep + h % p.rep;
   const int u = (int)((int64_t)t0 * p.rep / rows + b) + row / rows;
   const int64_t unit = (int64_t)(units - 1 - u) * c.G + g;
@@ -491,9 +505,11 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__
     const float* x = p.part + ((unit * p.splits * 2 + s) * BM + row % BM) * (HD + 2);
     const int64_t step = (int64_t)2 * BM * (HD + 2);
     float M = NONE, L = 0.f, a[D] = {};
+    bool cut = false;
 #pragma unroll 4
     for (int i = 0; i < p.splits; ++i, x += step) {
       const float2 ml = *reinterpret_cast<const float2*>(x + HD);
+      cut = cut || ml.y < 0.f;
       float2 v[D / 2];
 #pragma unroll
       for (int d = 0; d < D / 2; ++d) v[d] = *reinterpret_cast<const float2*>(x + lane * D + 2 * d);
@@ -505,6 +521,11 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__
         a[2 * d] = fmaf(a[2 * d], f, v[d].x * e);
         a[2 * d + 1] = fmaf(a[2 * d + 1], f, v[d].y * e);
       }
+    }
+    if (cut) {                                     // of either map: the row is zeros
+#pragma unroll
+      for (int d = 0; d < D; ++d) res[d] = 0.f;
+      break;
     }
     float w = L == 0.f ? 0.f : 1.f / L;
     if (p.maps == 2) w *= (map ? -p.lam[h] : 1.f) / (1.f - p.lam[h] + 1e-8f);

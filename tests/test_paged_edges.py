@@ -165,3 +165,63 @@ def test_offsets_that_do_not_start_at_zero(dev, first, new, lens):
         got = ops.paged_attention(q, caches[0], table, cu + first, i32(lens, dev), max(new), **kw)
         assert (got[:first] == 0).all()
         close(got[first:], *plain(q[first:], caches[0], table, new, lens, **kw0))
+
+
+def dirty(shape, dtype, dev):
+    """Memory that the next allocation of its size gets, full of NaN."""
+    torch.full(shape, math.nan, dtype=dtype, device=dev)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("diff", [False, True])
+def test_rows_that_are_not_computed_are_zeros(diff):
+    from mamformer_b200.fault import KernelTimeoutError, PagedCacheError, check_device_status
+    from mamformer_b200.ops._ext import require_native
+    C = require_native()
+    check_device_status()
+
+    def run(q, cu, lens, max_new):
+        dirty(q.shape, q.dtype, "cuda")
+        return ops.paged_attention(q, cache, table, cu, lens, max_new, **pair(q, diff))
+
+    # sequence 1 has more tokens than max_new says
+    new, lens = [1, 30, 2], [40, 90, 70]
+    cache, table = filled(lens, 16, 2, 128, "cuda")
+    q = rand((sum(new), 4, 128), torch.bfloat16, "cuda", 3)
+    cu, ln = offsets(new, "cuda"), i32(lens, "cuda")
+    want, tol = plain(q, cache, table, new, lens, **pair(q, diff))
+    got = run(q, cu, ln, 2)
+    assert (got[1:31] == 0).all()
+    for rows in (slice(0, 1), slice(31, 33)):
+        close(got[rows], want[rows], tol[rows])
+    with pytest.raises(PagedCacheError, match="lengths"):
+        check_device_status()
+    # offsets that fall, or run past the queries
+    q = rand((600, 4, 128), torch.bfloat16, "cuda", 4)
+    for bad in ([0, 5, 3, 8], [0, 2, 4, 900], [0, 200, 100, 600], [-5, 0, 5, 9], [0, 1, 2, -1]):
+        for max_new in (2, 40, 200):
+            got = run(q, i32(bad, "cuda"), ln, max_new)
+            assert got.isfinite().all() and (max_new == 200 or (got == 0).all())
+            with pytest.raises(PagedCacheError, match="lengths"):
+                check_device_status()
+    # a length that the table has no room for
+    ln, new, lens = i32([40, (1 << 31) - 1, 70], "cuda"), [1, 1, 2], [40, 90, 70]
+    want, tol = plain(q[:4], cache, table, new, lens, **pair(q[:4], diff))
+    got = run(q[:4], offsets(new, "cuda"), ln, 2)
+    for rows in (slice(0, 1), slice(2, 4)):                 # the other sequences'
+        close(got[rows], want[rows], tol[rows])
+    with pytest.raises(PagedCacheError):
+        check_device_status()
+    # waits that run out
+    for new, lens in (([1, 2], [60000, 70]), ([200], [9000]), ([90, 1], [2000, 300]), ([2000], [2000])):
+        cache, table = filled(lens, 64, 2, 128, "cuda")
+        q = rand((sum(new), 4, 128), torch.bfloat16, "cuda", 3)
+        had = C.paged_attention_wait_limit(-1)
+        try:
+            got = run(q, offsets(new, "cuda"), i32(lens, "cuda"), max(new))
+            torch.cuda.synchronize()
+        finally:
+            C.paged_attention_wait_limit(had)
+        assert (got == 0).all()
+        with pytest.raises(KernelTimeoutError):
+            check_device_status()
