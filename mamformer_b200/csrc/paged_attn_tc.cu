@@ -323,8 +323,9 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
       int e = (int)(__float_as_uint(mx) >> 23) - 127;       // rows of zeros and rows with infinities stay as they are
       if (e == -127 || e == 128) e = 0;
       e = max(-126, min(126, e));
-      const float down = pow2(-e);
-      rs = p.scale_log2 * pow2(e);
+      // the factor of the scores is not negative, so that the largest product is the largest score: its sign is q's
+      const float down = p.scale_log2 < 0.f ? -pow2(-e) : pow2(-e);
+      rs = fabsf(p.scale_log2) * pow2(e);
       uint8_t* qrow = sm + s * QB + r * 128;
 #pragma unroll
       for (int k = 0; k < HD / 8; ++k) {
@@ -354,14 +355,17 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
       *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(gr.k);
       const int kbase = (kt0 + j) * BN;
       if (__any_sync(0xffffffffu, !(gr.all && kbase >= lo && kbase + BN - 1 <= hi))) {
+        // scaled first, masked then: a factor may be 0, and 0 times -inf is NaN
 #pragma unroll
         for (int k = 0; k < BN; ++k) {
           const int key = kbase + k;
-          sv[k] = (key >= lo && key <= hi && f[k >> 4] != 0.f) ? sv[k] : -INFINITY;
+          sv[k] = (key >= lo && key <= hi && f[k >> 4] != 0.f) ? sv[k] * (f[k >> 4] * rs) : -INFINITY;
         }
-        // a masked group's factor: -inf stays -inf
 #pragma unroll
-        for (int k = 0; k < 4; ++k) f[k] = f[k] != 0.f ? f[k] : 1.f;
+        for (int k = 0; k < 4; ++k) f[k] = 1.f;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[k] *= rs;
       }
       float mx = -INFINITY;
 #pragma unroll
@@ -369,7 +373,6 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
         float a[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) a[q] = fmaxf(fmaxf(sv[16 * k + q], sv[16 * k + 4 + q]), fmaxf(sv[16 * k + 8 + q], sv[16 * k + 12 + q]));
-        f[k] *= rs;
         mx = fmaxf(mx, fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])) * f[k]);
       }
       float fo = gr.fo;

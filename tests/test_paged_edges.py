@@ -225,3 +225,30 @@ def test_rows_that_are_not_computed_are_zeros(diff):
         assert (got == 0).all()
         with pytest.raises(KernelTimeoutError):
             check_device_status()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("scale", [0.0, -0.1, -1e-30, 0.3])
+@pytest.mark.parametrize("diff", [False, True])
+@pytest.mark.parametrize("new,lens", [([1, 3], [70, 33]), ([130, 70], [130, 400])])
+def test_score_factors_of_any_sign(dev, scale, diff, new, lens):
+    cache, table = filled(lens, 32, 2, 128, dev)
+    q = rand((sum(new), 4, 128), torch.bfloat16, dev, 1)
+    kw = dict(pair(q, diff), scale=scale)
+    close(ops.paged_attention(q, cache, table, offsets(new, dev), i32(lens, dev), max(new), **kw), *plain(q, cache, table, new, lens, **kw))
+    windowed = dict(kw, window=20)
+    close(ops.paged_attention(q, cache, table, offsets(new, dev), i32(lens, dev), max(new), **windowed),
+          *plain(q, cache, table, new, lens, **windowed))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("size", [2.0 ** -60, 2.0 ** -120, 2.0 ** 40])
+@pytest.mark.parametrize("new,lens", [([1, 3], [70, 33]), ([130, 70], [130, 400])])
+def test_zero_keys_and_queries_of_any_size(dev, size, new, lens):
+    """Keys of zeros have the smallest block scale there is: the scores' factor underflows with small queries."""
+    table, P = tables(lens, 16, dev)
+    cache = pool(P, 1, 16, 64, dev)
+    v = rand((sum(lens), 1, 64), torch.float32, dev, 2)
+    ops.kv_append(torch.zeros_like(v), v, cache, table, offsets(lens, dev), i32(lens, dev), max(lens))
+    q = (rand((sum(new), 2, 64), torch.float32, dev, 1) * size).bfloat16()
+    close(ops.paged_attention(q, cache, table, offsets(new, dev), i32(lens, dev), max(new)), *plain(q, cache, table, new, lens))
