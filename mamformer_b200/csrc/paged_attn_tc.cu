@@ -10,8 +10,11 @@
 //                   e4m3 -> f16 (exact) into a ring of 128-byte-swizzled tiles; codes past the end become 0
 //   warp 10         TMEM allocation, MMA issue: S = Q K^T (M 128, N 64), O += P V (N = head size, P in TMEM)
 // The blocks' scales are powers of two and stay out of the products: a key's goes into the factor of its
-// score, a value's (relative to a reference that O is kept in) into the exponent of its weight, so a 16-token
-// group costs four multiplications per row.  Where there are fewer tiles than SMs, several CTAs share a tile's
+// score, a value's into the exponent of its weight.  O is kept in units of 2^(m + r): m is the row's running maximum of
+// the scores, which the sum of weights is kept in, and r a whole number that brings m + r to its running maximum of
+// score + log2 of the value scale.  So the f16 weights keep their bits for what the row sees, whatever the values of
+// other pages are, and the largest score's is a power of two.  A 16-token group costs a handful of operations per row.
+// Where there are fewer tiles than SMs, several CTAs share a tile's
 // keys and a second kernel joins them.  Online softmax with lazy rescaling as in flash_tc.cu.  Every
 // wait is bounded; a wait that runs out records a code, and the CTA winds down.
 //
@@ -81,9 +84,8 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)
 // What the softmax needs to know of a tile's four 16-token groups.
 struct __align__(16) Groups {
   float k[4];          // scale of the keys, 0: the group is not there
-  float e[4];          // weights enter P V as 2^e times themselves: e is the exponent of the value scale over vref
-  float c[4];          // 2^-e
-  float vref, fo;      // the scale that O's values are in, and what it takes O there from the tile before
+  float v[4];          // log2 of the scale of the values
+  float c[4];          // 1 / scale of the values
   int all;             // all four groups are there
 };
 
@@ -168,7 +170,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
     constexpr int RS = NC / CR;                              // rows between a thread's chunks: 8 or 16
     const int ct = threadIdx.x - 256, r0c = ct / CR, cc = ct % CR;
     uint4 kx[N], vx[N];                                      // chunk i: token i RS + r0c, dims 16 cc ..
-    float ks = 0.f, vs = 0.f, vref = 0.f, fo = 1.f;          // ks, vs: of group lane % 4
+    float ks = 0.f, vs = 0.f;                                // of group lane % 4
     auto look_up = [&](int j) {                              // the page of group lane % 4 of tile j
       const int slot = (kt0 + j) * BN + (lane & 3) * 16;
       if (j >= ntile || slot >= key_hi) return -2;
@@ -219,23 +221,13 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
       const int st = j % ST;
       if (j >= ST) ok = __all_sync(0xffffffffu, wait(&kv_empty[st], (uint32_t)((j / ST - 1) & 1), p.wait));
       if (!ok) break;
-      // the reference for O's values: the tile's largest value scale, once that is 2^6 away from it.  Scales
-      // below 2^-60 of it add nothing to O.
-      float vmax = fmaxf(vs, __shfl_xor_sync(0xffffffffu, vs, 1));
-      vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 2));
-      fo = 1.f;
-      if (vref == 0.f) vref = vmax;
-      else if (vmax > vref * 64.f || (vmax < vref * 0.015625f && vmax > vref * 8.6736174e-19f)) {
-        fo = vref / vmax;
-        vref = vmax;
-      }
       const bool all = __all_sync(0xffffffffu, ks != 0.f);
       if (ct < 4) {
-        const int e = vs > 0.f ? max(-100, ((int)__float_as_uint(vs) - (int)__float_as_uint(vref)) >> 23) : 0;
+        const int e = vs > 0.f ? (int)(__float_as_uint(vs) >> 23) - 127 : 0;
         groups[st].k[ct] = ks;
-        groups[st].e[ct] = (float)e;
-        groups[st].c[ct] = pow2(-e);
-        if (ct == 0) { groups[st].vref = vref; groups[st].fo = fo; groups[st].all = all; }
+        groups[st].v[ct] = (float)e;
+        groups[st].c[ct] = pow2(max(-126, -e));
+        if (ct == 0) groups[st].all = all;
       }
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -341,7 +333,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
     }
     // slots [lo, hi] that the row sees; rows past the last one (zeros) see everything and are not written
     const int hi = row_ok ? min(len - 1, at) : 0x7fffffff, lo = row_ok && p.window > 0 ? at - p.window + 1 : 0;
-    float m = NONE, l = 0.f;
+    float m = NONE, r2 = 0.f, unit = 1.f, l = 0.f;           // r2: r of the head comment;  unit = 2^r2
     bool ok = true;
     for (int j = 0; j < ntile && ok; ++j) {
       const int buf = j & 1, st = j % ST;
@@ -367,20 +359,26 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
 #pragma unroll
         for (int k = 0; k < 4; ++k) f[k] *= rs;
       }
-      float mx = -INFINITY;
+      float mx = -INFINITY, vx = -INFINITY;
+      float gv[4];
+      *reinterpret_cast<float4*>(gv) = *reinterpret_cast<const float4*>(gr.v);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         float a[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) a[q] = fmaxf(fmaxf(sv[16 * k + q], sv[16 * k + 4 + q]), fmaxf(sv[16 * k + 8 + q], sv[16 * k + 12 + q]));
-        mx = fmaxf(mx, fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])) * f[k]);
+        a[0] = fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])) * f[k];
+        mx = fmaxf(mx, a[0]);
+        vx = fmaxf(vx, a[0] + gv[k]);
       }
-      float fo = gr.fo;
-      if (mx > m + LAZY) {
-        const float g2 = ex2(m - mx);                       // 0 for the first key of a row
-        l *= g2;
-        fo *= g2;
-        m = mx;
+      float fo = 1.f;
+      if (mx > m + LAZY || vx > m + r2 + LAZY) {            // both rise once one of them is outgrown
+        const float m1 = fmaxf(m, mx), r1 = rintf(fmaxf(vx, m + r2) - m1);
+        l *= ex2(m - m1);                                   // 0 for the first key of a row
+        fo = ex2((m - m1) + (r2 - r1));
+        m = m1;
+        r2 = r1;
+        unit = pow2((int)fminf(fmaxf(r1, -126.f), 126.f));
       }
       if (j > 0 && __any_sync(0xffffffffu, fo != 1.f)) {
         ok = __all_sync(0xffffffffu, wait(&o_done[s * 2 + ((j - 1) & 1)], (uint32_t)(((j - 1) >> 1) & 1), p.wait));
@@ -398,7 +396,9 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
       float pk_[BN / 2];                                    // P as f16 pairs, bit patterns in fp32 registers
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float neg = gr.e[k] - m;
+        // Weights of a group whose scale is below 2^-60 of the reference enter as if it were that, which is as little
+        // as nothing in O; this keeps them, and so their sum for l, in range.
+        const float neg = fmaxf(gv[k] - r2, -60.f) - m;
         const uint64_t ff = pk(f[k], f[k]), nn = pk(neg, neg);
         uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
         }
         float a, a2;
         unpk(add2(sum[0], sum[1]), a, a2);
-        l = fmaf(a + a2, gr.c[k], l);
+        l = fmaf(a + a2, fminf(gr.c[k] * unit, 1.1529215e18f), l);         // 2^60
       }
       tst32(tl + (uint32_t)(s * 128 + buf * 64), pk_);      // over this row's S, which is in registers
       fence_before();
@@ -423,7 +423,6 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
       ok = __all_sync(0xffffffffu, wait(&o_done[s * 2 + ((ntile - 1) & 1)], (uint32_t)(((ntile - 1) >> 1) & 1), p.wait));
       fence_after();
     }
-    const float vref = ntile > 0 ? groups[(ntile - 1) % ST].vref : 0.f;
     T* out = (T*)p.out + ((int64_t)(t0 + i) * p.H + h) * HD;
     if (p.splits == 1) {
       // Rows of zeros: no row sees a key, and then there is no wait for O either, which orders the exchange below after
@@ -449,11 +448,11 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
         if (ntile > 0 && ok) tld32(tl + (uint32_t)(O_COL + s * HD + cc), o);
 #pragma unroll
         for (int k = 0; k < 32; k += 2)
-          *reinterpret_cast<float2*>(dst + cc + k) = ntile > 0 && ok ? make_float2(o[k] * vref, o[k + 1] * vref) : make_float2(0.f, 0.f);
+          *reinterpret_cast<float2*>(dst + cc + k) = ntile > 0 && ok ? make_float2(o[k] * unit, o[k + 1] * unit) : make_float2(0.f, 0.f);
       }
       ok = false;                                  // nothing more to write
     }
-    const float inv = l == 0.f ? 0.f : vref / l;
+    const float inv = l == 0.f ? 0.f : unit / l;
     float lam = 0.f, den = 1.f;
     if (p.maps == 2 && row_ok) { lam = p.lam[h]; den = 1.f / (1.f - lam + 1e-8f); }
     float* xrow = reinterpret_cast<float*>(sm) + r * (HD + 4);        // stream B's row; Q and the ring are free now

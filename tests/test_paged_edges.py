@@ -252,3 +252,31 @@ def test_zero_keys_and_queries_of_any_size(dev, size, new, lens):
     ops.kv_append(torch.zeros_like(v), v, cache, table, offsets(lens, dev), i32(lens, dev), max(lens))
     q = (rand((sum(new), 2, 64), torch.float32, dev, 1) * size).bfloat16()
     close(ops.paged_attention(q, cache, table, offsets(new, dev), i32(lens, dev), max(new)), *plain(q, cache, table, new, lens))
+
+
+SPREADS = [[1.0, 2.0 ** -8], [1.0, 2.0 ** -14], [2.0 ** -26, 1.0], [1.0, 2.0 ** 20], [1e-5, 500.0], [1.0, 2.0 ** 40, 2.0 ** -40, 1.0],
+           [0.0, 1.0], [1e-20, 0.0, 1e20, 3.0, 2.0 ** 55]]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("gain", SPREADS)
+@pytest.mark.parametrize("hd,page", [(64, 16), (128, 32), (128, 64)])
+@pytest.mark.parametrize("diff", [False, True])
+@pytest.mark.parametrize("new,lens", [([1, 1, 1], [40, 100, 150]), ([5, 3], [60, 33]), ([150, 90], [150, 200])])
+def test_pages_of_values_of_any_size(dev, gain, hd, page, diff, new, lens):
+    """Neighbouring pages' values differ by up to 2^120; a row is held to the values that it sees."""
+    cache, table = filled(lens, page, 1, hd, dev, gain)
+    q = rand((sum(new), 4, hd), torch.bfloat16, dev, 3)
+    kw = pair(q, diff)
+    got = ops.paged_attention(q, cache, table, offsets(new, dev), i32(lens, dev), max(new), **kw)
+    close(got, *plain(q, cache, table, new, lens, **kw))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gain", SPREADS)
+@pytest.mark.parametrize("new,lens", [([1], [9000]), ([70], [4000])])
+def test_parts_of_values_of_any_size(gain, new, lens):
+    """The same where several CTAs share a row's keys."""
+    cache, table = filled(lens, 16, 2, 64, "cuda", gain)
+    q = rand((sum(new), 4, 64), torch.bfloat16, "cuda", 3)
+    close(ops.paged_attention(q, cache, table, offsets(new, "cuda"), i32(lens, "cuda"), max(new)), *plain(q, cache, table, new, lens))
