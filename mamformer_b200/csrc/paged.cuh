@@ -104,12 +104,8 @@ __device__ __forceinline__ int sequence_of(const int* cu, int B, int t) {
 // Offsets of sequence b that rise and stay within the T packed tokens.
 __device__ __forceinline__ bool in_order(const Cache& c, int b) { return c.cu[b] >= 0 && c.cu[b] <= c.cu[b + 1] && c.cu[b + 1] <= c.T; }
 
-// Slots of sequence b; a length that the block table has no room for is recorded and cut to it.
-__device__ __forceinline__ int cached_length(const Cache& c, int b, int* err) {
-  const int len = c.lens[b], n = max(0, min(len, c.W << c.shift));
-  if (n != len) atomicCAS(err, 0, (int)ERR_LENGTH);
-  return n;
-}
+// The slots of a sequence that the block table has room for.
+__device__ __forceinline__ int cached_length(const Cache& c, int len) { return max(0, min(len, c.W << c.shift)); }
 
 }  // namespace paged
 }  // namespace mamf

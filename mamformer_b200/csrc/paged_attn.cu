@@ -130,13 +130,15 @@ __device__ __forceinline__ void set_range(const Params& p, Item& it) {
 }
 template <int ROWS>
 __device__ __forceinline__ bool set_sequence(const Params& p, Item& it, int b) {
+  const Cache& c = p.c;
+  const int t0 = c.cu[b], t1 = c.cu[b + 1], len = c.lens[b];
   it.b = b;
-  it.t0 = p.c.cu[b];
-  it.n = p.c.cu[b + 1] - it.t0;
-  if (it.n <= 0) return false;
+  it.t0 = t0;
+  it.n = t1 - t0;
+  if (t0 < 0 || t1 <= t0 || t1 > c.T) return false;             // what does not fit is the join kernel's to report
   it.rows = it.n * p.rep * p.maps;
-  if (it.rows > p.few) return false;                            // the chunk kernel's, or too_many
-  it.len = cached_length(p.c, b, &g_err);
+  if (it.rows > p.few) return false;
+  it.len = cached_length(c, len);
   it.g = it.rt = 0;
   set_range<ROWS>(p, it);
   return true;
@@ -161,11 +163,6 @@ __device__ __forceinline__ int64_t tiles_of(const Params& p, int b) {
       n += it.nt;
     }
   return n * p.c.G;
-}
-
-// More new tokens than the caller's max_new, by which this kernel was left to do it all.
-__device__ __forceinline__ bool too_many(const Params& p, int b) {
-  return !p.chunked && (int64_t)(p.c.cu[b + 1] - p.c.cu[b]) * p.rep * p.maps > p.few;
 }
 
 template <int HD> constexpr int stage_bytes() { return 2 * STEP * HD; }
@@ -219,38 +216,24 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
   // ---- this CTA's share [first, last) of the list of tiles ----
   const int chunk = (c.B + NT - 1) / NT;
   int64_t mine = 0;
-  bool odd = false;
+  bool broken = false;                              // offsets out of order: nothing is done here
   for (int i = 0; i < chunk; ++i) {
     const int b = tid * chunk + i;
     if (b < c.B) {
-      odd = odd || !in_order(c, b) || too_many(p, b);
       mine += tiles_of<ROWS>(p, b);
+      broken = broken || !in_order(c, b);
     }
   }
+  broken = __any_sync(0xffffffffu, broken);
   int64_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
-  if (lane == 31) s_pre[w] = incl;
+  if (lane == 31) s_pre[w] = broken ? 1LL << 60 : incl;
   if (tid == 0) { s_b = -1; s_cut = 0; }
-  if (__syncthreads_or(odd)) {
-    // sequences of too many tokens are left out and get zeros; offsets that are not in order give nothing but zeros
-    bool broken = false;
-    for (int b = tid; b < c.B; b += NT) broken = broken || !in_order(c, b);
-    broken = __syncthreads_or(broken);
-    if (tid == 0) record(ERR_LENGTH);
-    for (int t = blockIdx.x; t < c.T; t += gridDim.x) {
-      const int b = broken ? -1 : sequence_of(c.cu, c.B, t);
-      if (broken || (b >= 0 && too_many(p, b)))
-        for (int i = tid; i < p.H * HD; i += NT) ((T*)p.out)[(int64_t)t * p.H * HD + i] = from_f<T>(0.f);
-    }
-    if (broken) {
-      if (tid == 0) p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
-      return;
-    }
-  }
+  __syncthreads();
   int64_t total = 0, before = 0;
 #pragma unroll
   for (int i = 0; i < NW; ++i) {
@@ -281,7 +264,7 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
     for (int64_t i = end + (int64_t)blockIdx.x * NT + tid; i < c.T * row; i += (int64_t)gridDim.x * NT)
       ((T*)p.out)[i] = from_f<T>(0.f);
   }
-  if (first >= last) return;
+  if (first >= last || total >> 60) return;
 
   Item it;                                          // of the tile being computed
   set_sequence<ROWS>(p, it, s_b);
@@ -681,13 +664,37 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
   for (; waited < issued; ++waited) drain_tile(bar + waited % ST * 8, (uint32_t)(waited / ST & 1));
 }
 
+// What the split kernel has left out, by one block: offsets or lengths that do not fit are recorded, sequences of more
+// tokens than max_new get zeros, and offsets out of order give nothing but zeros.
+template <typename T>
+__device__ __noinline__ void left_out(const Params& p, int hd) {
+  const Cache& c = p.c;
+  auto too_many = [&](int b) { return !p.chunked && (int64_t)(c.cu[b + 1] - c.cu[b]) * p.rep * p.maps > p.few; };
+  bool broken = false, odd = false;
+  for (int b = threadIdx.x; b < c.B; b += NJ) {
+    broken = broken || !in_order(c, b);
+    odd = odd || too_many(b) || cached_length(c, c.lens[b]) != c.lens[b];
+  }
+  if (!__syncthreads_or(odd || broken)) return;
+  broken = __syncthreads_or(broken);
+  if (threadIdx.x == 0) record(ERR_LENGTH);
+  for (int t = 0; t < c.T; ++t) {
+    const int b = broken ? -1 : sequence_of(c.cu, c.B, t);
+    if (broken || (b >= 0 && too_many(b)))
+      for (int i = threadIdx.x; i < p.H * hd; i += NJ) ((T*)p.out)[(int64_t)t * p.H * hd + i] = from_f<T>(0.f);
+  }
+}
+
 // Joins the parts of an item that ran over several CTAs: block = the CTA in which it ended.
 template <typename T, int HD, int NR>
-__global__ void __launch_bounds__(NJ) join_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(NJ, 2) join_kernel(const __grid_constant__ Params p) {
   constexpr int ROWS = 8 * NR;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 j = p.joins[blockIdx.x];
-  if (j.x < 0) return;
+  if (j.x < 0) {
+    if (blockIdx.x == 0) left_out<T>(p, HD);          // no item ends in the first CTA that began before it
+    return;
+  }
   const int t0 = j.x, row0 = (j.z >> 16) * ROWS, n_rows = min(ROWS, j.y - row0), g = j.z & 0xffff;
   const int c0 = j.w >> 1, parts = blockIdx.x - c0 + 1, per = p.rep * p.maps;
   // the warps share the rows, and a row's warps its parts, each under a running maximum; the two maps of a head
@@ -697,43 +704,53 @@ __global__ void __launch_bounds__(NJ) join_kernel(const __grid_constant__ Params
   __shared__ float2 sums[W];                           // {maximum, sum}
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, r = w % n_rows, gr = w / n_rows, groups = W / n_rows;
   if (gr < groups) {
-    float M = NONE, L = 0.f, a[D] = {};
-    bool cut = false;
-#pragma unroll 8
-    for (int i = gr; i < parts; i += groups) {
-      const float* x = p.part + (((int64_t)(c0 + i) * 2 + (i == 0 ? j.w & 1 : 0)) * ROWS + r) * (HD + 2);
-      const float2 ml = *reinterpret_cast<const float2*>(x + HD);
-      float2 v[D / 2];
+    float M = NONE, L = 0.f, least = 0.f, a[D] = {};   // least: negative where a part was cut short
+    for (int i0 = gr; i0 < parts; i0 += 4 * groups) {   // four parts are on their way at once
+      float2 ml[4], v[4][D / 2];
 #pragma unroll
-      for (int d = 0; d < D / 2; ++d) v[d] = *reinterpret_cast<const float2*>(x + lane * D + 2 * d);
-      const float mn = fmaxf(M, ml.x), f = ex2(M - mn), e = ex2(ml.x - mn);
-      M = mn;
-      cut = cut || ml.y < 0.f;
-      L = fmaf(L, f, ml.y * e);
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * groups;
+        ml[u] = make_float2(NONE, 0.f);
 #pragma unroll
-      for (int d = 0; d < D / 2; ++d) {
-        a[2 * d] = fmaf(a[2 * d], f, v[d].x * e);
-        a[2 * d + 1] = fmaf(a[2 * d + 1], f, v[d].y * e);
+        for (int d = 0; d < D / 2; ++d) v[u][d] = make_float2(0.f, 0.f);
+        if (i < parts) {
+          const float* x = p.part + (((int64_t)(c0 + i) * 2 + (i == 0 ? j.w & 1 : 0)) * ROWS + r) * (HD + 2);
+          ml[u] = *reinterpret_cast<const float2*>(x + HD);
+#pragma unroll
+          for (int d = 0; d < D / 2; ++d) v[u][d] = *reinterpret_cast<const float2*>(x + lane * D + 2 * d);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float mn = fmaxf(M, ml[u].x), f = ex2(M - mn), e = ex2(ml[u].x - mn);
+        M = mn;
+        least = fminf(least, ml[u].y);
+        L = fmaf(L, f, ml[u].y * e);
+#pragma unroll
+        for (int d = 0; d < D / 2; ++d) {
+          a[2 * d] = fmaf(a[2 * d], f, v[u][d].x * e);
+          a[2 * d + 1] = fmaf(a[2 * d + 1], f, v[u][d].y * e);
+        }
       }
     }
 #pragma unroll
     for (int d = 0; d < D; ++d) vals[w][lane * D + d] = a[d];
-    if (lane == 0) sums[w] = make_float2(M, cut ? -1.f : L);
+    if (lane == 0) sums[w] = make_float2(M, least < 0.f ? -1.f : L);
   }
   __syncthreads();
   auto value = [&](int row, int d) {
     float M = NONE, L = 0.f, x = 0.f;
-    bool cut = false;                                // a part that a wait's end has cut short
+    float least = 0.f;
     for (int i = row; i < groups * n_rows; i += n_rows) {
       M = fmaxf(M, sums[i].x);
-      cut = cut || sums[i].y < 0.f;
+      least = fminf(least, sums[i].y);
     }
     for (int i = row; i < groups * n_rows; i += n_rows) {
       const float e = ex2(sums[i].x - M);
       x = fmaf(vals[i][d], e, x);
       L = fmaf(sums[i].y, e, L);
     }
-    return cut || L == 0.f ? 0.f : x / L;
+    return least < 0.f || L == 0.f ? 0.f : x / L;
   };
   for (int i = threadIdx.x; i < ROWS / p.maps * HD; i += NJ) {
     const int rr = i / HD * p.maps, d = i % HD;
@@ -771,7 +788,6 @@ void launch_split(const Params& p, const CUtensorMap& mk, const CUtensorMap& mv)
   }
   fn<<<p.ctas, NT, SMEM, stream()>>>(p, mk, mv);
   MAMF_LAUNCH_CHECK();
-  if (p.ctas == 1) return;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(p.ctas);
   cfg.blockDim = dim3(NJ);

@@ -109,9 +109,13 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
       ((T*)p.out)[i] = from_f<T>(0.f);
     if (blockIdx.x == gridDim.x - 1) {             // one CTA, of rows that see little, looks at all offsets
       bool odd = false;
-      for (int i = threadIdx.x; i < c.B; i += NT) odd = odd || !in_order(c, i);
+      bool long_one = false;
+      for (int i = threadIdx.x; i < c.B; i += NT) {
+        odd = odd || !in_order(c, i);
+        long_one = long_one || cached_length(c, c.lens[i]) != c.lens[i];
+      }
+      if (long_one || odd) atomicCAS(&g_err, 0, (int)ERR_LENGTH);
       if (__syncthreads_or(odd)) {                 // no unit may have some rows: none of the call's results count
-        if (threadIdx.x == 0) atomicCAS(&g_err, 0, (int)ERR_LENGTH);
         for (int64_t i = threadIdx.x; i < c.T * row; i += NT) ((T*)p.out)[i] = from_f<T>(0.f);
       }
     }
@@ -129,7 +133,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
       if ((int64_t)c.cu[mid] * p.rep / rows + mid <= u) b = mid; else hi = mid - 1;
     }
   }
-  const int t0 = c.cu[b], n = c.cu[b + 1] - t0, len = cached_length(c, b, &g_err);
+  const int t0 = c.cu[b], n = c.cu[b + 1] - t0, len = cached_length(c, c.lens[b]);
   const int64_t tile64 = u - ((int64_t)t0 * p.rep / rows + b);
   if (!in_order(c, b) || (int64_t)n * p.rep * p.maps <= p.few || tile64 < 0 || tile64 * rows >= (int64_t)n * p.rep) return;
   const int r0 = (int)tile64 * rows, total = n * p.rep;    // first row of the tile, rows of the sequence
@@ -507,11 +511,11 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__
     const float* x = p.part + ((unit * p.splits * 2 + s) * BM + row % BM) * (HD + 2);
     const int64_t step = (int64_t)2 * BM * (HD + 2);
     float M = NONE, L = 0.f, a[D] = {};
-    bool cut = false;
+    float least = 0.f;                             // negative where a part was cut short
 #pragma unroll 4
     for (int i = 0; i < p.splits; ++i, x += step) {
       const float2 ml = *reinterpret_cast<const float2*>(x + HD);
-      cut = cut || ml.y < 0.f;
+      least = fminf(least, ml.y);
       float2 v[D / 2];
 #pragma unroll
       for (int d = 0; d < D / 2; ++d) v[d] = *reinterpret_cast<const float2*>(x + lane * D + 2 * d);
@@ -524,7 +528,7 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__
         a[2 * d + 1] = fmaf(a[2 * d + 1], f, v[d].y * e);
       }
     }
-    if (cut) {                                     // of either map: the row is zeros
+    if (least < 0.f) {                             // of either map: the row is zeros
 #pragma unroll
       for (int d = 0; d < D; ++d) res[d] = 0.f;
       break;
