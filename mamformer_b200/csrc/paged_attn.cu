@@ -37,6 +37,7 @@ constexpr float NONE = -1e30f;                 // maximum of no scores: 2^(score
 // 158; one map, 8 sequences of 8000, 16 / 4 heads: 32 rows 55 and 78, 64 rows 83 and 94.
 constexpr int FEW = 64;
 constexpr float LAZY = 8.f;                    // log2 by which a row may outgrow its reference maximum
+constexpr float SLACK = 64.f;                  // value scales of up to this times O's unit are not looked at
 
 __device__ int g_err = 0, g_wait_err = 0;
 __device__ __forceinline__ void record(int code) { atomicCAS(&g_err, 0, code); }
@@ -336,8 +337,15 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
   float rs[NR][2];                        // score factor of rows 2 t4, 2 t4 + 1
   int lim[NR][2], low[NR][2];             // slots (low, lim] that the row sees
   int all_lo = 0, all_hi = 0;             // slots [all_lo, all_hi] that every row sees
+  // m: a row's running maximum of the scores, which l is kept in.  O is kept in units of 2^(m + off), off a whole number
+  // that brings m + off to the row's running maximum of score + log2 of the value scale: what a page of other values
+  // holds takes no bits from a row that gives it no weight.
   float m[NR][2], l[NR][2], o[NR][MT][4];
-  float vref = 0.f;
+  int noff[NR][2];                        // -off, as what it adds to the exponent bits of a scale
+  // 2^-off times a scale, between 0 and 2^126: keys of no weight may have any scale
+  auto ratio_of = [&](float vs, int nr, int x) {
+    return __int_as_float(__viaddmin_s32_relu((int)__float_as_uint(vs), noff[nr][x], 253 << 23));
+  };
   auto load_rows = [&]() {
     const int per = p.rep * p.maps, at0 = it.len - it.n;
     all_hi = min(it.len - 1, at0 + it.rt * ROWS / per);
@@ -387,13 +395,13 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
         low[nr][x] = rr < it.rows && p.window > 0 ? it.len - it.n + rr / per - p.window : -1;
         m[nr][x] = NONE;
         l[nr][x] = 0.f;
+        noff[nr][x] = 0;
       }
 #pragma unroll
       for (int j = 0; j < MT; ++j)
 #pragma unroll
         for (int x = 0; x < 4; ++x) o[nr][j][x] = 0.f;
     }
-    vref = 0.f;
   };
 
   // rows of this lane in the fragments: token tk (K) and tv[0], tv[1] (V), and the same + 8, which is
@@ -435,13 +443,15 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
         }
       }
   };
-  auto raise = [&](float (&s)[NR][4]) {
+  auto raise = [&](float (&s)[NR][4], float vs) {
     bool grow = false;
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-      for (int x = 0; x < 2; ++x) grow = grow || fmaxf(s[nr][x], s[nr][x + 2]) > m[nr][x] + LAZY;
+      for (int x = 0; x < 2; ++x)
+        grow = grow || fmaxf(s[nr][x], s[nr][x + 2]) > m[nr][x] + LAZY || ratio_of(vs, nr, x) > SLACK;
     if (!__any_sync(0xffffffffu, grow)) return;
+    const float lv = (float)((int)(__float_as_uint(vs) >> 23) - 127);
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
@@ -450,34 +460,19 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        if (mx > m[nr][x]) {
-          const float f = ex2(m[nr][x] - mx);
-          m[nr][x] = mx;
-          l[nr][x] *= f;
+        const float m0 = m[nr][x], off = (float)(-(noff[nr][x] >> 23)), m1 = fmaxf(m0, mx);
+        const float to = mx + lv > m0 + off ? mx + lv : m0 + off;
+        const float u1 = fminf(fmaxf(rintf(to - m1), -126.f), 126.f);
+        const float f = ex2((m0 - m1) + (off - u1));
+        l[nr][x] *= ex2(m0 - m1);
+        m[nr][x] = m1;
+        noff[nr][x] = -((int)u1 << 23);
 #pragma unroll
-          for (int j = 0; j < MT; ++j) { o[nr][j][x] *= f; o[nr][j][x + 2] *= f; }
-        }
+        for (int j = 0; j < MT; ++j) { o[nr][j][x] *= f; o[nr][j][x + 2] *= f; }
       }
   };
-  // P V of one tile.  O is in units of vref; a block whose scale is within 2^6 of it goes in through P (at
-  // most 2^14 then), a larger or smaller one changes vref, and one below 2^-60 of it is below O's last bit.
+  // P V of one tile.  The weights that enter it are at most 2^LAZY * SLACK.
   auto values = [&](uint32_t vb, float vs, int slot0, float (&s)[NR][4]) {
-    float ratio = 1.f;
-    if (vs != vref) {
-      if (vref == 0.f) vref = vs;
-      else if (vs > vref * 64.f || (vs < vref * 0.015625f && vs > vref * 8.6736174e-19f)) {
-        const float f = vref / vs;
-#pragma unroll
-        for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-          for (int j = 0; j < MT; ++j)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) o[nr][j][x] *= f;
-        vref = vs;
-      } else if (vs > vref * 8.6736174e-19f) {
-        ratio = __uint_as_float(__float_as_uint(vs) - __float_as_uint(vref) + (127u << 23));      // powers of two
-      } else ratio = 0.f;
-    }
     uint32_t pf[NR][2];
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
@@ -486,9 +481,10 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
       for (int x = 0; x < 4; ++x) {
         e[x] = ex2(s[nr][x] - m[nr][x & 1]);
         l[nr][x & 1] += e[x];
+        e[x] *= ratio_of(vs, nr, x & 1);
       }
-      pf[nr][0] = transposed(pack_h2(e[0] * ratio, e[1] * ratio));
-      pf[nr][1] = transposed(pack_h2(e[2] * ratio, e[3] * ratio));
+      pf[nr][0] = transposed(pack_h2(e[0], e[1]));
+      pf[nr][1] = transposed(pack_h2(e[2], e[3]));
     }
     // O^T: tokens tv[0], tv[1] and the same + 8, dims HD / 8 * g8 ..
     uint32_t vw[4][HD / 32];
@@ -529,12 +525,17 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
   // Warps 3, 2, 1 pass their joined state on through shared memory, lane by lane; warp 0 writes the result.
   float* merge = reinterpret_cast<float*>(smem + NW * ST * SB) + lane;
   auto finish = [&](int64_t item_start, bool ends) {
+    float unit[NR][2];
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) unit[nr][x] = __int_as_float((127 << 23) - noff[nr][x]);
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
       for (int j = 0; j < MT; ++j)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) o[nr][j][x] *= vref;
+        for (int x = 0; x < 4; ++x) o[nr][j][x] *= unit[nr][x & 1];
 #pragma unroll 1
     for (int turn = NW - 1; turn >= 0; --turn) {
       if (w == turn && turn < NW - 1) {
@@ -639,7 +640,7 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
     if (ok && ksr[0] != 0.f) {
       float s[NR][4];
       scores(here, ksr[0], slot0, s);
-      raise(s);
+      raise(s, vsr[0]);
       values(here + STEP * HD, vsr[0], slot0, s);
     }
     __syncwarp();                                  // the tile is read before its place is filled again

@@ -280,3 +280,28 @@ def test_parts_of_values_of_any_size(gain, new, lens):
     cache, table = filled(lens, 16, 2, 64, "cuda", gain)
     q = rand((sum(new), 4, 64), torch.bfloat16, "cuda", 3)
     close(ops.paged_attention(q, cache, table, offsets(new, "cuda"), i32(lens, "cuda"), max(new)), *plain(q, cache, table, new, lens))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("new,window", [([3], 120), ([16], 130), ([60], 130)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_a_window_hides_huge_values(dev, new, window, hd):
+    """The first rows of a tile see the end of a page of huge values, the others do not."""
+    lens = [new[0] + 134]
+    cache, table = filled(lens, 16, 1, hd, dev, [2.0 ** 90] + [1.0, 2.0 ** -10] * 6)
+    q = rand((sum(new), 2, hd), torch.bfloat16, dev, 3)
+    got = ops.paged_attention(q, cache, table, offsets(new, dev), i32(lens, dev), max(new), window=window)
+    close(got, *plain(q, cache, table, new, lens, window=window))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_keys_without_weight_have_huge_values(dev):
+    """Scores push the pages of huge values below fp32's smallest weight; what is left are the other pages' values."""
+    lens, hd = [150], 64
+    table, P = tables(lens, 16, dev)
+    cache = pool(P, 1, 16, hd, dev)
+    k, v = rand((150, 1, hd), torch.float32, dev, 1), rand((150, 1, hd), torch.float32, dev, 2)
+    k[:64], v[:64] = -20.0, v[:64] * 2.0 ** 100
+    ops.kv_append(k, v, cache, table, offsets(lens, dev), i32(lens, dev), 150)
+    q = torch.full((1, 2, hd), 1.0, dtype=torch.bfloat16, device=dev)
+    close(ops.paged_attention(q, cache, table, offsets([1], dev), i32(lens, dev), 1), *plain(q, cache, table, [1], lens))
