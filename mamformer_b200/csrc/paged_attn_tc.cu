@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
     float ks = 0.f, vs = 0.f;                                // of group lane % 4
     auto look_up = [&](int j) {                              // the page of group lane % 4 of tile j
       const int slot = (kt0 + j) * BN + (lane & 3) * 16;
-      if (j >= ntile || slot >= key_hi) return -2;
+      if (j >= ntile || slot >= key_hi || slot + 16 <= key_lo) return -2;      // nothing to see there: no page is asked for
       const int w = slot >> c.shift;
       const int pg = w < c.W ? c.table[(int64_t)b * c.W + w] : -1;
       return (unsigned)pg < (unsigned)c.P ? pg : -1;

@@ -288,7 +288,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, 
     """Causal attention of packed queries (T, H, hd) over the paged cache, H / G query heads per KV head -> (T, H, hd).
 
     Arguments as in :func:`kv_append`, called after it: query i of a sequence's n sees slots up to
-    kv_lens - n + i, with ``window`` > 0 only the last ``window`` of them.  With ``q2`` and ``lam`` (H,) fp32, the
+    kv_lens - n + i, with ``window`` > 0 only the last ``window`` of them; block table entries of pages below that may be
+    anything.  With ``q2`` and ``lam`` (H,) fp32, the
     differential form (softmax(q k) v - lam softmax(q2 k) v) / (1 - lam + 1e-8).  A query that sees nothing, and
     rows past cu_seqlens[-1], give 0.  No gradient."""
     _no_gradient("paged_attention", q) if q2 is None or lam is None else _no_gradient("paged_attention", q, q2, lam)

@@ -434,14 +434,15 @@ def paged_attention(q, cache, block_table, cu_seqlens, kv_lens, q2, lam, window,
         n = cu[b + 1] - cu[b]
         if n == 0:
             continue
-        pages = block_table[b, :(L + page - 1) // page].long()
+        below = max(0, L - n - window + 1) // page if window > 0 else 0       # pages that no query sees
+        pages = block_table[b, below:(L + page - 1) // page].long()
 
         def held(codes, s):
             x = codes.view(torch.uint8)[pages].view(torch.float8_e4m3fn).to(acc) * s[pages][..., None, None].to(acc)
-            return x.transpose(0, 1).reshape(G, -1, x.shape[-1])[:, :L].repeat_interleave(q.shape[1] // G, 0)
+            return x.transpose(0, 1).reshape(G, -1, x.shape[-1])[:, :L - below * page].repeat_interleave(q.shape[1] // G, 0)
 
         kx, vx = held(cache.k, cache.k_scale), held(cache.v, cache.v_scale)
-        dist = torch.arange(L - n, L, device=q.device)[:, None] - torch.arange(L, device=q.device)
+        dist = torch.arange(L - n, L, device=q.device)[:, None] - torch.arange(below * page, L, device=q.device)
         hide = (dist < 0) | (dist >= window) if window > 0 else dist < 0
         maps = []
         for x in (q,) if q2 is None else (q, q2):

@@ -305,3 +305,25 @@ def test_keys_without_weight_have_huge_values(dev):
     ops.kv_append(k, v, cache, table, offsets(lens, dev), i32(lens, dev), 150)
     q = torch.full((1, 2, hd), 1.0, dtype=torch.bfloat16, device=dev)
     close(ops.paged_attention(q, cache, table, offsets([1], dev), i32(lens, dev), 1), *plain(q, cache, table, [1], lens))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("page,window", [(16, 40), (32, 33), (64, 70)])
+@pytest.mark.parametrize("diff", [False, True])
+@pytest.mark.parametrize("new,lens", [([1, 2], [300, 170]), ([90, 150], [300, 170]), ([90], [2500])])
+def test_pages_below_a_window_may_be_given_back(dev, page, window, diff, new, lens):
+    """Pages that no query sees: another sequence's now, here full of NaN, or no page at all."""
+    from mamformer_b200.fault import check_device_status
+    cache, table = filled(lens, page, 2, 128, dev)
+    P = cache.k.shape[0]
+    unused = min(set(range(P)) - set(table.flatten().tolist()))
+    q = rand((sum(new), 4, 128), torch.bfloat16, dev, 3)
+    kw = dict(pair(q, diff), window=window)
+    want, tol = plain(q, cache, table, new, lens, **kw)
+    check_device_status()
+    for gone in (unused, -1, P + 5):
+        t = table.clone()
+        for b, (n, L) in enumerate(zip(new, lens)):
+            t[b, :max(0, L - n + 1 - window) // page] = gone
+        close(ops.paged_attention(q, cache, t, offsets(new, dev), i32(lens, dev), max(new), **kw), want, tol)
+        check_device_status()
