@@ -93,11 +93,11 @@ std::vector<at::Tensor> kv_append(at::Tensor k, at::Tensor v, at::Tensor ck, at:
                                   at::Tensor table, at::Tensor cu, at::Tensor lens, int64_t max_new,
                                   c10::optional<at::Tensor> cos, c10::optional<at::Tensor> sin,
                                   c10::optional<at::Tensor> pos, std::vector<at::Tensor> queries);
-int64_t kv_append_error();
+int64_t kv_append_error(bool clear);
 at::Tensor paged_attention(at::Tensor q1, c10::optional<at::Tensor> q2, c10::optional<at::Tensor> lam, at::Tensor ck,
                            at::Tensor cv, at::Tensor ks, at::Tensor vs, at::Tensor table, at::Tensor cu, at::Tensor lens,
                            int64_t max_new, int64_t window, double scale);
-int64_t paged_attention_error();
+int64_t paged_attention_error(bool clear);
 int64_t paged_attention_wait_limit(int64_t cycles);
 void gemm_ag(std::vector<int64_t> a_ptrs, int64_t shard_rows, int64_t lda, int64_t rank, at::Tensor B, bool b_mn,
              at::Tensor D);
@@ -167,9 +167,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("token_scores_bwd", &mamf::token_scores_bwd);
   m.def("token_scores", &mamf::token_scores);
   m.def("kv_append", &mamf::kv_append);
-  m.def("kv_append_error", &mamf::kv_append_error);
+  m.def("kv_append_error", &mamf::kv_append_error, py::arg("clear") = true);
   m.def("paged_attention", &mamf::paged_attention);
-  m.def("paged_attention_error", &mamf::paged_attention_error);
+  m.def("paged_attention_error", &mamf::paged_attention_error, py::arg("clear") = true);
   m.def("paged_attention_wait_limit", &mamf::paged_attention_wait_limit);
   m.def("gemm_ag", &mamf::gemm_ag);
   m.def("gemm_rs", &mamf::gemm_rs);

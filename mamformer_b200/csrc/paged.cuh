@@ -16,7 +16,7 @@
 namespace mamf {
 namespace paged {
 
-// Codes of paged_error(): the access was skipped, nothing else was.
+// What the kernels record; *_error() gives the codes met since they were cleared, code c as bit c.
 enum : int { ERR_PAGE = 1, ERR_LENGTH = 2, ERR_POSITION = 3, ERR_WAIT = 4 };
 
 struct Cache {
@@ -71,7 +71,15 @@ constexpr long long WAIT_CYCLES = 500000000LL;
 // csrc/paged_attn_tc.cu: sequences of more than `few` rows (of any number where few is 0, and then rows past
 // the last sequence are cleared too)
 void paged_chunk_attention(const Attn& p, int hd, bool bf16);
-int paged_chunk_error();
+int64_t paged_chunk_error(bool clear);
+
+// The code in a device word, 0 or one of the above, as a bit.
+template <typename Word> inline int64_t take_code(Word& word, bool clear) {
+  int v = 0, z = 0;
+  MAMF_CUDA_CHECK(cudaMemcpyFromSymbol(&v, word, sizeof(int)));
+  if (v && clear) MAMF_CUDA_CHECK(cudaMemcpyToSymbol(word, &z, sizeof(int)));
+  return v ? 1LL << v : 0;
+}
 
 // A tensor whose rows of adjacent values start on 16-byte boundaries: t itself, or a copy of it.
 inline at::Tensor rows16(const at::Tensor& t) {

@@ -879,14 +879,8 @@ at::Tensor paged_attention(at::Tensor q1, c10::optional<at::Tensor> q2, c10::opt
   return out;
 }
 
-int64_t paged_attention_error() {
-  int v = 0, w = 0, z = 0;
-  MAMF_CUDA_CHECK(cudaMemcpyFromSymbol(&v, pa::g_err, sizeof(int)));
-  MAMF_CUDA_CHECK(cudaMemcpyFromSymbol(&w, pa::g_wait_err, sizeof(int)));
-  if (v) MAMF_CUDA_CHECK(cudaMemcpyToSymbol(pa::g_err, &z, sizeof(int)));
-  if (w) MAMF_CUDA_CHECK(cudaMemcpyToSymbol(pa::g_wait_err, &z, sizeof(int)));
-  const int t = paged::paged_chunk_error();
-  return w ? w : v ? v : t;
+int64_t paged_attention_error(bool clear) {
+  return paged::take_code(pa::g_err, clear) | paged::take_code(pa::g_wait_err, clear) | paged::paged_chunk_error(clear);
 }
 
 }  // namespace mamf

@@ -577,14 +577,7 @@ void paged_chunk_attention(const Attn& p, int hd, bool bf16) {
   if (bf16) { if (hd == 128) ptc::launch<__nv_bfloat16, 128>(p); else ptc::launch<__nv_bfloat16, 64>(p); }
   else { if (hd == 128) ptc::launch<__half, 128>(p); else ptc::launch<__half, 64>(p); }
 }
-int paged_chunk_error() {
-  int v = 0, w = 0, z = 0;
-  MAMF_CUDA_CHECK(cudaMemcpyFromSymbol(&v, ptc::g_err, sizeof(int)));
-  MAMF_CUDA_CHECK(cudaMemcpyFromSymbol(&w, ptc::g_wait_err, sizeof(int)));
-  if (v) MAMF_CUDA_CHECK(cudaMemcpyToSymbol(ptc::g_err, &z, sizeof(int)));
-  if (w) MAMF_CUDA_CHECK(cudaMemcpyToSymbol(ptc::g_wait_err, &z, sizeof(int)));
-  return w ? w : v;
-}
+int64_t paged_chunk_error(bool clear) { return take_code(ptc::g_err, clear) | take_code(ptc::g_wait_err, clear); }
 }  // namespace paged
 
 }  // namespace mamf

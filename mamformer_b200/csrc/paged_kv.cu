@@ -388,14 +388,6 @@ std::vector<at::Tensor> kv_append(at::Tensor k, at::Tensor v, at::Tensor ck, at:
   return outs;
 }
 
-int64_t kv_append_error() {
-  int v = 0;
-  MAMF_CUDA_CHECK(cudaMemcpyFromSymbol(&v, kva::g_err, sizeof(int)));
-  if (v) {
-    int z = 0;
-    MAMF_CUDA_CHECK(cudaMemcpyToSymbol(kva::g_err, &z, sizeof(int)));
-  }
-  return v;
-}
+int64_t kv_append_error(bool clear) { return paged::take_code(kva::g_err, clear); }
 
 }  // namespace mamf

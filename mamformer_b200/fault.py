@@ -71,8 +71,6 @@ def check_device_status(clear: bool = True) -> None:
         fn = getattr(C, name, None)
         if fn is not None:
             attn = attn or int(fn())
-    # the paged-cache kernels' words; also cleared by the read itself
-    paged = int(C.kv_append_error()) or int(C.paged_attention_error())
     if comm:
         raise CommTimeoutError(f"cross-GPU barrier timed out waiting for peer {comm - 100}")
     if gemm:
@@ -80,12 +78,26 @@ def check_device_status(clear: bool = True) -> None:
     if attn:
         raise KernelTimeoutError(f"tcgen05 attention kernel reported code {attn} "
                                  "(a pipeline wait timed out, or a checked index was out of range)")
-    if paged == 4:
-        raise KernelTimeoutError("paged attention: a pipeline wait timed out")
-    if paged:
-        what = {1: "a block table entry that is not a page of the pool", 2: "lengths that do not fit the new tokens",
-                3: "a position outside the rotation tables"}.get(paged, f"code {paged}")
-        raise PagedCacheError(f"paged KV cache: {what}")
+    check_paged_status(clear)
+
+
+_PAGED_CODES = {1: "a block table entry that is not a page of the pool", 2: "lengths that do not fit the new tokens",
+                3: "a position outside the rotation tables", 4: "a pipeline wait timed out"}
+
+
+def check_paged_status(clear: bool = True) -> None:
+    """Raise if a paged-cache kernel of the current GPU recorded a timeout or a skipped access; ``clear`` forgets all
+    that was recorded, of both operators."""
+    from mamformer_b200.ops._ext import ext
+    C = ext()
+    if C is None or not torch.cuda.is_available():
+        return
+    append, attention = int(C.kv_append_error(clear)), int(C.paged_attention_error(clear))
+    codes = [c for c in range(1, 32) if (append | attention) >> c & 1]
+    if not codes:
+        return
+    what = "; ".join(_PAGED_CODES.get(c, f"code {c}") for c in reversed(codes))
+    raise (KernelTimeoutError if 4 in codes else PagedCacheError)(f"paged KV cache: {what}")
 
 
 class Heartbeat:

@@ -327,3 +327,69 @@ def test_pages_below_a_window_may_be_given_back(dev, page, window, diff, new, le
             t[b, :max(0, L - n + 1 - window) // page] = gone
         close(ops.paged_attention(q, cache, t, offsets(new, dev), i32(lens, dev), max(new), **kw), want, tol)
         check_device_status()
+
+
+@pytest.mark.gpu
+def test_one_check_reads_every_word():
+    """The append and both attention kernels have recorded something; with clear=False it stays."""
+    from mamformer_b200.fault import KernelTimeoutError, PagedCacheError, check_device_status
+    from mamformer_b200.ops._ext import require_native
+    C = require_native()
+    check_device_status()
+    cache, table = filled([40, 300], 16, 1, 64, "cuda")
+    q = rand((101, 2, 64), torch.bfloat16, "cuda", 1)
+    kv = rand((2, 1, 64), torch.bfloat16, "cuda", 2)
+    bad = table.clone()
+    bad[:, 2] = -1
+    two, both = offsets([1, 1], "cuda"), i32([40, 300], "cuda")
+
+    had = C.paged_attention_wait_limit(0)
+    C.paged_attention_wait_limit(had)
+    for timeout, error in ((False, PagedCacheError), (True, KernelTimeoutError)):
+        ops.kv_append(kv, kv, cache, bad, two, i32([40, 40], "cuda"), 1)
+        ops.paged_attention(q[:2], cache, bad, two, both, 1)
+        if timeout:
+            C.paged_attention_wait_limit(-1)
+        try:
+            ops.paged_attention(q, cache, table, offsets([1, 100], "cuda"), both, 100)
+            torch.cuda.synchronize()
+        finally:
+            C.paged_attention_wait_limit(had)
+        for _ in range(2):
+            with pytest.raises(error, match="page of the pool"):
+                check_device_status(clear=False)
+        with pytest.raises(error, match="page of the pool"):
+            check_device_status()
+        check_device_status()
+
+
+@pytest.mark.parametrize("comm,gemm", [(101, 0), (0, 7)])
+def test_an_earlier_error_leaves_the_paged_words(monkeypatch, comm, gemm):
+    """Another kernel's error is raised first; the paged ones are there for the next check.  (The words are fakes.)"""
+    from mamformer_b200 import fault
+    from mamformer_b200.ops import _ext
+    words = {"comm": comm, "gemm": gemm, "append": 1 << 1, "attention": 1 << 4}
+
+    class Fake:
+        comm_error = staticmethod(lambda: words["comm"])
+        gemm_error = staticmethod(lambda: words["gemm"])
+        comm_clear_error = staticmethod(lambda: words.update(comm=0))
+        gemm_clear_error = staticmethod(lambda: words.update(gemm=0))
+
+    def read(name):
+        def f(clear=True):
+            v = words[name]
+            if clear:
+                words[name] = 0
+            return v
+        return staticmethod(f)
+
+    Fake.kv_append_error, Fake.paged_attention_error = read("append"), read("attention")
+    monkeypatch.setattr(_ext, "ext", lambda: Fake)
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    with pytest.raises(fault.CommTimeoutError if comm else fault.KernelTimeoutError, match="peer 1" if comm else "GEMM"):
+        fault.check_device_status()
+    for clear in (False, True):
+        with pytest.raises(fault.KernelTimeoutError, match="timed out; a block table entry"):
+            fault.check_device_status(clear)
+    fault.check_device_status()
