@@ -17,6 +17,7 @@ import os
 from typing import List, NamedTuple, Optional, Sequence
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 import torch.nn.functional as F
 
 from mamformer_b200.ops import reference as ref
@@ -219,12 +220,19 @@ class TokenScores(NamedTuple):
 _SCORE_TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
+def _transformed() -> bool:
+    """Inside forward-mode differentiation or a torch.func transform, whose tensors a kernel call would take for plain
+    ones: their tangents would be lost."""
+    return forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active()
+
+
 def token_scores(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, temperature: float = 1.0,
                  ignore_index: int = -100) -> TokenScores:
     """Under p = softmax(logits / temperature): log p of ``targets``, the entropy of p, and the ``top_k`` (at most
     32) most likely tokens with their log probabilities, ties to the lower id.
 
-    logits (.., V) bf16 / f16 / fp32 (other types run the eager form), targets (..) int64.  Differentiable in all three scores.  Rows whose target is
+    logits (.., V) bf16 / f16 / fp32 (other types run the eager form, and so do forward-mode differentiation
+    and torch.func transforms), targets (..) int64.  Differentiable once in all three scores.  Rows whose target is
     ``ignore_index`` give 0, ids -1 and no gradient, and are not read; a logit of -inf has probability 0; a row of
     -inf only gives log probabilities of -inf, entropy 0 and no gradient."""
     shape = logits.shape
@@ -234,14 +242,14 @@ def token_scores(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, te
         raise ValueError(f"token_scores: temperature must be positive, got {temperature}")
     if not (0 <= top_k <= 32 and top_k <= shape[-1]):
         raise ValueError(f"token_scores: top_k from 0 to {min(32, shape[-1])}, got {top_k}")
-    if _native(logits) and "token_scores" in NATIVE and logits.dtype in _SCORE_TYPES:
+    if _native(logits) and "token_scores" in NATIVE and logits.dtype in _SCORE_TYPES and not _transformed():
         return TokenScores(*_nat().token_scores(logits, targets, top_k, temperature, ignore_index))
     return TokenScores(*ref.token_scores(logits, targets, top_k, temperature, ignore_index))
 
 
 def token_log_probs(logits: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
     """log_softmax(logits)[..., target] without materialising the full log-softmax; 0 where the target is -100."""
-    if _native(logits) and "token_scores" in NATIVE and logits.dtype in _SCORE_TYPES:
+    if _native(logits) and "token_scores" in NATIVE and logits.dtype in _SCORE_TYPES and not _transformed():
         return _nat().token_scores(logits, targets, 0, 1.0, -100)[0]
     lf = logits.float()
     lp = lf.gather(-1, targets.masked_fill(targets == -100, 0).unsqueeze(-1)).squeeze(-1) - torch.logsumexp(lf, dim=-1)
@@ -261,6 +269,10 @@ def _no_gradient(what: str, *tensors: torch.Tensor) -> None:
         for t in tensors:
             if t.requires_grad:
                 raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
+    if _transformed():
+        for t in tensors:
+            if torch._C._functorch.is_functorch_wrapped_tensor(t) or forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} has no gradient: neither forward-mode differentiation nor torch.func transforms")
 
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, cu_seqlens: torch.Tensor,

@@ -1,0 +1,78 @@
+"""ops.token_scores and ops.token_log_probs where they can go wrong: derivatives of other kinds than one backward pass,
+function transforms, targets outside the vocabulary, shapes.
+
+Tolerances: fp32 results of a few hundred terms of size 1, each to 2^-22: 1e-5."""
+
+import math
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+from mamformer_b200 import ops
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def rows(dev, R=5, V=300, dtype=torch.float32, seed=1):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(R, V, generator=g).to(dtype).to(dev)
+    t = torch.randint(0, V, (R,), generator=g).to(dev)
+    return x, t, torch.randn(R, V, generator=g).to(dtype).to(dev)
+
+
+def plain_log_probs(x, t):
+    return torch.log_softmax(x.double(), -1).gather(-1, t[..., None])[..., 0]
+
+
+def near(a, b):
+    assert a.shape == b.shape and ((a.double() - b.double()).abs() <= 1e-5).all()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_forward_mode_derivatives(dev):
+    x, t, dx = rows(dev)
+    p = torch.softmax(x.double(), -1)
+    want = dx.double().gather(-1, t[:, None])[:, 0] - (p * dx).sum(-1)
+    lp = torch.log_softmax(x.double(), -1)
+    want_ent = -(p * (dx - (p * dx).sum(-1, keepdim=True)) * (lp + 1)).sum(-1)
+    with fwd.dual_level():
+        d = fwd.make_dual(x, dx)
+        near(fwd.unpack_dual(ops.token_log_probs(d, t)).tangent, want)
+        s = ops.token_scores(d, t, top_k=2)
+        near(fwd.unpack_dual(s.log_probs).tangent, want)
+        near(fwd.unpack_dual(s.entropy).tangent, want_ent)
+        near(ops.token_log_probs(x, t), plain_log_probs(x, t))
+    out, tangent = torch.func.jvp(lambda z: ops.token_log_probs(z, t), (x,), (dx,))
+    near(out, plain_log_probs(x, t))
+    near(tangent, want)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_function_transforms(dev):
+    x, t, _ = rows(dev)
+    near(torch.func.vmap(ops.token_log_probs)(x, t), plain_log_probs(x, t))
+    near(torch.func.vmap(lambda a, b: ops.token_scores(a, b, top_k=3).log_probs)(x, t), plain_log_probs(x, t))
+    got = torch.func.grad(lambda z: ops.token_log_probs(z, t).sum())(x)
+    want, = torch.autograd.grad(plain_log_probs(z := x.double().requires_grad_(True), t).sum(), z)
+    near(got, want)
+    h = torch.func.hessian(lambda z: ops.token_log_probs(z, t[:1]).sum())(x[:1, :20].contiguous().clamp(-2, 2)) \
+        if t[0] < 20 else torch.func.hessian(lambda z: ops.token_log_probs(z, t[:1] * 0).sum())(x[:1, :20].contiguous())
+    assert h.shape == (1, 20, 1, 20) and h.isfinite().all() and h.abs().max() > 0
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_paged_operators_refuse_tangents_and_transforms(dev):
+    from test_paged_cache import filled, i32, offsets
+    cache, table = filled([5], 16, 1, 64, dev)
+    q = torch.ones(1, 2, 64, dtype=torch.bfloat16, device=dev)
+    k = torch.ones(1, 1, 64, dtype=torch.bfloat16, device=dev)
+    args = cache, table, offsets([1], dev), i32([5], dev), 1
+    with fwd.dual_level():
+        ops.paged_attention(q, *args)
+        with pytest.raises(RuntimeError, match="no gradient"):
+            ops.paged_attention(fwd.make_dual(q, q), *args)
+        with pytest.raises(RuntimeError, match="no gradient"):
+            ops.kv_append(fwd.make_dual(k, k), k, *args)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        torch.func.vmap(lambda x: ops.paged_attention(x, *args))(q[None])
