@@ -605,7 +605,50 @@ struct Scores : torch::autograd::Function<Scores> {
   }
 };
 
+// Log probabilities alone, differentiable any number of times: the first gradient is the kernel's, those of the
+// gradient are of torch's operations.
+struct LogProbsGrad : torch::autograd::Function<LogProbsGrad> {
+  static at::Tensor forward(AutogradContext* ctx, at::Tensor logits, at::Tensor target, at::Tensor stats, at::Tensor ent,
+                            at::Tensor top_id, at::Tensor g, int64_t ignore_index) {
+    ctx->save_for_backward({logits, target, g});
+    ctx->saved_data["ignore_index"] = ignore_index;
+    return token_scores_bwd(logits, target, ignore_index, 1.0, stats, ent, top_id, g, c10::nullopt, c10::nullopt);
+  }
+  // dx_j = g (d_jt - p_j): with w the gradient of dx, that of g is w_t - sum p w, that of x_j is -g p_j (w_j - sum p w)
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto v = ctx->get_saved_variables();
+    const at::Tensor &logits = v[0], &target = v[1], &g = v[2];
+    const int64_t V = logits.size(-1);
+    const at::Tensor live = (target != ctx->saved_data["ignore_index"].toInt()) & (target >= 0) & (target < V);
+    const at::Tensor w = grads[0].to(at::kFloat), p = at::softmax(logits.to(at::kFloat), -1);
+    const at::Tensor away = w - (p * w).sum(-1, true);
+    const at::Tensor dg = away.gather(-1, target.clamp(0, V - 1).unsqueeze(-1)).squeeze(-1);
+    const at::Tensor dx = -(g * live).unsqueeze(-1) * p * away, none;
+    return {dx.to(logits.scalar_type()), none, none, none, none, dg * live, none};
+  }
+};
+
+struct LogProbs : torch::autograd::Function<LogProbs> {
+  static at::Tensor forward(AutogradContext* ctx, at::Tensor logits, at::Tensor target, int64_t ignore_index) {
+    const auto r = token_scores_fwd(logits, target, ignore_index, 1.0, 0, true);
+    ctx->save_for_backward({logits, target, r[4], r[1], r[3]});
+    ctx->saved_data["ignore_index"] = ignore_index;
+    return r[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto v = ctx->get_saved_variables();
+    return {LogProbsGrad::apply(v[0], v[1], v[2], v[3], v[4], g[0].to(at::kFloat).contiguous(),
+                                ctx->saved_data["ignore_index"].toInt()),
+            at::Tensor(), at::Tensor()};
+  }
+};
+
 }  // namespace ts
+
+// -> log probabilities, differentiable in logits as often as needed
+at::Tensor token_log_probs(at::Tensor logits, at::Tensor target, int64_t ignore_index) {
+  return ts::LogProbs::apply(logits, target, ignore_index);
+}
 
 // -> log_probs, entropy, top_log_probs, top_ids, differentiable in logits
 std::vector<at::Tensor> token_scores(at::Tensor logits, at::Tensor target, int64_t ignore_index, double temperature,

@@ -250,7 +250,7 @@ def token_scores(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, te
 def token_log_probs(logits: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
     """log_softmax(logits)[..., target] without materialising the full log-softmax; 0 where the target is -100."""
     if _native(logits) and "token_scores" in NATIVE and logits.dtype in _SCORE_TYPES and not _transformed():
-        return _nat().token_scores(logits, targets, 0, 1.0, -100)[0]
+        return _nat().token_log_probs(logits, targets, -100)
     lf = logits.float()
     lp = lf.gather(-1, targets.masked_fill(targets == -100, 0).unsqueeze(-1)).squeeze(-1) - torch.logsumexp(lf, dim=-1)
     return lp.masked_fill(targets == -100, 0.0)

@@ -423,6 +423,13 @@ def token_scores(logits, targets, top_k, temperature, ignore_index):
     return _C.token_scores_fwd(logits, targets, ignore_index, temperature, top_k, False)
 
 
+def token_log_probs(logits, targets, ignore_index):
+    targets = targets.contiguous()
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _C.token_log_probs(logits, targets, ignore_index)
+    return _C.token_scores_fwd(logits, targets, ignore_index, 1.0, 0, False)[0]
+
+
 @_register("kv_append", "csrc/paged_kv.cu")
 def kv_append(k, v, cache, block_table, cu_seqlens, kv_lens, max_new, cos, sin, positions, queries):
     return _C.kv_append(k, v, *cache, block_table, cu_seqlens, kv_lens, max_new, cos, sin, positions, queries)

@@ -76,3 +76,39 @@ def test_paged_operators_refuse_tangents_and_transforms(dev):
             ops.kv_append(fwd.make_dual(k, k), k, *args)
     with pytest.raises(RuntimeError, match="no gradient"):
         torch.func.vmap(lambda x: ops.paged_attention(x, *args))(q[None])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_second_derivatives_of_log_probs(dev, dtype):
+    x, t, w = rows(dev, dtype=dtype)
+    t[2] = -100
+    g = torch.linspace(-1, 2, 5, device=dev)
+
+    def second(x, g, w, f, live):
+        d, = torch.autograd.grad(f(x)[live], x, g[live], create_graph=True)
+        return d, *torch.autograd.grad((d * w).sum(), (x, g))
+
+    live = t != -100
+    got = second(x.clone().requires_grad_(True), g.clone().requires_grad_(True), w, lambda z: ops.token_log_probs(z, t), live)
+    want = second(x.double().requires_grad_(True), g.double().requires_grad_(True), w.double(),
+                  lambda z: plain_log_probs(z, t.clamp(min=0)), live)
+    # bf16: the first gradient is rounded once (2^-8 of itself), and so is the second; their sums over w see sqrt(300) of those
+    for a, b in zip(got, want):
+        unit = 1e-5 if dtype == torch.float32 else 2.0 ** -7
+        assert ((a.double() - b).abs() <= unit * (1 + b.abs())).all()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_third_derivative_of_log_probs(dev):
+    x, t, w = rows(dev, R=2, V=9)
+
+    def third(x, f):
+        for _ in range(3):
+            x_, = torch.autograd.grad(f, x, create_graph=True)
+            f = (x_ * w.to(x.dtype)).sum()
+        return x_
+
+    a = x.clone().requires_grad_(True)
+    b = x.double().requires_grad_(True)
+    near(third(a, ops.token_log_probs(a, t).sum()), third(b, plain_log_probs(b, t).sum()))
