@@ -238,6 +238,8 @@ def token_scores(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, te
     shape = logits.shape
     if len(shape) < 1 or targets.shape != shape[:-1]:
         raise ValueError(f"token_scores: targets {tuple(targets.shape)} for logits {tuple(shape)}")
+    if targets.is_floating_point():
+        raise ValueError(f"token_scores: integer targets, got {targets.dtype}")
     if not temperature > 0:
         raise ValueError(f"token_scores: temperature must be positive, got {temperature}")
     if not (0 <= top_k <= 32 and top_k <= shape[-1]):
@@ -248,7 +250,11 @@ def token_scores(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, te
 
 
 def token_log_probs(logits: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
-    """log_softmax(logits)[..., target] without materialising the full log-softmax; 0 where the target is -100."""
+    """log_softmax(logits)[..., target] without materialising the full log-softmax; 0 where the target is -100.
+    targets (..) int64 for logits (.., V)."""
+    if targets.dtype != torch.int64 or targets.shape != logits.shape[:-1]:
+        raise ValueError(f"token_log_probs: int64 targets {tuple(logits.shape[:-1])} for logits {tuple(logits.shape)}, "
+                         f"got {targets.dtype} {tuple(targets.shape)}")
     if _native(logits) and "token_scores" in NATIVE and logits.dtype in _SCORE_TYPES and not _transformed():
         return _nat().token_log_probs(logits, targets, -100)
     lf = logits.float()

@@ -112,3 +112,15 @@ def test_third_derivative_of_log_probs(dev):
     a = x.clone().requires_grad_(True)
     b = x.double().requires_grad_(True)
     near(third(a, ops.token_log_probs(a, t).sum()), third(b, plain_log_probs(b, t).sum()))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_targets_of_another_shape_or_type_are_refused(dev):
+    x = torch.randn(2, 3, 11, device=dev)
+    for shape in ((6,), (3, 2), (2, 3, 1), (1, 3), ()):
+        for f in (ops.token_log_probs, ops.token_scores):
+            with pytest.raises(ValueError):
+                f(x, torch.zeros(shape, dtype=torch.long, device=dev))
+    for f in (ops.token_log_probs, ops.token_scores):
+        with pytest.raises(ValueError):
+            f(x, torch.zeros(2, 3, device=dev))
