@@ -86,6 +86,7 @@ std::vector<at::Tensor> token_scores_fwd(at::Tensor logits, at::Tensor target, i
                                          int64_t top_k, bool want_stats);
 std::vector<at::Tensor> token_scores(at::Tensor logits, at::Tensor target, int64_t ignore_index, double temperature,
                                      int64_t top_k);
+int64_t token_scores_error(bool clear);
 at::Tensor token_log_probs(at::Tensor logits, at::Tensor target, int64_t ignore_index);
 at::Tensor token_scores_bwd(at::Tensor logits, at::Tensor target, int64_t ignore_index, double temperature,
                             at::Tensor stats, at::Tensor ent, at::Tensor top_id, c10::optional<at::Tensor> g_lp,
@@ -167,6 +168,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("temperature"), py::arg("top_k"), py::arg("want_stats") = true);
   m.def("token_scores_bwd", &mamf::token_scores_bwd);
   m.def("token_scores", &mamf::token_scores);
+  m.def("token_scores_error", &mamf::token_scores_error, py::arg("clear") = true);
   m.def("token_log_probs", &mamf::token_log_probs);
   m.def("kv_append", &mamf::kv_append);
   m.def("kv_append_error", &mamf::kv_append_error, py::arg("clear") = true);

@@ -10,7 +10,8 @@
 // rows of the type's lowest value finite at every temperature.  A logit of -inf has probability 0 and
 // adds nothing to S1 (d is clamped at DMIN, where exp is 0).  A row of -inf only has no distribution:
 // its log probabilities are -inf, its entropy and gradient 0.  NaN and +inf make the row NaN.
-// Rows whose target is `ignore_index` (or outside the vocabulary) are not read: results 0, ids -1.
+// Rows whose target is `ignore_index` are not read: results 0, ids -1.  Nor are those of another target outside the
+// vocabulary: NaN, ids -1, no gradient, and an error word.
 //
 // 3686 x 128000 bf16: forward 160 us (5.9 TB/s; with 20 alternatives 210 us), gradient 311-328 us (5.9 TB/s).
 // DRAM bounds both, one exponential per logit (the MUFU at 60-70%) comes next.
@@ -26,6 +27,8 @@ constexpr int MAXK = 32;          // alternatives per row
 constexpr int CAP = 1024;         // candidates kept in shared memory for the selection
 constexpr float DMIN = -1e30f;
 constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ int g_err = 0;         // 1: a target outside the vocabulary
 
 struct Rows {                     // row r starts at base + (r / n1) * s0 + (r % n1) * s1 elements
   int64_t n1, s0, s1;
@@ -162,11 +165,13 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 3 : 5) scores_fwd_kernel(const
   const int64_t tgt = p.target[row];
   if (tgt == p.ignore || tgt < 0 || tgt >= p.V) {
     if (rank > 0) return;
+    const float none = tgt == p.ignore ? 0.f : NAN;
     if (tid == 0) {
-      p.lp[row] = 0.f; p.ent[row] = 0.f;
+      if (tgt != p.ignore) g_err = 1;
+      p.lp[row] = none; p.ent[row] = none;
       if (p.stats) { p.stats[2 * row] = -INFINITY; p.stats[2 * row + 1] = 0.f; }
     }
-    if (tid < p.k) { p.top_lp[row * p.k + tid] = 0.f; p.top_id[row * p.k + tid] = -1; }
+    if (tid < p.k) { p.top_lp[row * p.k + tid] = none; p.top_id[row * p.k + tid] = -1; }
     return;
   }
   const T* x = logits + p.rows.at(row);
@@ -507,6 +512,14 @@ void launch_fwd(const T* x, const FwdParams& p, int64_t R) {
 }
 
 }  // namespace ts
+
+// 1 where a target was outside the vocabulary since this was cleared
+int64_t token_scores_error(bool clear) {
+  int v = 0, z = 0;
+  MAMF_CUDA_CHECK(cudaMemcpyFromSymbol(&v, ts::g_err, sizeof(int)));
+  if (v && clear) MAMF_CUDA_CHECK(cudaMemcpyToSymbol(ts::g_err, &z, sizeof(int)));
+  return v;
+}
 
 // logits (.., V), up to two leading dimensions of any strides without a copy; target (..) int64.
 // -> log_probs, entropy (like target, fp32), top_log_probs, top_ids (.., k), and for the gradient stats (R, 2)

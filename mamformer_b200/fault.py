@@ -48,6 +48,10 @@ class PagedCacheError(RuntimeError):
     """A paged-cache kernel met a page, length or position out of range and skipped that access."""
 
 
+class TargetRangeError(RuntimeError):
+    """token_scores or token_log_probs met a target outside the vocabulary."""
+
+
 class RankFailureError(RuntimeError):
     """Another rank reported a failure or stopped sending heartbeats."""
 
@@ -79,6 +83,9 @@ def check_device_status(clear: bool = True) -> None:
         raise KernelTimeoutError(f"tcgen05 attention kernel reported code {attn} "
                                  "(a pipeline wait timed out, or a checked index was out of range)")
     check_paged_status(clear)
+    scores = getattr(C, "token_scores_error", None)
+    if scores is not None and int(scores(clear)):
+        raise TargetRangeError("token scores: a target outside the vocabulary (its scores are NaN)")
 
 
 _PAGED_CODES = {1: "a block table entry that is not a page of the pool", 2: "lengths that do not fit the new tokens",

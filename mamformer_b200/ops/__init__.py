@@ -234,7 +234,8 @@ def token_scores(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, te
     logits (.., V) bf16 / f16 / fp32 (other types run the eager form, and so do forward-mode differentiation
     and torch.func transforms), targets (..) int64.  Differentiable once in all three scores.  Rows whose target is
     ``ignore_index`` give 0, ids -1 and no gradient, and are not read; a logit of -inf has probability 0; a row of
-    -inf only gives log probabilities of -inf, entropy 0 and no gradient."""
+    -inf only gives log probabilities of -inf, entropy 0 and no gradient.  Another target outside the vocabulary
+    gives NaN, ids -1 and no gradient, and on the GPU ``fault.check_device_status`` raises afterwards."""
     shape = logits.shape
     if len(shape) < 1 or targets.shape != shape[:-1]:
         raise ValueError(f"token_scores: targets {tuple(targets.shape)} for logits {tuple(shape)}")
@@ -251,14 +252,21 @@ def token_scores(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, te
 
 def token_log_probs(logits: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
     """log_softmax(logits)[..., target] without materialising the full log-softmax; 0 where the target is -100.
-    targets (..) int64 for logits (.., V)."""
+    targets (..) int64 for logits (.., V).  A target outside the vocabulary is an error: on the GPU the result is NaN and
+    ``fault.check_device_status`` raises.  Differentiable any number of times; forward-mode differentiation and
+    torch.func transforms run the eager form."""
     if targets.dtype != torch.int64 or targets.shape != logits.shape[:-1]:
         raise ValueError(f"token_log_probs: int64 targets {tuple(logits.shape[:-1])} for logits {tuple(logits.shape)}, "
                          f"got {targets.dtype} {tuple(targets.shape)}")
     if _native(logits) and "token_scores" in NATIVE and logits.dtype in _SCORE_TYPES and not _transformed():
         return _nat().token_log_probs(logits, targets, -100)
     lf = logits.float()
-    lp = lf.gather(-1, targets.masked_fill(targets == -100, 0).unsqueeze(-1)).squeeze(-1) - torch.logsumexp(lf, dim=-1)
+    pick = targets.masked_fill(targets == -100, 0)
+    if logits.is_cuda:                                # an index out of range would fault there
+        pick = pick.clamp(0, logits.shape[-1] - 1)
+    lp = lf.gather(-1, pick.unsqueeze(-1)).squeeze(-1) - torch.logsumexp(lf, dim=-1)
+    if logits.is_cuda:
+        lp = torch.where(pick == targets, lp, math.nan)
     return lp.masked_fill(targets == -100, 0.0)
 
 

@@ -366,7 +366,9 @@ def token_scores(logits, targets, top_k: int, temperature: float, ignore_index: 
     """(log_probs, entropy, top_log_probs, top_ids); differentiable through autograd."""
     x = logits if logits.dtype == torch.float64 else logits.float()
     V = x.shape[-1]
-    live = (targets != ignore_index) & (targets >= 0) & (targets < V)
+    inside = (targets >= 0) & (targets < V)
+    live = (targets != ignore_index) & inside
+    rest = torch.where((targets != ignore_index) & ~inside, math.nan, 0.0).to(x.dtype)      # of rows that are not scored
     m = x.detach().amax(-1, keepdim=True)
     none = m == -math.inf
     u = torch.where(none, 0.0, x - m) / temperature
@@ -379,8 +381,8 @@ def token_scores(logits, targets, top_k: int, temperature: float, ignore_index: 
         torch.empty(*x.shape[:-1], 0, dtype=torch.long, device=x.device)
     pick = torch.cat([targets.clamp(0, V - 1).unsqueeze(-1), ids], -1)
     lp = torch.where(none, -math.inf, u.gather(-1, pick) - lse)
-    lp = torch.where(live.unsqueeze(-1), lp, 0.0)
-    return lp[..., 0], torch.where(live, ent, 0.0), lp[..., 1:], torch.where(live.unsqueeze(-1), ids, -1)
+    lp = torch.where(live.unsqueeze(-1), lp, rest.unsqueeze(-1))
+    return lp[..., 0], torch.where(live, ent, rest), lp[..., 1:], torch.where(live.unsqueeze(-1), ids, -1)
 
 
 def block_scale(amax: torch.Tensor) -> torch.Tensor:

@@ -124,3 +124,37 @@ def test_targets_of_another_shape_or_type_are_refused(dev):
     for f in (ops.token_log_probs, ops.token_scores):
         with pytest.raises(ValueError):
             f(x, torch.zeros(2, 3, device=dev))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_targets_outside_the_vocabulary_are_not_silent(dev):
+    """NaN in that row, no gradient from it, and on the GPU an error word."""
+    from mamformer_b200.fault import TargetRangeError, check_device_status
+    check_device_status()
+    x, t, _ = rows(dev)
+    good = ops.token_scores(x, t, top_k=2)
+    for bad in (300, -1, 1 << 40):
+        t2 = t.clone()
+        t2[3] = bad
+        x.requires_grad_(True)
+        s = ops.token_scores(x, t2, top_k=2)
+        assert s.log_probs[3].isnan() and s.entropy[3].isnan() and s.top_log_probs[3].isnan().all() and (s.top_ids[3] == -1).all()
+        keep = [0, 1, 2, 4]
+        for a, b in zip(s, good):
+            assert torch.equal(a[keep], b[keep])
+        d, = torch.autograd.grad(s.log_probs[keep].sum(), x)
+        assert (d[3] == 0).all() and d.isfinite().all()
+        x.requires_grad_(False)
+        if dev == "cuda":
+            with pytest.raises(TargetRangeError, match="vocabulary"):
+                check_device_status()
+            assert ops.token_log_probs(x.double(), t2)[3].isnan()
+            assert ops.token_log_probs(x, t2)[3].isnan()
+            with pytest.raises(TargetRangeError, match="vocabulary"):
+                check_device_status()
+        else:
+            with pytest.raises((RuntimeError, IndexError)):
+                ops.token_log_probs(x, t2)
+    t[1] = -100
+    assert ops.token_scores(x, t).log_probs[1] == 0
+    check_device_status()
