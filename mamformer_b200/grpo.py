@@ -27,6 +27,7 @@ from typing import List, Optional, Tuple
 
 import torch
 
+from mamformer_b200.fault import check_device_status
 from mamformer_b200.rewards import RewardCalculator
 from mamformer_b200.sgrpo import StochasticGRPOConfig, sample_token_mask
 
@@ -239,6 +240,10 @@ class GRPOTrainer:
         if self.global_step % c.grad_accum == 0:
             self.optimizer.zero_grad()
         (loss / c.grad_accum).backward()
+        if self.device.type == "cuda":                   # before the weights take what a kernel has given up on
+            torch.cuda.current_stream(self.device).synchronize()
+            with torch.cuda.device(self.device):
+                check_device_status()
         self.global_step += 1
         if self.global_step % c.grad_accum == 0:
             self.optimizer.step()

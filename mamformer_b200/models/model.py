@@ -445,6 +445,8 @@ class MamformerForCausalLM(GenerationMixin, nn.Module):
             generated = torch.cat([generated, nxt], dim=-1)
             if eos_token_id is not None:
                 alive = alive & (nxt.squeeze(-1) != eos_token_id)
+        if paged is not None:
+            paged.check()
         return generated
 
     @torch.no_grad()

@@ -9,7 +9,7 @@ power-of-two scale per page and KV head (:class:`mamformer_b200.ops.PagedKV`), o
     out = cache.layer(i).attend(q, k, v, cos, sin)   # per attention layer: append, then attend
 
 A layer's pages are allocated when it first attends.  Sequences may differ in length and in the number of new
-tokens; :meth:`release` gives a finished sequence's pages back.  What a page holds is rounded to 4 significant
+tokens; :meth:`release` gives a finished sequence's pages back; :meth:`check` raises what the kernels recorded.  What a page holds is rounded to 4 significant
 bits, so decoded logits differ from an unquantised cache's by that rounding.
 """
 
@@ -134,6 +134,15 @@ class PagedKVCache:
         self.block_table[b] = -1
         self.kv_lens = self.kv_lens.clone()
         self.kv_lens[b] = 0
+
+    def check(self) -> None:
+        """Wait for the steps so far and raise what their kernels recorded: PagedCacheError for a page, length or
+        position out of range, KernelTimeoutError.  :meth:`MamformerForCausalLM.generate` does so before it returns."""
+        if self.block_table.is_cuda:
+            from mamformer_b200.fault import check_paged_status
+            with torch.cuda.device(self.block_table.device):
+                torch.cuda.current_stream().synchronize()
+                check_paged_status()
 
     def _allocate(self, device) -> ops.PagedKV:
         shape = (self.n_pages, self.n_kv_heads, self.page_size, self.head_dim)

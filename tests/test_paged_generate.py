@@ -220,3 +220,46 @@ def test_refusals():
         att(x, use_cache=True, cache=cache)
     with torch.no_grad(), pytest.raises(ValueError, match="rows"):
         att(x[:, :1], use_cache=True, cache=cache)
+
+
+@pytest.mark.gpu
+def test_errors_on_the_device_reach_the_caller(monkeypatch):
+    """A page outside the pool is raised by generate and by a GRPO step, which leaves the weights alone."""
+    from mamformer_b200.fault import PagedCacheError, check_device_status
+    from mamformer_b200.grpo import GRPOConfig, GRPOTrainer
+    from mamformer_b200.tokenizer import MamformerTokenizer
+    from mamformer_b200.utils.precision import to_compute_dtype
+    torch.manual_seed(1)
+    check_device_status()
+    cfg = small_config()
+    model = MamformerForCausalLM(cfg).eval().cuda()
+    trainer = GRPOTrainer(model, MamformerTokenizer(), GRPOConfig(group_size=2, gen_max_tokens=3), compute_dtype=torch.bfloat16)
+    before = [p.detach().clone() for p in trainer.policy.parameters()]
+    batch = {"input_ids": torch.randint(0, 200, (2, 9)), "ground_truth": ["4", "5"], "reward_type": ["math", "math"],
+             "test_cases": [[], []], "reward_weights": [None, None]}
+    score = trainer.score
+    spoiled = PagedKVCache(1, 1, 64, 1, 10)
+
+    def spoil(*args):
+        spoiled.extend(1)
+        q = torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16, device="cuda")
+        spoiled.block_table.fill_(-1)
+        with torch.no_grad():
+            spoiled.layer(0).attend(q, q[:, :, :1], q[:, :, :1], torch.ones(1, 32, device="cuda"), torch.zeros(1, 32, device="cuda"))
+        return score(*args)
+
+    monkeypatch.setattr(trainer, "score", spoil)
+    with pytest.raises(PagedCacheError, match="page of the pool"):
+        trainer.step(batch)
+    assert all(torch.equal(a, b) for a, b in zip(before, trainer.policy.parameters()))
+    extend = PagedKVCache.extend
+
+    def broken(self, new):
+        extend(self, new)
+        self.block_table.fill_(-1)
+
+    monkeypatch.setattr(PagedKVCache, "extend", broken)
+    half = to_compute_dtype(MamformerForCausalLM(cfg).eval(), torch.bfloat16).cuda()
+    with pytest.raises(PagedCacheError, match="page of the pool"):
+        half.generate(torch.randint(0, 200, (2, 9), device="cuda"), max_new_tokens=2, temperature=0.0, kv_cache="paged")
+    check_device_status()
