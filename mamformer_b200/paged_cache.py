@@ -80,13 +80,18 @@ class PagedKVCache:
     @classmethod
     def for_model(cls, model, batch: int, max_len: int, page_size: int = 64) -> "PagedKVCache":
         """A cache with a place for every layer of a Mamformer model."""
-        c = model.config
+        heads = set()                                            # of the modules: a tensor-parallel rank holds its share
         for layer in model.model.layers:
             att = layer.attention
+            if att is None:
+                continue
             full = getattr(att, "full_attn", att)
+            heads.add((full.n_kv_heads, full.head_dim))
             if getattr(full, "sliding_window", 0) > 0 and full.window_mode != "causal":
                 raise ValueError("the paged cache attends causally: sliding windows need window_mode='causal'")
-        return cls(len(model.model.layers), c.n_kv_heads, c.head_dim, batch, max_len, page_size,
+        if len(heads) != 1:
+            raise ValueError(f"the paged cache takes layers of one number and size of KV heads, got {sorted(heads)}")
+        return cls(len(model.model.layers), *heads.pop(), batch, max_len, page_size,
                    device=next(model.parameters()).device)
 
     def layer(self, i: int) -> PagedLayer:

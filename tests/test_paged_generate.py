@@ -263,3 +263,15 @@ def test_errors_on_the_device_reach_the_caller(monkeypatch):
     with pytest.raises(PagedCacheError, match="page of the pool"):
         half.generate(torch.randint(0, 200, (2, 9), device="cuda"), max_new_tokens=2, temperature=0.0, kv_cache="paged")
     check_device_status()
+
+
+def test_a_tensor_parallel_rank_holds_its_heads():
+    model = MamformerForCausalLM(small_config())
+    for layer in model.model.layers:
+        att = getattr(layer, "attention", None)
+        if att is not None:
+            att.full_attn.n_kv_heads = 7                              # what sharding leaves on the module
+    assert PagedKVCache.for_model(model, 1, 10).n_kv_heads == 7
+    model.model.layers[0].attention.full_attn.n_kv_heads = 3
+    with pytest.raises(ValueError, match="one number"):
+        PagedKVCache.for_model(model, 1, 10)
