@@ -312,6 +312,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, 
                     kv_lens: torch.Tensor, max_new: int, q2: Optional[torch.Tensor] = None,
                     lam: Optional[torch.Tensor] = None, window: int = 0, scale: Optional[float] = None) -> torch.Tensor:
     """Causal attention of packed queries (T, H, hd) over the paged cache, H / G query heads per KV head -> (T, H, hd).
+    On the GPU the queries are bf16 or f16.
 
     Arguments as in :func:`kv_append`, called after it: query i of a sequence's n sees slots up to
     kv_lens - n + i, with ``window`` > 0 only the last ``window`` of them; block table entries of pages below that may be

@@ -20,6 +20,7 @@ from typing import List, Optional, Sequence, Union
 import torch
 
 from mamformer_b200 import ops
+from mamformer_b200.utils.precision import compute_dtype_of
 
 PAGE_SIZES = (16, 32, 64, 128)
 
@@ -89,6 +90,10 @@ class PagedKVCache:
             heads.add((full.n_kv_heads, full.head_dim))
             if getattr(full, "sliding_window", 0) > 0 and full.window_mode != "causal":
                 raise ValueError("the paged cache attends causally: sliding windows need window_mode='causal'")
+        dtype = compute_dtype_of(model)
+        if next(model.parameters()).is_cuda and dtype == torch.float32 and not torch.is_autocast_enabled("cuda"):
+            raise ValueError("the paged attention kernels take bf16 or f16 queries: convert the model first "
+                             "(utils.precision.to_compute_dtype; scripts/generate.py --bf16)")
         if len(heads) != 1:
             raise ValueError(f"the paged cache takes layers of one number and size of KV heads, got {sorted(heads)}")
         return cls(len(model.model.layers), *heads.pop(), batch, max_len, page_size,

@@ -275,3 +275,13 @@ def test_a_tensor_parallel_rank_holds_its_heads():
     model.model.layers[0].attention.full_attn.n_kv_heads = 3
     with pytest.raises(ValueError, match="one number"):
         PagedKVCache.for_model(model, 1, 10)
+
+
+@pytest.mark.gpu
+def test_fp32_models_are_refused_before_anything_is_cached():
+    model = MamformerForCausalLM(small_config()).eval().cuda()
+    ids = torch.randint(0, 200, (1, 5), device="cuda")
+    with pytest.raises(ValueError, match="bf16"):
+        model.generate(ids, max_new_tokens=2, kv_cache="paged")
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        PagedKVCache.for_model(model, 1, 10)
