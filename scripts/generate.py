@@ -44,6 +44,8 @@ def generate_text(model, tok, prompt, args):
     dev = next(model.parameters()).device
     ids = torch.tensor([tok.encode(prompt, add_bos=True)], device=dev)
     model.config.generation.repetition_penalty = args.repetition_penalty
+    if args.kv_cache != "dense" and (args.num_beams > 1 or (args.thinking and args.thinking != "NoThink")):
+        raise ValueError("--kv_cache paged goes with sampling: beams and thinking modes copy their cache between paths")
     if args.thinking and args.thinking != "NoThink":
         tc = ThinkingConfig.from_preset(args.thinking, args.think_budget, args.num_paths, args.summary_budget,
                                         args.show_thinking)

@@ -285,3 +285,18 @@ def test_fp32_models_are_refused_before_anything_is_cached():
         model.generate(ids, max_new_tokens=2, kv_cache="paged")
     with torch.autocast("cuda", dtype=torch.bfloat16):
         PagedKVCache.for_model(model, 1, 10)
+
+
+@pytest.mark.parametrize("extra", [["--num_beams", "2"], ["--thinking", "FastThink"]])
+def test_the_script_refuses_what_the_paged_cache_does_not_do(extra):
+    import sys
+    sys.path.insert(0, os.path.join(ROOT, "scripts"))
+    try:
+        import generate as script
+    finally:
+        sys.path.pop(0)
+    from mamformer_b200.tokenizer import MamformerTokenizer
+    args = script.build_parser().parse_args(["--config", "x", "--kv_cache", "paged", "--max_new_tokens", "2"] + extra)
+    model = MamformerForCausalLM(small_config()).eval()
+    with pytest.raises(ValueError, match="paged"):
+        script.generate_text(model, MamformerTokenizer(), "a", args)
