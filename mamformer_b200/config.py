@@ -308,7 +308,7 @@ _SUBCONFIGS = [
 ]
 _TOP_LEVEL = ["name", "model_type", "description", "d_model", "n_layers", "n_heads",
               "n_kv_heads", "head_dim", "d_ff", "vocab_size", "max_seq_len",
-              "tie_word_embeddings", "use_sliding_window", "sliding_window", "dropout",
+              "tie_word_embeddings", "use_sliding_window", "sliding_window", "window_mode", "dropout",
               "rms_norm_eps", "initializer_range"]
 
 
@@ -331,6 +331,9 @@ class MamformerConfig:
     tie_word_embeddings: bool = True
     use_sliding_window: bool = False
     sliding_window: int = 4096
+    # "reference": keys with 0 <= key - query < W, as the reference masks them; "causal": 0 <= query - key < W, which
+    # the paged cache needs
+    window_mode: str = "reference"
     mamba: MambaConfig = field(default_factory=MambaConfig)
     rope: RopeConfig = field(default_factory=RopeConfig)
     moe: MoEConfig = field(default_factory=MoEConfig)
@@ -361,6 +364,8 @@ class MamformerConfig:
                              f"({self.d_model // self.n_heads})")
         if self.d_ff <= 0:
             raise ValueError(f"d_ff ({self.d_ff}) must be positive")
+        if self.window_mode not in ("reference", "causal"):
+            raise ValueError(f"window_mode must be 'reference' or 'causal', got {self.window_mode!r}")
         if self.mamba.dt_rank == "auto":
             self.mamba.dt_rank = math.ceil(self.d_model / 32)
         if self.generation.max_context == 8192 and self.max_seq_len != 8192:
@@ -461,10 +466,14 @@ class MamformerConfig:
         return self.num_active_parameters / 1e9
 
     # -- serialisation --------------------------------------------------------------------
+    def _written(self) -> list:
+        """The top-level fields of a file: ``window_mode``, which is not the reference's, only where it is set."""
+        return [k for k in _TOP_LEVEL if k != "window_mode" or self.window_mode != "reference"]
+
     def to_dict(self) -> dict:
         """Flat dict with the shared ``<prefix>_<field>`` key names."""
         out = {k: getattr(self, k) for k in ["name", "model_type", "description"]}
-        out.update({k: getattr(self, k) for k in _TOP_LEVEL if k not in out})
+        out.update({k: getattr(self, k) for k in self._written() if k not in out})
         for attr, prefix, _cls, names in _SUBCONFIGS:
             sub = getattr(self, attr)
             for n in names:
@@ -474,7 +483,7 @@ class MamformerConfig:
 
     def to_nested_dict(self) -> dict:
         """Nested layout (``model:`` block with sub-config sections)."""
-        out = {k: getattr(self, k) for k in _TOP_LEVEL}
+        out = {k: getattr(self, k) for k in self._written()}
         for attr, _prefix, _cls, names in _SUBCONFIGS:
             sub = getattr(self, attr)
             out[attr] = {n: getattr(sub, n) for n in names}

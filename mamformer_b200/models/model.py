@@ -127,7 +127,7 @@ def block_kwargs(config: MamformerConfig, lt: dict, i: int) -> dict:
         comm_moe_n_heads=c.communicative_moe.n_comm_heads,
         comm_moe_depth=c.communicative_moe.comm_depth,
         comm_moe_dropout=c.communicative_moe.comm_dropout,
-        window_mode=getattr(c, "window_mode", "reference"),
+        window_mode=c.window_mode,
     )
 
 

@@ -89,7 +89,8 @@ class PagedKVCache:
             full = getattr(att, "full_attn", att)
             heads.add((full.n_kv_heads, full.head_dim))
             if getattr(full, "sliding_window", 0) > 0 and full.window_mode != "causal":
-                raise ValueError("the paged cache attends causally: sliding windows need window_mode='causal'")
+                raise ValueError("the paged cache attends causally: sliding windows need window_mode='causal' "
+                                 "(a field of the config; --window_mode of the scripts)")
         dtype = compute_dtype_of(model)
         if next(model.parameters()).is_cuda and dtype == torch.float32 and not torch.is_autocast_enabled("cuda"):
             raise ValueError("the paged attention kernels take bf16 or f16 queries: convert the model first "

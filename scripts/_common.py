@@ -36,11 +36,13 @@ def load_config(path_or_preset: str):
     return MamformerConfig.from_preset(path_or_preset)
 
 
-def load_model(config_path: str, checkpoint=None, device="cpu", dtype=None):
+def load_model(config_path: str, checkpoint=None, device="cpu", dtype=None, window_mode=None):
     import torch
     from mamformer_b200 import MamformerForCausalLM
     from mamformer_b200.checkpoint import load_model_state
     cfg = load_config(config_path)
+    if window_mode is not None:
+        cfg.window_mode = window_mode
     model = MamformerForCausalLM(cfg)
     if checkpoint:
         ck = torch.load(checkpoint, map_location="cpu", weights_only=False)

@@ -32,6 +32,8 @@ def build_parser():
     p.add_argument("--bf16", action="store_true")
     p.add_argument("--kv_cache", default="dense", choices=("dense", "paged"),
                    help="paged: keys and values in 8-bit pages (sampling only)")
+    p.add_argument("--window_mode", default=None, choices=("reference", "causal"),
+                   help="sliding windows of the model, in place of its config's (the paged cache needs causal ones)")
     p.add_argument("--seed", type=int, default=42, help="seeds the weights of a model built without a checkpoint "
                                                          "and the sampling")
     return p
@@ -67,7 +69,7 @@ def main(argv=None):
     args = build_parser().parse_args(argv)
     torch.manual_seed(args.seed)
     model, cfg = _common.load_model(args.config, args.checkpoint, args.device,
-                                    torch.bfloat16 if args.bf16 else None)
+                                    torch.bfloat16 if args.bf16 else None, args.window_mode)
     tok = MamformerTokenizer()
     if args.prompt is not None:
         print(generate_text(model, tok, args.prompt, args))

@@ -28,6 +28,8 @@ def build_parser():
     p.add_argument("--gen_top_k", type=int, default=50)
     p.add_argument("--gen_kv_cache", default="dense", choices=("dense", "paged"),
                    help="paged: rollouts keep keys and values in 8-bit pages")
+    p.add_argument("--window_mode", default=None, choices=("reference", "causal"),
+                   help="sliding windows of the model, in place of its config's (the paged cache needs causal ones)")
     p.add_argument("--entropy_beta", type=float, default=0.0, help="weight of the policy's token entropy in the loss")
     p.add_argument("--batch_size", type=int, default=4)
     p.add_argument("--gradient_accumulation_steps", type=int, default=1)
@@ -69,7 +71,7 @@ def main(argv=None):
     rank, world, local, device = _common.init_distributed()
     log = setup_logging(rank)
     ck = None if args.checkpoint.lower() == "none" else args.checkpoint
-    policy, cfg = _common.load_model(args.config, ck, device)
+    policy, cfg = _common.load_model(args.config, ck, device, window_mode=args.window_mode)
     policy.train()
     tok = MamformerTokenizer()
     gcfg = GRPOConfig(group_size=args.group_size, gen_max_tokens=args.gen_max_tokens,

@@ -300,3 +300,31 @@ def test_the_script_refuses_what_the_paged_cache_does_not_do(extra):
     model = MamformerForCausalLM(small_config()).eval()
     with pytest.raises(ValueError, match="paged"):
         script.generate_text(model, MamformerTokenizer(), "a", args)
+
+
+def test_configs_set_the_window_mode(tmp_path):
+    for name in ("pro-7b", "ultra-7b", "ultra-37b"):
+        c = MamformerConfig.from_yaml(os.path.join(ROOT, "configs", f"{name}.yaml"))
+        assert c.use_sliding_window and c.window_mode == "reference" and "window_mode" not in c.to_dict()
+    cfg = small_config()
+    d = cfg.to_dict()
+    d.update(use_sliding_window=True, sliding_window=8)
+    with pytest.raises(ValueError, match="window_mode"):
+        PagedKVCache.for_model(MamformerForCausalLM(MamformerConfig.from_dict(d)), 1, 10)
+    with pytest.raises(ValueError, match="window_mode"):
+        MamformerConfig.from_dict({**d, "window_mode": "both"})
+    path = str(tmp_path / "c.yaml")
+    for nested in (False, True):
+        MamformerConfig.from_dict({**d, "window_mode": "causal"}).to_yaml(path, nested)
+        cfg = MamformerConfig.from_yaml(path)
+        assert cfg.window_mode == "causal"
+    torch.manual_seed(0)
+    model = MamformerForCausalLM(cfg).eval()
+    ids = torch.randint(0, 200, (2, 21))
+    paged = PagedKVCache.for_model(model, 2, 30)
+    paged.extend(21)
+    with torch.no_grad():
+        a = model(ids, use_cache=True, cache=paged.layer_caches(), return_logits=True)["logits"].double()
+        b = model(ids, use_cache=True, return_logits=True)["logits"].double()
+    assert (a - b).norm() <= 2.0 ** -4 * b.norm()
+    assert model.generate(ids, max_new_tokens=3, temperature=0.0, kv_cache="paged").shape == (2, 24)
