@@ -341,10 +341,16 @@ class KDADiffAttention(nn.Module):
         self.last_choice = "full" if full else "linear"
         if dynamic:
             want = "full" if full else "linear"
-            cache = cache if (cache is None or cache.get("attn_type") == want) else None
+            paged = cache.get("paged") if cache is not None else None
+            if cache is not None and cache.get("attn_type") != want:
+                # a layer that turns back to full attention attends to what comes from here on, on either cache
+                cache = {"attn_type": "full", "paged": paged.restart()} if full and paged is not None else None
         mod = self.full_attn if full else self.linear_attn
-        return mod(x, attention_mask=attention_mask, use_cache=use_cache, cache=cache,
-                   h_states=h_states, rope_offset=rope_offset)
+        out, new_cache = mod(x, attention_mask=attention_mask, use_cache=use_cache, cache=cache,
+                             h_states=h_states, rope_offset=rope_offset)
+        if dynamic and not full and new_cache is not None and paged is not None:
+            new_cache["paged"] = paged                     # for when the gate turns to full attention again
+        return out, new_cache
 
     def get_lambda_values(self) -> torch.Tensor:
         return (self.linear_attn.get_lambda_values() + self.full_attn.get_lambda_values()) / 2.0

@@ -32,6 +32,13 @@ class PagedLayer:
         self.owner = owner
         self.index = index
         self.kv: Optional[ops.PagedKV] = None
+        self._skipped: Optional[torch.Tensor] = None             # tokens of each sequence from before the last restart
+
+    def restart(self) -> "PagedLayer":
+        """Forget the layer's tokens from before the current step, for a layer that has taken no part in the steps
+        before it.  The block table stays: the layer then uses its first pages."""
+        self._skipped = self.owner.kv_lens - self.owner._added
+        return self
 
     def attend(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
                q2: Optional[torch.Tensor] = None, lam: Optional[torch.Tensor] = None, window: int = 0,
@@ -48,8 +55,9 @@ class PagedLayer:
             raise ValueError(f"paged cache: {queries[0].shape[0]} query rows in a step of {o.tokens} tokens")
         pos = o._positions(cos.shape[0], q.device)
         kf, vf = flat(k), flat(v)
-        queries = ops.kv_append(kf, vf, self.kv, o.block_table, o.cu_seqlens, o.kv_lens, o.max_new, cos, sin, pos, queries)
-        out = ops.paged_attention(queries[0], self.kv, o.block_table, o.cu_seqlens, o.kv_lens, o.max_new,
+        lens = o.kv_lens if self._skipped is None else o.kv_lens - self._skipped
+        queries = ops.kv_append(kf, vf, self.kv, o.block_table, o.cu_seqlens, lens, o.max_new, cos, sin, pos, queries)
+        out = ops.paged_attention(queries[0], self.kv, o.block_table, o.cu_seqlens, lens, o.max_new,
                                   q2=queries[1] if q2 is not None else None, lam=lam, window=window, scale=scale)
         return out.view(q.shape)
 
@@ -145,6 +153,10 @@ class PagedKVCache:
         self.block_table[b] = -1
         self.kv_lens = self.kv_lens.clone()
         self.kv_lens[b] = 0
+        for layer in self.layers:
+            if layer._skipped is not None:
+                layer._skipped = layer._skipped.clone()
+                layer._skipped[b] = 0
 
     def check(self) -> None:
         """Wait for the steps so far and raise what their kernels recorded: PagedCacheError for a page, length or

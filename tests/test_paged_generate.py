@@ -328,3 +328,40 @@ def test_configs_set_the_window_mode(tmp_path):
         b = model(ids, use_cache=True, return_logits=True)["logits"].double()
     assert (a - b).norm() <= 2.0 ** -4 * b.norm()
     assert model.generate(ids, max_new_tokens=3, temperature=0.0, kv_cache="paged").shape == (2, 24)
+
+
+@pytest.mark.parametrize("dev,dtype", DEVICES)
+def test_a_gated_layer_stays_on_the_paged_cache(dev, dtype, monkeypatch):
+    """full, linear, full: as on the dense cache, the layer attends to what comes after the last turn, and stays paged."""
+    from mamformer_b200.models.kda_diff import KDADiffAttention
+    torch.manual_seed(0)
+    B, H, G, hd, d = 2, 4, 2, 64, 256
+    mod = KDADiffAttention(d, H, G, hd, kernel_dim=64, latent_dim=64, use_state_injection=False, use_dynamic_ratio=True).to(dev, dtype)
+    for p in mod.parameters():
+        if p.dim() == 2:
+            torch.nn.init.normal_(p, std=p.shape[1] ** -0.5)
+    for m in (mod.full_attn, mod.linear_attn):
+        m.lambda_raw.data = m.lambda_raw.data.float()
+    turns = [True, True, False, False, True, True, False, True]
+    counts = [18, 1, 1, 1, 1, 1, 1, 1]
+    x = torch.randn(B, sum(counts), d).to(dev, dtype)
+    h = torch.zeros(B, 1, 4, device=dev)
+    owner = PagedKVCache(1, G, hd, B, sum(counts), page_size=16, device=dev)
+    calls = []
+    real = ops.paged_attention
+    monkeypatch.setattr(ops, "paged_attention", lambda *a, **k: calls.append(a[4].tolist()) or real(*a, **k))
+    paged, dense, at = {"attn_type": "full", "paged": owner.layer(0)}, None, 0
+    for full, n in zip(turns, counts):
+        monkeypatch.setattr(mod, "choose_full", lambda h: full)
+        owner.extend(n)
+        with torch.no_grad():
+            a, paged = mod(x[:, at:at + n], use_cache=True, cache=paged, h_states=h)
+            b, dense = mod(x[:, at:at + n], use_cache=True, cache=dense, h_states=h)
+        assert paged["attn_type"] == ("full" if full else "linear") and paged["paged"] is owner.layer(0)
+        at += n
+        # the stored values' rounding, 2^-4 of each, on the full turns
+        assert (a - b).double().norm() <= (2.0 ** -3 if full else 2.0 ** -20) * b.double().norm(), (full, at)
+    assert calls == [[18, 18], [19, 19], [1, 1], [2, 2], [1, 1]]
+    owner.release(0)
+    owner.extend([3, 0])
+    assert owner.layer(0)._skipped.tolist()[0] == 0
