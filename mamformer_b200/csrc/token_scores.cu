@@ -463,7 +463,8 @@ static Rows rows_of(const at::Tensor& logits) {
 }
 
 static int64_t check(const at::Tensor& logits, const at::Tensor& target, double temperature, int64_t top_k) {
-  TORCH_CHECK(temperature > 0 && std::isfinite(temperature), "token_scores: temperature must be positive and finite, got ", temperature);
+  // 1 / T is finite in fp32, and exp(DMIN / T), the weight of a logit of -inf, is 0
+  TORCH_CHECK(temperature >= 1e-30 && temperature <= 1e27, "token_scores: temperature from 1e-30 to 1e27, got ", temperature);
   TORCH_CHECK(logits.is_cuda() && target.is_cuda() && logits.device() == target.device(),
               "token_scores: logits and targets on one GPU");
   TORCH_CHECK(target.scalar_type() == at::kLong && target.is_contiguous(), "token_scores: contiguous int64 targets");

@@ -241,8 +241,8 @@ def token_scores(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, te
         raise ValueError(f"token_scores: targets {tuple(targets.shape)} for logits {tuple(shape)}")
     if targets.is_floating_point():
         raise ValueError(f"token_scores: integer targets, got {targets.dtype}")
-    if not temperature > 0:
-        raise ValueError(f"token_scores: temperature must be positive, got {temperature}")
+    if not 1e-30 <= temperature <= 1e27:
+        raise ValueError(f"token_scores: temperature from 1e-30 to 1e27, got {temperature}")
     if not (0 <= top_k <= 32 and top_k <= shape[-1]):
         raise ValueError(f"token_scores: top_k from 0 to {min(32, shape[-1])}, got {top_k}")
     if _native(logits) and "token_scores" in NATIVE and logits.dtype in _SCORE_TYPES and not _transformed():

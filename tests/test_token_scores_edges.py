@@ -158,3 +158,20 @@ def test_targets_outside_the_vocabulary_are_not_silent(dev):
     t[1] = -100
     assert ops.token_scores(x, t).log_probs[1] == 0
     check_device_status()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_temperatures_at_the_ends_of_their_range(dev):
+    """Very cold: all weight on the largest logit; very hot: all that are not -inf alike, those of -inf still nothing."""
+    x, t, _ = rows(dev, R=3, V=700)
+    x[:, 5] = 9.0
+    x[:, 100:110] = -math.inf
+    t[:] = 5
+    cold = ops.token_scores(x, t, top_k=2, temperature=1e-30)
+    assert (cold.log_probs == 0).all() and (cold.entropy.abs() < 1e-6).all() and (cold.top_ids[:, 0] == 5).all()
+    hot = ops.token_scores(x, t, temperature=1e27)
+    near(hot.log_probs, torch.full((3,), -math.log(690), device=dev))
+    near(hot.entropy, torch.full((3,), math.log(690), device=dev))
+    for bad in (1e-31, 1e-45, 1e28, math.inf):
+        with pytest.raises(ValueError):
+            ops.token_scores(x, t, temperature=bad)
