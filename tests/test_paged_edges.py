@@ -393,3 +393,22 @@ def test_an_earlier_error_leaves_the_paged_words(monkeypatch, comm, gemm):
         with pytest.raises(fault.KernelTimeoutError, match="timed out; a block table entry"):
             fault.check_device_status(clear)
     fault.check_device_status()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("size", [60.0, 1e-4, 2.0 ** -20, 3e4])
+@pytest.mark.parametrize("diff", [False, True])
+def test_large_and_tiny_scores_of_many_rows(dev, size, diff):
+    """Scores of several hundred and more, and of next to nothing, in chunks of a prompt."""
+    new, lens = [130, 70], [130, 400]
+    cache, table = filled(lens, 32, 2, 128, dev, seed=7)
+    q = (rand((sum(new), 4, 128), torch.float32, dev, 3) * size).bfloat16()
+    kw = pair(q, diff)
+    got = ops.paged_attention(q, cache, table, offsets(new, dev), i32(lens, dev), max(new), **kw)
+    assert got.isfinite().all()
+    # a score of size s carries 2^-24 s of rounding in each of its 128 products, and the weights carry that much; values
+    # are below 5, times (1 + lam) / (1 - lam)
+    slack = 2.0 ** -24 * 128 * size * 12
+    if slack < 0.1:
+        want, tol = plain(q, cache, table, new, lens, **kw)
+        close(got, want, tol + slack * 5.0 * (9.0 if diff else 1.0))
