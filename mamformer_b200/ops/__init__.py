@@ -218,12 +218,13 @@ class TokenScores(NamedTuple):
 
 
 _SCORE_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+_func_active = torch._C._are_functorch_transforms_active
 
 
 def _transformed() -> bool:
     """Inside forward-mode differentiation or a torch.func transform, whose tensors a kernel call would take for plain
     ones: their tangents would be lost."""
-    return forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active()
+    return forward_ad._current_level >= 0 or _func_active()
 
 
 def token_scores(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, temperature: float = 1.0,
