@@ -19,7 +19,7 @@
 // so a fragment is one 16-byte read and no shuffles; so is the order of the 8 tokens of a fragment (`token`).
 //
 // 64 sequences of 300 to 8191 slots, 32 / 8 heads of 128, two maps (566 MB): 125 us, 4.5 TB/s, of which 8 us
-// are the start and 6 the join; with the arithmetic left out 105 us.  One token on 131000 slots: 62 us.
+// are the start and 6 the join.  One token on 131000 slots: 62.6 us.
 #include "paged.cuh"
 #include "tc5.cuh"
 
@@ -34,7 +34,8 @@ constexpr int TILE = STEP * NW;                // tokens per tile
 constexpr float NONE = -1e30f;                 // maximum of no scores: 2^(score - NONE) is never formed, 2^(NONE - m) is 0
 // Rows of a sequence and KV head above which the chunk kernel takes over.  This kernel and the chunk kernel, 16
 // sequences of 2000-6000 slots, 32 / 8 heads, two maps: 24 rows 89 and 157 us, 32 rows 90 and 158, 64 rows 160 and
-// 158; one map, 8 sequences of 8000, 16 / 4 heads: 32 rows 55 and 78, 64 rows 83 and 94.
+// 158; one map, 8 sequences of 8000, 16 / 4 heads: 32 rows 55 and 78, 64 rows 83 and 94 (of when the rule was set; since
+// then 64 rows 84, and 80 rows 81 in the chunk kernel).
 constexpr int FEW = 64;
 constexpr float LAZY = 8.f;                    // log2 by which a row may outgrow its reference maximum
 constexpr float SLACK = 64.f;                  // value scales of up to this times O's unit are not looked at

@@ -14,11 +14,15 @@
 // the scores, which the sum of weights is kept in, and r a whole number that brings m + r to its running maximum of
 // score + log2 of the value scale.  So the f16 weights keep their bits for what the row sees, whatever the values of
 // other pages are, and the largest score's is a power of two.  A 16-token group costs a handful of operations per row.
-// Where there are fewer tiles than SMs, several CTAs share a tile's
-// keys and a second kernel joins them.  Online softmax with lazy rescaling as in flash_tc.cu.  Every
-// wait is bounded; a wait that runs out records a code, and the CTA winds down.
+// Where there are fewer tiles than SMs, several CTAs share a tile's keys and a second kernel joins them.  Online softmax
+// with lazy rescaling as in flash_tc.cu.  Every wait is bounded; a wait that runs out records a code, and the CTA winds
+// down and leaves zeros.
 //
-// 2 x 2048 tokens on 10240 cached, 32 / 8 heads of 128, two maps: 1.72 ms, 877 TFLOP/s.  A pair of tiles takes
+// P is rounded to f16: 11 bits of a weight, where bf16 would keep 8, and a second product for the lower bits would be half
+// of the tensor work again; its sum is fp32.  In bf16 the result's own rounding hides it; f16 results of short runs are 2.9e-4
+// from 64 bits, 2.1e-4 with fp32 arithmetic.
+//
+// 2 x 2048 tokens on 10240 cached, 32 / 8 heads of 128, two maps: 1.74 ms, 871 TFLOP/s.  A pair of tiles takes
 // 2,670 cycles; the products' own time is 1,024.  It is bound by the hand-offs: the products of the scores
 // take 70-80 cycles each (32 at the full rate, N = 64), those of the values 160-190 (64), and a tile's
 // conversion 1,130 with 1,550 until the next one's loads are there; without the exponentials it is as slow.

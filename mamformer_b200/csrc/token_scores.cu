@@ -40,6 +40,8 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+// Good to 2^-22.  With that and the multiplication by a rounded 1 / T, scores of 32000 fp32 logits are 1.2e-7 of their size
+// from 64 bits, where torch's exp and a division by T come to 6.6e-8: the pass is next to the MUFU's bound as it is.
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -477,9 +479,11 @@ static int64_t check(const at::Tensor& logits, const at::Tensor& target, double 
   return R;
 }
 
-// CTAs per row: 8, 4 or 2 where that many per row stay resident at one per SM and each has 16 KB of the row.
-// 20 alternatives of 128000 logits: 64 rows 16.5 us with one, 15.6 with two, 18.6 with four; 200 rows 24.7 with
-// one or two, 39 with four.
+// CTAs per row: 8, 4 or 2 where that many per row stay resident at one per SM and each has 16 KB of the row.  Rows of
+// 128000 bf16, us with 1, 2, 4 and 8:
+//   k = 0     9 rows 14.9, 11.5, 9.1, 8.6    30 rows 16.5, 12.5, 10.5, 10.4   74 rows 16.5, 12.5, 14.4, 18.6
+//   k = 20    9 rows 18.8, 16.9, 16.6, 19.0  30 rows 20.7, 18.6, 17.7, 20.7   74 rows 20.8, 18.6, 22.7, 41.2
+// from 75 rows on 2 is no better than 1.  The 16 KB edge is flat: 30 rows of 16000 to 64000, k = 0, within 20%.
 static int cluster_of(int64_t R, int64_t row_bytes) {
   int cl = 1;
   while (cl < 8 && R * cl * 2 <= num_sms() && row_bytes >= 32768 * cl) cl *= 2;
@@ -499,9 +503,15 @@ void launch_fwd(const T* x, const FwdParams& p, int64_t R) {
   cfg.numAttrs = CL > 1 ? 1 : 0;
   MAMF_CUDA_CHECK(cudaLaunchKernelEx(&cfg, scores_fwd_kernel<T, CL, NT>, x, p));
 }
-// 512 threads have a row done sooner; 256 waste less at its end, which counts once every SM has several rows
-// (3686 x 128000 bf16: 160 us, with 512 174), unless the search for many alternatives is most of that (k = 20:
-// 229 us, with 512 209).
+// 512 threads have a row done sooner; 256 waste less at its end, which counts once every SM has three rows, unless the
+// search for many alternatives is most of that.  Rows of 128000 bf16, us with 512 / 256 threads:
+//   rows      148          443          500          900          3686
+//   k = 0     16.7 / 22.8  27.7 / 29.0  35.1 / 34.4  53.5 / 53.5  170 / 159
+//   k = 8     20.7 / 26.2  33.0 / 34.0  41.2 / 39.2  62.9 / 64.0  201 / 190
+//   k = 12    20.8 / 26.9  33.0 / 35.3  43.0 / 40.8  63.8 / 69.2  211 / 202
+//   k = 20    20.8 / 28.9  35.1 / 38.3  45.3 / 43.5  67.8 / 76.2  222 / 231
+// So k > 8 is a middle of edges between 4 and 20.  Shorter rows favour 256 earlier, which the rule does not follow: 600
+// rows of 16000, k = 8, 24.7 / 16.6.
 template <typename T>
 void launch_fwd(const T* x, const FwdParams& p, int64_t R) {
   const int cl = cluster_of(R, p.V * (int64_t)sizeof(T));

@@ -264,13 +264,13 @@ def _paged(B, new, lens, H, G, hd, page, diff):
     return cache, table, cu, ln, q, (q2 if diff else None), (torch.full((H,), 0.5, device="cuda") if diff else None)
 
 
-def case_paged_attention(B=64, new=1, lens=4096, H=32, G=8, hd=128, page=64):
-    """Differential attention over the paged 8-bit cache: a decode step, or (new > 1) a chunk of a prompt."""
+def case_paged_attention(B=64, new=1, lens=4096, H=32, G=8, hd=128, page=64, diff=True):
+    """Attention over the paged 8-bit cache: a decode step, or (new > 1) a chunk of a prompt."""
     from mamformer_b200 import ops
-    cache, table, cu, ln, q, q2, lam = _paged(B, new, lens, H, G, hd, page, True)
-    pairs = B * sum(lens - new + i + 1 for i in range(new))
-    return ((lambda: ops.paged_attention(q, cache, table, cu, ln, new, q2=q2, lam=lam)), 8.0 * pairs * H * hd,
-            B * lens * G * hd * 2 + 3 * q.numel() * 2)
+    cache, table, cu, ln, q, q2, lam = _paged(B, new, lens, H, G, hd, page, diff)
+    pairs, maps = B * sum(lens - new + i + 1 for i in range(new)), 2 if diff else 1
+    return ((lambda: ops.paged_attention(q, cache, table, cu, ln, new, q2=q2, lam=lam)), 4.0 * maps * pairs * H * hd,
+            B * lens * G * hd * 2 + (maps + 1) * q.numel() * 2)
 
 
 def case_kv_append(B=16, new=1024, H=32, G=8, hd=128, page=64):
@@ -296,6 +296,28 @@ def case_token_scores(R=4096, V=128000, k=0, backward=False):
     return (lambda: _C.token_scores_bwd(x, t, -100, 1.0, stats, ent, ids, g, g, None)), 0.0, x.numel() * 4
 
 
+def case_scores_small(R=50, V=1500, k=5):
+    """A whole small pass through torch's engine: scores, alternatives and gradient."""
+    from mamformer_b200 import ops
+    x = torch.randn(R, V, device="cuda").bfloat16().requires_grad_(True)
+    t = torch.randint(0, V, (R,), device="cuda")
+    g, gk = torch.randn(R, device="cuda"), torch.randn(R, k, device="cuda")
+
+    def run():
+        s = ops.token_scores(x, t, top_k=k)
+        torch.autograd.grad((s.log_probs, s.entropy, s.top_log_probs), x, (g, g, gk))
+    return run, 0.0, x.numel() * 6
+
+
+def case_scores_constrained(R=200, V=128000, k=20, finite=10):
+    """Fewer finite logits than alternatives: the rest are -inf, which are more ties than are kept as candidates."""
+    from mamformer_b200.ops.native import _C
+    x = torch.full((R, V), -float("inf"), device="cuda").bfloat16()
+    x[:, 100:100 + finite] = torch.randn(R, finite, device="cuda").bfloat16()
+    t = torch.full((R,), 100, device="cuda")
+    return (lambda: _C.token_scores_fwd(x, t, -100, 1.0, k, False)), 0.0, x.numel() * 2
+
+
 CASES = {"gemm": case_gemm, "grouped": case_grouped, "wgrad": case_wgrad, "scan": case_scan,
          "scan_bwd": lambda: case_scan(backward=True), "linear_attn": case_linear_attn,
          "linear_attn_bwd": lambda: case_linear_attn(backward=True), "ce": case_ce, "moe": case_moe,
@@ -308,6 +330,11 @@ CASES = {"gemm": case_gemm, "grouped": case_grouped, "wgrad": case_wgrad, "scan"
          "conv": case_conv, "conv_bwd": lambda: case_conv(backward=True), "groupnorm": case_groupnorm,
          "groupnorm_bwd": lambda: case_groupnorm(backward=True), "kv_append": case_kv_append,
          "paged_decode": case_paged_attention, "paged_chunk": lambda: case_paged_attention(4, 1024, 8192),
+         "paged_chunk_single": lambda: case_paged_attention(4, 1024, 8192, diff=False),
+         "paged_64_rows": lambda: case_paged_attention(8, 16, 8000, 16, 4, diff=False),
+         "paged_80_rows": lambda: case_paged_attention(8, 20, 8000, 16, 4, diff=False),
+         "paged_tail": lambda: case_paged_attention(1, 100, 14100),
+         "scores_small": case_scores_small, "scores_constrained": case_scores_constrained,
          "token_scores": case_token_scores, "token_scores_top": lambda: case_token_scores(k=20),
          "token_scores_bwd": lambda: case_token_scores(backward=True)}
 
