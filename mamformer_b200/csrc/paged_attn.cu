@@ -667,7 +667,8 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
 }
 
 // What the split kernel has left out, by one block: offsets or lengths that do not fit are recorded, sequences of more
-// tokens than max_new get zeros, and offsets out of order give nothing but zeros.
+// tokens than max_new get zeros, and offsets out of order give nothing but zeros.  The look at them needs nothing of that
+// kernel and is over before it ends; after it, it cost a short call 1.5 us.
 template <typename T>
 __device__ __noinline__ void left_out(const Params& p, int hd) {
   const Cache& c = p.c;
@@ -677,7 +678,9 @@ __device__ __noinline__ void left_out(const Params& p, int hd) {
     broken = broken || !in_order(c, b);
     odd = odd || too_many(b) || cached_length(c, c.lens[b]) != c.lens[b];
   }
-  if (!__syncthreads_or(odd || broken)) return;
+  odd = __syncthreads_or(odd || broken);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!odd) return;
   broken = __syncthreads_or(broken);
   if (threadIdx.x == 0) record(ERR_LENGTH);
   for (int t = 0; t < c.T; ++t) {
@@ -691,12 +694,13 @@ __device__ __noinline__ void left_out(const Params& p, int hd) {
 template <typename T, int HD, int NR>
 __global__ void __launch_bounds__(NJ, 2) join_kernel(const __grid_constant__ Params p) {
   constexpr int ROWS = 8 * NR;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int4 j = p.joins[blockIdx.x];
-  if (j.x < 0) {
-    if (blockIdx.x == 0) left_out<T>(p, HD);          // no item ends in the first CTA that began before it
+  if (blockIdx.x == 0) {                               // no item ends in the first CTA that began before it
+    left_out<T>(p, HD);
     return;
   }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 j = p.joins[blockIdx.x];
+  if (j.x < 0) return;
   const int t0 = j.x, row0 = (j.z >> 16) * ROWS, n_rows = min(ROWS, j.y - row0), g = j.z & 0xffff;
   const int c0 = j.w >> 1, parts = blockIdx.x - c0 + 1, per = p.rep * p.maps;
   // the warps share the rows, and a row's warps its parts, each under a running maximum; the two maps of a head
