@@ -830,6 +830,7 @@ at::Tensor paged_attention(at::Tensor q1, c10::optional<at::Tensor> q2, c10::opt
   Params p{};
   p.c = check_cache("paged_attention", Layer{ck, cv, ks, vs, table, cu, lens}, T, hd);
   TORCH_CHECK(H >= 1 && p.c.G >= 1 && H % p.c.G == 0, "paged_attention: ", H, " query heads over ", p.c.G, " KV heads");
+  TORCH_CHECK(std::isfinite((float)(scale * 1.4426950408889634)), "paged_attention: a finite scale, got ", scale);
   TORCH_CHECK(window >= 0 && max_new >= 0, "paged_attention: window and max_new must not be negative");
   q1 = rows16(q1);
   p.q1 = q1.data_ptr(); p.st1 = q1.stride(0); p.sh1 = q1.stride(1);

@@ -355,14 +355,15 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
       *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(gr.k);
       const int kbase = (kt0 + j) * BN;
       if (__any_sync(0xffffffffu, !(gr.all && kbase >= lo && kbase + BN - 1 <= hi))) {
-        // scaled first, masked then: a factor may be 0, and 0 times -inf is NaN
 #pragma unroll
         for (int k = 0; k < BN; ++k) {
           const int key = kbase + k;
-          sv[k] = (key >= lo && key <= hi && f[k >> 4] != 0.f) ? sv[k] * (f[k >> 4] * rs) : -INFINITY;
+          sv[k] = (key >= lo && key <= hi && f[k >> 4] != 0.f) ? sv[k] : -INFINITY;
         }
+        // a factor that is 0, or underflows, would make a masked score's -inf NaN; products are below 2^18, so that this
+        // one's scores are 0 all the same
 #pragma unroll
-        for (int k = 0; k < 4; ++k) f[k] = 1.f;
+        for (int k = 0; k < 4; ++k) f[k] = fmaxf(f[k] * rs, 1e-37f);
       } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k) f[k] *= rs;

@@ -412,3 +412,12 @@ def test_large_and_tiny_scores_of_many_rows(dev, size, diff):
     if slack < 0.1:
         want, tol = plain(q, cache, table, new, lens, **kw)
         close(got, want, tol + slack * 5.0 * (9.0 if diff else 1.0))
+
+
+@pytest.mark.gpu
+def test_score_factors_that_are_not_numbers_are_refused():
+    cache, table = filled([9], 16, 1, 64, "cuda")
+    q = rand((1, 2, 64), torch.bfloat16, "cuda", 1)
+    for scale in (math.nan, math.inf, -math.inf, 1e39):
+        with pytest.raises(RuntimeError, match="scale"):
+            ops.paged_attention(q, cache, table, offsets([1], "cuda"), i32([9], "cuda"), 1, scale=scale)
