@@ -101,6 +101,18 @@ at::Tensor paged_attention(at::Tensor q1, c10::optional<at::Tensor> q2, c10::opt
                            int64_t max_new, int64_t window, double scale);
 int64_t paged_attention_error(bool clear);
 int64_t paged_attention_wait_limit(int64_t cycles);
+std::vector<at::Tensor> kv4_append(at::Tensor k, at::Tensor v, at::Tensor blocks, c10::optional<at::Tensor> mass,
+                                   at::Tensor table, at::Tensor cu, at::Tensor lens, int64_t max_new,
+                                   c10::optional<at::Tensor> cos, c10::optional<at::Tensor> sin,
+                                   c10::optional<at::Tensor> pos, std::vector<at::Tensor> queries);
+std::vector<at::Tensor> kv4_read(at::Tensor blocks, at::Tensor table, at::Tensor cu, at::Tensor lens, int64_t T, at::ScalarType dtype);
+std::vector<at::Tensor> kv4_evict(at::Tensor blocks, at::Tensor mass, at::Tensor table, at::Tensor lens, int64_t budget,
+                                  int64_t recent, c10::optional<at::Tensor> out_table);
+int64_t kv4_error(bool clear);
+at::Tensor paged4_attention(at::Tensor q1, c10::optional<at::Tensor> q2, c10::optional<at::Tensor> lam, at::Tensor blocks,
+                            c10::optional<at::Tensor> mass, at::Tensor table, at::Tensor cu, at::Tensor lens,
+                            int64_t max_new, int64_t window, double scale);
+int64_t paged4_attention_error(bool clear);
 void gemm_ag(std::vector<int64_t> a_ptrs, int64_t shard_rows, int64_t lda, int64_t rank, at::Tensor B, bool b_mn,
              at::Tensor D);
 void gemm_rs(at::Tensor A, at::Tensor B, bool b_mn, std::vector<int64_t> d_ptrs, int64_t shard_rows, int64_t ldd,
@@ -175,6 +187,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("paged_attention", &mamf::paged_attention);
   m.def("paged_attention_error", &mamf::paged_attention_error, py::arg("clear") = true);
   m.def("paged_attention_wait_limit", &mamf::paged_attention_wait_limit);
+  m.def("kv4_append", &mamf::kv4_append);
+  m.def("kv4_read", &mamf::kv4_read);
+  m.def("kv4_evict", &mamf::kv4_evict);
+  m.def("kv4_error", &mamf::kv4_error, py::arg("clear") = true);
+  m.def("paged4_attention", &mamf::paged4_attention);
+  m.def("paged4_attention_error", &mamf::paged4_attention_error, py::arg("clear") = true);
   m.def("gemm_ag", &mamf::gemm_ag);
   m.def("gemm_rs", &mamf::gemm_rs);
 }

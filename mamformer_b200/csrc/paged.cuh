@@ -1,6 +1,7 @@
-// Shared by the paged 8-bit KV cache kernels (paged_kv.cu, paged_attn.cu).
+// Shared by the paged KV cache kernels: of the 8-bit cache (paged_kv.cu, paged_attn.cu, paged_attn_tc.cu) and, in what
+// both have alike, of the 4-bit one (paged4.cuh).
 //
-// One layer's cache is four tensors:
+// One layer's 8-bit cache is four tensors:
 //   k, v              (P, G, page, hd) e4m3 codes; the `page` tokens of one KV head are contiguous
 //   k_scale, v_scale  (P, G) fp32 powers of two, one for each block of `page` tokens and head
 // and a block table (B, W) int32 gives the page of slots [j * page, (j + 1) * page) of a sequence.
@@ -19,12 +20,27 @@ namespace paged {
 // What the kernels record; *_error() gives the codes met since they were cleared, code c as bit c.
 enum : int { ERR_PAGE = 1, ERR_LENGTH = 2, ERR_POSITION = 3, ERR_WAIT = 4 };
 
-struct Cache {
-  uint8_t *k, *v;
-  float *ks, *vs;
+struct Table {
   const int *table, *cu, *lens;
   int P, G, page, shift, W, B, T;        // page = 1 << shift
 };
+struct Cache : Table {
+  uint8_t *k, *v;
+  float *ks, *vs;
+};
+
+// The block table, offsets and lengths (contiguous, on one GPU) of a cache of P pages of `page` tokens and G heads.
+// cu null: an operator that takes no new tokens.
+inline Table check_table(const char* what, const at::Tensor& table, const at::Tensor* cu, const at::Tensor& lens, int64_t P,
+                         int64_t G, int64_t page, int64_t T) {
+  for (const at::Tensor* t : {&table, cu, &lens})
+    TORCH_CHECK(!t || t->scalar_type() == at::kInt, what, ": int32 block table, offsets and lengths");
+  const int64_t B = lens.numel();
+  TORCH_CHECK(table.dim() == 2 && table.size(0) == B && (!cu || cu->numel() == B + 1), what, ": a block table row and an offset for each of ", B, " sequences");
+  TORCH_CHECK(P < (1LL << 31) && G <= 65535 && table.size(1) * page < (1LL << 31) && T < (1LL << 31) && B < (1 << 24), what, ": sizes");
+  return Table{table.data_ptr<int>(), cu ? cu->data_ptr<int>() : nullptr, lens.data_ptr<int>(), (int)P, (int)G, (int)page,
+               page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7, (int)table.size(1), (int)B, (int)T};
+}
 
 struct Layer { at::Tensor k, v, ks, vs, table, cu, lens; };
 
@@ -39,22 +55,22 @@ inline Cache check_cache(const char* what, const Layer& l, int64_t T, int64_t hd
   TORCH_CHECK(page == 16 || page == 32 || page == 64 || page == 128, what, ": pages of 16, 32, 64 or 128 tokens, got ", page);
   for (const at::Tensor* t : {&l.ks, &l.vs})
     TORCH_CHECK(t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) == P && t->size(1) == G, what, ": fp32 scales (P, G)");
-  for (const at::Tensor* t : {&l.table, &l.cu, &l.lens})
-    TORCH_CHECK(t->scalar_type() == at::kInt, what, ": int32 block table, offsets and lengths");
-  const int64_t B = l.lens.numel();
-  TORCH_CHECK(l.table.dim() == 2 && l.table.size(0) == B && l.cu.numel() == B + 1, what, ": a block table row and an offset for each of ", B, " sequences");
   TORCH_CHECK(aligned16(l.k.data_ptr()) && aligned16(l.v.data_ptr()), what, ": 16-byte aligned pages");
-  TORCH_CHECK(P < (1LL << 31) && G <= 65535 && l.table.size(1) * page < (1LL << 31) && T < (1LL << 31) && B < (1 << 24), what, ": sizes");
-  return Cache{(uint8_t*)l.k.data_ptr(), (uint8_t*)l.v.data_ptr(), l.ks.data_ptr<float>(), l.vs.data_ptr<float>(),
-               l.table.data_ptr<int>(), l.cu.data_ptr<int>(), l.lens.data_ptr<int>(), (int)P, (int)G, (int)page,
-               page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7, (int)l.table.size(1), (int)B, (int)T};
+  Cache c;
+  static_cast<Table&>(c) = check_table(what, l.table, &l.cu, l.lens, P, G, page, T);
+  c.k = (uint8_t*)l.k.data_ptr();
+  c.v = (uint8_t*)l.v.data_ptr();
+  c.ks = l.ks.data_ptr<float>();
+  c.vs = l.vs.data_ptr<float>();
+  return c;
 }
 
-// What both attention kernels are given.
-struct Attn {
-  Cache c;
+// What the attention kernels of a cache are given.
+template <class C> struct AttnOf {
+  C c;
   const void *q1, *q2;                 // packed queries (T, H, hd); q2 null: one map
   void* out;                           // (T, H, hd), contiguous
+  float* lse;                          // (T, H, maps) log2 of each row's sum of weights, +inf for none; null: not asked for
   const float* lam;
   int64_t st1, sh1, st2, sh2;          // token and head strides of q1, q2 in elements
   int H, rep, maps, window;            // rep = H / G query heads per KV head
@@ -63,10 +79,12 @@ struct Attn {
   float scale_log2;
   long long wait;                      // cycles after which a wait gives up; negative: at once, without a look
 };
+using Attn = AttnOf<Cache>;
 
 // Cycles of a wait, about 0.25 s, where the longest takes microseconds; paged_attention_wait_limit() sets another number
 // for the waits that a test lets run out.
 constexpr long long WAIT_CYCLES = 500000000LL;
+long long attention_wait_limit();
 
 // csrc/paged_attn_tc.cu: sequences of more than `few` rows (of any number where few is 0, and then rows past
 // the last sequence are cleared too)
@@ -110,10 +128,10 @@ __device__ __forceinline__ int sequence_of(const int* cu, int B, int t) {
 }
 
 // Offsets of sequence b that rise and stay within the T packed tokens.
-__device__ __forceinline__ bool in_order(const Cache& c, int b) { return c.cu[b] >= 0 && c.cu[b] <= c.cu[b + 1] && c.cu[b + 1] <= c.T; }
+__device__ __forceinline__ bool in_order(const Table& c, int b) { return c.cu[b] >= 0 && c.cu[b] <= c.cu[b + 1] && c.cu[b + 1] <= c.T; }
 
 // The slots of a sequence that the block table has room for.
-__device__ __forceinline__ int cached_length(const Cache& c, int len) { return max(0, min(len, c.W << c.shift)); }
+__device__ __forceinline__ int cached_length(const Table& c, int len) { return max(0, min(len, c.W << c.shift)); }
 
 }  // namespace paged
 }  // namespace mamf

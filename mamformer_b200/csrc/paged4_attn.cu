@@ -1,0 +1,803 @@
+// Attention over the paged 4-bit cache (layout in paged4.cuh), for few query rows per KV head: single tokens and short
+// runs of tokens; with the weights that each slot receives, where they are asked for.
+//
+//   S = scale q . k,  P = 2^(S log2 e - r),  O = sum P v / sum P,   causal, optional window;
+//   differential: (O1 - lam O2) / (1 - lam + 1e-8);   mass[slot] += sum over rows and maps of P / sum P
+//
+// The work is the list of (sequence, KV head, row tile) items, each a run of 64-token tiles; the grid's CTAs take equal
+// contiguous shares of that list, so one long sequence fills the GPU as well as many short ones.  An item that ends in
+// another CTA than it began in leaves partial (r, l, O) in a workspace and a second small kernel joins them in order
+// (results do not depend on timing).
+//
+// A CTA is 4 warps; warp w takes tokens 16 w .. 16 w + 15 of each tile, which is one block of the cache, through a ring
+// of its own: one bulk copy a block, issued by one lane.  It never waits for the other warps inside an item.  The 16
+// tokens are the M rows of mma.m16n8k16 (f16 operands, fp32 sums): S^T = K Q^T and O^T = V^T P^T with up to 8 query rows
+// as N; 16 rows take two.  A code becomes its f16 value in three instructions for two dims, exactly, so the products are
+// those of the stored values; the rows of q are scaled by a power of two to [1, 2) first, which f16 holds exactly down to
+// 2^-14 of a row's largest value.  P is rounded to f16 (11 bits; bf16 would keep 8) at up to 2^15, so that weights down to
+// 2^-21 of a row's largest keep all of their bits, whatever values they are given to.  The order of the head's dims in the
+// products is free as long as both sides agree: a lane takes 16 adjacent bytes of a key's codes and 8 of a value's.
+//
+// Received weights: the scores of up to 16 rows are left in a workspace (4 bytes a row and slot, a small part of which the
+// L2 does not keep), and a last kernel turns them into weights with each row's joined sum; longer runs of tokens have
+// them computed from the keys once more (weights_kernel).
+#include "paged4.cuh"
+#include "paged_split.cuh"
+
+namespace mamf {
+namespace pa4 {
+
+using namespace split;
+using namespace paged4;
+
+// Rows of a sequence and KV head above which the chunk kernel takes over.
+constexpr int FEW = 64;
+constexpr float LIFT = 7.f, LAZY = 8.f;        // a row's largest weight is 2^LIFT when its reference is set, and may outgrow it
+constexpr int KEEP = 16;                       // rows whose scores are left for the received weights, at most
+
+struct Params : Attn4 {
+  int ctas;
+  float* part;        // [ctas][2][rows][HD + 2]: O (not divided), r, l
+  int4* joins;        // [ctas]: {t0, rows, g | rt << 16, 2 c0 + place} of the item that ends in this CTA after it
+                      // began in CTA c0 (its part there is in `place`), or {-1, ..}
+  float* scores;      // [B][G][cap][stride] scores (log2) of up to `stride` rows, where weights are asked for
+  int64_t cap;        // slots that a sequence can have
+  int stride;
+};
+
+__device__ __forceinline__ uint32_t lds4(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+
+constexpr int ST = 4;                          // blocks of a warp's ring
+// resident CTAs per SM: the latency of a warp's chain (products, exponentials, products) is hidden by other
+// warps, so there are as many as the registers of a row tile allow without spills (128, 168 or 255)
+template <int HD, int NR> constexpr int residents() { return NR == 1 ? 4 : HD == 64 ? 3 : 2; }
+template <int HD, int NR> constexpr int merge_words() { return NR * (HD / 4 + 4); }      // of a lane
+template <int HD, int NR> constexpr int smem_bytes() {
+  return 1024 + NW * ST * BLOCK<HD> + 32 * 4 * merge_words<HD, NR>();
+}
+
+template <typename T, int HD, int NR>
+__global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __grid_constant__ Params p) {
+  constexpr int ROWS = 8 * NR;
+  constexpr int KW = HD / 32;                    // words of a K row per lane, and of the parameters of a row's two halves
+  constexpr int VW = HD / 64;                    // words of a V row per lane
+  constexpr int MT = HD / 16;                    // 16-dim tiles of O^T
+  constexpr int SB = BLOCK<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t bars[NW][ST];
+  __shared__ int64_t s_pre[NT / 32];
+  __shared__ int64_t s_begin;
+  __shared__ int s_b, s_cut;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g8 = lane >> 2, t4 = lane & 3;
+  const Cache4& c = p.c;
+  asm volatile("griddepcontrol.launch_dependents;");      // the join kernel waits for this grid's end by itself
+
+  // ---- this CTA's share [first, last) of the list of tiles ----
+  const int chunk = (c.B + NT - 1) / NT;
+  int64_t mine = 0;
+  bool broken = false;                              // offsets out of order: nothing is done here
+  for (int i = 0; i < chunk; ++i) {
+    const int b = tid * chunk + i;
+    if (b < c.B) {
+      mine += tiles_of<ROWS>(p, b);
+      broken = broken || !in_order(c, b);
+    }
+  }
+  broken = __any_sync(0xffffffffu, broken);
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) s_pre[w] = broken ? 1LL << 60 : incl;
+  if (tid == 0) { s_b = -1; s_cut = 0; }
+  __syncthreads();
+  int64_t total = 0, before = 0;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    if (i < w) before += s_pre[i];
+    total += s_pre[i];
+  }
+  incl += before;
+  const int64_t share = (total + p.ctas - 1) / p.ctas;
+  const int64_t first = blockIdx.x * share, last = min(total, first + share);
+  if (incl - mine <= first && first < incl) {      // one thread at most
+    int64_t at = incl - mine;
+    int b = tid * chunk;
+    for (;; ++b) {
+      const int64_t n = tiles_of<ROWS>(p, b);
+      if (first < at + n) break;
+      at += n;
+    }
+    s_b = b;
+    s_begin = at;
+  }
+  __syncthreads();
+  if (tid == 0) p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  // rows before the first and past the last sequence
+  {
+    const int64_t row = (int64_t)p.H * HD;
+    const int64_t front = c.B > 0 ? min(max(0, c.cu[0]), c.T) * row : 0, end = c.B > 0 ? max(0, c.cu[c.B]) * row : 0;
+    for (int64_t i = (int64_t)blockIdx.x * NT + tid; i < front; i += (int64_t)gridDim.x * NT) ((T*)p.out)[i] = from_f<T>(0.f);
+    for (int64_t i = end + (int64_t)blockIdx.x * NT + tid; i < c.T * row; i += (int64_t)gridDim.x * NT)
+      ((T*)p.out)[i] = from_f<T>(0.f);
+  }
+  if (first >= last || total >> 60) return;
+
+  Item it;                                          // of the tile being computed
+  set_sequence<ROWS>(p, it, s_b);
+  int64_t start = s_begin;                          // list position of the item's first tile
+  while (first >= start + it.nt) { start += it.nt; next_item<ROWS>(p, it); }
+
+  // ---- ring: the issue side runs ST - 1 tiles ahead ----
+  const uint32_t ring = su32(smem) + w * ST * SB, bar = su32(bars[w]);
+  if (lane < ST) tc5::bar_init(&bars[w][lane], 1);
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  __syncwarp();
+  Item is = it;
+  int to_issue = (int)(last - first), issued = 0, waited = 0;
+  int is_left = it.nt - (int)(first - start);                        // tiles of the item still to be looked up
+  int is_slot = (it.k0 + (int)(first - start)) * TILE + w * STEP;     // the warp's first token of the tile
+  const int* is_table = c.table + (int64_t)is.b * c.W;
+  // the page of the warp's 16 tokens of a tile: -2 nothing to see there, -1 not a page of the pool
+  int pg;
+  auto look_up = [&]() {
+    pg = -2;
+    if (is_slot < is.hi && is_slot + STEP > is.lo) {
+      const int j = is_slot >> c.shift;
+      pg = j < c.W ? is_table[j] : -1;
+    }
+  };
+  look_up();
+  int flying = 0;                        // bit i: the i-th next tile's tokens are there
+  bool ok = true;
+  auto issue = [&](uint32_t stage_at, uint32_t bar_at) {
+    flying >>= 1;
+    if (to_issue <= 0) return;
+    ++issued;
+    const bool there = (unsigned)pg < (unsigned)c.P;
+    if (there) flying |= 1 << (ST - 1);
+    if (lane == 0) {
+      if (there) {
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar_at), "r"(SB) : "memory");
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                     ::"r"(stage_at), "l"(block_of<HD>(c, pg, is.g, is_slot)), "r"(SB), "r"(bar_at) : "memory");
+      } else {
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar_at) : "memory");
+        if (pg != -2) record(ERR_PAGE);
+      }
+    }
+    if (--to_issue > 0) {
+      is_slot += TILE;
+      if (--is_left == 0) {
+        next_item<ROWS>(p, is);
+        is_left = is.nt;
+        is_slot = is.k0 * TILE + w * STEP;
+        is_table = c.table + (int64_t)is.b * c.W;
+      }
+      look_up();
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < ST - 1; ++s) issue(ring + s * SB, bar + s * 8);
+
+  // ---- state of the current item ----
+  uint32_t qf[NR][MT][2];
+  float rs[NR][2];                        // score factor of rows 2 t4, 2 t4 + 1
+  int lim[NR][2], low[NR][2];             // slots (low, lim] that the row sees
+  int all_lo = 0, all_hi = 0;             // slots [all_lo, all_hi] that every row sees
+  float r[NR][2], l[NR][2], o[NR][MT][4]; // weights are 2^(score - r), at most 2^(LIFT + LAZY)
+  float* scores_at = nullptr;             // of slot 0 and this lane's first row
+  auto load_rows = [&]() {
+    const int per = p.rep * p.maps, at0 = it.len - it.n;
+    if (p.scores) scores_at = it.rows <= p.stride ? p.scores + ((int64_t)it.b * c.G + it.g) * p.cap * p.stride + 2 * t4 : nullptr;
+    all_hi = min(it.len - 1, at0 + it.rt * ROWS / per);
+    all_lo = p.window > 0 ? at0 + min(it.n - 1, (it.rt * ROWS + ROWS - 1) / per) - p.window + 1 : 0;
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+      const int row = it.rt * ROWS + nr * 8 + g8;
+      float f[KW][8];
+      float mx = 0.f;
+      if (row < it.rows) {
+        const int i = row / per, h = it.g * p.rep + (row % per) / p.maps, map = row % p.maps;
+        const T* q = map ? (const T*)p.q2 + (int64_t)(it.t0 + i) * p.st2 + (int64_t)h * p.sh2
+                         : (const T*)p.q1 + (int64_t)(it.t0 + i) * p.st1 + (int64_t)h * p.sh1;
+#pragma unroll
+        for (int i2 = 0; i2 < KW / 2; ++i2) q_row16(q + t4 * (HD / 4) + 16 * i2, &f[2 * i2][0]);
+#pragma unroll
+        for (int i2 = 0; i2 < KW; ++i2)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fabsf(f[i2][j]));
+      } else {
+#pragma unroll
+        for (int i2 = 0; i2 < KW; ++i2)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[i2][j] = 0.f;
+      }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      // 2^e <= mx < 2^(e + 1); rows of zeros and rows with infinities stay as they are
+      int e = (int)(__float_as_uint(mx) >> 23) - 127;
+      if (e == -127 || e == 128) e = 0;
+      e = max(-126, min(126, e));
+      const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
+      // as the codes of a word are decoded: dims (0, 4) and (1, 5), then (2, 6) and (3, 7)
+#pragma unroll
+      for (int i2 = 0; i2 < KW; ++i2)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) qf[nr][2 * i2 + y][j] = pack_h2(f[i2][2 * y + j] * down, f[i2][2 * y + j + 4] * down);
+      const float mine_rs = p.scale_log2 * up;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        rs[nr][x] = __shfl_sync(0xffffffffu, mine_rs, (2 * t4 + x) * 4);
+        const int rr = it.rt * ROWS + nr * 8 + 2 * t4 + x;
+        // rows past the last one are rows of zeros that see everything: they ask for no mask and are not written
+        lim[nr][x] = rr < it.rows ? min(it.len - 1, it.len - it.n + rr / per) : 0x7fffffff;
+        low[nr][x] = rr < it.rows && p.window > 0 ? it.len - it.n + rr / per - p.window : -1;
+        r[nr][x] = NONE;
+        l[nr][x] = 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < MT; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[nr][j][x] = 0.f;
+    }
+  };
+
+  // K rows of this lane in the fragments: tokens g8 and g8 + 8, dims HD / 4 t4 ..;  V: tokens 2 t4, 2 t4 + 1 and the same
+  // + 8, dims HD / 8 g8 ..
+  const uint32_t k_at = g8 * (HD / 2) + t4 * (HD / 8), kp_at = PARAMS<HD> + g8 * (HD / 16);
+  const uint32_t v_at = HALF<HD> + 2 * t4 * (HD / 2) + g8 * (HD / 16), vp_at = HALF<HD> + PARAMS<HD> + 2 * t4 * (HD / 16);
+  auto scores = [&](uint32_t kb, int slot0, float (&s)[NR][4]) {
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) s[nr][x] = 0.f;
+    uint32_t kw[2][KW];
+    Levels lv[2][KW / 2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      if (HD == 128) {
+        const uint4 v = lds16(kb + k_at + x * 8 * (HD / 2));
+        const uint2 pw = lds8(kb + kp_at + x * 8 * (HD / 16));
+        kw[x][0] = v.x; kw[x][1] = v.y; kw[x][KW - 2] = v.z; kw[x][KW - 1] = v.w;
+        lv[x][0] = levels_of(pw.x); lv[x][KW / 2 - 1] = levels_of(pw.y);
+      } else {
+        const uint2 v = lds8(kb + k_at + x * 8 * (HD / 2));
+        kw[x][0] = v.x; kw[x][1] = v.y;
+        lv[x][0] = levels_of(lds4(kb + kp_at + x * 8 * (HD / 16)));
+      }
+    }
+    // S^T: word i holds runs 2 i, 2 i + 1 of the lane's dims, of groups (0, 1) or (2, 3)
+#pragma unroll
+    for (int i = 0; i < KW; ++i) {
+      uint32_t a[4], b[4];
+      decode(kw[0][i], lv[0][i % (KW / 2)], a);
+      decode(kw[1][i], lv[1][i % (KW / 2)], b);
+#pragma unroll
+      for (int nr = 0; nr < NR; ++nr) {
+        mma(s[nr], a[0], b[0], a[1], b[1], qf[nr][2 * i][0], qf[nr][2 * i][1]);
+        mma(s[nr], a[2], b[2], a[3], b[3], qf[nr][2 * i + 1][0], qf[nr][2 * i + 1][1]);
+      }
+    }
+    const bool all = slot0 + STEP - 1 <= all_hi && slot0 >= all_lo;
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        s[nr][x] *= rs[nr][x & 1];
+        if (!all) {
+          const int slot = slot0 + g8 + (x >> 1) * 8;
+          if (slot > lim[nr][x & 1] || slot <= low[nr][x & 1]) s[nr][x] = -INFINITY;
+        }
+      }
+    if (scores_at) {                              // rows 2 t4 and 2 t4 + 1 of tokens g8 and g8 + 8
+#pragma unroll
+      for (int nr = 0; nr < NR; ++nr)
+        if (nr * 8 + 2 * t4 < p.stride) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            *reinterpret_cast<float2*>(scores_at + (int64_t)(slot0 + g8 + 8 * x) * p.stride + nr * 8) = make_float2(s[nr][2 * x], s[nr][2 * x + 1]);
+        }
+    }
+  };
+  auto raise = [&](float (&s)[NR][4]) {
+    bool grow = false;
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) grow = grow || fmaxf(s[nr][x], s[nr][x + 2]) > r[nr][x] + (LIFT + LAZY);
+    if (!__any_sync(0xffffffffu, grow)) return;
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        float mx = fmaxf(s[nr][x], s[nr][x + 2]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float r1 = fmaxf(r[nr][x], mx - LIFT), f = ex2(r[nr][x] - r1);
+        r[nr][x] = r1;
+        l[nr][x] *= f;
+#pragma unroll
+        for (int j = 0; j < MT; ++j) { o[nr][j][x] *= f; o[nr][j][x + 2] *= f; }
+      }
+  };
+  // P V of one tile
+  auto values = [&](uint32_t vb, int slot0, float (&s)[NR][4]) {
+    uint32_t pf[NR][2];
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+      float e[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        e[x] = ex2(s[nr][x] - r[nr][x & 1]);
+        l[nr][x & 1] += e[x];
+      }
+      pf[nr][0] = transposed(pack_h2(e[0], e[1]));
+      pf[nr][1] = transposed(pack_h2(e[2], e[3]));
+    }
+    // O^T: tokens 2 t4 (x = 0), 2 t4 + 1, and the same + 8 (x = 2, 3)
+    uint32_t vw[4][VW], pw[4][VW];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int row = (x & 1) + (x >> 1) * 8;
+      if (HD == 128) {
+        const uint2 v = lds8(vb + v_at + row * (HD / 2)), u = lds8(vb + vp_at + row * (HD / 16));
+        vw[x][0] = v.x; vw[x][VW - 1] = v.y;
+        pw[x][0] = u.x; pw[x][VW - 1] = u.y;
+      } else {
+        vw[x][0] = lds4(vb + v_at + row * (HD / 2));
+        pw[x][0] = lds4(vb + vp_at + row * (HD / 16));
+      }
+    }
+    if (slot0 + 16 > it.hi) {                          // what is past the end may be anything: zeros
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (slot0 + 2 * t4 + (x & 1) + (x >> 1) * 8 >= it.hi) {
+#pragma unroll
+          for (int i = 0; i < VW; ++i) pw[x][i] = 0;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < VW; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {                    // the word's lower and upper four dims, of one group each
+        const uint32_t sel = h ? 0x7632u : 0x5410u;
+        uint32_t a[4], b[4];
+        decode(__byte_perm(vw[0][i], vw[1][i], sel), levels_of(__byte_perm(pw[0][i], pw[1][i], sel)), a);
+        decode(__byte_perm(vw[2][i], vw[3][i], sel), levels_of(__byte_perm(pw[2][i], pw[3][i], sel)), b);
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) {
+          mma(o[nr][4 * i + 2 * h], a[0], a[1], b[0], b[1], pf[nr][0], pf[nr][1]);          // dims HD / 8 g8 + 8 i + 4 h, + 1
+          mma(o[nr][4 * i + 2 * h + 1], a[2], a[3], b[2], b[3], pf[nr][0], pf[nr][1]);      // + 2, + 3
+        }
+      }
+  };
+
+  // Warps 3, 2, 1 pass their joined state on through shared memory, lane by lane; warp 0 writes the result.
+  float* merge = reinterpret_cast<float*>(smem + NW * ST * SB) + lane;
+  auto finish = [&](int64_t item_start, bool ends) {
+#pragma unroll 1
+    for (int turn = NW - 1; turn >= 0; --turn) {
+      if (w == turn && turn < NW - 1) {
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float mm = merge[(nr * 4 + x) * 32], M = fmaxf(r[nr][x], mm);
+            const float a = ex2(r[nr][x] - M), b = ex2(mm - M);
+            r[nr][x] = M;
+            l[nr][x] = fmaf(l[nr][x], a, merge[(nr * 4 + 2 + x) * 32] * b);
+#pragma unroll
+            for (int j = 0; j < MT; ++j)
+#pragma unroll
+              for (int z = x; z < 4; z += 2) o[nr][j][z] = fmaf(o[nr][j][z], a, merge[(NR * 4 + (nr * MT + j) * 4 + z) * 32] * b);
+          }
+      }
+      if (w == turn && turn > 0) {
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) { merge[(nr * 4 + x) * 32] = r[nr][x]; merge[(nr * 4 + 2 + x) * 32] = l[nr][x]; }
+#pragma unroll
+          for (int j = 0; j < MT; ++j)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) merge[(NR * 4 + (nr * MT + j) * 4 + x) * 32] = o[nr][j][x];
+        }
+      }
+      if (turn > 0) __syncthreads();
+    }
+    if (w == 0) {
+      const bool whole = ends && item_start >= first, cut = *(volatile int*)&s_cut != 0;
+      float* part = p.part + ((int64_t)blockIdx.x * 2 + (item_start > first ? 1 : 0)) * ROWS * (HD + 2);
+      const int per = p.rep * p.maps;
+#pragma unroll
+      for (int nr = 0; nr < NR; ++nr) {
+        float f0[2];                                     // 1 / sum over the row's lanes
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float M = r[nr][x];
+          float L = l[nr][x];
+          L += __shfl_xor_sync(0xffffffffu, L, 4);
+          L += __shfl_xor_sync(0xffffffffu, L, 8);
+          L += __shfl_xor_sync(0xffffffffu, L, 16);
+          if (cut) L = -1.f;                             // in a part: the join writes zeros
+          f0[x] = cut || L == 0.f ? 0.f : 1.f / L;
+          const int part_row = nr * 8 + 2 * t4 + x;
+          if (whole && p.lse && g8 == 0) {
+            const int row = it.rt * ROWS + part_row;
+            if (row < it.rows)
+              p.lse[(int64_t)(it.t0 + row / per) * p.H * p.maps + it.g * per + row % per] = cut || L == 0.f ? INFINITY : M + log2f(L);
+          }
+          if (!whole) {
+            float* dst = part + part_row * (HD + 2);
+#pragma unroll
+            for (int j = 0; j < MT; ++j)
+              *reinterpret_cast<float2*>(dst + g8 * (HD / 8) + 2 * j) = make_float2(o[nr][j][x], o[nr][j][x + 2]);
+            if (g8 == 0) *reinterpret_cast<float2*>(dst + HD) = make_float2(M, L);
+          }
+        }
+        if (!whole) continue;
+        // rows 2 t4 and 2 t4 + 1 are two heads, or the two maps of one
+        const int row = it.rt * ROWS + nr * 8 + 2 * t4;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (row + x >= it.rows || (x == 1 && p.maps == 2)) continue;
+          const int tok = it.t0 + (row + x) / per, h = it.g * p.rep + (row + x) % per / p.maps;
+          float wa = f0[x], wb = 0.f;
+          if (p.maps == 2) {
+            const float lam = p.lam[h], den = 1.f / (1.f - lam + 1e-8f);
+            wa *= den;
+            wb = -lam * den * f0[1];
+          }
+          T* out = (T*)p.out + ((int64_t)tok * p.H + h) * HD + g8 * (HD / 8);
+#pragma unroll
+          for (int j = 0; j < MT; j += 4) {
+            Vec16<T> v;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float a0 = o[nr][j + k][x] * wa, a1 = o[nr][j + k][x + 2] * wa;
+              v.v[2 * k] = from_f<T>(p.maps == 2 ? fmaf(o[nr][j + k][1], wb, a0) : a0);
+              v.v[2 * k + 1] = from_f<T>(p.maps == 2 ? fmaf(o[nr][j + k][3], wb, a1) : a1);
+            }
+            st16(out + 2 * j, v);
+          }
+        }
+      }
+      if (ends && !whole && lane == 0) {
+        const int64_t c0 = item_start / share;       // CTA and place of the item's first part
+        p.joins[blockIdx.x] = make_int4(it.t0, it.rows, it.g | it.rt << 16, (int)(2 * c0 + (item_start > c0 * share ? 1 : 0)));
+      }
+    }
+    __syncthreads();
+  };
+
+  load_rows();
+  int tiles = it.nt - (int)(first - start);                           // of the item, still to be done
+  int slot0 = (it.k0 + (int)(first - start)) * TILE + w * STEP;
+  uint32_t here = ring, bar_here = bar, phase = 0, there = ring + (ST - 1) * SB, bar_there = bar + (ST - 1) * 8;
+  for (int left = (int)(last - first); left > 0; --left) {
+    if (ok) {
+      issue(there, bar_there);
+      ok = wait_tile(bar_here, phase, p.wait);
+      waited += ok;
+      if (!ok) s_cut = 1;                          // this item's rows and the next ones' are zeros
+    }
+    if (ok && (flying & 1)) {
+      float s[NR][4];
+      scores(here, slot0, s);
+      raise(s);
+      values(here, slot0, s);
+    }
+    __syncwarp();                                  // the tile is read before its place is filled again
+    there = here;
+    bar_there = bar_here;
+    here += SB;
+    bar_here += 8;
+    if (here == ring + ST * SB) { here = ring; bar_here = bar; phase ^= 1; }
+    slot0 += TILE;
+    if (--tiles == 0 || left == 1) {
+      finish(start, tiles == 0);
+      if (left > 1) {
+        start += it.nt;
+        next_item<ROWS>(p, it);
+        tiles = it.nt;
+        slot0 = it.k0 * TILE + w * STEP;
+        load_rows();
+      }
+    }
+  }
+  // after a wait that ran out: the copies that are still under way into this CTA's memory
+  for (; waited < issued; ++waited) drain_tile(bar + waited % ST * 8, (uint32_t)(waited / ST & 1));
+}
+
+// ---- received weights ------------------------------------------------------------------------------
+// From the scores that the split kernel has left: a thread per slot.
+constexpr int NK = 256;
+__global__ void __launch_bounds__(NK) kept_weights_kernel(const __grid_constant__ Params p) {
+  const Cache4& c = p.c;
+  const int g = blockIdx.y, b = blockIdx.z;
+  Item it;
+  if (!in_order(c, b) || !set_sequence<2 * 8>(p, it, b) || it.rows > p.stride) return;
+  const int per = p.rep * p.maps;
+  const float* lse = p.lse + (int64_t)it.t0 * p.H * p.maps + g * per;
+  for (int slot = it.lo / STEP * STEP + blockIdx.x * NK + threadIdx.x; slot < it.hi; slot += gridDim.x * NK) {
+    const int pg = c.table[(int64_t)b * c.W + (slot >> c.shift)];
+    if (pg < 0 || pg >= c.P) continue;                  // recorded where its keys were looked for
+    const float* s = p.scores + (((int64_t)b * c.G + g) * p.cap + slot) * p.stride;
+    float sum = 0.f;
+    for (int row = 0; row < it.rows; ++row) {
+      const float of = lse[(int64_t)(row / per) * p.H * p.maps + row % per];
+      if (of != INFINITY) sum += ex2(s[row] - of);      // rows cut short have not left all of their scores
+    }
+    c.mass[(((int64_t)pg * c.G + g) << c.shift) + (slot & (c.page - 1))] += sum;
+  }
+}
+
+// From the keys, for sequences of more rows: a CTA takes 256 slots of a KV head, 32 per warp, whose keys stay in registers
+// as the M rows of the products while all rows of the sequence that see some of them pass by in tiles of 64 as N.
+constexpr int WW = 8, WK = 32, WR = 64;          // warps, slots of a warp, rows of a tile
+template <typename T, int HD>
+__global__ void __launch_bounds__(WW * 32) weights_kernel(const __grid_constant__ Params p) {
+  constexpr int KW = HD / 32, MT = HD / 16, QS = HD / 2 + 4;       // QS: words of a row, with a shift of banks
+  const Cache4& c = p.c;
+  const int g = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g8 = lane >> 2, t4 = lane & 3;
+  if (!in_order(c, b)) return;
+  const int t0 = c.cu[b], n = c.cu[b + 1] - t0, per = p.rep * p.maps, len = cached_length(c, c.lens[b]);
+  const int64_t rows = (int64_t)n * per;
+  if (rows == 0 || rows <= p.stride || (rows > p.few && !p.chunked)) return;      // the other kernel's, or left out altogether
+  const int at0 = len - n, base = blockIdx.x * (WW * WK);
+  if (base >= len) return;
+  // tokens [i0, i1) see some slot of the CTA's
+  const int i0 = max(0, base - at0);
+  const int last = min(base + WW * WK, len) - 1;
+  const int i1 = p.window > 0 ? (int)min((int64_t)n, (int64_t)last + p.window - at0) : n;
+  if (i0 >= i1) return;
+  __shared__ __align__(16) uint32_t q[WR * QS];
+  __shared__ float factor[WR], sum_of[WR];
+  __shared__ int sees[WR];                          // the row's slot
+
+  // keys: word i of tokens g8, g8 + 8 of each block
+  const int slot0 = base + w * WK;
+  uint32_t a[WK / 16][MT][4];
+  int pages[WK / 16];
+#pragma unroll
+  for (int m = 0; m < WK / 16; ++m) {
+    const int slot = slot0 + 16 * m;
+    int pg = -1;
+    if (slot < len) {
+      pg = c.table[(int64_t)b * c.W + (slot >> c.shift)];
+      if (pg < 0 || pg >= c.P) pg = -1;
+    }
+    pages[m] = pg;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int row = g8 + 8 * x;
+      const bool there = pg >= 0 && slot + row < len;
+#pragma unroll
+      for (int i = 0; i < KW; ++i) {
+        uint32_t word = 0, params = 0;
+        if (there) {
+          const uint8_t* blk = block_of<HD>(c, pg, g, slot);
+          word = *reinterpret_cast<const uint32_t*>(blk + row * (HD / 2) + t4 * (HD / 8) + 4 * i);
+          params = *reinterpret_cast<const uint32_t*>(blk + PARAMS<HD> + row * (HD / 16) + 4 * (i % (KW / 2)));
+        }
+        uint32_t h[4];
+        decode(word, levels_of(params), h);
+        a[m][2 * i][x] = h[0];
+        a[m][2 * i][x + 2] = h[1];
+        a[m][2 * i + 1][x] = h[2];
+        a[m][2 * i + 1][x + 2] = h[3];
+      }
+    }
+  }
+  float sum[WK / 16][2] = {};
+  const int64_t end = (int64_t)i1 * per;
+  for (int64_t first = (int64_t)i0 * per; first < end; first += WR) {
+    __syncthreads();
+    // four threads a row: dims HD / 4 (tid & 3) .., in the order of the keys' fragments
+    {
+      const int64_t row = first + (tid >> 2);
+      const int i = (int)(row / per), j = (int)(row % per), h = g * p.rep + j / p.maps, map = j % p.maps;
+      float f[KW][8], mx = 0.f;
+      const bool there = row < end;
+      if (there) {
+        const T* src = map ? (const T*)p.q2 + (int64_t)(t0 + i) * p.st2 + (int64_t)h * p.sh2
+                           : (const T*)p.q1 + (int64_t)(t0 + i) * p.st1 + (int64_t)h * p.sh1;
+#pragma unroll
+        for (int x = 0; x < KW / 2; ++x) q_row16(src + (tid & 3) * (HD / 4) + 16 * x, &f[2 * x][0]);
+      } else {
+#pragma unroll
+        for (int x = 0; x < KW; ++x)
+#pragma unroll
+          for (int y = 0; y < 8; ++y) f[x][y] = 0.f;
+      }
+#pragma unroll
+      for (int x = 0; x < KW; ++x)
+#pragma unroll
+        for (int y = 0; y < 8; ++y) mx = fmaxf(mx, fabsf(f[x][y]));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      int e = (int)(__float_as_uint(mx) >> 23) - 127;
+      if (e == -127 || e == 128) e = 0;
+      e = max(-126, min(126, e));
+      const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
+      uint32_t* to = q + (tid >> 2) * QS + (tid & 3) * (HD / 8);
+#pragma unroll
+      for (int x = 0; x < KW; ++x)
+        *reinterpret_cast<uint4*>(to + 4 * x) = make_uint4(pack_h2(f[x][0] * down, f[x][4] * down), pack_h2(f[x][1] * down, f[x][5] * down),
+                                                           pack_h2(f[x][2] * down, f[x][6] * down), pack_h2(f[x][3] * down, f[x][7] * down));
+      if ((tid & 3) == 0) {
+        factor[tid >> 2] = p.scale_log2 * up;
+        sum_of[tid >> 2] = there ? p.lse[(int64_t)(t0 + i) * p.H * p.maps + g * per + j] : INFINITY;
+        sees[tid >> 2] = at0 + i;
+      }
+    }
+    __syncthreads();
+    const int low_row = sees[0], high_row = (int)(at0 + (min(first + WR, end) - 1) / per);
+    const bool all = slot0 + WK - 1 <= low_row && (p.window == 0 || slot0 > high_row - p.window);
+    if (slot0 > high_row) continue;
+#pragma unroll 1
+    for (int col = 0; col < WR; col += 8) {
+      float s[WK / 16][4] = {};
+      const uint32_t* src = q + (col + g8) * QS + t4 * (HD / 8);
+#pragma unroll
+      for (int i = 0; i < KW; ++i) {
+        const uint4 v = *reinterpret_cast<const uint4*>(src + 4 * i);
+#pragma unroll
+        for (int m = 0; m < WK / 16; ++m) {
+          mma(s[m], a[m][2 * i][0], a[m][2 * i][1], a[m][2 * i][2], a[m][2 * i][3], v.x, v.y);
+          mma(s[m], a[m][2 * i + 1][0], a[m][2 * i + 1][1], a[m][2 * i + 1][2], a[m][2 * i + 1][3], v.z, v.w);
+        }
+      }
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {                    // rows col + 2 t4, + 1
+        const int rr = col + 2 * t4 + y;
+        const float f = factor[rr], ls = sum_of[rr];
+        const int at = sees[rr];
+#pragma unroll
+        for (int m = 0; m < WK / 16; ++m)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int slot = slot0 + 16 * m + g8 + 8 * x;
+            const float e = ex2(fmaf(s[m][y + 2 * x], f, -ls));
+            if (all || (slot <= at && (p.window == 0 || slot > at - p.window))) sum[m][x] += e;
+          }
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < WK / 16; ++m)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      float v = sum[m][x];
+      v += __shfl_xor_sync(0xffffffffu, v, 1);
+      v += __shfl_xor_sync(0xffffffffu, v, 2);
+      const int slot = slot0 + 16 * m + g8 + 8 * x;
+      if (t4 == 0 && pages[m] >= 0 && slot < len)
+        c.mass[(((int64_t)pages[m] * c.G + g) << c.shift) + (slot & (c.page - 1))] += v;
+    }
+}
+
+template <typename T, int HD, int NR>
+void launch_split(const Params& p) {
+  auto fn = split_kernel<T, HD, NR>;
+  constexpr int SMEM = smem_bytes<HD, NR>();
+  static bool set[64] = {};                              // by device; the attribute stays
+  int dev = 0;
+  MAMF_CUDA_CHECK(cudaGetDevice(&dev));
+  if (dev >= 64 || !set[dev]) {
+    MAMF_CUDA_CHECK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+    if (dev < 64) set[dev] = true;
+  }
+  fn<<<p.ctas, NT, SMEM, stream()>>>(p);
+  MAMF_LAUNCH_CHECK();
+  launch_join<T, HD, NR>(p);
+}
+
+}  // namespace pa4
+
+// q1, q2 (T, H, hd) bf16 or f16 packed queries -> (T, H, hd)
+at::Tensor paged4_attention(at::Tensor q1, c10::optional<at::Tensor> q2, c10::optional<at::Tensor> lam, at::Tensor blocks,
+                            c10::optional<at::Tensor> mass, at::Tensor table, at::Tensor cu, at::Tensor lens,
+                            int64_t max_new, int64_t window, double scale) {
+  using namespace pa4;
+  TORCH_CHECK(q1.is_cuda() && q1.dim() == 3 && q1.device() == blocks.device() && (q1.scalar_type() == at::kBFloat16 || q1.scalar_type() == at::kHalf),
+              "paged_attention: bf16 or f16 queries (T, H, hd) on the cache's GPU");
+  c10::cuda::CUDAGuard guard(q1.device());
+  const int64_t T = q1.size(0), H = q1.size(1), hd = q1.size(2);
+  Params p{};
+  p.c = check_cache4("paged_attention", blocks, mass, table, &cu, lens, T, hd);
+  TORCH_CHECK(H >= 1 && p.c.G >= 1 && H % p.c.G == 0, "paged_attention: ", H, " query heads over ", p.c.G, " KV heads");
+  TORCH_CHECK(std::isfinite((float)(scale * 1.4426950408889634)), "paged_attention: a finite scale, got ", scale);
+  TORCH_CHECK(window >= 0 && max_new >= 0, "paged_attention: window and max_new must not be negative");
+  q1 = rows16(q1);
+  p.q1 = q1.data_ptr(); p.st1 = q1.stride(0); p.sh1 = q1.stride(1);
+  if (q2.has_value()) {
+    TORCH_CHECK(lam.has_value() && q2->is_cuda() && q2->device() == q1.device() && q2->sizes() == q1.sizes() && q2->scalar_type() == q1.scalar_type(),
+                "paged_attention: q2 like q1, with lam");
+    TORCH_CHECK(lam->is_cuda() && lam->device() == q1.device() && lam->scalar_type() == at::kFloat && lam->is_contiguous() && lam->numel() == H,
+                "paged_attention: fp32 lam (H)");
+    q2 = rows16(*q2);
+    p.q2 = q2->data_ptr(); p.st2 = q2->stride(0); p.sh2 = q2->stride(1);
+    p.lam = lam->data_ptr<float>();
+  } else {
+    TORCH_CHECK(!lam.has_value(), "paged_attention: lam without q2");
+  }
+  at::Tensor out = at::empty({T, H, hd}, q1.options());
+  if (T == 0) return out;
+  TORCH_CHECK(p.c.P >= 1, "paged_attention: a pool without pages");
+  p.out = out.data_ptr();
+  p.H = (int)H;
+  p.window = (int)std::min<int64_t>(window, 1LL << 30);
+  p.scale_log2 = (float)(scale * 1.4426950408889634);
+  p.wait = attention_wait_limit();
+  p.rep = (int)(H / p.c.G);
+  p.maps = p.q2 ? 2 : 1;
+  p.cap = (int64_t)p.c.W * p.c.page;
+  TORCH_CHECK(T * H < (1LL << 31), "paged_attention: sizes");
+  // Sequences of up to FEW rows go to the split kernel, longer runs of tokens to the chunk kernel; where all
+  // have the same number of tokens one of them does everything.
+  const int64_t most_rows = std::max<int64_t>(1, std::min(max_new, T)) * p.rep * p.maps;
+  p.chunked = most_rows > FEW && p.c.B > 0;
+  const bool alone = p.chunked && T == p.c.B * max_new;
+  p.few = alone ? 0 : (int)std::min<int64_t>(most_rows, FEW);
+  at::Tensor sums, kept;
+  if (mass.has_value() && p.c.B > 0) {
+    TORCH_CHECK(p.c.B < 65536, "paged_attention: received weights of at most 65535 sequences");
+    sums = at::empty({T, H, p.maps}, q1.options().dtype(at::kFloat));
+    p.lse = sums.data_ptr<float>();
+    if (!alone) {
+      p.stride = (int)((std::min<int64_t>(p.few, KEEP) + 1) / 2 * 2);
+      kept = at::empty({p.c.B * (int64_t)p.c.G * p.cap * p.stride}, q1.options().dtype(at::kFloat));
+      p.scores = kept.data_ptr<float>();
+    }
+  }
+  const bool bf16 = q1.scalar_type() == at::kBFloat16;
+  if (p.chunked) chunk_attention(p, (int)hd, bf16);
+  if (!alone) {
+    // one query row tile holds 8 rows, or 16 where a sequence can have more than 8
+    const int nr = p.few > 8 ? 2 : 1, rows = 8 * nr;
+    const int64_t row_tiles = (p.few + rows - 1) / rows;
+    const int64_t most = std::max<int64_t>(1, (int64_t)p.c.B * p.c.G * row_tiles * std::max<int64_t>(1, (p.cap + TILE - 1) / TILE));
+    p.ctas = (int)std::min<int64_t>(most, (nr == 1 ? residents<128, 1>() : hd == 64 ? residents<64, 2>() : residents<128, 2>()) * num_sms());
+    const int64_t part = (int64_t)p.ctas * 2 * rows * (hd + 2);
+    at::Tensor ws = at::empty({part + 4 * p.ctas}, q1.options().dtype(at::kFloat));
+    p.joins = reinterpret_cast<int4*>(ws.data_ptr<float>());
+    p.part = ws.data_ptr<float>() + 4 * p.ctas;
+    auto go = [&](auto t) {
+      using E = decltype(t);
+      if (hd == 128) { if (nr == 1) launch_split<E, 128, 1>(p); else launch_split<E, 128, 2>(p); }
+      else { if (nr == 1) launch_split<E, 64, 1>(p); else launch_split<E, 64, 2>(p); }
+    };
+    if (bf16) go(__nv_bfloat16()); else go(__half());
+  }
+  if (p.lse) {
+    if (p.scores) {
+      kept_weights_kernel<<<dim3((unsigned)((p.cap + 4 * NK - 1) / (4 * NK)), (unsigned)p.c.G, (unsigned)p.c.B), NK, 0, stream()>>>(p);
+      MAMF_LAUNCH_CHECK();
+    }
+    if (most_rows > p.stride) {
+      const dim3 grid((unsigned)((p.cap + WW * WK - 1) / (WW * WK)), (unsigned)p.c.G, (unsigned)p.c.B);
+      if (hd == 128) { if (bf16) weights_kernel<__nv_bfloat16, 128><<<grid, WW * 32, 0, stream()>>>(p); else weights_kernel<__half, 128><<<grid, WW * 32, 0, stream()>>>(p); }
+      else { if (bf16) weights_kernel<__nv_bfloat16, 64><<<grid, WW * 32, 0, stream()>>>(p); else weights_kernel<__half, 64><<<grid, WW * 32, 0, stream()>>>(p); }
+      MAMF_LAUNCH_CHECK();
+    }
+  }
+  return out;
+}
+
+int64_t paged4_attention_error(bool clear) {
+  return paged::take_code(split::g_err, clear) | paged::take_code(split::g_wait_err, clear) | paged4::chunk_error(clear);
+}
+
+}  // namespace mamf

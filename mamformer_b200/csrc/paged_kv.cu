@@ -1,4 +1,4 @@
-// Appending keys and values to the paged 8-bit cache, with the rotation of the keys (and of up to two
+// Appending keys and values to the paged caches, with the rotation of the keys (and of up to two
 // query tensors) on the way.  The reference grows (B, S, G, hd) tensors with torch.cat each step
 // (mamformer/layers/attention.py:143-149, kda_diff.py:813-818) and rotates in a pass of its own.
 //
@@ -20,7 +20,7 @@
 // 20,000 prompt tokens, 8 KV heads and two query tensors of 32 heads of 128 (792 MB): 156 us, 5.1 TB/s; the CTAs
 // alternate between loads and stores.  One token each of 200 sequences: 10 us, the chain offsets - table -
 // scale - rotation and the launch.
-#include "paged.cuh"
+#include "paged4.cuh"
 
 namespace mamf {
 namespace kva {
@@ -34,14 +34,20 @@ __device__ __forceinline__ void record(int code) { atomicCAS(&g_err, 0, code); }
 
 struct Src { const void* p; int64_t st, sh; };       // token and head strides in elements
 
-struct Params {
-  Cache c;
+struct Rows {
   Src k, v, q[2];
   void* qo[2];
   const float *cos, *sin;                            // (n_pos, hd / 2) with row stride rot, null: no rotation
   int64_t rot;
   const int64_t* pos;                                // (T)
-  int n_pos, H, units, per_seq, max_new, nq;
+  int n_pos, H, nq, units;
+};
+struct Params : Rows {
+  Cache c;
+  int per_seq, max_new;
+};
+struct Params4 : Rows {
+  paged4::Cache4 c;
 };
 
 // 8 consecutive values of a token's head as floats
@@ -68,7 +74,7 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const float* 
 // cos and sin of 8 dims at token t's position
 struct Turn { float c[8], s[8]; };
 template <int HD>
-__device__ __forceinline__ Turn turn_of(const Params& p, int t, int d) {
+__device__ __forceinline__ Turn turn_of(const Rows& p, int t, int d) {
   int64_t pos = p.pos[t];
   if (pos < 0 || pos >= p.n_pos) { record(ERR_POSITION); pos = pos < 0 ? 0 : p.n_pos - 1; }
   Turn r;
@@ -210,10 +216,10 @@ __device__ __forceinline__ void append_block(const Params& p) {
 // One token per CTA at a time; a thread takes the same 16 dims of its heads in every tensor.  The rows are
 // requested before the position, whose load the tables' loads wait for.
 template <typename T, int HD>
-__device__ __forceinline__ void rotate_queries(const Params& p, int block, int blocks) {
+__device__ __forceinline__ void rotate_queries(const Rows& p, int tokens, int block, int blocks) {
   constexpr int TPT = HD / 16;
   const int d = (threadIdx.x % TPT) * 8;
-  for (int t = block; t < p.c.T; t += blocks)
+  for (int t = block; t < tokens; t += blocks)
     for (int h = threadIdx.x / TPT; h < p.H; h += NT / TPT) {
       constexpr int N = 16 / sizeof(T), L = 16 / N;
       Vec16<T> raw[2][L];
@@ -244,7 +250,7 @@ __global__ void __launch_bounds__(NT, NP == 1 ? 4 : NP == 2 ? 3 : 2) append_kern
   if ((int)blockIdx.x < p.units) append_block<T, HD, NP>(p);
   else {
     const int qb = gridDim.x - p.units, layer = blockIdx.y + gridDim.y * blockIdx.z;
-    rotate_queries<T, HD>(p, (blockIdx.x - p.units) + qb * layer, qb * gridDim.y * gridDim.z);
+    rotate_queries<T, HD>(p, p.c.T, (blockIdx.x - p.units) + qb * layer, qb * gridDim.y * gridDim.z);
   }
 }
 
@@ -253,7 +259,7 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(NT, 4) append_one_kernel(const __grid_constant__ Params p) {
   constexpr int TPT = HD / 16;
   if ((int)blockIdx.x >= p.units) {
-    rotate_queries<T, HD>(p, blockIdx.x - p.units, gridDim.x - p.units);
+    rotate_queries<T, HD>(p, p.c.T, blockIdx.x - p.units, gridDim.x - p.units);
     return;
   }
   const Cache& c = p.c;
@@ -328,23 +334,11 @@ void launch(Params& p) {
   else append_kernel<T, HD, 4><<<grid, NT, 0, stream()>>>(p);
 }
 
-}  // namespace kva
-
-// k, v (T, G, hd), queries (T, H, hd): packed new tokens of any strides (rows that are not on 16-byte
-// boundaries are copied first).  Writes the cache; returns the rotated queries, contiguous.
-std::vector<at::Tensor> kv_append(at::Tensor k, at::Tensor v, at::Tensor ck, at::Tensor cv, at::Tensor ks, at::Tensor vs,
-                                  at::Tensor table, at::Tensor cu, at::Tensor lens, int64_t max_new,
-                                  c10::optional<at::Tensor> cos, c10::optional<at::Tensor> sin,
-                                  c10::optional<at::Tensor> pos, std::vector<at::Tensor> queries) {
-  using namespace kva;
-  TORCH_CHECK(k.is_cuda() && k.dim() == 3 && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() &&
-              k.device() == ck.device() && v.device() == ck.device(), "kv_append: k and v (T, G, hd) of one type on the cache's GPU");
-  c10::cuda::CUDAGuard guard(k.device());
+// The inputs' pointers, and room for the rotated queries.  Tensors whose rows are not on 16-byte boundaries are replaced by
+// copies.
+std::vector<at::Tensor> take_rows(Rows& p, at::Tensor& k, at::Tensor& v, c10::optional<at::Tensor>& cos,
+                                  c10::optional<at::Tensor>& sin, c10::optional<at::Tensor>& pos, std::vector<at::Tensor>& queries) {
   const int64_t T = k.size(0), hd = k.size(2);
-  Params p{};
-  p.c = check_cache("kv_append", Layer{ck, cv, ks, vs, table, cu, lens}, T, hd);
-  TORCH_CHECK(k.size(1) == p.c.G, "kv_append: ", p.c.G, " KV heads in the cache, got ", k.size(1));
-  TORCH_CHECK(max_new >= 0, "kv_append: max_new must not be negative");
   auto src = [&](at::Tensor& t) {
     t = rows16(t);
     return Src{t.data_ptr(), t.stride(0), t.stride(1)};
@@ -373,16 +367,173 @@ std::vector<at::Tensor> kv_append(at::Tensor k, at::Tensor v, at::Tensor ck, at:
                 q.scalar_type() == k.scalar_type() && q.sizes() == queries[0].sizes(), "kv_append: queries (T, H, hd) of k's type");
     outs.push_back(at::empty(q.sizes(), q.options(), at::MemoryFormat::Contiguous));
   }
-  if (T == 0 || p.c.B == 0) return outs;
   p.k = src(k);
   p.v = src(v);
   p.nq = (int)queries.size();
   for (int i = 0; i < p.nq; ++i) { p.q[i] = src(queries[i]); p.qo[i] = outs[i].data_ptr(); }
   p.H = p.nq ? (int)queries[0].size(1) : 0;
+  return outs;
+}
+
+// ---- the 4-bit cache -------------------------------------------------------------------------------
+// 16 values of a token (8 of each half, from dim d) of keys or values: parameters by all lanes of the token together,
+// codes and, by one lane or two, the parameters into the block.  Dims d .. d + 3 and d + 4 .. d + 7 are of two groups.
+template <int HD>
+__device__ __forceinline__ void put_codes4(uint8_t* half_block, int row, int sub, float* x) {
+  using namespace paged4;
+  constexpr int J = HD / 32;
+  float lo[2], hi[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    lo[r] = hi[r] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float& y = x[8 * h + 4 * r + e];
+        y = storable(y);
+        lo[r] = fminf(lo[r], y);
+        hi[r] = fmaxf(hi[r], y);
+      }
+  }
+  // the lanes whose runs are of the same two groups: every second one of 8 for four groups, all 4 for two
+#pragma unroll
+  for (int o = HD / 32; o >= J / 2; o >>= 1)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      lo[r] = fminf(lo[r], __shfl_xor_sync(0xffffffffu, lo[r], o));
+      hi[r] = fmaxf(hi[r], __shfl_xor_sync(0xffffffffu, hi[r], o));
+    }
+  const Group g[2] = {group_of(lo[0], hi[0]), group_of(lo[1], hi[1])};
+  if (half_block == nullptr) return;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w |= code_of(x[8 * h + e], g[e / 4]) << (4 * e);
+    *reinterpret_cast<uint32_t*>(half_block + row * (HD / 2) + h * (HD / 4) + sub * 4) = w;
+  }
+  if (sub < J / 2) *reinterpret_cast<uint32_t*>(half_block + PARAMS<HD> + (row * (J / 2) + sub) * 4) = param_of(g[0]) | param_of(g[1]) << 16;
+}
+
+// A group of TPT lanes does the keys and values of one token, of every gridDim.y-th head.
+template <typename T, int HD>
+__global__ void __launch_bounds__(NT, 3) append4_kernel(const __grid_constant__ Params4 p) {
+  constexpr int TPT = HD / 16;
+  if ((int)blockIdx.x >= p.units) {
+    const int qb = gridDim.x - p.units;
+    rotate_queries<T, HD>(p, p.c.T, (blockIdx.x - p.units) + qb * blockIdx.y, qb * gridDim.y);
+    return;
+  }
+  const paged4::Cache4& c = p.c;
+  if (blockIdx.x + blockIdx.y == 0)
+    for (int b = threadIdx.x; b < c.B; b += NT)
+      if (!in_order(c, b)) record(ERR_LENGTH);
+  const int sub = threadIdx.x % TPT, d = sub * 8;
+  const int64_t item = ((int64_t)blockIdx.x * NT + threadIdx.x) / TPT;
+  const int t = (int)min(item, (int64_t)c.T);
+  bool ok = t < c.T;
+  int b = -1, slot = 0, pg = -1;
+  if (ok) {
+    // the usual step: every sequence has one token
+    b = t < c.B && c.cu[t] == t && c.cu[t + 1] == t + 1 ? t : sequence_of(c.cu, c.B, t);
+    ok = b >= 0;
+  }
+  if (ok) {
+    const int t0 = c.cu[b], n = c.cu[b + 1] - t0, end = c.lens[b];
+    slot = end - n + (t - t0);
+    ok = in_order(c, b) && t >= t0 && t - t0 < n && end - n >= 0;
+    if (!ok && sub == 0) record(ERR_LENGTH);
+  }
+  if (ok) {
+    const int j = slot >> c.shift;
+    pg = j < c.W ? c.table[(int64_t)b * c.W + j] : -1;
+    ok = pg >= 0 && pg < c.P;
+    if (!ok && sub == 0) record(ERR_PAGE);
+  }
+  const bool turn_keys = p.cos != nullptr;
+  Turn turn;
+  if (ok && turn_keys) turn = turn_of<HD>(p, t, d);
+  // all lanes of a warp stay in the loop for its shuffles
+  for (int g = blockIdx.y; g < c.G; g += gridDim.y) {
+    float x[16], y[16];
+    uint8_t* blk = nullptr;
+    if (ok) {
+      const T* k = (const T*)p.k.p + (int64_t)t * p.k.st + (int64_t)g * p.k.sh + d;
+      const T* v = (const T*)p.v.p + (int64_t)t * p.v.st + (int64_t)g * p.v.sh + d;
+      load8(k, x);
+      load8(k + HD / 2, x + 8);
+      load8(v, y);
+      load8(v + HD / 2, y + 8);
+      if (turn_keys) rotate8(turn, x, x + 8);
+      blk = paged4::block_of<HD>(c, pg, g, slot);
+      if (c.mass && sub == 0) c.mass[(((int64_t)pg * c.G + g) << c.shift) + (slot & (c.page - 1))] = 0.f;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] = y[e] = 0.f;
+    }
+    put_codes4<HD>(blk, slot & 15, sub, x);
+    put_codes4<HD>(blk ? blk + paged4::HALF<HD> : nullptr, slot & 15, sub, y);
+  }
+}
+
+template <typename T, int HD>
+void launch4(Params4& p) {
+  p.units = (int)(((int64_t)p.c.T * (HD / 16) + NT - 1) / NT);
+  const int64_t qblocks = p.nq ? std::min<int64_t>(p.c.T, 1 << 16) : 0;
+  // as many ways to share the heads as give every SM some CTAs: the look-ups in front of a token's heads are paid per way
+  const int ways = (int)std::max<int64_t>(1, std::min<int64_t>(p.c.G, 8LL * num_sms() / p.units));
+  const dim3 grid((unsigned)(p.units + (qblocks + ways - 1) / ways), (unsigned)ways);
+  append4_kernel<T, HD><<<grid, NT, 0, stream()>>>(p);
+}
+
+}  // namespace kva
+
+// k, v (T, G, hd), queries (T, H, hd): packed new tokens of any strides (rows that are not on 16-byte
+// boundaries are copied first).  Writes the cache; returns the rotated queries, contiguous.
+std::vector<at::Tensor> kv_append(at::Tensor k, at::Tensor v, at::Tensor ck, at::Tensor cv, at::Tensor ks, at::Tensor vs,
+                                  at::Tensor table, at::Tensor cu, at::Tensor lens, int64_t max_new,
+                                  c10::optional<at::Tensor> cos, c10::optional<at::Tensor> sin,
+                                  c10::optional<at::Tensor> pos, std::vector<at::Tensor> queries) {
+  using namespace kva;
+  TORCH_CHECK(k.is_cuda() && k.dim() == 3 && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() &&
+              k.device() == ck.device() && v.device() == ck.device(), "kv_append: k and v (T, G, hd) of one type on the cache's GPU");
+  c10::cuda::CUDAGuard guard(k.device());
+  const int64_t T = k.size(0), hd = k.size(2);
+  Params p{};
+  p.c = check_cache("kv_append", Layer{ck, cv, ks, vs, table, cu, lens}, T, hd);
+  TORCH_CHECK(k.size(1) == p.c.G, "kv_append: ", p.c.G, " KV heads in the cache, got ", k.size(1));
+  TORCH_CHECK(max_new >= 0, "kv_append: max_new must not be negative");
+  std::vector<at::Tensor> outs = take_rows(p, k, v, cos, sin, pos, queries);
+  if (T == 0 || p.c.B == 0) return outs;
   p.max_new = (int)std::min<int64_t>(max_new, T);
   TORCH_CHECK(T * p.c.G * 2 < (1LL << 31), "kv_append: sizes");
   MAMF_DISPATCH_FLOAT_BF16(k.scalar_type(), "kv_append", [&] {
     if (hd == 128) launch<scalar_t, 128>(p); else launch<scalar_t, 64>(p);
+  });
+  MAMF_LAUNCH_CHECK();
+  return outs;
+}
+
+// The same into the 4-bit cache; new slots of `mass` are set to 0.
+std::vector<at::Tensor> kv4_append(at::Tensor k, at::Tensor v, at::Tensor blocks, c10::optional<at::Tensor> mass,
+                                   at::Tensor table, at::Tensor cu, at::Tensor lens, int64_t max_new,
+                                   c10::optional<at::Tensor> cos, c10::optional<at::Tensor> sin,
+                                   c10::optional<at::Tensor> pos, std::vector<at::Tensor> queries) {
+  using namespace kva;
+  TORCH_CHECK(k.is_cuda() && k.dim() == 3 && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() &&
+              k.device() == blocks.device() && v.device() == blocks.device(), "kv_append: k and v (T, G, hd) of one type on the cache's GPU");
+  c10::cuda::CUDAGuard guard(k.device());
+  const int64_t T = k.size(0), hd = k.size(2);
+  Params4 p{};
+  p.c = paged4::check_cache4("kv_append", blocks, mass, table, &cu, lens, T, hd);
+  TORCH_CHECK(k.size(1) == p.c.G, "kv_append: ", p.c.G, " KV heads in the cache, got ", k.size(1));
+  TORCH_CHECK(max_new >= 0, "kv_append: max_new must not be negative");
+  std::vector<at::Tensor> outs = take_rows(p, k, v, cos, sin, pos, queries);
+  if (T == 0 || p.c.B == 0) return outs;
+  TORCH_CHECK(T * (hd / 16) < (1LL << 31), "kv_append: sizes");
+  MAMF_DISPATCH_FLOAT_BF16(k.scalar_type(), "kv_append", [&] {
+    if (hd == 128) launch4<scalar_t, 128>(p); else launch4<scalar_t, 64>(p);
   });
   MAMF_LAUNCH_CHECK();
   return outs;

@@ -94,13 +94,15 @@ _PAGED_CODES = {1: "a block table entry that is not a page of the pool", 2: "len
 
 def check_paged_status(clear: bool = True) -> None:
     """Raise if a paged-cache kernel of the current GPU recorded a timeout or a skipped access; ``clear`` forgets all
-    that was recorded, of both operators."""
+    that was recorded, of all of them."""
     from mamformer_b200.ops._ext import ext
     C = ext()
     if C is None or not torch.cuda.is_available():
         return
-    append, attention = int(C.kv_append_error(clear)), int(C.paged_attention_error(clear))
-    codes = [c for c in range(1, 32) if (append | attention) >> c & 1]
+    seen = 0
+    for word in (C.kv_append_error, C.paged_attention_error, C.kv4_error, C.paged4_attention_error):
+        seen |= int(word(clear))
+    codes = [c for c in range(1, 32) if seen >> c & 1]
     if not codes:
         return
     what = "; ".join(_PAGED_CODES.get(c, f"code {c}") for c in reversed(codes))

@@ -41,7 +41,8 @@ class GRPOConfig:
     gen_temperature: float = 0.8
     gen_top_k: int = 50
     gen_top_p: float = 0.95
-    gen_kv_cache: str = "dense"            # "paged": 8-bit pages and the paged attention kernels for rollouts
+    gen_kv_cache: str = "dense"            # "paged", "paged4": 8-bit or 4-bit pages and the paged attention kernels for rollouts
+    gen_kv_budget: Optional[int] = None    # "paged4": tokens that a rollout's cache is cut to
     kl_beta: float = 0.04
     entropy_beta: float = 0.0              # weight of the policy's mean token entropy, which is rewarded
     learning_rate: float = 1e-6
@@ -153,7 +154,7 @@ class GRPOTrainer:
         outs = []
         for t in rollout_temperatures(c.gen_temperature, c.group_size):
             g = self.policy.generate(prompt_ids, max_new_tokens=c.gen_max_tokens, temperature=t, top_k=c.gen_top_k,
-                                     top_p=c.gen_top_p, kv_cache=c.gen_kv_cache)
+                                     top_p=c.gen_top_p, kv_cache=c.gen_kv_cache, kv_budget=c.gen_kv_budget)
             outs.append(g[:, prompt_ids.shape[1]:])
         self.policy.train()
         return outs

@@ -405,12 +405,17 @@ class MamformerForCausalLM(GenerationMixin, nn.Module):
                  temperature: Optional[float] = None, top_k: Optional[int] = None,
                  top_p: Optional[float] = None, eos_token_id: Optional[int] = None,
                  pad_token_id: Optional[int] = None,
-                 thinking_config: Optional[object] = None, kv_cache: str = "dense") -> Union[torch.Tensor, dict]:
+                 thinking_config: Optional[object] = None, kv_cache: str = "dense",
+                 kv_budget: Optional[int] = None) -> Union[torch.Tensor, dict]:
         """Sample up to ``max_new_tokens`` per row.  ``kv_cache="paged"`` keeps the full-attention layers' K / V in
         8-bit pages (:class:`mamformer_b200.paged_cache.PagedKVCache`) instead of growing tensors, and attends with
-        the paged kernels."""
-        if kv_cache not in ("dense", "paged"):
-            raise ValueError(f"kv_cache must be 'dense' or 'paged', got {kv_cache!r}")
+        the paged kernels; ``"paged4"`` does so in 4 bits.  With the latter, ``kv_budget`` bounds what a sequence keeps:
+        whenever it holds a page more than that, it is cut to the budget, of which a quarter are its last tokens and the
+        rest those that received the most attention weight."""
+        if kv_cache not in ("dense", "paged", "paged4"):
+            raise ValueError(f"kv_cache must be 'dense', 'paged' or 'paged4', got {kv_cache!r}")
+        if kv_budget is not None and (kv_cache != "paged4" or kv_budget < 1):
+            raise ValueError(f"kv_budget: a number of tokens for kv_cache='paged4', got {kv_budget} for {kv_cache!r}")
         if (thinking_config is not None and getattr(thinking_config, "enabled", False)
                 and getattr(thinking_config, "is_active", False)):
             if kv_cache != "dense":
@@ -424,15 +429,20 @@ class MamformerForCausalLM(GenerationMixin, nn.Module):
         B = input_ids.shape[0]
         generated = input_ids.clone()
         cache = paged = None
-        if kv_cache == "paged":
+        if kv_cache != "dense":
             from mamformer_b200.paged_cache import PagedKVCache
-            paged = PagedKVCache.for_model(self, B, input_ids.shape[1] + max_new_tokens)
+            page, most = 64, input_ids.shape[1] + max_new_tokens
+            if kv_budget is not None:
+                most = min(most, max(input_ids.shape[1], kv_budget + page))
+            paged = PagedKVCache.for_model(self, B, most, page, bits=4 if kv_cache == "paged4" else 8, weights=kv_budget is not None)
         alive = torch.ones(B, dtype=torch.bool, device=input_ids.device)
         for _ in range(max_new_tokens):
             if not bool(alive.any()):
                 break
             cur = generated if cache is None else generated[:, -1:]
             if paged is not None:
+                if kv_budget is not None and cache is not None and paged.lens[0] >= kv_budget + paged.page_size:
+                    paged.evict(kv_budget, kv_budget // 4)
                 paged.extend(cur.shape[1])
                 cache = paged.layer_caches() if cache is None else cache
             out = self.forward(cur, use_cache=True, cache=cache, return_logits=True)

@@ -14,7 +14,7 @@ from __future__ import annotations
 
 import math
 import os
-from typing import List, NamedTuple, Optional, Sequence
+from typing import List, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -27,7 +27,8 @@ __all__ = [
     "rms_norm", "rope", "swiglu", "causal_conv1d_silu", "selective_scan", "mamba_inner",
     "linear_diff_attention", "diff_attention", "attention", "head_group_norm", "router_topk",
     "expert_histogram", "moe_routed", "moe_expert_outputs", "linear_cross_entropy",
-    "fused_ce_available", "token_log_probs", "token_scores", "TokenScores", "PagedKV", "kv_append", "paged_attention",
+    "fused_ce_available", "token_log_probs", "token_scores", "TokenScores", "PagedKV", "PagedKV4", "kv_append",
+    "kv_read", "paged_attention", "kv_evict",
     "NATIVE", "has_native", "force_reference",
 ]
 
@@ -279,6 +280,19 @@ class PagedKV(NamedTuple):
     v_scale: torch.Tensor
 
 
+class PagedKV4(NamedTuple):
+    """One layer's paged 4-bit cache, and the attention weight that its slots have received where that is kept.
+
+    A block holds 16 tokens of a KV head: key codes (16, hd / 2), key parameters (16, hd / 32) of 16 bits, and the
+    same of the values.  A byte holds two dims, the even one in its low half.  Group j of hd / 32 is the 32 dims d with
+    (d / 4) % (hd / 32) == j; its parameter is the f16 pattern of a scale s with the zero point z in the low 4 bits,
+    and a code n stands for s (n - z), exactly an f16.  Values within a group are rounded to sixteen levels that span
+    them and 0, evenly.  The range is f16's: larger values and infinities become its largest, NaN becomes 0, and
+    levels are 2^-20 apart at least."""
+    blocks: torch.Tensor                       # (P, G, page / 16, 18 hd) uint8
+    mass: Optional[torch.Tensor] = None        # (P, G, page) fp32
+
+
 def _no_gradient(what: str, *tensors: torch.Tensor) -> None:
     if torch.is_grad_enabled():
         for t in tensors:
@@ -290,7 +304,7 @@ def _no_gradient(what: str, *tensors: torch.Tensor) -> None:
                 raise RuntimeError(f"{what} has no gradient: neither forward-mode differentiation nor torch.func transforms")
 
 
-def kv_append(k: torch.Tensor, v: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
+def kv_append(k: torch.Tensor, v: torch.Tensor, cache: Union[PagedKV, PagedKV4], block_table: torch.Tensor, cu_seqlens: torch.Tensor,
               kv_lens: torch.Tensor, max_new: int, cos: Optional[torch.Tensor] = None,
               sin: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
               queries: Sequence[torch.Tensor] = ()) -> List[torch.Tensor]:
@@ -302,14 +316,19 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, cache: PagedKV, block_table: tor
     and ``positions`` (T,) int64, keys and up to two query tensors (T, H, hd) are rotated on the way (halves, as
     :func:`rope`).  A page that takes new tokens must belong to one sequence only.  On the GPU a page or length out
     of range is skipped and a position is clamped to the tables, and ``fault.check_device_status`` raises
-    afterwards.  No gradient."""
+    afterwards.  No gradient.
+
+    ``cache`` is a :class:`PagedKV` or a :class:`PagedKV4`; of the latter, the new slots' ``mass`` becomes 0."""
     _no_gradient("kv_append", k, v, *queries)
+    if isinstance(cache, PagedKV4):
+        f = _nat().kv4_append if _native(k) and "kv4_append" in NATIVE else ref.kv4_append
+        return f(k, v, cache, block_table, cu_seqlens, kv_lens, max_new, cos, sin, positions, queries)
     if _native(k) and "kv_append" in NATIVE:
         return _nat().kv_append(k, v, cache, block_table, cu_seqlens, kv_lens, max_new, cos, sin, positions, queries)
     return ref.kv_append(k, v, cache, block_table, cu_seqlens, kv_lens, cos, sin, positions, queries)
 
 
-def paged_attention(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
+def paged_attention(q: torch.Tensor, cache: Union[PagedKV, PagedKV4], block_table: torch.Tensor, cu_seqlens: torch.Tensor,
                     kv_lens: torch.Tensor, max_new: int, q2: Optional[torch.Tensor] = None,
                     lam: Optional[torch.Tensor] = None, window: int = 0, scale: Optional[float] = None) -> torch.Tensor:
     """Causal attention of packed queries (T, H, hd) over the paged cache, H / G query heads per KV head -> (T, H, hd).
@@ -319,12 +338,59 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, 
     kv_lens - n + i, with ``window`` > 0 only the last ``window`` of them; block table entries of pages below that may be
     anything.  With ``q2`` and ``lam`` (H,) fp32, the
     differential form (softmax(q k) v - lam softmax(q2 k) v) / (1 - lam + 1e-8).  A query that sees nothing, and
-    rows past cu_seqlens[-1], give 0.  No gradient."""
+    rows past cu_seqlens[-1], give 0.  No gradient.
+
+    ``cache`` is a :class:`PagedKV` or a :class:`PagedKV4`.  With ``cache.mass`` of the latter, each slot's mass grows by
+    the softmax weights that it receives, summed over the queries, the heads of its group and both maps, in fp32 and in
+    the same order every time; its pages must then belong to one sequence each."""
     _no_gradient("paged_attention", q) if q2 is None or lam is None else _no_gradient("paged_attention", q, q2, lam)
     scale = q.shape[-1] ** -0.5 if scale is None else scale
+    if isinstance(cache, PagedKV4):
+        f = _nat().paged4_attention if _native(q) and "paged4_attention" in NATIVE else ref.paged4_attention
+        return f(q, cache, block_table, cu_seqlens, kv_lens, max_new, q2, lam, window, scale)
     if _native(q) and "paged_attention" in NATIVE:
         return _nat().paged_attention(q, cache, block_table, cu_seqlens, kv_lens, max_new, q2, lam, window, scale)
     return ref.paged_attention(q, cache, block_table, cu_seqlens, kv_lens, q2, lam, window, scale)
+
+
+def kv_read(cache: PagedKV4, block_table: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor, tokens: int,
+            dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values that a 4-bit cache holds of each sequence's last tokens, packed: (tokens, G, hd) each.
+
+    Rows cu_seqlens[b] : cu_seqlens[b + 1] are the last of sequence b's kv_lens[b] tokens (zeros in front of a shorter
+    one, and in rows of no sequence), as :func:`kv_append` took them, keys rotated.  f16 and fp32 hold them exactly."""
+    if not isinstance(cache, PagedKV4):
+        raise TypeError(f"kv_read: a PagedKV4, got {type(cache).__name__}")
+    if dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError(f"kv_read: bf16, f16 or fp32, got {dtype}")
+    if tokens < 0:
+        raise ValueError(f"kv_read: tokens must not be negative, got {tokens}")
+    if _native(cache.blocks) and "kv_read" in NATIVE:
+        return _nat().kv_read(cache, block_table, cu_seqlens, kv_lens, tokens, dtype)
+    return ref.kv_read(cache, block_table, cu_seqlens, kv_lens, tokens, dtype)
+
+
+def kv_evict(cache: PagedKV4, block_table: torch.Tensor, kv_lens: torch.Tensor, budget: int, recent: int = 0,
+             out_table: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Cut every sequence of a 4-bit cache to ``budget`` tokens, each KV head by itself: the last ``recent`` ones stay, and
+    of the others those of the largest ``cache.mass`` (ties to the earlier slot).
+
+    The kept tokens move, in order, with their mass, to slots 0 .. budget - 1; sequences of up to ``budget`` tokens keep
+    all of theirs.  Without ``out_table`` that is in place.  With it (B, W') int32 they go to its pages, which must be no
+    page of ``block_table``'s, and what block_table names stays as it is: a prompt that other sequences share, for
+    instance.  Returns the kept slots (B, G, budget) int32, -1 past a shorter sequence's end, and the new lengths (B,)
+    int32.  Keys stay rotated as they were appended.  Sliding windows count slots, so they do not go with a cache that
+    has been evicted from.  On the GPU, tokens of pages out of range stay where they are and
+    ``fault.check_device_status`` raises afterwards.  A positive NaN counts as heavier than infinity."""
+    if not isinstance(cache, PagedKV4):
+        raise TypeError(f"kv_evict: a PagedKV4 (the 8-bit cache's pages share a scale), got {type(cache).__name__}")
+    if cache.mass is None:
+        raise ValueError("kv_evict: a cache with mass")
+    if budget < 1 or not 0 <= recent <= budget:
+        raise ValueError(f"kv_evict: 0 <= recent <= budget and budget >= 1, got {recent} and {budget}")
+    if _native(cache.blocks) and "kv_evict" in NATIVE:
+        return _nat().kv_evict(cache, block_table, kv_lens, budget, recent, out_table)
+    return ref.kv_evict(cache, block_table, kv_lens, budget, recent, out_table)
 
 
 # Register native ops (import has no side effects when the extension is absent).

@@ -438,3 +438,23 @@ def kv_append(k, v, cache, block_table, cu_seqlens, kv_lens, max_new, cos, sin, 
 @_register("paged_attention", "csrc/paged_attn.cu")
 def paged_attention(q, cache, block_table, cu_seqlens, kv_lens, max_new, q2, lam, window, scale):
     return _C.paged_attention(q, q2, lam, *cache, block_table, cu_seqlens, kv_lens, max_new, window, scale)
+
+
+@_register("kv4_append", "csrc/paged_kv.cu")
+def kv4_append(k, v, cache, block_table, cu_seqlens, kv_lens, max_new, cos, sin, positions, queries):
+    return _C.kv4_append(k, v, *cache, block_table, cu_seqlens, kv_lens, max_new, cos, sin, positions, queries)
+
+
+@_register("kv_read", "csrc/paged4_kv.cu")
+def kv_read(cache, block_table, cu_seqlens, kv_lens, tokens, dtype):
+    return tuple(_C.kv4_read(cache.blocks, block_table, cu_seqlens, kv_lens, tokens, dtype))
+
+
+@_register("paged4_attention", "csrc/paged4_attn.cu + csrc/paged4_attn_tc.cu")
+def paged4_attention(q, cache, block_table, cu_seqlens, kv_lens, max_new, q2, lam, window, scale):
+    return _C.paged4_attention(q, q2, lam, *cache, block_table, cu_seqlens, kv_lens, max_new, window, scale)
+
+
+@_register("kv_evict", "csrc/paged4_kv.cu")
+def kv_evict(cache, block_table, kv_lens, budget, recent, out_table):
+    return tuple(_C.kv4_evict(*cache, block_table, kv_lens, budget, recent, out_table))

@@ -457,3 +457,143 @@ def paged_attention(q, cache, block_table, cu_seqlens, kv_lens, q2, lam, window,
             o = (o - w * maps[1]) / (1.0 - w + 1e-8)
         out[cu[b]:cu[b + 1]] = o.transpose(0, 1).to(q.dtype)
     return out
+
+
+# ---- the 4-bit cache (layout in ops.PagedKV4) -----------------------------------------------------------
+def kv4_levels(x: torch.Tensor):
+    """fp32 (.., hd) -> codes (.., hd / 2) uint8, parameters (.., hd / 32) int16.  The scale is a fifteenth of a group's
+    range, 0 in it, rounded up to 7 significant bits (to a multiple of 2^-20 below 2^-14)."""
+    J = x.shape[-1] // 32
+    x = torch.where(x.isnan(), 0.0, x).clamp(-65504.0, 65504.0).unflatten(-1, (8, J, 4))
+    lo, hi = x.amin((-3, -1)).clamp(max=0.0), x.amax((-3, -1)).clamp(min=0.0)
+    s = (hi - lo) * 0.06666666
+    up = ((s.view(torch.int32) + 0x1FFFF) & ~0x1FFFF).view(torch.float32)
+    s = torch.where(s < 2.0 ** -14, torch.ceil(s * 2.0 ** 20) * 2.0 ** -20, up).clamp(min=2.0 ** -20)
+    z = torch.round(-lo * s.reciprocal()).clamp(0.0, 15.0)
+    s = s.clamp(max=4352.0)
+    n = (torch.round(x * s.reciprocal()[..., None, :, None]) + z[..., None, :, None]).clamp(0.0, 15.0)
+    n = n.to(torch.uint8).flatten(-3)
+    return n[..., 0::2] | n[..., 1::2] << 4, s.half().view(torch.int16) | z.to(torch.int16)
+
+
+def kv4_values(codes: torch.Tensor, params: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    n = torch.stack([codes & 15, codes >> 4], -1).flatten(-2).unflatten(-1, (8, params.shape[-1], 4)).to(dtype)
+    s, z = (params & -16).view(torch.float16).to(dtype), (params & 15).to(dtype)
+    return (s[..., None, :, None] * (n - z[..., None, :, None])).flatten(-3)
+
+
+def kv4_parts(blocks: torch.Tensor):
+    """Views of the blocks: key codes, key parameters, value codes, value parameters, (P, G, page / 16, 16, ..)."""
+    hd = blocks.shape[-1] // 18
+    out = []
+    for x in (blocks[..., :9 * hd], blocks[..., 9 * hd:]):
+        out += [x[..., :8 * hd].unflatten(-1, (16, hd // 2)), x[..., 8 * hd:].view(torch.int16).unflatten(-1, (16, hd // 32))]
+    return out
+
+
+def _slots(table, page, slot):
+    """Where slots of a sequence are: page, block of the page, row of the block."""
+    return table[slot // page].long(), slot % page // 16, slot % 16
+
+
+def _check4(what, cache, hd):
+    if cache.blocks.dtype != torch.uint8 or cache.blocks.dim() != 4 or cache.blocks.shape[3] != 18 * hd or hd not in (64, 128):
+        raise ValueError(f"{what}: heads of {hd} dims for blocks {tuple(cache.blocks.shape)} {cache.blocks.dtype}")
+
+
+def kv4_append(k, v, cache, block_table, cu_seqlens, kv_lens, max_new, cos, sin, positions, queries):
+    if k.shape != v.shape or k.dim() != 3 or k.shape[1] != cache.blocks.shape[1]:
+        raise ValueError(f"kv_append: k {tuple(k.shape)}, v {tuple(v.shape)} for blocks {tuple(cache.blocks.shape)}")
+    _check4("kv_append", cache, k.shape[2])
+
+    def turn(x):
+        c, s = cos[positions].unsqueeze(1), sin[positions].unsqueeze(1)
+        a, b = x.float().chunk(2, -1)
+        return torch.cat([a * c - b * s, b * c + a * s], -1)
+
+    page = 16 * cache.blocks.shape[2]
+    parts = kv4_parts(cache.blocks)
+    new = kv4_levels(turn(k) if cos is not None else k.float()) + kv4_levels(v.float())
+    cu = cu_seqlens.tolist()
+    for b, end in enumerate(kv_lens.tolist()):
+        at = _slots(block_table[b], page, torch.arange(end - (cu[b + 1] - cu[b]), end, device=k.device))
+        for to, x in zip(parts, new):
+            to[at[0], :, at[1], at[2]] = x[cu[b]:cu[b + 1]]
+        if cache.mass is not None:
+            cache.mass[at[0], :, 16 * at[1] + at[2]] = 0.0
+    return [turn(q).to(q.dtype) for q in queries]
+
+
+def kv_read(cache, block_table, cu_seqlens, kv_lens, tokens, dtype):
+    page, G, hd = 16 * cache.blocks.shape[2], cache.blocks.shape[1], cache.blocks.shape[3] // 18
+    _check4("kv_read", cache, hd)
+    parts = kv4_parts(cache.blocks)
+    out = [torch.zeros(tokens, G, hd, dtype=dtype, device=cache.blocks.device) for _ in range(2)]
+    cu = cu_seqlens.tolist()
+    for b, end in enumerate(kv_lens.tolist()):
+        n = min(end, cu[b + 1] - cu[b])
+        at = _slots(block_table[b], page, torch.arange(end - n, end, device=cache.blocks.device))
+        for i, x in enumerate(out):
+            codes, params = (y[at[0], :, at[1], at[2]] for y in parts[2 * i:2 * i + 2])
+            x[cu[b + 1] - n:cu[b + 1]] = kv4_values(codes, params).to(dtype)
+    return tuple(out)
+
+
+def paged4_attention(q, cache, block_table, cu_seqlens, kv_lens, max_new, q2, lam, window, scale):
+    page, G = 16 * cache.blocks.shape[2], cache.blocks.shape[1]
+    if q.dim() != 3 or q.shape[1] % G or (q2 is None) != (lam is None):
+        raise ValueError(f"paged_attention: q {tuple(q.shape)} for blocks {tuple(cache.blocks.shape)}")
+    _check4("paged_attention", cache, q.shape[2])
+    acc = torch.float64 if q.dtype == torch.float64 else torch.float32
+    out = torch.zeros_like(q)
+    parts = kv4_parts(cache.blocks)
+    cu = cu_seqlens.tolist()
+    for b, L in enumerate(kv_lens.tolist()):
+        n = cu[b + 1] - cu[b]
+        if n == 0:
+            continue
+        below = max(0, L - n - window + 1) // page * page if window > 0 else 0       # pages that no query sees
+        at = _slots(block_table[b], page, torch.arange(below, L, device=q.device))
+        kx, vx = (kv4_values(*(y[at[0], :, at[1], at[2]] for y in parts[i:i + 2]), acc).transpose(0, 1)
+                  .repeat_interleave(q.shape[1] // G, 0) for i in (0, 2))
+        dist = torch.arange(L - n, L, device=q.device)[:, None] - torch.arange(below, L, device=q.device)
+        hide = (dist < 0) | (dist >= window) if window > 0 else dist < 0
+        maps = []
+        for x in (q,) if q2 is None else (q, q2):
+            s = (x[cu[b]:cu[b + 1]].transpose(0, 1).to(acc) @ kx.transpose(1, 2)) * scale
+            p = torch.softmax(s.masked_fill(hide, -math.inf), -1)
+            p = torch.where(hide.all(-1)[:, None], 0.0, p)
+            maps.append(p @ vx)
+            if cache.mass is not None:
+                cache.mass[at[0], :, 16 * at[1] + at[2]] += p.sum(1).unflatten(0, (G, -1)).sum(1).T.float()
+        o = maps[0]
+        if q2 is not None:
+            w = lam.view(-1, 1, 1).to(acc)
+            o = (o - w * maps[1]) / (1.0 - w + 1e-8)
+        out[cu[b]:cu[b + 1]] = o.transpose(0, 1).to(q.dtype)
+    return out
+
+
+def kv_evict(cache, block_table, kv_lens, budget, recent, out_table):
+    page, G = 16 * cache.blocks.shape[2], cache.blocks.shape[1]
+    to_table = block_table if out_table is None else out_table
+    if to_table.shape[0] != block_table.shape[0] or to_table.shape[1] * page < min(budget, block_table.shape[1] * page):
+        raise ValueError(f"kv_evict: out_table {tuple(to_table.shape)} for {block_table.shape[0]} sequences of {budget} tokens")
+    B = block_table.shape[0]
+    kept = torch.full((B, G, budget), -1, dtype=torch.int32, device=block_table.device)
+    parts = kv4_parts(cache.blocks) + [cache.mass.unflatten(2, (-1, 16))]
+    for b, L in enumerate(kv_lens.tolist()):
+        slots = torch.arange(L, device=block_table.device)
+        for g in range(G):
+            keep = slots
+            if L > budget:
+                at = _slots(block_table[b], page, slots[:L - recent])
+                bits = (cache.mass[at[0], g, 16 * at[1] + at[2]] + 0.0).view(torch.int32).long()
+                order = torch.where(bits < 0, -(bits & 0x7FFFFFFF), bits)
+                first = torch.sort(order, descending=True, stable=True).indices[:budget - recent]
+                keep = torch.cat([first.sort().values, slots[L - recent:]])
+            kept[b, g, :len(keep)] = keep.to(torch.int32)
+            src, dst = _slots(block_table[b], page, keep), _slots(to_table[b], page, slots[:len(keep)])
+            for x in parts:
+                x[dst[0], g, dst[1], dst[2]] = x[src[0], g, src[1], src[2]]
+    return kept, kv_lens.clamp(max=budget)

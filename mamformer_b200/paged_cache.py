@@ -1,4 +1,4 @@
-"""Paged 8-bit KV cache of a batch of sequences.
+"""Paged KV cache of a batch of sequences, in 8 or 4 bits.
 
 The cache a decoding batch keeps instead of growing (B, S, G, hd) tensors with ``torch.cat`` (reference
 ``layers/attention.py:143-149``, ``kda_diff.py:813-818``): pages of ``page_size`` tokens, e4m3 codes with one
@@ -11,6 +11,13 @@ power-of-two scale per page and KV head (:class:`mamformer_b200.ops.PagedKV`), o
 A layer's pages are allocated when it first attends.  Sequences may differ in length and in the number of new
 tokens; :meth:`release` gives a finished sequence's pages back; :meth:`check` raises what the kernels recorded.  What a page holds is rounded to 4 significant
 bits, so decoded logits differ from an unquantised cache's by that rounding.
+
+``bits=4`` takes 9 bytes for 16 dims instead of 16: sixteen even levels for each 32 dims of a token's head
+(:class:`mamformer_b200.ops.PagedKV4`).  With ``weights=True`` such a cache adds up the attention weight that each slot
+receives, and :meth:`evict` cuts the sequences to a budget by it, every layer and KV head by itself:
+
+    cache = PagedKVCache(..., bits=4, weights=True)
+    cache.evict(budget=2048, recent=512)             # between steps: the last 512 tokens and the heaviest others stay
 """
 
 from __future__ import annotations
@@ -31,7 +38,7 @@ class PagedLayer:
     def __init__(self, owner: "PagedKVCache", index: int) -> None:
         self.owner = owner
         self.index = index
-        self.kv: Optional[ops.PagedKV] = None
+        self.kv: Union[ops.PagedKV, ops.PagedKV4, None] = None
         self._skipped: Optional[torch.Tensor] = None             # tokens of each sequence from before the last restart
 
     def restart(self) -> "PagedLayer":
@@ -47,6 +54,8 @@ class PagedLayer:
         cos, sin (S, hd / 2): the rotation of the step's S positions.  Or packed (T, H, hd) with a row of cos / sin
         per token, where the step's counts differ.  Returns a tensor like q."""
         o = self.owner
+        if window > 0 and o.evicted:
+            raise ValueError("paged cache: sliding windows count slots, and evicted tokens' are gone")
         if self.kv is None:
             self.kv = o._allocate(q.device)
         flat = lambda x: x.reshape(-1, *x.shape[-2:])  # noqa: E731
@@ -64,12 +73,19 @@ class PagedLayer:
 
 class PagedKVCache:
     def __init__(self, n_layers: int, n_kv_heads: int, head_dim: int, batch: int, max_len: int, page_size: int = 64,
-                 n_pages: Optional[int] = None, device: Union[str, torch.device] = "cuda") -> None:
+                 n_pages: Optional[int] = None, device: Union[str, torch.device] = "cuda", bits: int = 8,
+                 weights: bool = False) -> None:
+        if bits not in (4, 8):
+            raise ValueError(f"the paged cache holds 4 or 8 bits, got {bits}")
+        if weights and bits != 4:
+            raise ValueError("received weights are kept by the 4-bit cache")
         if page_size not in PAGE_SIZES:
             raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
         if head_dim not in (64, 128):
             raise ValueError(f"the paged cache holds heads of 64 or 128 dims, got {head_dim}")
         self.n_kv_heads, self.head_dim, self.page_size = n_kv_heads, head_dim, page_size
+        self.bits, self.weights = bits, weights
+        self.evicted = False                                     # slots are no longer positions
         self.batch = batch
         self.width = max(1, -(-max_len // page_size))            # pages of a sequence
         self.n_pages = n_pages if n_pages is not None else batch * self.width
@@ -87,8 +103,10 @@ class PagedKVCache:
         self._pos: dict = {}
 
     @classmethod
-    def for_model(cls, model, batch: int, max_len: int, page_size: int = 64) -> "PagedKVCache":
-        """A cache with a place for every layer of a Mamformer model."""
+    def for_model(cls, model, batch: int, max_len: int, page_size: int = 64, bits: int = 8,
+                  weights: bool = False) -> "PagedKVCache":
+        """A cache with a place for every layer of a Mamformer model.  ``weights``: one that is going to be evicted
+        from, so without sliding windows."""
         heads = set()                                            # of the modules: a tensor-parallel rank holds its share
         for layer in model.model.layers:
             att = layer.attention
@@ -99,6 +117,8 @@ class PagedKVCache:
             if getattr(full, "sliding_window", 0) > 0 and full.window_mode != "causal":
                 raise ValueError("the paged cache attends causally: sliding windows need window_mode='causal' "
                                  "(a field of the config; --window_mode of the scripts)")
+            if getattr(full, "sliding_window", 0) > 0 and weights:
+                raise ValueError("sliding windows count slots: they do not go with eviction")
         dtype = compute_dtype_of(model)
         if next(model.parameters()).is_cuda and dtype == torch.float32 and not torch.is_autocast_enabled("cuda"):
             raise ValueError("the paged attention kernels take bf16 or f16 queries: convert the model first "
@@ -106,7 +126,7 @@ class PagedKVCache:
         if len(heads) != 1:
             raise ValueError(f"the paged cache takes layers of one number and size of KV heads, got {sorted(heads)}")
         return cls(len(model.model.layers), *heads.pop(), batch, max_len, page_size,
-                   device=next(model.parameters()).device)
+                   device=next(model.parameters()).device, bits=bits, weights=weights)
 
     def layer(self, i: int) -> PagedLayer:
         return self.layers[i]
@@ -158,6 +178,38 @@ class PagedKVCache:
                 layer._skipped = layer._skipped.clone()
                 layer._skipped[b] = 0
 
+    def evict(self, budget: int, recent: int = 0) -> None:
+        """Cut every sequence of more than ``budget`` tokens to that many, between steps: in each layer and KV head by
+        itself the last ``recent`` ones stay and, of the others, those that have received the most attention weight.
+        What the sequences then no longer need of their pages is given back."""
+        if not self.weights:
+            raise ValueError("evict: a cache with weights=True")
+        if budget < 1 or not 0 <= recent <= budget:
+            raise ValueError(f"evict: 0 <= recent <= budget and budget >= 1, got {recent} and {budget}")
+        if max(self.lens, default=0) <= budget:
+            return
+        left = self.kv_lens.clamp(max=budget)
+        for layer in self.layers:
+            if layer.kv is None:
+                continue
+            lens = self.kv_lens if layer._skipped is None else self.kv_lens - layer._skipped
+            _, lens = ops.kv_evict(layer.kv, self.block_table, lens, budget, recent)
+            if layer._skipped is not None:
+                layer._skipped = left - lens
+        self.kv_lens = left
+        self.lens = [min(n, budget) for n in self.lens]
+        self.evicted = True
+        rows, cols = [], []
+        for b, (n, pages) in enumerate(zip(self.lens, self._pages)):
+            need = -(-n // self.page_size)
+            while len(pages) > need:
+                self._free.append(pages.pop())
+                rows.append(b)
+                cols.append(len(pages))
+        if rows:
+            r, c = torch.tensor([rows, cols], device=self.block_table.device).unbind()
+            self.block_table[r, c] = -1
+
     def check(self) -> None:
         """Wait for the steps so far and raise what their kernels recorded: PagedCacheError for a page, length or
         position out of range, KernelTimeoutError.  :meth:`MamformerForCausalLM.generate` does so before it returns."""
@@ -167,7 +219,11 @@ class PagedKVCache:
                 torch.cuda.current_stream().synchronize()
                 check_paged_status()
 
-    def _allocate(self, device) -> ops.PagedKV:
+    def _allocate(self, device) -> Union[ops.PagedKV, ops.PagedKV4]:
+        if self.bits == 4:
+            blocks = torch.empty(self.n_pages, self.n_kv_heads, self.page_size // 16, 18 * self.head_dim, dtype=torch.uint8, device=device)
+            mass = torch.zeros(self.n_pages, self.n_kv_heads, self.page_size, device=device) if self.weights else None
+            return ops.PagedKV4(blocks, mass)
         shape = (self.n_pages, self.n_kv_heads, self.page_size, self.head_dim)
         code = lambda: torch.empty(shape, dtype=torch.float8_e4m3fn, device=device)  # noqa: E731
         return ops.PagedKV(code(), code(), torch.ones(shape[:2], device=device), torch.ones(shape[:2], device=device))

@@ -30,8 +30,10 @@ def build_parser():
     p.add_argument("--summary_budget", type=int, default=0)
     p.add_argument("--show_thinking", action="store_true")
     p.add_argument("--bf16", action="store_true")
-    p.add_argument("--kv_cache", default="dense", choices=("dense", "paged"),
-                   help="paged: keys and values in 8-bit pages (sampling only)")
+    p.add_argument("--kv_cache", default="dense", choices=("dense", "paged", "paged4"),
+                   help="paged, paged4: keys and values in 8-bit or 4-bit pages (sampling only)")
+    p.add_argument("--kv_budget", type=int, default=None,
+                   help="with --kv_cache paged4: tokens that the cache is cut to, by received attention weight")
     p.add_argument("--window_mode", default=None, choices=("reference", "causal"),
                    help="sliding windows of the model, in place of its config's (the paged cache needs causal ones)")
     p.add_argument("--seed", type=int, default=42, help="seeds the weights of a model built without a checkpoint "
@@ -47,7 +49,7 @@ def generate_text(model, tok, prompt, args):
     ids = torch.tensor([tok.encode(prompt, add_bos=True)], device=dev)
     model.config.generation.repetition_penalty = args.repetition_penalty
     if args.kv_cache != "dense" and (args.num_beams > 1 or (args.thinking and args.thinking != "NoThink")):
-        raise ValueError("--kv_cache paged goes with sampling: beams and thinking modes copy their cache between paths")
+        raise ValueError(f"--kv_cache {args.kv_cache} goes with sampling: beams and thinking modes copy their cache between paths")
     if args.thinking and args.thinking != "NoThink":
         tc = ThinkingConfig.from_preset(args.thinking, args.think_budget, args.num_paths, args.summary_budget,
                                         args.show_thinking)
@@ -59,7 +61,7 @@ def generate_text(model, tok, prompt, args):
                                  eos_token_id=tok.eos_token_id)
     else:
         seq = model.generate(ids, max_new_tokens=args.max_new_tokens, temperature=args.temperature,
-                             top_k=args.top_k, top_p=args.top_p, eos_token_id=tok.eos_token_id, kv_cache=args.kv_cache)
+                             top_k=args.top_k, top_p=args.top_p, eos_token_id=tok.eos_token_id, kv_cache=args.kv_cache, kv_budget=args.kv_budget)
     return tok.decode(seq[0, ids.shape[1]:].tolist(), skip_special_tokens=not args.show_thinking)
 
 
