@@ -20,9 +20,16 @@ namespace paged4 {
 
 using namespace paged;
 
+// Constants of the decoding below.  They come with the launch and not with the code, where the compiler would write them
+// into a register anew for every use of a pair of constants: an instruction takes one.
+struct Base {
+  uint32_t one = 0x64006400u;                        // 1024 in both halves
+  uint32_t back = 0xF380F380u;                       // -15360
+};
 struct Cache4 : Table {
   uint8_t* blocks;
   float* mass;                                       // (P, G, page) received weights, or null
+  Base base;
 };
 
 template <int HD> constexpr int HALF = 9 * HD;        // bytes of a block's keys, or values, with their parameters
@@ -38,7 +45,7 @@ inline Cache4 check_cache4(const char* what, const at::Tensor& blocks, const c10
   const int64_t P = blocks.size(0), G = blocks.size(1), page = 16 * blocks.size(2);
   TORCH_CHECK(page == 16 || page == 32 || page == 64 || page == 128, what, ": pages of 16, 32, 64 or 128 tokens, got ", page);
   TORCH_CHECK(aligned16(blocks.data_ptr()), what, ": 16-byte aligned blocks");
-  Cache4 c;
+  Cache4 c{};
   static_cast<Table&>(c) = check_table(what, table, cu, lens, P, G, page, T);
   c.blocks = (uint8_t*)blocks.data_ptr();
   c.mass = nullptr;
@@ -68,23 +75,36 @@ __device__ __forceinline__ uint32_t hmul(uint32_t a, uint32_t b) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-// What two groups' parameters give: for codes in the low four bits of a half, and for those in the next four.
+__device__ __forceinline__ uint32_t hfma(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+// (a & mask) | 1024 in both halves, in one instruction; written as two operators it became two
+template <uint32_t MASK> __device__ __forceinline__ uint32_t pick(uint32_t a, uint32_t one) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "n"(MASK), "r"(one));
+  return r;
+}
+// What two groups' parameters give: for codes in the low four bits of a half, and for those in the next four.  The integer
+// units are what bounds the decoding, so the second pair comes from the first by f16 arithmetic (exact: 16 (1024 + z) -
+// 15360 = 1024 + 16 z).
 struct Levels { uint32_t z0, s0, z4, s4; };
-__device__ __forceinline__ Levels levels_of(uint32_t params) {
+__device__ __forceinline__ Levels levels_of(uint32_t params, const Base& base) {
   Levels l;
-  l.z0 = (params & 0x000F000Fu) | 0x64006400u;
-  l.z4 = ((params << 4) & 0x00F000F0u) | 0x64006400u;
+  l.z0 = pick<0x000F000Fu>(params, base.one);
   l.s0 = params & 0xFFF0FFF0u;
+  l.z4 = hfma(l.z0, 0x4C004C00u, base.back);         // 16
   l.s4 = hmul(l.s0, 0x2C002C00u);                    // 1 / 16
   return l;
 }
 // The 16-bit halves of w hold the codes of two groups, four each: code i of both as the halves of h[i].
-__device__ __forceinline__ void decode(uint32_t w, const Levels& l, uint32_t (&h)[4]) {
+__device__ __forceinline__ void decode(uint32_t w, const Levels& l, const Base& base, uint32_t (&h)[4]) {
   const uint32_t u = w >> 8;
-  h[0] = hmul(hsub((w & 0x000F000Fu) | 0x64006400u, l.z0), l.s0);
-  h[1] = hmul(hsub((w & 0x00F000F0u) | 0x64006400u, l.z4), l.s4);
-  h[2] = hmul(hsub((u & 0x000F000Fu) | 0x64006400u, l.z0), l.s0);
-  h[3] = hmul(hsub((u & 0x00F000F0u) | 0x64006400u, l.z4), l.s4);
+  h[0] = hmul(hsub(pick<0x000F000Fu>(w, base.one), l.z0), l.s0);
+  h[1] = hmul(hsub(pick<0x00F000F0u>(w, base.one), l.z4), l.s4);
+  h[2] = hmul(hsub(pick<0x000F000Fu>(u, base.one), l.z0), l.s0);
+  h[3] = hmul(hsub(pick<0x00F000F0u>(u, base.one), l.z4), l.s4);
 }
 
 // ---- values -> codes -------------------------------------------------------------------------------

@@ -32,6 +32,8 @@ using namespace paged4;
 
 // Rows of a sequence and KV head above which the chunk kernel takes over.
 constexpr int FEW = 64;
+constexpr int NB = 2, STEP = 16 * NB;          // blocks and tokens of a warp per tile
+constexpr int TILE = STEP * NW;                // tokens per tile
 constexpr float LIFT = 7.f, LAZY = 8.f;        // a row's largest weight is 2^LIFT when its reference is set, and may outgrow it
 constexpr int KEEP = 16;                       // rows whose scores are left for the received weights, at most
 
@@ -51,13 +53,19 @@ __device__ __forceinline__ uint32_t lds4(uint32_t a) {
   return v;
 }
 
-constexpr int ST = 4;                          // blocks of a warp's ring
+// mma() onto zeros
+__device__ __forceinline__ void mma_new(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+constexpr int ST = 2;                          // tiles of a warp's ring
 // resident CTAs per SM: the latency of a warp's chain (products, exponentials, products) is hidden by other
 // warps, so there are as many as the registers of a row tile allow without spills (128, 168 or 255)
 template <int HD, int NR> constexpr int residents() { return NR == 1 ? 4 : HD == 64 ? 3 : 2; }
 template <int HD, int NR> constexpr int merge_words() { return NR * (HD / 4 + 4); }      // of a lane
 template <int HD, int NR> constexpr int smem_bytes() {
-  return 1024 + NW * ST * BLOCK<HD> + 32 * 4 * merge_words<HD, NR>();
+  return 1024 + NW * ST * NB * BLOCK<HD> + 32 * 4 * merge_words<HD, NR>();
 }
 
 template <typename T, int HD, int NR>
@@ -66,13 +74,17 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
   constexpr int KW = HD / 32;                    // words of a K row per lane, and of the parameters of a row's two halves
   constexpr int VW = HD / 64;                    // words of a V row per lane
   constexpr int MT = HD / 16;                    // 16-dim tiles of O^T
-  constexpr int SB = BLOCK<HD>;
+  constexpr int SB = NB * BLOCK<HD>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t bars[NW][ST];
   __shared__ int64_t s_pre[NT / 32];
   __shared__ int64_t s_begin;
   __shared__ int s_b, s_cut;
+  // What the warps need at an item's ends only, and so keep out of registers: its description for the tiles being computed
+  // and for those being fetched, and the slots (x, y] that each of its rows sees.
+  __shared__ Item s_item[NW][2];
+  __shared__ int2 s_sees[NW][8 * NR];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g8 = lane >> 2, t4 = lane & 3;
   const Cache4& c = p.c;
   asm volatile("griddepcontrol.launch_dependents;");      // the join kernel waits for this grid's end by itself
@@ -84,7 +96,7 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
   for (int i = 0; i < chunk; ++i) {
     const int b = tid * chunk + i;
     if (b < c.B) {
-      mine += tiles_of<ROWS>(p, b);
+      mine += tiles_of<ROWS, TILE>(p, b);
       broken = broken || !in_order(c, b);
     }
   }
@@ -111,7 +123,7 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
     int64_t at = incl - mine;
     int b = tid * chunk;
     for (;; ++b) {
-      const int64_t n = tiles_of<ROWS>(p, b);
+      const int64_t n = tiles_of<ROWS, TILE>(p, b);
       if (first < at + n) break;
       at += n;
     }
@@ -130,58 +142,104 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
   }
   if (first >= last || total >> 60) return;
 
-  Item it;                                          // of the tile being computed
-  set_sequence<ROWS>(p, it, s_b);
+  Item& it = s_item[w][0];                          // of the tile being computed
+  Item& is = s_item[w][1];                          // of the next tile to be fetched
+  int done = 0;                                     // tiles of the first item that are other CTAs'
   int64_t start = s_begin;                          // list position of the item's first tile
-  while (first >= start + it.nt) { start += it.nt; next_item<ROWS>(p, it); }
+  {
+    Item x;
+    set_sequence<ROWS, TILE>(p, x, s_b);
+    while (first >= start + x.nt) { start += x.nt; next_item<ROWS, TILE>(p, x); }
+    it = is = x;                                    // every lane writes the same
+    done = (int)(first - start);
+  }
+  auto advance = [&](Item& s) {
+    Item x = s;
+    next_item<ROWS, TILE>(p, x);
+    __syncwarp();
+    s = x;
+    __syncwarp();
+  };
 
   // ---- ring: the issue side runs ST - 1 tiles ahead ----
   const uint32_t ring = su32(smem) + w * ST * SB, bar = su32(bars[w]);
   if (lane < ST) tc5::bar_init(&bars[w][lane], 1);
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   __syncwarp();
-  Item is = it;
   int to_issue = (int)(last - first), issued = 0, waited = 0;
-  int is_left = it.nt - (int)(first - start);                        // tiles of the item still to be looked up
-  int is_slot = (it.k0 + (int)(first - start)) * TILE + w * STEP;     // the warp's first token of the tile
-  const int* is_table = c.table + (int64_t)is.b * c.W;
-  // the page of the warp's 16 tokens of a tile: -2 nothing to see there, -1 not a page of the pool
-  int pg;
+  int is_left, is_slot, is_lo, is_hi, is_g, is_at = 0;     // tiles of the item not fetched yet, the warp's first token of the next
+  // Pages of the item's next 32 tiles, a tile per lane, asked for while the tile before them is being computed: those of
+  // the warp's first block and, where a page is one block, of its second.
+  int pages[NB];
   auto look_up = [&]() {
-    pg = -2;
-    if (is_slot < is.hi && is_slot + STEP > is.lo) {
-      const int j = is_slot >> c.shift;
-      pg = j < c.W ? is_table[j] : -1;
+    const int* table = c.table + (int64_t)is.b * c.W;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int first_slot = is_slot + lane * TILE + 16 * i, last_slot = first_slot + (c.shift == 4 ? 15 : STEP - 1);
+      // only of what some row sees: below a window there may be no page
+      const int j = first_slot >> c.shift;
+      pages[i] = -1;
+      if ((i == 0 || c.shift == 4) && first_slot < is_hi && last_slot >= is_lo && j < c.W) pages[i] = table[j];
     }
+    is_at = 0;
   };
-  look_up();
-  int flying = 0;                        // bit i: the i-th next tile's tokens are there
+  auto fetch_item = [&](int skip) {
+    is_left = is.nt - skip;
+    is_slot = (is.k0 + skip) * TILE + w * STEP;
+    is_lo = is.lo;
+    is_hi = is.hi;
+    is_g = is.g;
+    look_up();
+  };
+  fetch_item(done);
+  int flying = 0;                        // NB bits for each tile on its way, the next one's lowest: which blocks are there
   bool ok = true;
   auto issue = [&](uint32_t stage_at, uint32_t bar_at) {
-    flying >>= 1;
+    flying >>= NB;
     if (to_issue <= 0) return;
     ++issued;
-    const bool there = (unsigned)pg < (unsigned)c.P;
-    if (there) flying |= 1 << (ST - 1);
+    int pg[NB];
+    pg[0] = __shfl_sync(0xffffffffu, pages[0], is_at);
+#pragma unroll
+    for (int i = 1; i < NB; ++i) pg[i] = c.shift == 4 ? __shfl_sync(0xffffffffu, pages[i], is_at) : pg[0];
+    int there = 0;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int slot = is_slot + 16 * i;
+      const bool sees = slot < is_hi && slot + 16 > is_lo, page = (unsigned)pg[i] < (unsigned)c.P;
+      there |= (sees && page) << i;
+      bad = bad || (sees && !page);
+    }
+    flying |= there << NB * (ST - 1);
     if (lane == 0) {
-      if (there) {
-        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar_at), "r"(SB) : "memory");
-        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                     ::"r"(stage_at), "l"(block_of<HD>(c, pg, is.g, is_slot)), "r"(SB), "r"(bar_at) : "memory");
-      } else {
+      if (bad) record(ERR_PAGE);
+      if (there)
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar_at), "r"(__popc(there) * BLOCK<HD>) : "memory");
+      else
         asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar_at) : "memory");
-        if (pg != -2) record(ERR_PAGE);
+      // blocks of one page are adjacent
+      const bool whole = there == (1 << NB) - 1 && c.shift > 4;
+      if (there & 1)
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                     ::"r"(stage_at), "l"(block_of<HD>(c, pg[0], is_g, is_slot)), "r"(whole ? SB : BLOCK<HD>), "r"(bar_at) : "memory");
+      if (!whole) {
+#pragma unroll
+        for (int i = 1; i < NB; ++i)
+          if (there >> i & 1)
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                         ::"r"(stage_at + i * BLOCK<HD>), "l"(block_of<HD>(c, pg[i], is_g, is_slot + 16 * i)), "r"(BLOCK<HD>), "r"(bar_at) : "memory");
       }
     }
     if (--to_issue > 0) {
       is_slot += TILE;
+      ++is_at;
       if (--is_left == 0) {
-        next_item<ROWS>(p, is);
-        is_left = is.nt;
-        is_slot = is.k0 * TILE + w * STEP;
-        is_table = c.table + (int64_t)is.b * c.W;
+        advance(is);
+        fetch_item(0);
+      } else if (is_at == 32) {
+        look_up();
       }
-      look_up();
     }
   };
 #pragma unroll
@@ -190,13 +248,13 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
   // ---- state of the current item ----
   uint32_t qf[NR][MT][2];
   float rs[NR][2];                        // score factor of rows 2 t4, 2 t4 + 1
-  int lim[NR][2], low[NR][2];             // slots (low, lim] that the row sees
-  int all_lo = 0, all_hi = 0;             // slots [all_lo, all_hi] that every row sees
+  int it_hi = 0, all_lo = 0, all_hi = 0;             // slots [all_lo, all_hi] that every row sees
   float r[NR][2], l[NR][2], o[NR][MT][4]; // weights are 2^(score - r), at most 2^(LIFT + LAZY)
   float* scores_at = nullptr;             // of slot 0 and this lane's first row
   auto load_rows = [&]() {
     const int per = p.rep * p.maps, at0 = it.len - it.n;
     if (p.scores) scores_at = it.rows <= p.stride ? p.scores + ((int64_t)it.b * c.G + it.g) * p.cap * p.stride + 2 * t4 : nullptr;
+    it_hi = it.hi;
     all_hi = min(it.len - 1, at0 + it.rt * ROWS / per);
     all_lo = p.window > 0 ? at0 + min(it.n - 1, (it.rt * ROWS + ROWS - 1) / per) - p.window + 1 : 0;
 #pragma unroll
@@ -226,7 +284,9 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
       int e = (int)(__float_as_uint(mx) >> 23) - 127;
       if (e == -127 || e == 128) e = 0;
       e = max(-126, min(126, e));
-      const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
+      // The factor of the scores is above 0: the largest product is the largest score, and what is masked stays so.  A
+      // factor of 0, or one that underflows, gives scores of 0 all the same: products are below 2^25.
+      const float down = __uint_as_float((uint32_t)(127 - e) << 23 | (p.scale_log2 < 0.f ? 0x80000000u : 0u)), up = __uint_as_float((uint32_t)(127 + e) << 23);
       // as the codes of a word are decoded: dims (0, 4) and (1, 5), then (2, 6) and (3, 7)
 #pragma unroll
       for (int i2 = 0; i2 < KW; ++i2)
@@ -234,14 +294,10 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
         for (int y = 0; y < 2; ++y)
 #pragma unroll
           for (int j = 0; j < 2; ++j) qf[nr][2 * i2 + y][j] = pack_h2(f[i2][2 * y + j] * down, f[i2][2 * y + j + 4] * down);
-      const float mine_rs = p.scale_log2 * up;
+      const float mine_rs = fmaxf(fabsf(p.scale_log2) * up, 1e-37f);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         rs[nr][x] = __shfl_sync(0xffffffffu, mine_rs, (2 * t4 + x) * 4);
-        const int rr = it.rt * ROWS + nr * 8 + 2 * t4 + x;
-        // rows past the last one are rows of zeros that see everything: they ask for no mask and are not written
-        lim[nr][x] = rr < it.rows ? min(it.len - 1, it.len - it.n + rr / per) : 0x7fffffff;
-        low[nr][x] = rr < it.rows && p.window > 0 ? it.len - it.n + rr / per - p.window : -1;
         r[nr][x] = NONE;
         l[nr][x] = 0.f;
       }
@@ -250,17 +306,22 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
 #pragma unroll
         for (int x = 0; x < 4; ++x) o[nr][j][x] = 0.f;
     }
+    __syncwarp();
+    if (lane < ROWS) {
+      // rows past the last one are rows of zeros that see everything: they ask for no mask and are not written
+      const int row = it.rt * ROWS + lane, at = at0 + row / per;
+      s_sees[w][lane] = row < it.rows ? make_int2(p.window > 0 ? at - p.window : -1, min(it.len - 1, at)) : make_int2(-1, 0x7fffffff);
+    }
+    __syncwarp();
   };
 
   // K rows of this lane in the fragments: tokens g8 and g8 + 8, dims HD / 4 t4 ..;  V: tokens 2 t4, 2 t4 + 1 and the same
   // + 8, dims HD / 8 g8 ..
   const uint32_t k_at = g8 * (HD / 2) + t4 * (HD / 8), kp_at = PARAMS<HD> + g8 * (HD / 16);
   const uint32_t v_at = HALF<HD> + 2 * t4 * (HD / 2) + g8 * (HD / 16), vp_at = HALF<HD> + PARAMS<HD> + 2 * t4 * (HD / 16);
-  auto scores = [&](uint32_t kb, int slot0, float (&s)[NR][4]) {
-#pragma unroll
-    for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) s[nr][x] = 0.f;
+  const Base base = c.base;
+  // raw products of a block's keys
+  auto products = [&](uint32_t kb, float (&s)[NR][4]) {
     uint32_t kw[2][KW];
     Levels lv[2][KW / 2];
 #pragma unroll
@@ -269,77 +330,98 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
         const uint4 v = lds16(kb + k_at + x * 8 * (HD / 2));
         const uint2 pw = lds8(kb + kp_at + x * 8 * (HD / 16));
         kw[x][0] = v.x; kw[x][1] = v.y; kw[x][KW - 2] = v.z; kw[x][KW - 1] = v.w;
-        lv[x][0] = levels_of(pw.x); lv[x][KW / 2 - 1] = levels_of(pw.y);
+        lv[x][0] = levels_of(pw.x, base); lv[x][KW / 2 - 1] = levels_of(pw.y, base);
       } else {
         const uint2 v = lds8(kb + k_at + x * 8 * (HD / 2));
         kw[x][0] = v.x; kw[x][1] = v.y;
-        lv[x][0] = levels_of(lds4(kb + kp_at + x * 8 * (HD / 16)));
+        lv[x][0] = levels_of(lds4(kb + kp_at + x * 8 * (HD / 16)), base);
       }
     }
     // S^T: word i holds runs 2 i, 2 i + 1 of the lane's dims, of groups (0, 1) or (2, 3)
 #pragma unroll
     for (int i = 0; i < KW; ++i) {
       uint32_t a[4], b[4];
-      decode(kw[0][i], lv[0][i % (KW / 2)], a);
-      decode(kw[1][i], lv[1][i % (KW / 2)], b);
+      decode(kw[0][i], lv[0][i % (KW / 2)], base, a);
+      decode(kw[1][i], lv[1][i % (KW / 2)], base, b);
 #pragma unroll
       for (int nr = 0; nr < NR; ++nr) {
-        mma(s[nr], a[0], b[0], a[1], b[1], qf[nr][2 * i][0], qf[nr][2 * i][1]);
+        if (i == 0) mma_new(s[nr], a[0], b[0], a[1], b[1], qf[nr][0][0], qf[nr][0][1]);
+        else mma(s[nr], a[0], b[0], a[1], b[1], qf[nr][2 * i][0], qf[nr][2 * i][1]);
         mma(s[nr], a[2], b[2], a[3], b[3], qf[nr][2 * i + 1][0], qf[nr][2 * i + 1][1]);
       }
     }
-    const bool all = slot0 + STEP - 1 <= all_hi && slot0 >= all_lo;
+  };
+  // raw products of the tile's blocks, -inf where a row does not see the token; times rs they are the scores (log2)
+  auto scores = [&](uint32_t at, int slot0, int there, float (&s)[NB][NR][4]) {
 #pragma unroll
-    for (int nr = 0; nr < NR; ++nr)
+    for (int i = 0; i < NB; ++i) products(at + i * BLOCK<HD>, s[i]);
+    if (there != (1 << NB) - 1 || slot0 + STEP - 1 > all_hi || slot0 < all_lo) {
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        s[nr][x] *= rs[nr][x & 1];
-        if (!all) {
-          const int slot = slot0 + g8 + (x >> 1) * 8;
-          if (slot > lim[nr][x & 1] || slot <= low[nr][x & 1]) s[nr][x] = -INFINITY;
+      for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const int2 sees = s_sees[w][nr * 8 + 2 * t4 + y];
+#pragma unroll
+          for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int slot = slot0 + 16 * i + g8 + x * 8;
+              if (slot > sees.y || slot <= sees.x || !(there >> i & 1)) s[i][nr][2 * x + y] = -INFINITY;
+            }
         }
-      }
-    if (scores_at) {                              // rows 2 t4 and 2 t4 + 1 of tokens g8 and g8 + 8
+    }
+    if (scores_at) {                              // rows 2 t4 and 2 t4 + 1 of tokens g8 and g8 + 8 of each block
 #pragma unroll
       for (int nr = 0; nr < NR; ++nr)
         if (nr * 8 + 2 * t4 < p.stride) {
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
-            *reinterpret_cast<float2*>(scores_at + (int64_t)(slot0 + g8 + 8 * x) * p.stride + nr * 8) = make_float2(s[nr][2 * x], s[nr][2 * x + 1]);
+          for (int i = 0; i < NB; ++i)
+            if (there >> i & 1) {
+#pragma unroll
+              for (int x = 0; x < 2; ++x)
+                *reinterpret_cast<float2*>(scores_at + (int64_t)(slot0 + 16 * i + g8 + 8 * x) * p.stride + nr * 8) = make_float2(s[i][nr][2 * x] * rs[nr][0], s[i][nr][2 * x + 1] * rs[nr][1]);
+            }
         }
     }
   };
-  auto raise = [&](float (&s)[NR][4]) {
+  auto raise = [&](float (&s)[NB][NR][4]) {
+    float mx[NR][2];
     bool grow = false;
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-      for (int x = 0; x < 2; ++x) grow = grow || fmaxf(s[nr][x], s[nr][x + 2]) > r[nr][x] + (LIFT + LAZY);
+      for (int x = 0; x < 2; ++x) {
+        mx[nr][x] = fmaxf(s[0][nr][x], s[0][nr][x + 2]);
+#pragma unroll
+        for (int i = 1; i < NB; ++i) mx[nr][x] = fmaxf(mx[nr][x], fmaxf(s[i][nr][x], s[i][nr][x + 2]));
+        mx[nr][x] *= rs[nr][x];
+        grow = grow || mx[nr][x] > r[nr][x] + (LIFT + LAZY);
+      }
     if (!__any_sync(0xffffffffu, grow)) return;
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        float mx = fmaxf(s[nr][x], s[nr][x + 2]);
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        const float r1 = fmaxf(r[nr][x], mx - LIFT), f = ex2(r[nr][x] - r1);
+        float m = mx[nr][x];
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+        const float r1 = fmaxf(r[nr][x], m - LIFT), f = ex2(r[nr][x] - r1);
         r[nr][x] = r1;
         l[nr][x] *= f;
 #pragma unroll
         for (int j = 0; j < MT; ++j) { o[nr][j][x] *= f; o[nr][j][x + 2] *= f; }
       }
   };
-  // P V of one tile
-  auto values = [&](uint32_t vb, int slot0, float (&s)[NR][4]) {
+  // P V of one block
+  auto values = [&](uint32_t vb, int slot0, bool clear, float (&s)[NR][4]) {
     uint32_t pf[NR][2];
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
       float e[4];
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        e[x] = ex2(s[nr][x] - r[nr][x & 1]);
+        e[x] = ex2(fmaf(s[nr][x], rs[nr][x & 1], -r[nr][x & 1]));
         l[nr][x & 1] += e[x];
       }
       pf[nr][0] = transposed(pack_h2(e[0], e[1]));
@@ -359,10 +441,10 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
         pw[x][0] = lds4(vb + vp_at + row * (HD / 16));
       }
     }
-    if (slot0 + 16 > it.hi) {                          // what is past the end may be anything: zeros
+    if (clear) {                                       // what is past the end, or not there, may be anything: zeros
 #pragma unroll
       for (int x = 0; x < 4; ++x)
-        if (slot0 + 2 * t4 + (x & 1) + (x >> 1) * 8 >= it.hi) {
+        if (slot0 + 2 * t4 + (x & 1) + (x >> 1) * 8 >= it_hi) {
 #pragma unroll
           for (int i = 0; i < VW; ++i) pw[x][i] = 0;
         }
@@ -373,8 +455,8 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
       for (int h = 0; h < 2; ++h) {                    // the word's lower and upper four dims, of one group each
         const uint32_t sel = h ? 0x7632u : 0x5410u;
         uint32_t a[4], b[4];
-        decode(__byte_perm(vw[0][i], vw[1][i], sel), levels_of(__byte_perm(pw[0][i], pw[1][i], sel)), a);
-        decode(__byte_perm(vw[2][i], vw[3][i], sel), levels_of(__byte_perm(pw[2][i], pw[3][i], sel)), b);
+        decode(__byte_perm(vw[0][i], vw[1][i], sel), levels_of(__byte_perm(pw[0][i], pw[1][i], sel), base), base, a);
+        decode(__byte_perm(vw[2][i], vw[3][i], sel), levels_of(__byte_perm(pw[2][i], pw[3][i], sel), base), base, b);
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
           mma(o[nr][4 * i + 2 * h], a[0], a[1], b[0], b[1], pf[nr][0], pf[nr][1]);          // dims HD / 8 g8 + 8 i + 4 h, + 1
@@ -482,8 +564,8 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
   };
 
   load_rows();
-  int tiles = it.nt - (int)(first - start);                           // of the item, still to be done
-  int slot0 = (it.k0 + (int)(first - start)) * TILE + w * STEP;
+  int tiles = it.nt - done;                                            // of the item, still to be done
+  int slot0 = (it.k0 + done) * TILE + w * STEP;
   uint32_t here = ring, bar_here = bar, phase = 0, there = ring + (ST - 1) * SB, bar_there = bar + (ST - 1) * 8;
   for (int left = (int)(last - first); left > 0; --left) {
     if (ok) {
@@ -492,11 +574,16 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
       waited += ok;
       if (!ok) s_cut = 1;                          // this item's rows and the next ones' are zeros
     }
-    if (ok && (flying & 1)) {
-      float s[NR][4];
-      scores(here, slot0, s);
+    const int blocks = flying & ((1 << NB) - 1);
+    if (ok && blocks) {
+      float s[NB][NR][4];
+      scores(here, slot0, blocks, s);
       raise(s);
-      values(here, slot0, s);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const bool not_there = !(blocks >> i & 1);
+        values(here + i * BLOCK<HD>, not_there ? it_hi : slot0 + 16 * i, not_there || slot0 + 16 * (i + 1) > it_hi, s[i]);
+      }
     }
     __syncwarp();                                  // the tile is read before its place is filled again
     there = here;
@@ -509,7 +596,7 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
       finish(start, tiles == 0);
       if (left > 1) {
         start += it.nt;
-        next_item<ROWS>(p, it);
+        advance(it);
         tiles = it.nt;
         slot0 = it.k0 * TILE + w * STEP;
         load_rows();
@@ -527,10 +614,10 @@ __global__ void __launch_bounds__(NK) kept_weights_kernel(const __grid_constant_
   const Cache4& c = p.c;
   const int g = blockIdx.y, b = blockIdx.z;
   Item it;
-  if (!in_order(c, b) || !set_sequence<2 * 8>(p, it, b) || it.rows > p.stride) return;
+  if (!in_order(c, b) || !set_sequence<2 * 8, TILE>(p, it, b) || it.rows > p.stride) return;
   const int per = p.rep * p.maps;
   const float* lse = p.lse + (int64_t)it.t0 * p.H * p.maps + g * per;
-  for (int slot = it.lo / STEP * STEP + blockIdx.x * NK + threadIdx.x; slot < it.hi; slot += gridDim.x * NK) {
+  for (int slot = it.lo / 16 * 16 + blockIdx.x * NK + threadIdx.x; slot < it.hi; slot += gridDim.x * NK) {
     const int pg = c.table[(int64_t)b * c.W + (slot >> c.shift)];
     if (pg < 0 || pg >= c.P) continue;                  // recorded where its keys were looked for
     const float* s = p.scores + (((int64_t)b * c.G + g) * p.cap + slot) * p.stride;
@@ -592,7 +679,7 @@ __global__ void __launch_bounds__(WW * 32) weights_kernel(const __grid_constant_
           params = *reinterpret_cast<const uint32_t*>(blk + PARAMS<HD> + row * (HD / 16) + 4 * (i % (KW / 2)));
         }
         uint32_t h[4];
-        decode(word, levels_of(params), h);
+        decode(word, levels_of(params, c.base), c.base, h);
         a[m][2 * i][x] = h[0];
         a[m][2 * i][x + 2] = h[1];
         a[m][2 * i + 1][x] = h[2];

@@ -195,15 +195,16 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
     // further round: the banks of both differ.
     uint8_t* const at = ring + (cc >> 1) * (BN * 128) + r0c * 128;
     const int c0 = HD == 128 ? (cc & 1) * 4 : cc * 4, turn = HD == 128 ? cc & 2 : 0;
+    const Base base = c.base;
     auto store = [&](uint8_t* row, const uint4& x, const uint32_t (&params)[HD / 64]) {
       Levels lv[HD / 64];
 #pragma unroll
-      for (int i = 0; i < HD / 64; ++i) lv[i] = levels_of(params[i]);
+      for (int i = 0; i < HD / 64; ++i) lv[i] = levels_of(params[i], base);
       const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
       for (int m = 0; m < 4; ++m) {                          // words m and m + 2 are of the same groups
         uint32_t h[4];
-        decode(turn ? w[m ^ 2] : w[m], lv[HD == 128 ? m & 1 : 0], h);
+        decode(turn ? w[m ^ 2] : w[m], lv[HD == 128 ? m & 1 : 0], base, h);
         *reinterpret_cast<uint4*>(row + (((c0 + (m ^ turn)) ^ (r0c & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
       }
     };

@@ -35,9 +35,9 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const float* 
   }
 }
 // 8 dims of a word of codes
-__device__ __forceinline__ void values8(uint32_t w, uint32_t params, float* f) {
+__device__ __forceinline__ void values8(uint32_t w, uint32_t params, const Base& base, float* f) {
   uint32_t h[4];
-  decode(w, levels_of(params), h);
+  decode(w, levels_of(params, base), base, h);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h[e]));
@@ -82,8 +82,8 @@ __global__ void __launch_bounds__(NR) read_kernel(const Cache4 c, T* __restrict_
         const uint32_t w0 = *reinterpret_cast<const uint32_t*>(at + row * (HD / 2) + sub * 4);
         const uint32_t w1 = *reinterpret_cast<const uint32_t*>(at + row * (HD / 2) + HD / 4 + sub * 4);
         const uint32_t params = *reinterpret_cast<const uint32_t*>(at + PARAMS<HD> + (row * (J / 2) + sub % (J / 2)) * 4);
-        values8(w0, params, f + 16 * x);
-        values8(w1, params, f + 16 * x + 8);
+        values8(w0, params, c.base, f + 16 * x);
+        values8(w1, params, c.base, f + 16 * x + 8);
       }
     }
     const int64_t to = ((int64_t)t * c.G + g) * HD + d;

@@ -32,6 +32,8 @@ using namespace split;
 // 158; one map, 8 sequences of 8000, 16 / 4 heads: 32 rows 55 and 78, 64 rows 83 and 94 (of when the rule was set; since
 // then 64 rows 84, and 80 rows 81 in the chunk kernel).
 constexpr int FEW = 64;
+constexpr int STEP = 16;                       // tokens of a warp per tile
+constexpr int TILE = STEP * NW;                // tokens per tile
 constexpr float LAZY = 8.f;                    // log2 by which a row may outgrow its reference maximum
 constexpr float SLACK = 64.f;                  // value scales of up to this times O's unit are not looked at
 
@@ -97,7 +99,7 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
   for (int i = 0; i < chunk; ++i) {
     const int b = tid * chunk + i;
     if (b < c.B) {
-      mine += tiles_of<ROWS>(p, b);
+      mine += tiles_of<ROWS, TILE>(p, b);
       broken = broken || !in_order(c, b);
     }
   }
@@ -124,7 +126,7 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
     int64_t at = incl - mine;
     int b = tid * chunk;
     for (;; ++b) {
-      const int64_t n = tiles_of<ROWS>(p, b);
+      const int64_t n = tiles_of<ROWS, TILE>(p, b);
       if (first < at + n) break;
       at += n;
     }
@@ -144,9 +146,9 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
   if (first >= last || total >> 60) return;
 
   Item it;                                          // of the tile being computed
-  set_sequence<ROWS>(p, it, s_b);
+  set_sequence<ROWS, TILE>(p, it, s_b);
   int64_t start = s_begin;                          // list position of the item's first tile
-  while (first >= start + it.nt) { start += it.nt; next_item<ROWS>(p, it); }
+  while (first >= start + it.nt) { start += it.nt; next_item<ROWS, TILE>(p, it); }
 
   // ---- ring: the issue side runs ST - 1 tiles ahead ----
   const uint32_t ring = su32(smem) + w * ST * SB, bar = su32(bars[w]);
@@ -197,7 +199,7 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
     if (--to_issue > 0) {
       is_slot += TILE;
       if (--is_left == 0) {
-        next_item<ROWS>(p, is);
+        next_item<ROWS, TILE>(p, is);
         is_left = is.nt;
         is_slot = is.k0 * TILE + w * STEP;
         is_table = c.table + (int64_t)is.b * c.W;
@@ -530,7 +532,7 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
       finish(start, tiles == 0);
       if (left > 1) {
         start += it.nt;
-        next_item<ROWS>(p, it);
+        next_item<ROWS, TILE>(p, it);
         tiles = it.nt;
         slot0 = it.k0 * TILE + w * STEP;
         load_rows();

@@ -12,8 +12,6 @@ namespace split {
 using namespace paged;
 
 constexpr int NW = 4, NT = NW * 32, NJ = 512;
-constexpr int STEP = 16;                       // tokens of a warp per tile
-constexpr int TILE = STEP * NW;                // tokens per tile
 constexpr float NONE = -1e30f;                 // maximum of no scores: 2^(score - NONE) is never formed, 2^(NONE - m) is 0
 
 // The file's own words.
@@ -75,6 +73,7 @@ __device__ __forceinline__ void drain_tile(uint32_t bar, uint32_t parity) {
 }
 
 // One row tile of one KV head of one sequence.
+// ROWS: rows of a tile, TILE: tokens of a tile.
 struct Item {
   int b, g, rt;
   int t0, n, len;            // first packed token, new tokens, cached length
@@ -82,7 +81,7 @@ struct Item {
   int lo, hi, k0, nt;        // slots [lo, hi) that some row of the tile sees, first tile, tiles (at least 1)
 };
 
-template <int ROWS, class P>
+template <int ROWS, int TILE, class P>
 __device__ __forceinline__ void set_range(const P& p, Item& it) {
   const int per = p.rep * p.maps, first = it.len - it.n;
   const int i0 = it.rt * ROWS / per, i1 = min(it.n - 1, (it.rt * ROWS + ROWS - 1) / per);
@@ -91,7 +90,7 @@ __device__ __forceinline__ void set_range(const P& p, Item& it) {
   it.k0 = it.lo / TILE;
   it.nt = it.hi > it.lo ? (it.hi + TILE - 1) / TILE - it.k0 : 1;
 }
-template <int ROWS, class P>
+template <int ROWS, int TILE, class P>
 __device__ __forceinline__ bool set_sequence(const P& p, Item& it, int b) {
   const Table& c = p.c;
   const int t0 = c.cu[b], t1 = c.cu[b + 1], len = c.lens[b];
@@ -103,26 +102,26 @@ __device__ __forceinline__ bool set_sequence(const P& p, Item& it, int b) {
   if (it.rows > p.few) return false;
   it.len = cached_length(c, len);
   it.g = it.rt = 0;
-  set_range<ROWS>(p, it);
+  set_range<ROWS, TILE>(p, it);
   return true;
 }
-template <int ROWS, class P>
+template <int ROWS, int TILE, class P>
 __device__ __forceinline__ void next_item(const P& p, Item& it) {
-  if (ROWS > 8 && (it.rt + 1) * ROWS < it.rows) { ++it.rt; set_range<ROWS>(p, it); return; }
-  if (it.g + 1 < p.c.G) { ++it.g; it.rt = 0; set_range<ROWS>(p, it); return; }
+  if (ROWS > 8 && (it.rt + 1) * ROWS < it.rows) { ++it.rt; set_range<ROWS, TILE>(p, it); return; }
+  if (it.g + 1 < p.c.G) { ++it.g; it.rt = 0; set_range<ROWS, TILE>(p, it); return; }
   int b = it.b + 1;
-  while (b < p.c.B && !set_sequence<ROWS>(p, it, b)) ++b;
+  while (b < p.c.B && !set_sequence<ROWS, TILE>(p, it, b)) ++b;
   it.b = b;
 }
-template <int ROWS, class P>
+template <int ROWS, int TILE, class P>
 __device__ __forceinline__ int64_t tiles_of(const P& p, int b) {
   Item it;
-  if (!set_sequence<ROWS>(p, it, b)) return 0;
+  if (!set_sequence<ROWS, TILE>(p, it, b)) return 0;
   int64_t n = 0;
   if constexpr (ROWS == 8) n = it.nt;                           // 8 rows are all there can be
   else
     for (; it.rt * ROWS < it.rows; ++it.rt) {
-      set_range<ROWS>(p, it);
+      set_range<ROWS, TILE>(p, it);
       n += it.nt;
     }
   return n * p.c.G;
