@@ -3,11 +3,11 @@
 // Eviction keeps, for each sequence of more than `budget` tokens and each KV head by itself, the last `recent` tokens and of
 // the others the budget - recent of largest mass, ties to the lower slot, and moves them, in order, to slots 0 .. budget - 1.
 //
-// select: a cluster of CTAs per (sequence, head) finds the least kept mass by radix: 11, 11 and 10 bits of the weights' order
+// select: a cluster of CTAs per (sequence, head) finds the least kept mass by radix: four times 8 bits of the weights' order
 // as whole numbers, each pass a histogram in shared memory that the cluster's CTAs add up through distributed shared
-// memory.  A thread holds the 16 slots of a block, in order, so a scan of the threads' counts gives each kept slot its place.
-// move: 8 lanes per token copy its codes, parameters and mass.  To other pages in one pass; in place through a packed
-// copy, since the kept tokens' places overlap.
+// memory.  Weights lie in few bins of their leading bits, so the lanes of a warp count apart.  A thread holds the 16 slots of a block, in order, so a scan of the threads' counts gives each kept slot its place.
+// move: a warp gathers the tokens of two blocks and writes them whole.  To other pages in one pass; in place through a
+// packed copy, since the kept tokens' places overlap.
 #include "paged4.cuh"
 
 #include <cooperative_groups.h>
@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(NR) read_kernel(const Cache4 c, T* __restrict_
 }
 
 // ---- eviction: which slots -------------------------------------------------------------------------
-constexpr int NS = 512, KPT = 16, BINS = 2048;       // threads, slots of a thread, bins of a pass
+constexpr int KPT = 16, BINS = 256;                  // slots of a thread, bins of a pass
 constexpr int MOST = 8;                               // CTAs of a cluster
 
 struct Evict {
@@ -114,6 +114,7 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 }
 
 // Sums of (a, b) over the threads before this one, and over all.
+template <int NS>
 __device__ __forceinline__ int2 scan2(int2 v, int2& total, int2* sm) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   int2 x = v;
@@ -124,24 +125,27 @@ __device__ __forceinline__ int2 scan2(int2 v, int2& total, int2* sm) {
   }
   if (lane == 31) sm[w] = x;
   __syncthreads();
-  int2 before = make_int2(0, 0);
-  total = make_int2(0, 0);
-#pragma unroll
-  for (int i = 0; i < NS / 32; ++i) {
-    if (i < w) { before.x += sm[i].x; before.y += sm[i].y; }
-    total.x += sm[i].x;
-    total.y += sm[i].y;
-  }
+  // the warps' totals, a lane each
+  const int2 t = lane < NS / 32 ? sm[lane] : make_int2(0, 0);
+  total = make_int2(__reduce_add_sync(0xffffffffu, t.x), __reduce_add_sync(0xffffffffu, t.y));
+  const int2 before = make_int2(__reduce_add_sync(0xffffffffu, lane < w ? t.x : 0), __reduce_add_sync(0xffffffffu, lane < w ? t.y : 0));
   __syncthreads();
   return make_int2(before.x + x.x - v.x, before.y + x.y - v.y);
 }
 
-__global__ void __launch_bounds__(NS) select_kernel(const Evict p) {
+// NS threads, C CTAs of a cluster for each (sequence, head).
+template <int NS, int C>
+__global__ void __launch_bounds__(NS) select_kernel(const __grid_constant__ Evict p) {
   cg::cluster_group cluster = cg::this_cluster();
-  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  __shared__ int hist[2][BINS];                       // the passes take turns
-  __shared__ int2 sm[NS / 32], mine;
-  __shared__ int s_bin, s_above;
+  const int rank = C == 1 ? 0 : (int)cluster.block_rank();
+  auto everybody = [&]() { if (C == 1) __syncthreads(); else cluster.sync(); };
+  // lanes count by themselves, or every eighth together where there are few keys to count and the sums cost more
+  constexpr int L = NS == 1024 ? 32 : 8;
+  __shared__ int hist[BINS * (L + 1)];
+  __shared__ int sums[2][BINS];                       // of the lanes; the passes take turns
+  __shared__ int2 sm[32], mine[2];
+  __shared__ int s_bin[2], s_above[2];
+  asm volatile("griddepcontrol.launch_dependents;");  // the move waits for this grid's end by itself
   const Cache4& c = p.c;
   const int g = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
   const int len = cached_length(c, c.lens[b]), K = p.budget;
@@ -179,16 +183,13 @@ __global__ void __launch_bounds__(NS) select_kernel(const Evict p) {
     }
   };
   load(0);
-  uint32_t at = 0;                                    // the bits of the least kept weight found so far
-  for (int i = tid; i < 2 * BINS; i += NS) (&hist[0][0])[i] = 0;
+  for (int i = tid; i < BINS * (L + 1); i += NS) hist[i] = 0;
   __syncthreads();
-  int shift = 32;
+  uint32_t at = 0;                                    // the bits of the least kept weight found so far
 #pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {
-    const int bits = pass < 2 ? 11 : 10;
-    const uint32_t above = pass == 0 ? 0u : 0xFFFFFFFFu << shift;      // bits that are settled
-    shift -= bits;
-    int* h = hist[pass & 1];
+  for (int pass = 0; pass < 4; ++pass) {
+    const int shift = 24 - 8 * pass, turn = pass & 1;
+    const uint32_t above = pass == 0 ? 0u : 0xFFFFFFFFu << (shift + 8);      // bits that are settled
     if (want > 0)
 #pragma unroll 1
       for (int i = 0; i < batches; ++i) {
@@ -196,35 +197,37 @@ __global__ void __launch_bounds__(NS) select_kernel(const Evict p) {
         const int64_t s0 = first_of(i);
 #pragma unroll
         for (int e = 0; e < KPT; ++e)
-          if (s0 + e < old && (key[e] & above) == at) atomicAdd(&h[key[e] >> shift & ((1 << bits) - 1)], 1);
+          if (s0 + e < old && (key[e] & above) == at) atomicAdd(&hist[(key[e] >> shift & (BINS - 1)) * (L + 1) + tid % L], 1);
       }
-    cluster.sync();
-    // bins from the top: thread t takes BINS / NS of them, the highest first
-    constexpr int PER = BINS / NS;
-    int n[PER], sum = 0;
+    __syncthreads();
+    const int bin = BINS - 1 - tid;                   // from the top, a bin per thread
+    int n = 0;
+    if (tid < BINS) {
 #pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      const int bin = BINS - 1 - (tid * PER + e);
-      n[e] = 0;
-      for (int r = 0; r < C; ++r) n[e] += *cluster.map_shared_rank(&h[bin], r);
-      sum += n[e];
+      for (int k = 0; k < L; ++k) {
+        n += hist[bin * (L + 1) + k];
+        hist[bin * (L + 1) + k] = 0;                  // for the next pass
+      }
+      if (C > 1) sums[turn][bin] = n;
+    }
+    if (C > 1) {
+      cluster.sync();                                 // the pass before the last has been read by all, too
+      if (tid < BINS) {
+        int part[C];
+#pragma unroll
+        for (int r = 0; r < C; ++r) part[r] = *cluster.map_shared_rank(&sums[turn][bin], r);
+        n = 0;
+#pragma unroll
+        for (int r = 0; r < C; ++r) n += part[r];
+      }
     }
     int2 total;
-    int before = scan2(make_int2(sum, 0), total, sm).x;
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      if (before < want && want <= before + n[e]) { s_bin = BINS - 1 - (tid * PER + e); s_above = before; }
-      before += n[e];
-    }
-    if (want == 0 && tid == 0) { s_bin = (1 << bits) - 1; s_above = 0; }      // no place: nothing is as heavy
+    const int before = scan2<NS>(make_int2(n, 0), total, sm).x;
+    if (before < want && want <= before + n) { s_bin[turn] = bin; s_above[turn] = before; }
+    if (want == 0 && tid == 0) { s_bin[turn] = BINS - 1; s_above[turn] = 0; }      // no place: nothing is as heavy
     __syncthreads();
-    at |= (uint32_t)s_bin << shift;
-    want -= s_above;
-    cluster.sync();                                   // everybody has read this pass's bins
-    if (pass == 0) {                                  // for the third pass
-      for (int i = tid; i < BINS; i += NS) h[i] = 0;
-      __syncthreads();
-    }
+    at |= (uint32_t)s_bin[turn] << shift;
+    want -= s_above[turn];
   }
   // `want` of those as heavy as `at` are kept, the lowest slots, and all heavier ones
   int2 done = make_int2(0, 0);                        // heavier, and as heavy, in slots before the batch
@@ -236,15 +239,19 @@ __global__ void __launch_bounds__(NS) select_kernel(const Evict p) {
 #pragma unroll
     for (int e = 0; e < KPT; ++e)
       if (s0 + e < old) { v.x += key[e] > at; v.y += key[e] == at; }
-    int2 x = scan2(v, total, sm);
-    if (tid == 0) mine = total;
-    cluster.sync();
-    int2 batch = make_int2(0, 0);
-    for (int r = 0; r < C; ++r) {
-      const int2 o = *cluster.map_shared_rank(&mine, r);
-      if (r < rank) { x.x += o.x; x.y += o.y; }
-      batch.x += o.x;
-      batch.y += o.y;
+    int2 x = scan2<NS>(v, total, sm);
+    int2 batch = total;
+    if (C > 1) {
+      if (tid == 0) mine[i & 1] = total;              // the batches take turns
+      cluster.sync();
+      batch = make_int2(0, 0);
+#pragma unroll
+      for (int r = 0; r < C; ++r) {
+        const int2 o = *cluster.map_shared_rank(&mine[i & 1], r);
+        if (r < rank) { x.x += o.x; x.y += o.y; }
+        batch.x += o.x;
+        batch.y += o.y;
+      }
     }
     x.x += done.x;
     x.y += done.y;
@@ -258,119 +265,158 @@ __global__ void __launch_bounds__(NS) select_kernel(const Evict p) {
         x.x += heavier;
         x.y += same;
       }
-    cluster.sync();                                   // everybody has read `mine`
   }
   for (int i = rank * NS + tid; i < p.recent; i += C * NS) kept[K - p.recent + i] = old + i;
+  everybody();                                        // nobody leaves while its shared memory is read
+}
+
+template <int NS, int C> void launch_select(const Evict& p) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)C, (unsigned)p.c.G, (unsigned)p.c.B);
+  cfg.blockDim = dim3(NS);
+  cfg.stream = stream();
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)C;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = C > 1 ? 1 : 0;
+  MAMF_CUDA_CHECK(cudaLaunchKernelEx(&cfg, select_kernel<NS, C>, p));
 }
 
 // ---- eviction: the move ----------------------------------------------------------------------------
-constexpr int NM = 256, LANES = 8, UNROLL = 4;
-template <int HD> constexpr int RECORD = HD + HD / 8 + 16;          // a packed token: codes, parameters, mass
+constexpr int NM = 128, PAIR = 2;                                    // threads, blocks that a warp moves at once
+template <int HD> constexpr int PACKED = BLOCK<HD> + 64;             // a packed block: its tokens, their masses
 
 enum Mode { DIRECT, PACK, UNPACK };
 
-// A token's pieces by lane: lanes 0-3 keys, 4-7 values, 16 bytes of codes each (8 of 64 dims); lanes 0 and 4 the
-// parameters; lane 1 the mass.
+// A warp fills blocks of the kept tokens' places: lanes 4 t .. 4 t + 3 take the codes of tokens t and t + 8, 16 bytes a lane
+// of keys and of values (8 of 64 dims), lanes t and t + 16 the parameters of token t, lane t its mass.  What is written is
+// whole blocks.
 template <int HD> struct Piece {
-  uint4 code;
+  uint4 code[2][2];
   uint2 param;
   float mass;
 };
 template <int HD>
-__device__ __forceinline__ void get(Piece<HD>& x, const uint8_t* half, int row, int q, const float* mass, int lane) {
-  if (HD == 128) x.code = *reinterpret_cast<const uint4*>(half + row * (HD / 2) + q * 16);
-  else *reinterpret_cast<uint2*>(&x.code) = *reinterpret_cast<const uint2*>(half + row * (HD / 2) + q * 8);
-  if (q == 0) {
-    if (HD == 128) x.param = *reinterpret_cast<const uint2*>(half + PARAMS<HD> + row * (HD / 16));
-    else x.param.x = *reinterpret_cast<const uint32_t*>(half + PARAMS<HD> + row * (HD / 16));
-  }
-  if (lane == 1) x.mass = *mass;
+__device__ __forceinline__ void copy_codes(uint4& to, const uint8_t* from) {
+  if (HD == 128) to = *reinterpret_cast<const uint4*>(from);
+  else *reinterpret_cast<uint2*>(&to) = *reinterpret_cast<const uint2*>(from);
 }
 template <int HD>
-__device__ __forceinline__ void put(const Piece<HD>& x, uint8_t* half, int row, int q, float* mass, int lane) {
-  if (HD == 128) *reinterpret_cast<uint4*>(half + row * (HD / 2) + q * 16) = x.code;
-  else *reinterpret_cast<uint2*>(half + row * (HD / 2) + q * 8) = *reinterpret_cast<const uint2*>(&x.code);
-  if (q == 0) {
-    if (HD == 128) *reinterpret_cast<uint2*>(half + PARAMS<HD> + row * (HD / 16)) = x.param;
-    else *reinterpret_cast<uint32_t*>(half + PARAMS<HD> + row * (HD / 16)) = x.param.x;
-  }
-  if (lane == 1) *mass = x.mass;
+__device__ __forceinline__ void copy_codes(uint8_t* to, const uint4& from) {
+  if (HD == 128) *reinterpret_cast<uint4*>(to) = from;
+  else *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(&from);
 }
 
 template <int HD, int MODE>
-__global__ void __launch_bounds__(NM) move_kernel(const Evict p) {
+__global__ void __launch_bounds__(NM) move_kernel(const __grid_constant__ Evict p) {
   const Cache4& c = p.c;
-  const int lane = threadIdx.x % LANES, q = lane & 3, side = lane >> 2;
-  const int g = blockIdx.y, b = blockIdx.z;
-  const int64_t row0 = ((int64_t)b * c.G + g) * p.budget;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, g = blockIdx.y, b = blockIdx.z, q = lane & 3;
+  const int blocks = (p.budget + 15) >> 4;
+  const int first = (blockIdx.x * (NM / 32) + w) * PAIR;
+  if (first >= blocks) return;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int* kept = p.kept + ((int64_t)b * c.G + g) * p.budget;
   const int* table = c.table + (int64_t)b * c.W;
   const int* to = p.out_table + (int64_t)b * p.out_W;
-  constexpr int GROUPS = NM / LANES;
-  const int r0 = blockIdx.x * (GROUPS * UNROLL) + threadIdx.x / LANES;
-  int src[UNROLL];
-  uint8_t* dst[UNROLL];
-  float* dst_mass[UNROLL];
-  Piece<HD> x[UNROLL];
+  int src[PAIR], page[PAIR];                          // of token lane & 15: its slot and that one's page
+  uint8_t* dst[PAIR];
+  float* dst_mass[PAIR];
 #pragma unroll
-  for (int u = 0; u < UNROLL; ++u) {
-    const int r = r0 + u * GROUPS;
-    src[u] = r < p.budget ? p.kept[row0 + r] : -1;
-    if (MODE != DIRECT && src[u] == r) src[u] = -1;   // it stays
+  for (int u = 0; u < PAIR; ++u) {
+    const int r = (first + u) * 16 + (lane & 15);
+    src[u] = r < p.budget ? kept[r] : -1;
+    // in place, blocks whose tokens stay are left alone, by both passes
+    if (MODE != DIRECT && __all_sync(0xffffffffu, src[u] < 0 || src[u] == r)) src[u] = -1;
+  }
+#pragma unroll
+  for (int u = 0; u < PAIR; ++u) {
+    const int r0 = (first + u) * 16;
+    page[u] = 0;
     dst[u] = nullptr;
-    if (src[u] < 0) continue;
+    if (__all_sync(0xffffffffu, src[u] < 0)) continue;
+    if (MODE != UNPACK && src[u] >= 0) page[u] = table[src[u] >> c.shift];
     if (MODE == PACK) {
-      dst[u] = p.packed + (row0 + r) * RECORD<HD>;
+      dst[u] = p.packed + (((int64_t)b * c.G + g) * blocks + first + u) * PACKED<HD>;
+      dst_mass[u] = reinterpret_cast<float*>(dst[u] + BLOCK<HD>);
       continue;
     }
-    const int pg = to[r >> c.shift];
+    const int pg = to[r0 >> c.shift];
     if (pg >= 0 && pg < c.P) {
-      dst[u] = block_of<HD>(c, pg, g, r) + side * HALF<HD>;
-      dst_mass[u] = c.mass + (((int64_t)pg * c.G + g) << c.shift) + (r & (c.page - 1));
+      dst[u] = block_of<HD>(c, pg, g, r0);
+      dst_mass[u] = c.mass + (((int64_t)pg * c.G + g) << c.shift) + (r0 & (c.page - 1));
     } else if (lane == 0) {
       record(ERR_PAGE);
     }
   }
+  Piece<HD> x[PAIR];
 #pragma unroll
-  for (int u = 0; u < UNROLL; ++u) {
+  for (int u = 0; u < PAIR; ++u) {
     if (!dst[u]) continue;
-    const int r = r0 + u * GROUPS;
-    if (MODE == UNPACK) {
-      const uint8_t* rec = p.packed + (row0 + r) * RECORD<HD>;
-      if (HD == 128) x[u].code = *reinterpret_cast<const uint4*>(rec + lane * 16);
-      else *reinterpret_cast<uint2*>(&x[u].code) = *reinterpret_cast<const uint2*>(rec + lane * 8);
-      x[u].param = *reinterpret_cast<const uint2*>(rec + HD + side * 8);
-      x[u].mass = *reinterpret_cast<const float*>(rec + HD + 16);
-      continue;
+    if (MODE != UNPACK && src[u] >= 0 && (page[u] < 0 || page[u] >= c.P)) { src[u] = -1; record(ERR_PAGE); }
+    const uint8_t* packed = MODE == UNPACK ? p.packed + (((int64_t)b * c.G + g) * blocks + first + u) * PACKED<HD> : nullptr;
+    // where the token's block is, and its row of it
+    const int64_t mine = MODE == UNPACK ? 0 : src[u] >= 0 ? block_of<HD>(c, page[u], g, src[u]) - c.blocks : -1;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int t = (lane >> 2) + 8 * h, s = __shfl_sync(0xffffffffu, src[u], t);
+      const int64_t off = __shfl_sync(0xffffffffu, mine, t);
+      if (s < 0) continue;
+      const uint8_t* blk = MODE == UNPACK ? packed : c.blocks + off;
+      const int row = MODE == UNPACK ? t : s & 15;
+      copy_codes<HD>(x[u].code[h][0], blk + row * (HD / 2) + q * (HD / 8));
+      copy_codes<HD>(x[u].code[h][1], blk + HALF<HD> + row * (HD / 2) + q * (HD / 8));
     }
-    const int pg = table[src[u] >> c.shift];
-    if (pg < 0 || pg >= c.P) { dst[u] = nullptr; if (lane == 0) record(ERR_PAGE); continue; }
-    get<HD>(x[u], block_of<HD>(c, pg, g, src[u]) + side * HALF<HD>, src[u] & 15, q,
-            c.mass + (((int64_t)pg * c.G + g) << c.shift) + (src[u] & (c.page - 1)), lane);
+    if (src[u] >= 0) {
+      const uint8_t* blk = MODE == UNPACK ? packed : c.blocks + mine;
+      const int row = MODE == UNPACK ? lane & 15 : src[u] & 15;
+      const uint8_t* at = blk + (lane >> 4) * HALF<HD> + PARAMS<HD> + row * (HD / 16);
+      if (HD == 128) x[u].param = *reinterpret_cast<const uint2*>(at);
+      else x[u].param.x = *reinterpret_cast<const uint32_t*>(at);
+      if (lane < 16) x[u].mass = MODE == UNPACK ? reinterpret_cast<const float*>(packed + BLOCK<HD>)[row]
+                                                : c.mass[(((int64_t)page[u] * c.G + g) << c.shift) + (src[u] & (c.page - 1))];
+    }
   }
 #pragma unroll
-  for (int u = 0; u < UNROLL; ++u) {
+  for (int u = 0; u < PAIR; ++u) {
     if (!dst[u]) continue;
-    const int r = r0 + u * GROUPS;
-    if (MODE == PACK) {
-      if (HD == 128) *reinterpret_cast<uint4*>(dst[u] + lane * 16) = x[u].code;
-      else *reinterpret_cast<uint2*>(dst[u] + lane * 8) = *reinterpret_cast<const uint2*>(&x[u].code);
-      if (q == 0) *reinterpret_cast<uint2*>(dst[u] + HD + side * 8) = x[u].param;
-      if (lane == 1) *reinterpret_cast<float*>(dst[u] + HD + 16) = x[u].mass;
-    } else {
-      put<HD>(x[u], dst[u], r & 15, q, dst_mass[u], lane);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int t = (lane >> 2) + 8 * h;
+      if (__shfl_sync(0xffffffffu, src[u], t) < 0) continue;
+      copy_codes<HD>(dst[u] + t * (HD / 2) + q * (HD / 8), x[u].code[h][0]);
+      copy_codes<HD>(dst[u] + HALF<HD> + t * (HD / 2) + q * (HD / 8), x[u].code[h][1]);
+    }
+    if (src[u] >= 0) {
+      uint8_t* at = dst[u] + (lane >> 4) * HALF<HD> + PARAMS<HD> + (lane & 15) * (HD / 16);
+      if (HD == 128) *reinterpret_cast<uint2*>(at) = x[u].param;
+      else *reinterpret_cast<uint32_t*>(at) = x[u].param.x;
+      if (lane < 16) dst_mass[u][lane] = x[u].mass;
     }
   }
 }
 
-template <int HD> void launch_move(Evict& p, bool in_place) {
-  const dim3 grid((unsigned)((p.budget + NM / LANES * UNROLL - 1) / (NM / LANES * UNROLL)), (unsigned)p.c.G, (unsigned)p.c.B);
-  if (!in_place) { move_kernel<HD, DIRECT><<<grid, NM, 0, stream()>>>(p); MAMF_LAUNCH_CHECK(); return; }
-  const at::Tensor ws = at::empty({(int64_t)p.c.B * p.c.G * p.budget * RECORD<HD>}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA));
+template <int HD, int MODE> void launch_move(const Evict& p) {
+  const int per = NM / 32 * PAIR * 16;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((p.budget + per - 1) / per), (unsigned)p.c.G, (unsigned)p.c.B);
+  cfg.blockDim = dim3(NM);
+  cfg.stream = stream();
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = MODE == UNPACK ? 0 : 1;
+  MAMF_CUDA_CHECK(cudaLaunchKernelEx(&cfg, move_kernel<HD, MODE>, p));
+}
+template <int HD> void move_kept(Evict& p, bool in_place) {
+  if (!in_place) { launch_move<HD, DIRECT>(p); return; }
+  const int64_t blocks = (int64_t)p.c.B * p.c.G * ((p.budget + 15) / 16);
+  const at::Tensor ws = at::empty({blocks * PACKED<HD>}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA));
   p.packed = ws.data_ptr<uint8_t>();
-  move_kernel<HD, PACK><<<grid, NM, 0, stream()>>>(p);
-  MAMF_LAUNCH_CHECK();
-  move_kernel<HD, UNPACK><<<grid, NM, 0, stream()>>>(p);
-  MAMF_LAUNCH_CHECK();
+  launch_move<HD, PACK>(p);
+  launch_move<HD, UNPACK>(p);
 }
 
 }  // namespace kv4
@@ -427,22 +473,16 @@ std::vector<at::Tensor> kv4_evict(at::Tensor blocks, at::Tensor mass, at::Tensor
   p.lens_out = lens_out.data_ptr<int>();
   p.budget = (int)budget;
   p.recent = (int)recent;
-  // CTAs per (sequence, head): as many as the table's longest sequence fills, up to a cluster
-  int C = 1;
-  while (C < MOST && (int64_t)C * NS * KPT < (int64_t)p.c.W * p.c.page) C *= 2;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)C, (unsigned)p.c.G, (unsigned)p.c.B);
-  cfg.blockDim = dim3(NS);
-  cfg.stream = stream();
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)C;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  MAMF_CUDA_CHECK(cudaLaunchKernelEx(&cfg, select_kernel, p));
+  // As many threads and CTAs per (sequence, head) as the table's longest sequence has blocks for.
+  const int64_t threads = (int64_t)p.c.W * p.c.page / KPT;
+  if (threads <= 256) launch_select<256, 1>(p);
+  else if (threads <= 512) launch_select<512, 1>(p);
+  else if (threads <= 1024) launch_select<512, 2>(p);
+  else if (threads <= 2048) launch_select<512, 4>(p);
+  else if (threads <= 4096) launch_select<512, 8>(p);
+  else launch_select<1024, 8>(p);
   const bool in_place = to.data_ptr() == table.data_ptr();
-  if (hd == 128) launch_move<128>(p, in_place); else launch_move<64>(p, in_place);
+  if (hd == 128) move_kept<128>(p, in_place); else move_kept<64>(p, in_place);
   return {kept, lens_out};
 }
 
