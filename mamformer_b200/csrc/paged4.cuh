@@ -137,6 +137,8 @@ using Attn4 = AttnOf<Cache4>;
 // csrc/paged4_attn_tc.cu: sequences of more than `few` rows (of any number where few is 0, and then rows past the last
 // sequence are cleared too)
 void chunk_attention(const Attn4& p, int hd, bool bf16);
+// and the weights that their slots receive, of sequences of more than `kept` rows, from the rows' sums in p.lse
+void chunk_weights(const Attn4& p, int kept, int hd, bool bf16);
 int64_t chunk_error(bool clear);
 
 }  // namespace paged4

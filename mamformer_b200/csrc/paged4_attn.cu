@@ -20,12 +20,16 @@
 //
 // Received weights: the scores of up to 16 rows are left in a workspace (4 bytes a row and slot, a small part of which the
 // L2 does not keep), and a last kernel turns them into weights with each row's joined sum; longer runs of tokens have
-// them computed from the keys once more (weights_kernel).
+// them computed from the keys once more (paged4_attn_tc.cu).
 #include "paged4.cuh"
 #include "paged_split.cuh"
 
+#include <cooperative_groups.h>
+
 namespace mamf {
 namespace pa4 {
+
+namespace cg = cooperative_groups;
 
 using namespace split;
 using namespace paged4;
@@ -35,6 +39,12 @@ constexpr int FEW = 64;
 constexpr int NB = 2, STEP = 16 * NB;          // blocks and tokens of a warp per tile
 constexpr int TILE = STEP * NW;                // tokens per tile
 constexpr float LIFT = 7.f, LAZY = 8.f;        // a row's largest weight is 2^LIFT when its reference is set, and may outgrow it
+constexpr int MOST = 8;                        // CTAs of a cluster
+// Each item gets a cluster of its own where all of these fit on the GPU at once and a CTA has at most SHORT tiles, of the
+// longest sequence that the table has room for: no list to be shared, no second kernel.  Clusters and list, one map of 16 / 4
+// heads, us: 1 sequence of 700 slots 8.0 and 10.8, of 4000 12.4 and 12.4, of 8000 18.2 and 13.9; 16 of 700 10.9 and 13.4, of
+// 4000 19.3 and 23.0, of 8000 30.3 and 31.8; 64 of 700, with clusters of 8 in four waves, 38.2 and 20.2.
+constexpr int SHORT = 4;
 constexpr int KEEP = 16;                       // rows whose scores are left for the received weights, at most
 
 struct Params : Attn4 {
@@ -64,11 +74,13 @@ constexpr int ST = 2;                          // tiles of a warp's ring
 // warps, so there are as many as the registers of a row tile allow without spills (128, 168 or 255)
 template <int HD, int NR> constexpr int residents() { return NR == 1 ? 4 : HD == 64 ? 3 : 2; }
 template <int HD, int NR> constexpr int merge_words() { return NR * (HD / 4 + 4); }      // of a lane
-template <int HD, int NR> constexpr int smem_bytes() {
-  return 1024 + NW * ST * NB * BLOCK<HD> + 32 * 4 * merge_words<HD, NR>();
+template <int HD, int NR, bool ALONE> constexpr int smem_bytes() {
+  return 1024 + NW * ST * NB * BLOCK<HD> + 32 * 4 * merge_words<HD, NR>() + (ALONE ? 8 * NR * (HD + 2) * 4 : 0);
 }
 
-template <typename T, int HD, int NR>
+// ALONE: a cluster of CTAs for each item shares its tiles and joins its parts through distributed shared memory.  Else
+// contiguous shares of all items' tiles, and the join kernel.
+template <typename T, int HD, int NR, bool ALONE>
 __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __grid_constant__ Params p) {
   constexpr int ROWS = 8 * NR;
   constexpr int KW = HD / 32;                    // words of a K row per lane, and of the parameters of a row's two halves
@@ -89,6 +101,42 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
   const Cache4& c = p.c;
   asm volatile("griddepcontrol.launch_dependents;");      // the join kernel waits for this grid's end by itself
 
+  const int rank = ALONE ? (int)cg::this_cluster().block_rank() : 0;
+  int64_t first, last, share = 1;                   // this CTA's tiles, of the item or of the list
+  bool nothing;
+  if constexpr (ALONE) {
+    const int b = blockIdx.z, g = blockIdx.y % c.G;
+    bool broken = false;
+    for (int i = tid; i < c.B; i += NT) broken = broken || !in_order(c, i);
+    if (tid == 0) s_cut = 0;
+    broken = __syncthreads_or(broken);
+    Item x;
+    const bool mine = !broken && set_sequence<ROWS, TILE>(p, x, b);
+    first = last = 0;
+    nothing = !mine;
+    if (mine) {
+      x.g = g;
+      x.rt = blockIdx.y / c.G;
+      nothing = x.rt * ROWS >= x.rows;
+      if (!nothing) {
+        set_range<ROWS, TILE>(p, x);
+        const int C = gridDim.x, per = (x.nt + C - 1) / C;
+        first = min(x.nt, rank * per);
+        last = min(x.nt, rank * per + per);
+        s_item[w][0] = x;
+      }
+      if (tid == 0 && rank == 0 && cached_length(c, c.lens[b]) != c.lens[b]) record(ERR_LENGTH);
+    } else if (broken || c.cu[b + 1] > c.cu[b]) {   // offsets out of order anywhere: zeros everywhere; more rows than were said: its rows
+      const int64_t row = (int64_t)p.H * HD, C = gridDim.x;
+      const int64_t from = broken ? 0 : c.cu[b], to = broken ? c.T : c.cu[b + 1];
+      const int64_t step = C * NT * gridDim.y * (broken ? c.B : 1);
+      for (int64_t i = from * row + ((int64_t)((broken ? b : 0) * gridDim.y + blockIdx.y) * C + rank) * NT + tid; i < to * row; i += step) ((T*)p.out)[i] = from_f<T>(0.f);
+      if (p.lse)
+        for (int64_t i = from * p.H * p.maps + tid; i < to * p.H * p.maps; i += NT) p.lse[i] = INFINITY;
+      if (tid == 0) record(ERR_LENGTH);
+    }
+    if (broken) return;
+  } else {
   // ---- this CTA's share [first, last) of the list of tiles ----
   const int chunk = (c.B + NT - 1) / NT;
   int64_t mine = 0;
@@ -117,8 +165,9 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
     total += s_pre[i];
   }
   incl += before;
-  const int64_t share = (total + p.ctas - 1) / p.ctas;
-  const int64_t first = blockIdx.x * share, last = min(total, first + share);
+  share = (total + p.ctas - 1) / p.ctas;
+  first = blockIdx.x * share;
+  last = min(total, first + share);
   if (incl - mine <= first && first < incl) {      // one thread at most
     int64_t at = incl - mine;
     int b = tid * chunk;
@@ -132,22 +181,30 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
   }
   __syncthreads();
   if (tid == 0) p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  nothing = first >= last || total >> 60;
+  }
   // rows before the first and past the last sequence
   {
     const int64_t row = (int64_t)p.H * HD;
     const int64_t front = c.B > 0 ? min(max(0, c.cu[0]), c.T) * row : 0, end = c.B > 0 ? max(0, c.cu[c.B]) * row : 0;
-    for (int64_t i = (int64_t)blockIdx.x * NT + tid; i < front; i += (int64_t)gridDim.x * NT) ((T*)p.out)[i] = from_f<T>(0.f);
-    for (int64_t i = end + (int64_t)blockIdx.x * NT + tid; i < c.T * row; i += (int64_t)gridDim.x * NT)
-      ((T*)p.out)[i] = from_f<T>(0.f);
+    const int64_t at = (((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * NT + tid, step = (int64_t)gridDim.x * gridDim.y * gridDim.z * NT;
+    for (int64_t i = at; i < front; i += step) ((T*)p.out)[i] = from_f<T>(0.f);
+    for (int64_t i = end + at; i < c.T * row; i += step) ((T*)p.out)[i] = from_f<T>(0.f);
   }
-  if (first >= last || total >> 60) return;
+
+  if (nothing) return;                              // the CTAs of a cluster agree on this
 
   Item& it = s_item[w][0];                          // of the tile being computed
   Item& is = s_item[w][1];                          // of the next tile to be fetched
   int done = 0;                                     // tiles of the first item that are other CTAs'
-  int64_t start = s_begin;                          // list position of the item's first tile
-  {
+  int64_t start = 0;                                // list position of the item's first tile
+  if constexpr (ALONE) {
+    __syncwarp();
+    is = it;
+    done = (int)first;
+  } else {
     Item x;
+    start = s_begin;
     set_sequence<ROWS, TILE>(p, x, s_b);
     while (first >= start + x.nt) { start += x.nt; next_item<ROWS, TILE>(p, x); }
     it = is = x;                                    // every lane writes the same
@@ -467,6 +524,7 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
 
   // Warps 3, 2, 1 pass their joined state on through shared memory, lane by lane; warp 0 writes the result.
   float* merge = reinterpret_cast<float*>(smem + NW * ST * SB) + lane;
+  float* const s_part = reinterpret_cast<float*>(smem + NW * ST * SB + 32 * 4 * merge_words<HD, NR>());
   auto finish = [&](int64_t item_start, bool ends) {
 #pragma unroll 1
     for (int turn = NW - 1; turn >= 0; --turn) {
@@ -499,8 +557,8 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
       if (turn > 0) __syncthreads();
     }
     if (w == 0) {
-      const bool whole = ends && item_start >= first, cut = *(volatile int*)&s_cut != 0;
-      float* part = p.part + ((int64_t)blockIdx.x * 2 + (item_start > first ? 1 : 0)) * ROWS * (HD + 2);
+      const bool whole = (!ALONE || gridDim.x == 1) && ends && item_start >= first, cut = *(volatile int*)&s_cut != 0;
+      float* part = ALONE ? s_part : p.part + ((int64_t)blockIdx.x * 2 + (item_start > first ? 1 : 0)) * ROWS * (HD + 2);
       const int per = p.rep * p.maps;
 #pragma unroll
       for (int nr = 0; nr < NR; ++nr) {
@@ -555,7 +613,7 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
           }
         }
       }
-      if (ends && !whole && lane == 0) {
+      if (!ALONE && ends && !whole && lane == 0) {
         const int64_t c0 = item_start / share;       // CTA and place of the item's first part
         p.joins[blockIdx.x] = make_int4(it.t0, it.rows, it.g | it.rt << 16, (int)(2 * c0 + (item_start > c0 * share ? 1 : 0)));
       }
@@ -567,6 +625,7 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
   int tiles = it.nt - done;                                            // of the item, still to be done
   int slot0 = (it.k0 + done) * TILE + w * STEP;
   uint32_t here = ring, bar_here = bar, phase = 0, there = ring + (ST - 1) * SB, bar_there = bar + (ST - 1) * 8;
+  if (ALONE && first == last) finish(start, true);   // no tile is left for this CTA: a part of nothing
   for (int left = (int)(last - first); left > 0; --left) {
     if (ok) {
       issue(there, bar_there);
@@ -603,6 +662,51 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
       }
     }
   }
+  if (ALONE && gridDim.x > 1) {
+    // the cluster's parts, a row (or a head's pair of rows) per CTA and turn, 32 dims a warp
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const int C = gridDim.x, per = p.rep * p.maps, n_rows = min(ROWS, it.rows - it.rt * ROWS);
+    for (int rr = rank * p.maps; rr < n_rows; rr += C * p.maps) {
+      const int row = it.rt * ROWS + rr, tok = it.t0 + row / per, h = it.g * p.rep + row % per / p.maps;
+      for (int d = tid; d < HD; d += NT) {
+        float x[2] = {0.f, 0.f};
+        bool cut = false;
+        for (int map = 0; map < p.maps; ++map) {
+          const float* src = s_part + (rr + map) * (HD + 2);
+          float2 ml[MOST];
+          float v[MOST];
+#pragma unroll
+          for (int i = 0; i < MOST; ++i) {
+            ml[i] = make_float2(NONE, 0.f);
+            v[i] = 0.f;
+            if (i < C) {
+              const float* remote = cluster.map_shared_rank(src, i);
+              ml[i] = *reinterpret_cast<const float2*>(remote + HD);
+              v[i] = remote[d];
+            }
+          }
+          float M = NONE, L = 0.f, a = 0.f;
+#pragma unroll
+          for (int i = 0; i < MOST; ++i) M = fmaxf(M, ml[i].x);
+#pragma unroll
+          for (int i = 0; i < MOST; ++i) {
+            const float e = ex2(ml[i].x - M);
+            cut = cut || ml[i].y < 0.f;
+            L = fmaf(ml[i].y, e, L);
+            a = fmaf(v[i], e, a);
+          }
+          x[map] = L == 0.f ? 0.f : a / L;
+          if (p.lse && d == 0) p.lse[(int64_t)tok * p.H * p.maps + it.g * per + row % per + map] = L == 0.f ? INFINITY : M + log2f(L);
+        }
+        if (p.maps == 2) x[0] = (x[0] - p.lam[h] * x[1]) / (1.f - p.lam[h] + 1e-8f);
+        if (cut && p.lse && d == 0)
+          for (int map = 0; map < p.maps; ++map) p.lse[(int64_t)tok * p.H * p.maps + it.g * per + row % per + map] = INFINITY;
+        ((T*)p.out)[((int64_t)tok * p.H + h) * HD + d] = from_f<T>(cut ? 0.f : x[0]);
+      }
+    }
+    cluster.sync();                                 // nobody leaves while its part is read
+  }
   // after a wait that ran out: the copies that are still under way into this CTA's memory
   for (; waited < issued; ++waited) drain_tile(bar + waited % ST * 8, (uint32_t)(waited / ST & 1));
 }
@@ -616,169 +720,40 @@ __global__ void __launch_bounds__(NK) kept_weights_kernel(const __grid_constant_
   Item it;
   if (!in_order(c, b) || !set_sequence<2 * 8, TILE>(p, it, b) || it.rows > p.stride) return;
   const int per = p.rep * p.maps;
-  const float* lse = p.lse + (int64_t)it.t0 * p.H * p.maps + g * per;
+  __shared__ float lse[KEEP];
+  if (threadIdx.x < KEEP) {
+    const int row = threadIdx.x;
+    lse[row] = row < it.rows ? p.lse[(int64_t)(it.t0 + row / per) * p.H * p.maps + g * per + row % per] : INFINITY;
+  }
+  __syncthreads();
+  // rows cut short (+inf) have not left all of their scores
+  auto weight = [](float score, float of) { return of == INFINITY ? 0.f : ex2(score - of); };
   for (int slot = it.lo / 16 * 16 + blockIdx.x * NK + threadIdx.x; slot < it.hi; slot += gridDim.x * NK) {
     const int pg = c.table[(int64_t)b * c.W + (slot >> c.shift)];
     if (pg < 0 || pg >= c.P) continue;                  // recorded where its keys were looked for
+    float* to = c.mass + (((int64_t)pg * c.G + g) << c.shift) + (slot & (c.page - 1));
+    const float had = *to;
     const float* s = p.scores + (((int64_t)b * c.G + g) * p.cap + slot) * p.stride;
     float sum = 0.f;
-    for (int row = 0; row < it.rows; ++row) {
-      const float of = lse[(int64_t)(row / per) * p.H * p.maps + row % per];
-      if (of != INFINITY) sum += ex2(s[row] - of);      // rows cut short have not left all of their scores
+    if (p.stride % 4 == 0) {
+      for (int row = 0; row < it.rows; row += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(s + row);
+        sum += (weight(v.x, lse[row]) + weight(v.y, lse[row + 1])) + (weight(v.z, lse[row + 2]) + weight(v.w, lse[row + 3]));
+      }
+    } else {
+      for (int row = 0; row < it.rows; row += 2) {
+        const float2 v = *reinterpret_cast<const float2*>(s + row);
+        sum += weight(v.x, lse[row]) + weight(v.y, lse[row + 1]);
+      }
     }
-    c.mass[(((int64_t)pg * c.G + g) << c.shift) + (slot & (c.page - 1))] += sum;
+    *to = had + sum;
   }
 }
 
-// From the keys, for sequences of more rows: a CTA takes 256 slots of a KV head, 32 per warp, whose keys stay in registers
-// as the M rows of the products while all rows of the sequence that see some of them pass by in tiles of 64 as N.
-constexpr int WW = 8, WK = 32, WR = 64;          // warps, slots of a warp, rows of a tile
-template <typename T, int HD>
-__global__ void __launch_bounds__(WW * 32) weights_kernel(const __grid_constant__ Params p) {
-  constexpr int KW = HD / 32, MT = HD / 16, QS = HD / 2 + 4;       // QS: words of a row, with a shift of banks
-  const Cache4& c = p.c;
-  const int g = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g8 = lane >> 2, t4 = lane & 3;
-  if (!in_order(c, b)) return;
-  const int t0 = c.cu[b], n = c.cu[b + 1] - t0, per = p.rep * p.maps, len = cached_length(c, c.lens[b]);
-  const int64_t rows = (int64_t)n * per;
-  if (rows == 0 || rows <= p.stride || (rows > p.few && !p.chunked)) return;      // the other kernel's, or left out altogether
-  const int at0 = len - n, base = blockIdx.x * (WW * WK);
-  if (base >= len) return;
-  // tokens [i0, i1) see some slot of the CTA's
-  const int i0 = max(0, base - at0);
-  const int last = min(base + WW * WK, len) - 1;
-  const int i1 = p.window > 0 ? (int)min((int64_t)n, (int64_t)last + p.window - at0) : n;
-  if (i0 >= i1) return;
-  __shared__ __align__(16) uint32_t q[WR * QS];
-  __shared__ float factor[WR], sum_of[WR];
-  __shared__ int sees[WR];                          // the row's slot
-
-  // keys: word i of tokens g8, g8 + 8 of each block
-  const int slot0 = base + w * WK;
-  uint32_t a[WK / 16][MT][4];
-  int pages[WK / 16];
-#pragma unroll
-  for (int m = 0; m < WK / 16; ++m) {
-    const int slot = slot0 + 16 * m;
-    int pg = -1;
-    if (slot < len) {
-      pg = c.table[(int64_t)b * c.W + (slot >> c.shift)];
-      if (pg < 0 || pg >= c.P) pg = -1;
-    }
-    pages[m] = pg;
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int row = g8 + 8 * x;
-      const bool there = pg >= 0 && slot + row < len;
-#pragma unroll
-      for (int i = 0; i < KW; ++i) {
-        uint32_t word = 0, params = 0;
-        if (there) {
-          const uint8_t* blk = block_of<HD>(c, pg, g, slot);
-          word = *reinterpret_cast<const uint32_t*>(blk + row * (HD / 2) + t4 * (HD / 8) + 4 * i);
-          params = *reinterpret_cast<const uint32_t*>(blk + PARAMS<HD> + row * (HD / 16) + 4 * (i % (KW / 2)));
-        }
-        uint32_t h[4];
-        decode(word, levels_of(params, c.base), c.base, h);
-        a[m][2 * i][x] = h[0];
-        a[m][2 * i][x + 2] = h[1];
-        a[m][2 * i + 1][x] = h[2];
-        a[m][2 * i + 1][x + 2] = h[3];
-      }
-    }
-  }
-  float sum[WK / 16][2] = {};
-  const int64_t end = (int64_t)i1 * per;
-  for (int64_t first = (int64_t)i0 * per; first < end; first += WR) {
-    __syncthreads();
-    // four threads a row: dims HD / 4 (tid & 3) .., in the order of the keys' fragments
-    {
-      const int64_t row = first + (tid >> 2);
-      const int i = (int)(row / per), j = (int)(row % per), h = g * p.rep + j / p.maps, map = j % p.maps;
-      float f[KW][8], mx = 0.f;
-      const bool there = row < end;
-      if (there) {
-        const T* src = map ? (const T*)p.q2 + (int64_t)(t0 + i) * p.st2 + (int64_t)h * p.sh2
-                           : (const T*)p.q1 + (int64_t)(t0 + i) * p.st1 + (int64_t)h * p.sh1;
-#pragma unroll
-        for (int x = 0; x < KW / 2; ++x) q_row16(src + (tid & 3) * (HD / 4) + 16 * x, &f[2 * x][0]);
-      } else {
-#pragma unroll
-        for (int x = 0; x < KW; ++x)
-#pragma unroll
-          for (int y = 0; y < 8; ++y) f[x][y] = 0.f;
-      }
-#pragma unroll
-      for (int x = 0; x < KW; ++x)
-#pragma unroll
-        for (int y = 0; y < 8; ++y) mx = fmaxf(mx, fabsf(f[x][y]));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      int e = (int)(__float_as_uint(mx) >> 23) - 127;
-      if (e == -127 || e == 128) e = 0;
-      e = max(-126, min(126, e));
-      const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
-      uint32_t* to = q + (tid >> 2) * QS + (tid & 3) * (HD / 8);
-#pragma unroll
-      for (int x = 0; x < KW; ++x)
-        *reinterpret_cast<uint4*>(to + 4 * x) = make_uint4(pack_h2(f[x][0] * down, f[x][4] * down), pack_h2(f[x][1] * down, f[x][5] * down),
-                                                           pack_h2(f[x][2] * down, f[x][6] * down), pack_h2(f[x][3] * down, f[x][7] * down));
-      if ((tid & 3) == 0) {
-        factor[tid >> 2] = p.scale_log2 * up;
-        sum_of[tid >> 2] = there ? p.lse[(int64_t)(t0 + i) * p.H * p.maps + g * per + j] : INFINITY;
-        sees[tid >> 2] = at0 + i;
-      }
-    }
-    __syncthreads();
-    const int low_row = sees[0], high_row = (int)(at0 + (min(first + WR, end) - 1) / per);
-    const bool all = slot0 + WK - 1 <= low_row && (p.window == 0 || slot0 > high_row - p.window);
-    if (slot0 > high_row) continue;
-#pragma unroll 1
-    for (int col = 0; col < WR; col += 8) {
-      float s[WK / 16][4] = {};
-      const uint32_t* src = q + (col + g8) * QS + t4 * (HD / 8);
-#pragma unroll
-      for (int i = 0; i < KW; ++i) {
-        const uint4 v = *reinterpret_cast<const uint4*>(src + 4 * i);
-#pragma unroll
-        for (int m = 0; m < WK / 16; ++m) {
-          mma(s[m], a[m][2 * i][0], a[m][2 * i][1], a[m][2 * i][2], a[m][2 * i][3], v.x, v.y);
-          mma(s[m], a[m][2 * i + 1][0], a[m][2 * i + 1][1], a[m][2 * i + 1][2], a[m][2 * i + 1][3], v.z, v.w);
-        }
-      }
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {                    // rows col + 2 t4, + 1
-        const int rr = col + 2 * t4 + y;
-        const float f = factor[rr], ls = sum_of[rr];
-        const int at = sees[rr];
-#pragma unroll
-        for (int m = 0; m < WK / 16; ++m)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const int slot = slot0 + 16 * m + g8 + 8 * x;
-            const float e = ex2(fmaf(s[m][y + 2 * x], f, -ls));
-            if (all || (slot <= at && (p.window == 0 || slot > at - p.window))) sum[m][x] += e;
-          }
-      }
-    }
-  }
-#pragma unroll
-  for (int m = 0; m < WK / 16; ++m)
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      float v = sum[m][x];
-      v += __shfl_xor_sync(0xffffffffu, v, 1);
-      v += __shfl_xor_sync(0xffffffffu, v, 2);
-      const int slot = slot0 + 16 * m + g8 + 8 * x;
-      if (t4 == 0 && pages[m] >= 0 && slot < len)
-        c.mass[(((int64_t)pages[m] * c.G + g) << c.shift) + (slot & (c.page - 1))] += v;
-    }
-}
-
-template <typename T, int HD, int NR>
-void launch_split(const Params& p) {
-  auto fn = split_kernel<T, HD, NR>;
-  constexpr int SMEM = smem_bytes<HD, NR>();
+template <typename T, int HD, int NR, bool ALONE>
+void launch_split(const Params& p, int row_tiles, int cluster) {
+  auto fn = split_kernel<T, HD, NR, ALONE>;
+  constexpr int SMEM = smem_bytes<HD, NR, ALONE>();
   static bool set[64] = {};                              // by device; the attribute stays
   int dev = 0;
   MAMF_CUDA_CHECK(cudaGetDevice(&dev));
@@ -786,9 +761,28 @@ void launch_split(const Params& p) {
     MAMF_CUDA_CHECK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
     if (dev < 64) set[dev] = true;
   }
-  fn<<<p.ctas, NT, SMEM, stream()>>>(p);
-  MAMF_LAUNCH_CHECK();
-  launch_join<T, HD, NR>(p);
+  if (!ALONE) {
+    fn<<<p.ctas, NT, SMEM, stream()>>>(p);
+    MAMF_LAUNCH_CHECK();
+    launch_join<T, HD, NR>(p);
+    return;
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)cluster, (unsigned)(p.c.G * row_tiles), (unsigned)p.c.B);
+  cfg.blockDim = dim3(NT);
+  cfg.dynamicSmemBytes = SMEM;
+  cfg.stream = stream();
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  MAMF_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fn, p));
+}
+template <typename T, int HD, int NR>
+void launch_split(const Params& p, int row_tiles, int cluster) {
+  if (cluster) launch_split<T, HD, NR, true>(p, row_tiles, cluster); else launch_split<T, HD, NR, false>(p, 0, 0);
 }
 
 }  // namespace pa4
@@ -855,16 +849,28 @@ at::Tensor paged4_attention(at::Tensor q1, c10::optional<at::Tensor> q2, c10::op
     // one query row tile holds 8 rows, or 16 where a sequence can have more than 8
     const int nr = p.few > 8 ? 2 : 1, rows = 8 * nr;
     const int64_t row_tiles = (p.few + rows - 1) / rows;
-    const int64_t most = std::max<int64_t>(1, (int64_t)p.c.B * p.c.G * row_tiles * std::max<int64_t>(1, (p.cap + TILE - 1) / TILE));
-    p.ctas = (int)std::min<int64_t>(most, (nr == 1 ? residents<128, 1>() : hd == 64 ? residents<64, 2>() : residents<128, 2>()) * num_sms());
-    const int64_t part = (int64_t)p.ctas * 2 * rows * (hd + 2);
-    at::Tensor ws = at::empty({part + 4 * p.ctas}, q1.options().dtype(at::kFloat));
-    p.joins = reinterpret_cast<int4*>(ws.data_ptr<float>());
-    p.part = ws.data_ptr<float>() + 4 * p.ctas;
+    const int64_t tiles = std::max<int64_t>(1, (p.cap + TILE - 1) / TILE);
+    int cluster = 0;
+    at::Tensor ws;
+    const int64_t slots = (nr == 1 ? residents<128, 1>() : hd == 64 ? residents<64, 2>() : residents<128, 2>()) * num_sms();
+    const int64_t items = (int64_t)p.c.B * p.c.G * row_tiles;
+    if (items > 0 && !p.chunked) {
+      cluster = MOST;
+      while (cluster > 1 && (items * cluster > slots || cluster >= 2 * tiles)) cluster /= 2;
+      if (items * cluster > slots || tiles > SHORT * cluster) cluster = 0;
+    }
+    if (!cluster) {
+      const int64_t most = std::max<int64_t>(1, items * tiles);
+      p.ctas = (int)std::min<int64_t>(most, slots);
+      const int64_t part = (int64_t)p.ctas * 2 * rows * (hd + 2);
+      ws = at::empty({part + 4 * p.ctas}, q1.options().dtype(at::kFloat));
+      p.joins = reinterpret_cast<int4*>(ws.data_ptr<float>());
+      p.part = ws.data_ptr<float>() + 4 * p.ctas;
+    }
     auto go = [&](auto t) {
       using E = decltype(t);
-      if (hd == 128) { if (nr == 1) launch_split<E, 128, 1>(p); else launch_split<E, 128, 2>(p); }
-      else { if (nr == 1) launch_split<E, 64, 1>(p); else launch_split<E, 64, 2>(p); }
+      if (hd == 128) { if (nr == 1) launch_split<E, 128, 1>(p, (int)row_tiles, cluster); else launch_split<E, 128, 2>(p, (int)row_tiles, cluster); }
+      else { if (nr == 1) launch_split<E, 64, 1>(p, (int)row_tiles, cluster); else launch_split<E, 64, 2>(p, (int)row_tiles, cluster); }
     };
     if (bf16) go(__nv_bfloat16()); else go(__half());
   }
@@ -873,12 +879,7 @@ at::Tensor paged4_attention(at::Tensor q1, c10::optional<at::Tensor> q2, c10::op
       kept_weights_kernel<<<dim3((unsigned)((p.cap + 4 * NK - 1) / (4 * NK)), (unsigned)p.c.G, (unsigned)p.c.B), NK, 0, stream()>>>(p);
       MAMF_LAUNCH_CHECK();
     }
-    if (most_rows > p.stride) {
-      const dim3 grid((unsigned)((p.cap + WW * WK - 1) / (WW * WK)), (unsigned)p.c.G, (unsigned)p.c.B);
-      if (hd == 128) { if (bf16) weights_kernel<__nv_bfloat16, 128><<<grid, WW * 32, 0, stream()>>>(p); else weights_kernel<__half, 128><<<grid, WW * 32, 0, stream()>>>(p); }
-      else { if (bf16) weights_kernel<__nv_bfloat16, 64><<<grid, WW * 32, 0, stream()>>>(p); else weights_kernel<__half, 64><<<grid, WW * 32, 0, stream()>>>(p); }
-      MAMF_LAUNCH_CHECK();
-    }
+    if (most_rows > p.stride) chunk_weights(p, p.stride, (int)hd, bf16);
   }
   return out;
 }

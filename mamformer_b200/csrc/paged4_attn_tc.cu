@@ -542,9 +542,282 @@ void launch(const Attn4& attn) {
   }
 }
 
+// ---- received weights ------------------------------------------------------------------------------
+// mass[slot] += sum over rows of 2^(score - log2 of the row's sum): the scores once more, transposed, so that a thread sums
+// one slot's weights in a register and nothing is added up across threads or CTAs.
+//
+// rows_kernel lays the rows of q out once: tiles of 128 rows of a sequence and KV head as f16 in the order of the products'
+// operand, and behind each tile what a weight needs of its row, {factor, factor, -log2 sum, -log2 sum} of two rows.
+// weights_kernel: a CTA holds 256 slots of a KV head as two M = 128 operands, S^T = K Q^T, decoded once into shared memory;
+// the tiles with rows that see some of them pass by as N = 128.  10 warps:
+//   warps 0-3, 4-7  128 slots each (thread = slot = TMEM lane): S^T from TMEM, a fused multiply-add and an exponential a
+//                   weight, two at a time
+//   warp 8          one lane copies tiles into a ring of three
+//   warp 9          TMEM allocation, MMA issue; two accumulators for each half, so that the sums do not wait for a product
+// Bound by the exponentials: 16 a cycle and SM, 2,048 cycles for 256 slots and 128 rows.  256 slots rather than 128: each
+// tile of rows is read from the L2 half as often.
+constexpr int WR = 128, WK = 256, WQ = 3, NTW = 320;       // rows of a tile, slots of a CTA, ring
+template <int HD> constexpr int TILE_BYTES = WR * HD * 2 + WR * 8;
+template <int HD> constexpr int weights_smem() { return 1024 + WK * HD * 2 + WQ * ((TILE_BYTES<HD> + 1023) / 1024 * 1024); }
+
+struct Weights : Attn4 {
+  uint8_t* tiles;            // [unit * G + head][TILE_BYTES]
+  int kept;                  // sequences of up to this many rows are not taken
+};
+// Tiles of sequence b begin at unit cu[b] per / WR + b: it has ceil(n per / WR) or less.
+__device__ __forceinline__ int64_t first_unit(const Table& c, int b, int per) { return (int64_t)c.cu[b] * per / WR + b; }
+__device__ __forceinline__ bool takes(const Weights& p, int b) {
+  if (!in_order(p.c, b)) return false;
+  const int64_t rows = (int64_t)(p.c.cu[b + 1] - p.c.cu[b]) * p.rep * p.maps;
+  return rows > p.kept && (rows <= p.few || p.chunked);
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ Weights p) {
+  constexpr int LANES = HD / 8;                            // of a row, 8 dims each
+  const Cache4& c = p.c;
+  const int per = p.rep * p.maps, g = blockIdx.y;
+  int b = 0;
+  for (int hi = c.B - 1; b < hi;) {
+    const int mid = (b + hi + 1) >> 1;
+    if (first_unit(c, mid, per) <= (int64_t)blockIdx.x) b = mid; else hi = mid - 1;
+  }
+  if (!takes(p, b)) return;
+  const int t0 = c.cu[b];
+  const int64_t rows = (int64_t)(c.cu[b + 1] - t0) * per, row0 = ((int64_t)blockIdx.x - first_unit(c, b, per)) * WR;
+  if (row0 < 0 || row0 >= rows) return;
+  uint8_t* tile = p.tiles + ((int64_t)blockIdx.x * c.G + g) * TILE_BYTES<HD>;
+  float* facts = reinterpret_cast<float*>(tile + WR * HD * 2);
+  const int k = threadIdx.x % LANES;
+  constexpr int STEPS = WR * LANES / 256;
+  Vec16<T> x[STEPS];
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    const int64_t row = row0 + (s * 256 + threadIdx.x) / LANES;
+    const int i = (int)(row / per), j = (int)(row % per), h = g * p.rep + j / p.maps;
+    x[s].raw = make_uint4(0, 0, 0, 0);
+    if (row < rows)
+      x[s] = ld16(j % p.maps ? (const T*)p.q2 + (int64_t)(t0 + i) * p.st2 + (int64_t)h * p.sh2 + 8 * k
+                             : (const T*)p.q1 + (int64_t)(t0 + i) * p.st1 + (int64_t)h * p.sh1 + 8 * k);
+  }
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    const int r = (s * 256 + threadIdx.x) / LANES;
+    float mx = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(to_f(x[s].v[e])));
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    int e = (int)(__float_as_uint(mx) >> 23) - 127;        // as in the attention
+    if (e == -127 || e == 128) e = 0;
+    e = max(-126, min(126, e));
+    const float down = pow2(-e);
+    uint4 v;
+    v.x = h2(to_f(x[s].v[0]) * down, to_f(x[s].v[4]) * down);
+    v.y = h2(to_f(x[s].v[1]) * down, to_f(x[s].v[5]) * down);
+    v.z = h2(to_f(x[s].v[2]) * down, to_f(x[s].v[6]) * down);
+    v.w = h2(to_f(x[s].v[3]) * down, to_f(x[s].v[7]) * down);
+    *reinterpret_cast<uint4*>(tile + (k >> 3) * (WR * 128) + r * 128 + (((k & 7) ^ (r & 7)) << 4)) = v;
+    if (k == 0) {
+      const int64_t row = row0 + r;
+      facts[(r >> 1) * 4 + (r & 1)] = p.scale_log2 * pow2(e);
+      facts[(r >> 1) * 4 + (r & 1) + 2] = row < rows ? -p.lse[(t0 + row / per) * p.H * p.maps + g * per + row % per] : -INFINITY;
+    }
+  }
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(NTW, 1) weights_kernel(const __grid_constant__ Weights p) {
+  constexpr int KB2 = WR * HD * 2, STAGE = (TILE_BYTES<HD> + 1023) / 1024 * 1024;       // bytes of 128 slots, of a ring's place
+  const Cache4& c = p.c;
+  const int g = blockIdx.y, b = blockIdx.z, base = blockIdx.x * WK, per = p.rep * p.maps;
+  const int len = cached_length(c, c.lens[b]);
+  if (base >= len || !takes(p, b)) return;
+  bool odd = false;                                        // offsets out of order anywhere: not all tiles are there
+  for (int i = threadIdx.x; i < c.B; i += NTW) odd = odd || !in_order(c, i);
+  if (__syncthreads_or(odd)) return;
+  const int n = c.cu[b + 1] - c.cu[b], at0 = len - n;
+  const int64_t rows = (int64_t)n * per;
+  // tokens [i0, i1) see some slot of the CTA's
+  const int i0 = max(0, base - at0), last = min(base + WK, len) - 1;
+  const int i1 = p.window > 0 ? (int)min((int64_t)n, (int64_t)last + p.window - at0) : n;
+  if (i0 >= i1) return;
+  const int64_t j0 = (int64_t)i0 * per / WR;
+  const int ntile = (int)(((int64_t)i1 * per + WR - 1) / WR - j0);
+  const uint8_t* tiles = p.tiles + ((first_unit(c, b, per) + j0) * c.G + g) * TILE_BYTES<HD>;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = sm + 2 * KB2;
+  __shared__ uint64_t q_full[WQ], q_empty[WQ], s_full[4], s_empty[4], idle;
+  __shared__ uint32_t tmem_slot;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < WQ; ++i) { bar_init(&q_full[i], 1); bar_init(&q_empty[i], 9); }
+    for (int i = 0; i < 4; ++i) { bar_init(&s_full[i], 1); bar_init(&s_empty[i], 128); }
+    bar_init(&idle, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&tmem_slot)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  // keys: a 16-byte chunk of codes (32 dims) per thread and turn; slots past the end, or of no page, become zeros
+  for (int i = threadIdx.x; i < WK * (HD / 32); i += NTW) {
+    const int tok = i / (HD / 32), cc = i % (HD / 32), slot = base + tok;
+    uint4 x = make_uint4(0, 0, 0, 0);
+    uint32_t params[HD / 64] = {};
+    if (slot < len) {
+      const int pg = c.table[(int64_t)b * c.W + (slot >> c.shift)];
+      if (pg >= 0 && pg < c.P) {
+        const uint8_t* blk = block_of<HD>(c, pg, g, slot);
+        x = *reinterpret_cast<const uint4*>(blk + (tok & 15) * (HD / 2) + cc * 16);
+#pragma unroll
+        for (int k = 0; k < HD / 64; ++k) params[k] = reinterpret_cast<const uint32_t*>(blk + PARAMS<HD> + (tok & 15) * (HD / 16))[k];
+      }
+    }
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    uint8_t* row = sm + (tok >> 7) * KB2 + (cc >> 1) * (WR * 128) + (tok & 127) * 128;
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      uint32_t h[4];
+      decode(w[m], levels_of(params[HD == 128 ? m & 1 : 0], c.base), c.base, h);
+      *reinterpret_cast<uint4*>(row + ((((cc & 1) * 4 + m) ^ (tok & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+    }
+  }
+  fence_async_smem();
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == 8) {
+    // ------------------------------- rows -------------------------------
+    if (lane == 0) {
+      bool ok = true;
+      int j = 0;
+      for (; j < ntile; ++j) {
+        const int st = j % WQ;
+        if (j >= WQ) ok = wait(&q_empty[st], (uint32_t)((j / WQ - 1) & 1), p.wait);
+        if (!ok) break;
+        bar_expect_tx(&q_full[st], TILE_BYTES<HD>);
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                     ::"r"(su32(ring + st * STAGE)), "l"(tiles + (int64_t)j * c.G * TILE_BYTES<HD>), "r"(TILE_BYTES<HD>), "r"(su32(&q_full[st])) : "memory");
+      }
+      // after a wait that ran out: the copies that are still under way into this CTA's memory
+      if (!ok)
+        for (int k = max(0, j - WQ); k < j; ++k)
+          for (const long long t = clock64(); !try_once(&q_full[k % WQ], (uint32_t)((k / WQ) & 1)) && clock64() - t <= WAIT_CYCLES;) {}
+    }
+  } else if (warp == 9) {
+    // ------------------------------- MMA issue -------------------------------
+    if (lane == 0) {
+      constexpr uint32_t ID = idesc(WR, false);
+      bool ok = true;
+      for (int j = 0; j < ntile && ok; ++j) {
+        const int st = j % WQ;
+        ok = wait(&q_full[st], (uint32_t)((j / WQ) & 1), p.wait);
+        const uint32_t qb = su32(ring + st * STAGE);
+        for (int s = 0; s < 2 && ok; ++s) {
+          const int buf = 2 * s + (j & 1);
+          if (j >= 2) ok = wait(&s_empty[buf], (uint32_t)((j / 2 - 1) & 1), p.wait);
+          if (!ok) break;
+          fence_after();
+          const uint32_t ka = su32(sm + s * KB2);
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k)
+            mma_ss(tmem + (uint32_t)(buf * WR), sdesc(ka + (k >> 2) * (WR * 128) + (k & 3) * 32, 16, 1024),
+                   sdesc(qb + (k >> 2) * (WR * 128) + (k & 3) * 32, 16, 1024), ID, k > 0 ? 1u : 0u);
+          commit(&s_full[buf]);
+        }
+        if (ok) commit(&q_empty[st]);
+      }
+      // products under way read shared memory and write TMEM, both of which go when the CTA ends
+      commit(&idle);
+      for (const long long t = clock64(); !try_once(&idle, 0) && clock64() - t <= WAIT_CYCLES;) {}
+    }
+  } else {
+    // ------------------------------- sums -------------------------------
+    const int s = warp >> 2, r = (warp & 3) * 32 + lane, from = base + s * WR, slot = from + r;
+    const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
+    bool ok = true;
+    for (int j = 0; j < ntile && ok; ++j) {
+      const int st = j % WQ, buf = 2 * s + (j & 1);
+      // the tile's facts, too, are there
+      ok = __all_sync(0xffffffffu, wait(&q_full[st], (uint32_t)((j / WQ) & 1), p.wait) && wait(&s_full[buf], (uint32_t)((j >> 1) & 1), p.wait));
+      if (!ok) break;
+      fence_after();
+      const int64_t row0 = (j0 + j) * WR;
+      const int low = at0 + (int)(row0 / per), high = at0 + (int)((min(row0 + WR, rows) - 1) / per);
+      const bool all = from + WR - 1 <= low && (p.window == 0 || from > high - p.window);
+      const float* fact = reinterpret_cast<const float*>(ring + st * STAGE + KB2);
+#pragma unroll 1
+      for (int cc = 0; cc < WR; cc += 32) {
+        float v[32];
+        tld32(tl + (uint32_t)(buf * WR + cc), v);
+        if (cc == WR - 32) {                               // the accumulator is read
+          fence_before();
+          bar_arrive(&s_empty[buf]);
+        }
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) {
+          const float4 f = *reinterpret_cast<const float4*>(fact + 2 * (cc + k));
+          float e0, e1;
+          unpk(fma2(pk(v[k], v[k + 1]), pk(f.x, f.y), pk(f.z, f.w)), e0, e1);
+          e0 = ex2(e0);
+          e1 = ex2(e1);
+          if (!all) {
+            const int at = at0 + (int)((row0 + cc + k) / per), at1 = at0 + (int)((row0 + cc + k + 1) / per);
+            if (slot > at || (p.window > 0 && slot <= at - p.window)) e0 = 0.f;
+            if (slot > at1 || (p.window > 0 && slot <= at1 - p.window)) e1 = 0.f;
+          }
+          sum[k / 2 & 3] = add2(sum[k / 2 & 3], pk(e0, e1));
+        }
+      }
+      __syncwarp();
+      if (lane == 0) bar_arrive(&q_empty[st]);
+    }
+    float a, a2;
+    unpk(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), a, a2);
+    if (ok && slot < len) {
+      const int pg = c.table[(int64_t)b * c.W + (slot >> c.shift)];
+      if (pg >= 0 && pg < c.P) c.mass[(((int64_t)pg * c.G + g) << c.shift) + (slot & (c.page - 1))] += a + a2;
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+template <typename T, int HD>
+void launch_weights(const Attn4& attn, int kept) {
+  Weights p;
+  static_cast<Attn4&>(p) = attn;
+  p.kept = kept;
+  const int64_t units = (int64_t)p.c.T * p.rep * p.maps / WR + p.c.B;
+  TORCH_CHECK(units < (1LL << 31), "paged_attention: sizes");
+  const at::Tensor ws = at::empty({units * p.c.G * TILE_BYTES<HD>}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA));
+  p.tiles = ws.data_ptr<uint8_t>();
+  rows_kernel<T, HD><<<dim3((unsigned)units, (unsigned)p.c.G), 256, 0, stream()>>>(p);
+  MAMF_LAUNCH_CHECK();
+  auto fn = weights_kernel<T, HD>;
+  MAMF_CUDA_CHECK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, weights_smem<HD>()));
+  const int64_t tiles = ((int64_t)p.c.W * p.c.page + WK - 1) / WK;
+  fn<<<dim3((unsigned)tiles, (unsigned)p.c.G, (unsigned)p.c.B), NTW, weights_smem<HD>(), stream()>>>(p);
+  MAMF_LAUNCH_CHECK();
+}
+
 }  // namespace ptc4
 
 namespace paged4 {
+void chunk_weights(const Attn4& p, int kept, int hd, bool bf16) {
+  if (bf16) { if (hd == 128) ptc4::launch_weights<__nv_bfloat16, 128>(p, kept); else ptc4::launch_weights<__nv_bfloat16, 64>(p, kept); }
+  else { if (hd == 128) ptc4::launch_weights<__half, 128>(p, kept); else ptc4::launch_weights<__half, 64>(p, kept); }
+}
 void chunk_attention(const Attn4& p, int hd, bool bf16) {
   if (bf16) { if (hd == 128) ptc4::launch<__nv_bfloat16, 128>(p); else ptc4::launch<__nv_bfloat16, 64>(p); }
   else { if (hd == 128) ptc4::launch<__half, 128>(p); else ptc4::launch<__half, 64>(p); }
