@@ -760,19 +760,26 @@ __global__ void __launch_bounds__(NTW, 1) weights_kernel(const __grid_constant__
           fence_before();
           bar_arrive(&s_empty[buf]);
         }
+        // two loops: a question inside the one would put its pairs behind one another
+        if (all) {
 #pragma unroll
-        for (int k = 0; k < 32; k += 2) {
-          const float4 f = *reinterpret_cast<const float4*>(fact + 2 * (cc + k));
-          float e0, e1;
-          unpk(fma2(pk(v[k], v[k + 1]), pk(f.x, f.y), pk(f.z, f.w)), e0, e1);
-          e0 = ex2(e0);
-          e1 = ex2(e1);
-          if (!all) {
-            const int at = at0 + (int)((row0 + cc + k) / per), at1 = at0 + (int)((row0 + cc + k + 1) / per);
-            if (slot > at || (p.window > 0 && slot <= at - p.window)) e0 = 0.f;
-            if (slot > at1 || (p.window > 0 && slot <= at1 - p.window)) e1 = 0.f;
+          for (int k = 0; k < 32; k += 2) {
+            const float4 f = *reinterpret_cast<const float4*>(fact + 2 * (cc + k));
+            float e0, e1;
+            unpk(fma2(pk(v[k], v[k + 1]), pk(f.x, f.y), pk(f.z, f.w)), e0, e1);
+            sum[k / 2 & 3] = add2(sum[k / 2 & 3], pk(ex2(e0), ex2(e1)));
           }
-          sum[k / 2 & 3] = add2(sum[k / 2 & 3], pk(e0, e1));
+        } else {
+          int at = at0 + (int)((row0 + cc) / per), of = (int)((row0 + cc) % per);      // the row's slot, its place in its token
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            const float f = fact[4 * ((cc + k) >> 1) + (k & 1)], minus = fact[4 * ((cc + k) >> 1) + (k & 1) + 2];
+            const float e = slot > at || (p.window > 0 && slot <= at - p.window) ? 0.f : ex2(fmaf(v[k], f, minus));
+            sum[k & 3] = add2(sum[k & 3], pk(e, 0.f));
+            ++of;
+            at += of == per;
+            of = of == per ? 0 : of;
+          }
         }
       }
       __syncwarp();
