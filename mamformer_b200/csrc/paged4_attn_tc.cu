@@ -588,15 +588,14 @@ __global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ Weigh
   if (row0 < 0 || row0 >= rows) return;
   uint8_t* tile = p.tiles + ((int64_t)blockIdx.x * c.G + g) * TILE_BYTES<HD>;
   float* facts = reinterpret_cast<float*>(tile + WR * HD * 2);
-  const int k = threadIdx.x % LANES;
+  const int k = threadIdx.x % LANES, i0 = (int)(row0 / per), k0 = (int)(row0 % per);      // the first row's token, its place there
   constexpr int STEPS = WR * LANES / 256;
   Vec16<T> x[STEPS];
 #pragma unroll
   for (int s = 0; s < STEPS; ++s) {
-    const int64_t row = row0 + (s * 256 + threadIdx.x) / LANES;
-    const int i = (int)(row / per), j = (int)(row % per), h = g * p.rep + j / p.maps;
+    const int r = (s * 256 + threadIdx.x) / LANES, i = i0 + (k0 + r) / per, j = (k0 + r) % per, h = g * p.rep + j / p.maps;
     x[s].raw = make_uint4(0, 0, 0, 0);
-    if (row < rows)
+    if (row0 + r < rows)
       x[s] = ld16(j % p.maps ? (const T*)p.q2 + (int64_t)(t0 + i) * p.st2 + (int64_t)h * p.sh2 + 8 * k
                              : (const T*)p.q1 + (int64_t)(t0 + i) * p.st1 + (int64_t)h * p.sh1 + 8 * k);
   }
@@ -619,9 +618,8 @@ __global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ Weigh
     v.w = h2(to_f(x[s].v[3]) * down, to_f(x[s].v[7]) * down);
     *reinterpret_cast<uint4*>(tile + (k >> 3) * (WR * 128) + r * 128 + (((k & 7) ^ (r & 7)) << 4)) = v;
     if (k == 0) {
-      const int64_t row = row0 + r;
       facts[(r >> 1) * 4 + (r & 1)] = p.scale_log2 * pow2(e);
-      facts[(r >> 1) * 4 + (r & 1) + 2] = row < rows ? -p.lse[(t0 + row / per) * p.H * p.maps + g * per + row % per] : -INFINITY;
+      facts[(r >> 1) * 4 + (r & 1) + 2] = row0 + r < rows ? -p.lse[(int64_t)(t0 + i0 + (k0 + r) / per) * p.H * p.maps + g * per + (k0 + r) % per] : -INFINITY;
     }
   }
 }
