@@ -640,6 +640,9 @@ __global__ void __launch_bounds__(NTW, 1) weights_kernel(const __grid_constant__
   const int i0 = max(0, base - at0), last = min(base + WK, len) - 1;
   const int i1 = p.window > 0 ? (int)min((int64_t)n, (int64_t)last + p.window - at0) : n;
   if (i0 >= i1) return;
+  // The first slot that some row of the sequence sees.  A page below it may be another sequence's by now, whose CTA is adding
+  // to its weights: it is not touched, not even to add 0.
+  const int seen = p.window > 0 ? max(0, at0 - p.window + 1) : 0;
   const int64_t j0 = (int64_t)i0 * per / WR;
   const int ntile = (int)(((int64_t)i1 * per + WR - 1) / WR - j0);
   const uint8_t* tiles = p.tiles + ((first_unit(c, b, per) + j0) * c.G + g) * TILE_BYTES<HD>;
@@ -660,12 +663,12 @@ __global__ void __launch_bounds__(NTW, 1) weights_kernel(const __grid_constant__
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&tmem_slot)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  // keys: a 16-byte chunk of codes (32 dims) per thread and turn; slots past the end, or of no page, become zeros
+  // keys: a 16-byte chunk of codes (32 dims) per thread and turn; slots that nobody sees, or of no page, become zeros
   for (int i = threadIdx.x; i < WK * (HD / 32); i += NTW) {
     const int tok = i / (HD / 32), cc = i % (HD / 32), slot = base + tok;
     uint4 x = make_uint4(0, 0, 0, 0);
     uint32_t params[HD / 64] = {};
-    if (slot < len) {
+    if (slot >= seen && slot < len) {
       const int pg = c.table[(int64_t)b * c.W + (slot >> c.shift)];
       if (pg >= 0 && pg < c.P) {
         const uint8_t* blk = block_of<HD>(c, pg, g, slot);
@@ -785,7 +788,7 @@ __global__ void __launch_bounds__(NTW, 1) weights_kernel(const __grid_constant__
     }
     float a, a2;
     unpk(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), a, a2);
-    if (ok && slot < len) {
+    if (ok && slot >= seen && slot < len) {
       const int pg = c.table[(int64_t)b * c.W + (slot >> c.shift)];
       if (pg >= 0 && pg < c.P) c.mass[(((int64_t)pg * c.G + g) << c.shift) + (slot & (c.page - 1))] += a + a2;
     }
