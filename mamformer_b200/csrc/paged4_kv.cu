@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(NM) move_kernel(const __grid_constant__ Evict 
     page[u] = 0;
     dst[u] = nullptr;
     if (__all_sync(0xffffffffu, src[u] < 0)) continue;
-    if (MODE != UNPACK && src[u] >= 0) page[u] = table[src[u] >> c.shift];
+    if (src[u] >= 0) page[u] = table[src[u] >> c.shift];
     if (MODE == PACK) {
       dst[u] = p.packed + (((int64_t)b * c.G + g) * blocks + first + u) * PACKED<HD>;
       dst_mass[u] = reinterpret_cast<float*>(dst[u] + BLOCK<HD>);
@@ -354,7 +354,8 @@ __global__ void __launch_bounds__(NM) move_kernel(const __grid_constant__ Evict 
 #pragma unroll
   for (int u = 0; u < PAIR; ++u) {
     if (!dst[u]) continue;
-    if (MODE != UNPACK && src[u] >= 0 && (page[u] < 0 || page[u] >= c.P)) { src[u] = -1; record(ERR_PAGE); }
+    // no page: nothing comes of the token, also not out of the packed copy, where its place was never written
+    if (src[u] >= 0 && (page[u] < 0 || page[u] >= c.P)) { src[u] = -1; record(ERR_PAGE); }
     const uint8_t* packed = MODE == UNPACK ? p.packed + (((int64_t)b * c.G + g) * blocks + first + u) * PACKED<HD> : nullptr;
     // where the token's block is, and its row of it
     const int64_t mine = MODE == UNPACK ? 0 : src[u] >= 0 ? block_of<HD>(c, page[u], g, src[u]) - c.blocks : -1;

@@ -34,3 +34,57 @@ def test_entries_below_a_window_may_name_live_pages(dev, page, window, new, lens
         for _ in range(3):
             check(q, cache, t, new, lens, window=window)
             assert torch.equal(mass, cache.mass)
+
+
+# ---- eviction ------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("hd,page", [(64, 16), (128, 32)])
+@pytest.mark.parametrize("gone", [-1, 1 << 30])
+def test_evicted_tokens_of_a_bad_page_leave_their_new_slots_alone(in_place, hd, page, gone):
+    """Nothing but what a slot held, or the token that it is to hold, is in it afterwards, whatever memory held before."""
+    from mamformer_b200.fault import PagedCacheError, check_device_status
+    lens, G, budget, recent = [150, 90], 2, 70, 20
+    cache, table = filled(lens, page, G, hd, "cuda")
+    cache.mass.copy_(some_mass(cache.mass.shape, 1, "cuda") + 1.0)
+    bad = 140 // page                                                 # of the last tokens of sequence 0, which are kept whatever their weight
+    t = table.clone()
+    t[0, bad] = gone
+    to, P = None, cache.blocks.shape[0]
+    if not in_place:
+        new, extra = tables([budget] * 2, page, "cuda", 9)
+        cache = ops.PagedKV4(torch.cat([cache.blocks, pool(extra, G, page, hd, "cuda").blocks]), torch.cat([cache.mass, torch.full((extra, G, page), 8.0, device="cuda")]))
+        to = new + P
+    # what the cache holds of each token: its bytes and its weight
+    slots = lambda c: torch.cat([x.flatten(4) for x in _pieces(c)], -1).flatten(2, 3)                    # noqa: E731  (P, G, page, bytes)
+    check_device_status()
+    junk = [torch.full((1 << 15,), 0x5A, dtype=torch.uint8, device="cuda") for _ in range(64)]     # what a workspace may find
+    before = slots(cache).clone()
+    del junk
+    kept, left = ops.kv_evict(cache, t, i32(lens, "cuda"), budget, recent, out_table=to)
+    with pytest.raises(PagedCacheError, match="page"):
+        check_device_status()
+    after, where = slots(cache), t if in_place else to
+    assert left.tolist() == [70, 70]
+    unmoved = 0
+    for b in range(2):
+        for g in range(G):
+            for r, s in enumerate(kept[b, g].tolist()):
+                at = int(where[b, r // page])
+                if not 0 <= at < cache.blocks.shape[0]:
+                    continue
+                from_page = int(t[b, s // page])
+                ok = 0 <= from_page < P
+                unmoved += not ok
+                want = before[from_page, g, s % page] if ok else before[at, g, r % page]
+                assert torch.equal(after[at, g, r % page], want)
+    assert unmoved > 0
+
+
+def _pieces(cache):
+    """The bytes of each token of a cache, (P, G, page / 16, 16, ..) each: codes and parameters of keys and values, weight."""
+    hd = cache.blocks.shape[-1] // 18
+    out = []
+    for x in (cache.blocks[..., :9 * hd], cache.blocks[..., 9 * hd:]):
+        out += [x[..., :8 * hd].unflatten(-1, (16, hd // 2)), x[..., 8 * hd:].unflatten(-1, (16, hd // 16))]
+    return out + [cache.mass.view(torch.uint8).unflatten(-1, (-1, 16, 4))]
