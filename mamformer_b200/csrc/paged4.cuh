@@ -109,8 +109,10 @@ __device__ __forceinline__ void decode(uint32_t w, const Levels& l, const Base& 
 
 // ---- values -> codes -------------------------------------------------------------------------------
 // Scale and zero point of a group with extremes lo <= 0 <= hi.  The scale is a fifteenth of the range rounded up to 7
-// significant bits (to a multiple of 2^-20 below 2^-14), so that every value is within half a step of a level; its
-// largest keeps all levels within f16.  Elementwise fp32 roundings throughout, so that eager code finds the same codes.
+// significant bits (to a multiple of 2^-20 below 2^-14), so that every value is within half a step of a level.  No level may
+// leave f16: the largest scale is 65504 / max(zero, 15 - zero) rounded down to 7 bits, which above 4096 are multiples of 64.
+// It is met only where an extreme is above 60,900; the other end of such a group may then be off by up to a step.
+// Elementwise fp32 roundings throughout, so that eager code finds the same codes.
 struct Group { float scale, inv; int zero; };
 __device__ __forceinline__ Group group_of(float lo, float hi) {
   float s = __fmul_rn(__fsub_rn(hi, lo), 0.06666666f);          // 1/15, rounded down
@@ -119,7 +121,7 @@ __device__ __forceinline__ Group group_of(float lo, float hi) {
   s = fmaxf(s, 9.5367431640625e-7f);
   Group g;
   g.zero = (int)fminf(fmaxf(rintf(__fmul_rn(-lo, __frcp_rn(s))), 0.f), 15.f);
-  g.scale = fminf(s, 4352.f);
+  g.scale = s > 4352.f ? fminf(s, (float)(64 * (1023 / max(g.zero, 15 - g.zero)))) : s;      // 4352: of 15 levels on one side
   g.inv = __frcp_rn(g.scale);
   return g;
 }

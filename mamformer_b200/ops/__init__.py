@@ -286,9 +286,10 @@ class PagedKV4(NamedTuple):
     A block holds 16 tokens of a KV head: key codes (16, hd / 2), key parameters (16, hd / 32) of 16 bits, and the
     same of the values.  A byte holds two dims, the even one in its low half.  Group j of hd / 32 is the 32 dims d with
     (d / 4) % (hd / 32) == j; its parameter is the f16 pattern of a scale s with the zero point z in the low 4 bits,
-    and a code n stands for s (n - z), exactly an f16.  Values within a group are rounded to sixteen levels that span
-    them and 0, evenly.  The range is f16's: larger values and infinities become its largest, NaN becomes 0, and
-    levels are 2^-20 apart at least."""
+    and a code n stands for s (n - z), exactly an f16.  Values within a group are rounded to the nearest of sixteen even
+    levels that span them and 0, a fifteenth of that range apart, 1/64 of it more at most, and 2^-20 at least.  The range
+    is f16's: larger values and infinities become its largest, NaN becomes 0.  Levels stay within f16 too, so that in a
+    group that has values of both signs and some above 60,900 in size the end away from those may be off by a whole step."""
     blocks: torch.Tensor                       # (P, G, page / 16, 18 hd) uint8
     mass: Optional[torch.Tensor] = None        # (P, G, page) fp32
 

@@ -462,7 +462,8 @@ def paged_attention(q, cache, block_table, cu_seqlens, kv_lens, q2, lam, window,
 # ---- the 4-bit cache (layout in ops.PagedKV4) -----------------------------------------------------------
 def kv4_levels(x: torch.Tensor):
     """fp32 (.., hd) -> codes (.., hd / 2) uint8, parameters (.., hd / 32) int16.  The scale is a fifteenth of a group's
-    range, 0 in it, rounded up to 7 significant bits (to a multiple of 2^-20 below 2^-14)."""
+    range, 0 in it, rounded up to 7 significant bits (to a multiple of 2^-20 below 2^-14), and no more than keeps every level
+    within f16: 65504 / max(z, 15 - z), rounded down to a multiple of 64."""
     J = x.shape[-1] // 32
     x = torch.where(x.isnan(), 0.0, x).clamp(-65504.0, 65504.0).unflatten(-1, (8, J, 4))
     lo, hi = x.amin((-3, -1)).clamp(max=0.0), x.amax((-3, -1)).clamp(min=0.0)
@@ -470,7 +471,7 @@ def kv4_levels(x: torch.Tensor):
     up = ((s.view(torch.int32) + 0x1FFFF) & ~0x1FFFF).view(torch.float32)
     s = torch.where(s < 2.0 ** -14, torch.ceil(s * 2.0 ** 20) * 2.0 ** -20, up).clamp(min=2.0 ** -20)
     z = torch.round(-lo * s.reciprocal()).clamp(0.0, 15.0)
-    s = s.clamp(max=4352.0)
+    s = torch.minimum(s, 64.0 * torch.floor(1023.0 / torch.maximum(z, 15.0 - z)))
     n = (torch.round(x * s.reciprocal()[..., None, :, None]) + z[..., None, :, None]).clamp(0.0, 15.0)
     n = n.to(torch.uint8).flatten(-3)
     return n[..., 0::2] | n[..., 1::2] << 4, s.half().view(torch.int16) | z.to(torch.int16)

@@ -88,3 +88,60 @@ def _pieces(cache):
     for x in (cache.blocks[..., :9 * hd], cache.blocks[..., 9 * hd:]):
         out += [x[..., :8 * hd].unflatten(-1, (16, hd // 2)), x[..., 8 * hd:].unflatten(-1, (16, hd // 16))]
     return out + [cache.mass.view(torch.uint8).unflatten(-1, (-1, 16, 4))]
+
+
+# ---- the levels of wide groups -------------------------------------------------------------------------
+def wide(seed=1):
+    """Rows (T, 1, 64) whose two groups have any two ends within f16: both signs, one sign, symmetric, the largest."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.rand(600, 1, 64, generator=g)
+    top, low = 65504 * torch.rand(600, 1, 64, generator=g)[..., :1] ** 0.3, 65504 * torch.rand(600, 1, 1, generator=g) ** 0.3
+    top[::5], low[1::5], top[2::5], low[2::5] = 65504.0, 65504.0, 65504.0, 65504.0
+    top[3::5], low[3::5] = 40000.0, 40000.0
+    x = (top + low) * x - low
+    x[4::50] = x[4::50].abs()
+    x[9::50] = -x[9::50].abs()
+    x[..., :8], x[..., 8:16] = top, -low
+    return x.clamp(-65504.0, 65504.0)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_values_of_wide_groups(dev):
+    """Within half a step of the group's levels where these fit into f16 as they are; within a step for every group."""
+    x = wide().to(dev)
+    T = len(x)
+    table, P = tables([T], 32, dev)
+    cache = pool(P, 1, 32, 64, dev)
+    ops.kv_append(x, -x, cache, table, offsets([T], dev), i32([T], dev), T)
+    back = ops.kv_read(cache, table, offsets([T], dev), i32([T], dev), T, torch.float32)
+    for got, want in zip(back, (x.double(), -x.double())):
+        off, half = (got.double() - want).abs(), half_step(want)
+        assert got.abs().amax() <= 65504 and (off <= 2 * half).all()
+        for j in range(2):
+            of = (group_of(64) == j).to(dev)
+            fits = want[..., of].abs().amax(-1) <= 60900
+            assert fits.any() and not fits.all() and (off[..., of][fits] <= half[..., of][fits]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_both_devices_store_the_same_bytes_of_wide_groups(dtype):
+    x = wide(2).to(dtype)
+    T, got = len(x), []
+    for dev in ("cpu", "cuda"):
+        table, P = tables([T], 32, dev)
+        cache = ops.PagedKV4(torch.zeros(P, 1, 2, 18 * 64, dtype=torch.uint8, device=dev))
+        ops.kv_append(x.to(dev), -x.to(dev), cache, table, offsets([T], dev), i32([T], dev), T)
+        got.append(cache.blocks.cpu())
+    assert torch.equal(*got)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("new", [[3], [80]])
+def test_attention_over_wide_groups(dev, new):
+    """The products take what the cache holds, up to f16's largest."""
+    x = wide(3)[:200].to(dev)
+    table, P = tables([200], 16, dev)
+    cache = pool(P, 1, 16, 64, dev)
+    ops.kv_append(x.flip(0) * 2.0 ** -14, x, cache, table, offsets([200], dev), i32([200], dev), 200)
+    check(rand((sum(new), 2, 64), torch.bfloat16, dev, 3), cache, table, new, [200])
