@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
         long_one = long_one || cached_length(c, c.lens[i]) != c.lens[i];
       }
       if (long_one || odd) atomicCAS(&g_err, 0, (int)ERR_LENGTH);
-      if (__syncthreads_or(odd)) {                 // no unit may have some rows: none of the call's results count
+      if (__syncthreads_or(odd)) {                 // none of the call's results count, and nobody else writes any
         for (int64_t i = threadIdx.x; i < c.T * row; i += NT) ((T*)p.out)[i] = from_f<T>(0.f);
       }
     }
@@ -153,6 +153,10 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
     ntile = min(share, ntile - first);
   }
 
+  // Offsets out of order anywhere: some rows may be no unit's, or two units', so no unit leaves results.  The look at them is
+  // over by the time that the tensor memory is there.
+  bool odd = false;
+  for (int i = threadIdx.x; i < c.B; i += NT) odd = odd || !in_order(c, i);
   if (threadIdx.x == 0) {
     bar_init(&q_full, 256);
     bar_init(&ex_full, 128);
@@ -167,9 +171,13 @@ __global__ void __launch_bounds__(NT, 1) chunk_kernel(const __grid_constant__ Pa
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   fence_before();
-  __syncthreads();
+  odd = __syncthreads_or(odd);
   fence_after();
   const uint32_t tmem = tmem_slot;
+  if (odd) {
+    if (warp == 8 + NC / 32) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    return;
+  }
   uint8_t* ring = sm + 2 * QB;
 
   if (warp >= 8 && warp < 8 + NC / 32) {
@@ -499,6 +507,9 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__ Params p, int units) {
   constexpr int D = HD / 32;
   const Cache& c = p.c;
+  bool odd = false;                                // then there are no parts
+  for (int i = threadIdx.x; i < c.B; i += 256) odd = odd || !in_order(c, i);
+  if (__syncthreads_or(odd)) return;
   const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
   if (item >= (int64_t)c.T * p.H) return;

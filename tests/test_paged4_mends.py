@@ -145,3 +145,43 @@ def test_attention_over_wide_groups(dev, new):
     cache = pool(P, 1, 16, 64, dev)
     ops.kv_append(x.flip(0) * 2.0 ** -14, x, cache, table, offsets([200], dev), i32([200], dev), 200)
     check(rand((sum(new), 2, 64), torch.bfloat16, dev, 3), cache, table, new, [200])
+
+
+# ---- offsets out of order ------------------------------------------------------------------------------
+def cache_of(bits, lens, page, G, hd):
+    if bits == 4:
+        return filled(lens, page, G, hd, "cuda")
+    import test_paged_cache as eight
+    table, P = tables(lens, page, "cuda")
+    cache = eight.pool(P, G, page, hd, "cuda")
+    k, v = rand((sum(lens), G, hd), torch.float32, "cuda", 1), rand((sum(lens), G, hd), torch.float32, "cuda", 2)
+    ops.kv_append(k, v, cache, table, offsets(lens, "cuda"), i32(lens, "cuda"), max(lens))
+    return cache, table
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hd,diff", [(64, False), (128, True)])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("off,T,max_new", [([0, 200, 100], 200, 100), ([0, 200, 100], 600, 200), ([100, 0, 200], 200, 100), ([0, 300, 200, 600], 600, 200),
+                                           ([0, 90, 900], 180, 90), ([-5, 100, 200], 200, 100)])
+def test_offsets_out_of_order_give_zeros(bits, hd, diff, wide, off, T, max_new):
+    """With a table so wide that the chunk kernel's CTAs share keys, and without; weights stay as they were."""
+    from mamformer_b200.fault import PagedCacheError, check_device_status
+    lens = [300] * (len(off) - 1)
+    cache, table = cache_of(bits, lens, 64, 2, hd)
+    if wide:
+        table = torch.cat([table, torch.full((len(lens), 96), -1, dtype=torch.int32, device="cuda")], 1)
+    q = rand((T, 4, hd), torch.bfloat16, "cuda", 4)
+    check_device_status()
+    for _ in range(3):
+        junk = [torch.full((n,), 7.0, device="cuda") for n in (T * 4 * hd // 2, 1 << 22, 1 << 24)]      # what outputs and workspaces may find
+        del junk
+        got = ops.paged_attention(q, cache, table, i32(off, "cuda"), i32(lens, "cuda"), max_new, **pair(q, diff))
+        with pytest.raises(PagedCacheError, match="lengths"):
+            check_device_status()
+        assert (got == 0).all()
+        if bits == 4:
+            held_by = torch.zeros(cache.mass.shape[0], dtype=torch.bool, device="cuda")
+            held_by[table[table >= 0].long()] = True
+            assert ((cache.mass[held_by] == 0) | (cache.mass[held_by] == 3)).all()
