@@ -110,7 +110,8 @@ __device__ __forceinline__ void decode(uint32_t w, const Levels& l, const Base& 
 // ---- values -> codes -------------------------------------------------------------------------------
 // Scale and zero point of a group with extremes lo <= 0 <= hi.  The scale is a fifteenth of the range rounded up to 7
 // significant bits (to a multiple of 2^-20 below 2^-14), so that every value is within half a step of a level.  No level may
-// leave f16: the largest scale is 65504 / max(zero, 15 - zero) rounded down to 7 bits, which above 4096 are multiples of 64.
+// leave f16: the largest scale is 65504 / max(zero, 15 - zero) rounded down to 7 bits, which above 4096 are multiples of
+// 64: 64 floor(1023 / max(zero, 15 - zero)).
 // It is met only where an extreme is above 60,900; the other end of such a group may then be off by up to a step.
 // Elementwise fp32 roundings throughout, so that eager code finds the same codes.
 struct Group { float scale, inv; int zero; };
@@ -121,7 +122,9 @@ __device__ __forceinline__ Group group_of(float lo, float hi) {
   s = fmaxf(s, 9.5367431640625e-7f);
   Group g;
   g.zero = (int)fminf(fmaxf(rintf(__fmul_rn(-lo, __frcp_rn(s))), 0.f), 15.f);
-  g.scale = s > 4352.f ? fminf(s, (float)(64 * (1023 / max(g.zero, 15 - g.zero)))) : s;      // 4352: of 15 levels on one side
+  // 1023 / m for m = 8 .. 15, a byte each: a division cost a single-token append 1 us
+  const uint32_t units = __byte_perm(0x5D66717Fu, 0x44494E55u, (uint32_t)max(g.zero, 15 - g.zero) - 8u) & 0xFFu;
+  g.scale = fminf(s, 64.f * (float)units);
   g.inv = __frcp_rn(g.scale);
   return g;
 }
