@@ -85,7 +85,7 @@ class PagedKVCache:
             raise ValueError(f"the paged cache holds heads of 64 or 128 dims, got {head_dim}")
         self.n_kv_heads, self.head_dim, self.page_size = n_kv_heads, head_dim, page_size
         self.bits, self.weights = bits, weights
-        self.evicted = False                                     # slots are no longer positions
+        self._cut: set = set()                                   # sequences that were evicted from
         self.batch = batch
         self.width = max(1, -(-max_len // page_size))            # pages of a sequence
         self.n_pages = n_pages if n_pages is not None else batch * self.width
@@ -128,6 +128,11 @@ class PagedKVCache:
         return cls(len(model.model.layers), *heads.pop(), batch, max_len, page_size,
                    device=next(model.parameters()).device, bits=bits, weights=weights)
 
+    @property
+    def evicted(self) -> bool:
+        """Some sequence's slots are no longer its positions: tokens of it were evicted, and it has not been released since."""
+        return bool(self._cut)
+
     def layer(self, i: int) -> PagedLayer:
         return self.layers[i]
 
@@ -169,6 +174,7 @@ class PagedKVCache:
         """Give sequence b's pages back; it is empty afterwards."""
         self._free.extend(reversed(self._pages[b]))
         self._pages[b] = []
+        self._cut.discard(b)
         self.lens[b] = 0
         self.block_table[b] = -1
         self.kv_lens = self.kv_lens.clone()
@@ -197,8 +203,8 @@ class PagedKVCache:
             if layer._skipped is not None:
                 layer._skipped = left - lens
         self.kv_lens = left
+        self._cut.update(b for b, n in enumerate(self.lens) if n > budget)
         self.lens = [min(n, budget) for n in self.lens]
-        self.evicted = True
         rows, cols = [], []
         for b, (n, pages) in enumerate(zip(self.lens, self._pages)):
             need = -(-n // self.page_size)
