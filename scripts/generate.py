@@ -50,6 +50,8 @@ def generate_text(model, tok, prompt, args):
     model.config.generation.repetition_penalty = args.repetition_penalty
     if args.kv_cache != "dense" and (args.num_beams > 1 or (args.thinking and args.thinking != "NoThink")):
         raise ValueError(f"--kv_cache {args.kv_cache} goes with sampling: beams and thinking modes copy their cache between paths")
+    if args.kv_budget is not None and args.kv_cache != "paged4":
+        raise ValueError(f"--kv_budget goes with --kv_cache paged4, not {args.kv_cache}")
     if args.thinking and args.thinking != "NoThink":
         tc = ThinkingConfig.from_preset(args.thinking, args.think_budget, args.num_paths, args.summary_budget,
                                         args.show_thinking)

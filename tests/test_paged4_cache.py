@@ -39,3 +39,18 @@ def test_windows_after_the_evicted_sequences_were_released(dev, dtype):
             want, tol, _, _ = plain(q, c.layer(0).kv, c.block_table, new, c.lens, window=9)
             close(got, want, tol + (2.0 ** -18 if dtype == torch.float32 else 0.0))
     c.check()
+
+
+@pytest.mark.parametrize("flags", [["--num_beams", "2"], ["--thinking", "FastThink"], []])
+@pytest.mark.parametrize("kv", ["dense", "paged"])
+def test_generate_script_refuses_a_budget_that_it_would_not_keep(flags, kv):
+    from mamformer_b200.models.model import MamformerForCausalLM
+    from mamformer_b200.tokenizer import MamformerTokenizer
+    from scripts.generate import build_parser, generate_text
+    from test_paged_generate import small_config
+    parser = build_parser()
+    need = [x for a in parser._actions if a.required for x in (a.option_strings[0], "x")]
+    args = parser.parse_args(need + flags + ["--kv_cache", kv, "--kv_budget", "64", "--max_new_tokens", "1"])
+    model = MamformerForCausalLM(small_config()).eval()
+    with pytest.raises(ValueError, match="kv_budget" if kv == "dense" or not flags else "kv_"):
+        generate_text(model, MamformerTokenizer(), "x", args)
