@@ -152,9 +152,10 @@ class GRPOTrainer:
         c = self.cfg
         self.policy.eval()
         outs = []
+        budget = {} if c.gen_kv_budget is None else {"kv_budget": c.gen_kv_budget}      # a policy of another class may not know it
         for t in rollout_temperatures(c.gen_temperature, c.group_size):
             g = self.policy.generate(prompt_ids, max_new_tokens=c.gen_max_tokens, temperature=t, top_k=c.gen_top_k,
-                                     top_p=c.gen_top_p, kv_cache=c.gen_kv_cache, kv_budget=c.gen_kv_budget)
+                                     top_p=c.gen_top_p, kv_cache=c.gen_kv_cache, **budget)
             outs.append(g[:, prompt_ids.shape[1]:])
         self.policy.train()
         return outs

@@ -54,3 +54,16 @@ def test_generate_script_refuses_a_budget_that_it_would_not_keep(flags, kv):
     model = MamformerForCausalLM(small_config()).eval()
     with pytest.raises(ValueError, match="kv_budget" if kv == "dense" or not flags else "kv_"):
         generate_text(model, MamformerTokenizer(), "x", args)
+
+
+def test_rollouts_of_a_policy_without_a_budget():
+    """A policy of one's own whose generate() knows no budget goes on as before where none is set."""
+    from mamformer_b200.grpo import GRPOConfig, GRPOTrainer
+
+    class Policy(torch.nn.Module):
+        def generate(self, ids, max_new_tokens, temperature, top_k, top_p, kv_cache):
+            return torch.cat([ids, ids], 1)
+
+    trainer = GRPOTrainer.__new__(GRPOTrainer)
+    trainer.cfg, trainer.policy = GRPOConfig(group_size=2), Policy()
+    assert len(trainer.rollouts(torch.zeros(1, 3, dtype=torch.long))) == 2
