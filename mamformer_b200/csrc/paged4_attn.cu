@@ -18,9 +18,9 @@
 // 2^-21 of a row's largest keep all of their bits, whatever values they are given to.  The order of the head's dims in the
 // products is free as long as both sides agree: a lane takes 16 adjacent bytes of a key's codes and 8 of a value's.
 //
-// Received weights: the scores of up to 16 rows are left in a workspace (4 bytes a row and slot, a small part of which the
-// L2 does not keep), and a last kernel turns them into weights with each row's joined sum; longer runs of tokens have
-// them computed from the keys once more (paged4_attn_tc.cu).
+// Received weights: the scores of up to 16 rows are left in a workspace, 4 bytes a row and slot, for at most twice
+// the slots of the pool (a slot of the cache has 76 or 148 bytes), and a last kernel turns them into weights with each row's
+// joined sum; longer runs of tokens have them computed from the keys once more (paged4_attn_tc.cu).
 #include "paged4.cuh"
 #include "paged_split.cuh"
 
@@ -47,15 +47,27 @@ constexpr int MOST = 8;                        // CTAs of a cluster
 constexpr int SHORT = 4;
 constexpr int KEEP = 16;                       // rows whose scores are left for the received weights, at most
 
+// A sequence's scores: [G][n][stride] from slot `lo` on, behind those of `start` slots; start < 0: not kept.
+struct Place { int64_t start; int lo, n; };
+
 struct Params : Attn4 {
   int ctas;
   float* part;        // [ctas][2][rows][HD + 2]: O (not divided), r, l
   int4* joins;        // [ctas]: {t0, rows, g | rt << 16, 2 c0 + place} of the item that ends in this CTA after it
                       // began in CTA c0 (its part there is in `place`), or {-1, ..}
-  float* scores;      // [B][G][cap][stride] scores (log2) of up to `stride` rows, where weights are asked for
+  float* scores;      // scores (log2) of up to `stride` rows of a slot, where weights are asked for
+  const Place* places;                     // [B] where a sequence's scores are; null: at b cap, of all slots
   int64_t cap;        // slots that a sequence can have
   int stride;
 };
+
+// Slots in front of slot 0's scores of a sequence and KV head (less than 0 where slots in front of `lo` are left out), or NOT_KEPT.
+constexpr int64_t NOT_KEPT = -(1LL << 62);
+__device__ __forceinline__ int64_t scores_of(const Params& p, int b, int g) {
+  if (!p.places) return ((int64_t)b * p.c.G + g) * p.cap;
+  const Place at = p.places[b];
+  return at.start < 0 ? NOT_KEPT : at.start * p.c.G + (int64_t)g * at.n - at.lo;
+}
 
 __device__ __forceinline__ uint32_t lds4(uint32_t a) {
   uint32_t v;
@@ -310,7 +322,10 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
   float* scores_at = nullptr;             // of slot 0 and this lane's first row
   auto load_rows = [&]() {
     const int per = p.rep * p.maps, at0 = it.len - it.n;
-    if (p.scores) scores_at = it.rows <= p.stride ? p.scores + ((int64_t)it.b * c.G + it.g) * p.cap * p.stride + 2 * t4 : nullptr;
+    if (p.scores) {
+      const int64_t at = it.rows <= p.stride ? scores_of(p, it.b, it.g) : NOT_KEPT;
+      scores_at = at != NOT_KEPT ? p.scores + at * p.stride + 2 * t4 : nullptr;
+    }
     it_hi = it.hi;
     all_hi = min(it.len - 1, at0 + it.rt * ROWS / per);
     all_lo = p.window > 0 ? at0 + min(it.n - 1, (it.rt * ROWS + ROWS - 1) / per) - p.window + 1 : 0;
@@ -712,13 +727,56 @@ __global__ void __launch_bounds__(NT, residents<HD, NR>()) split_kernel(const __
 }
 
 // ---- received weights ------------------------------------------------------------------------------
+// Where each sequence's scores go when the workspace is as large as the pool: one block lays the pages that rows see end to
+// end.  They are one sequence's each, so they fit; what does not is recorded and left out.
+constexpr int NPL = 1024;
+__global__ void __launch_bounds__(NPL) places_kernel(const __grid_constant__ Params p, Place* places, int64_t room) {
+  const Cache4& c = p.c;
+  const int chunk = (c.B + NPL - 1) / NPL, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  auto place_of = [&](int b) {
+    Item it;
+    Place at{-1, 0, 0};
+    if (!in_order(c, b) || !set_sequence<2 * 8, TILE>(p, it, b) || it.rows > p.stride) return at;
+    at.start = 0;
+    at.lo = it.lo >> c.shift << c.shift;
+    at.n = max(0, ((it.hi + c.page - 1) >> c.shift << c.shift) - at.lo);
+    return at;
+  };
+  const int b0 = threadIdx.x * chunk, b1 = min(c.B, b0 + chunk);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += place_of(b).n;
+  __shared__ int64_t sums[NPL / 32];
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) sums[w] = incl;
+  __syncthreads();
+  for (int i = 0; i < w; ++i) incl += sums[i];
+  int64_t at = incl - mine;
+  for (int b = b0; b < b1; ++b) {
+    Place x = place_of(b);
+    if (x.start == 0) {
+      x.start = at;
+      at += x.n;
+      if (at > room) { x.start = -1; record(ERR_PAGE); }
+    }
+    places[b] = x;
+  }
+}
+
 // From the scores that the split kernel has left: a thread per slot.
 constexpr int NK = 256;
-__global__ void __launch_bounds__(NK) kept_weights_kernel(const __grid_constant__ Params p) {
+// all of an SM's threads resident: 32 registers; with 35, 64 sequences of up to 8191 slots took 20 us and not 17
+__global__ void __launch_bounds__(NK, 8) kept_weights_kernel(const __grid_constant__ Params p) {
   const Cache4& c = p.c;
   const int g = blockIdx.y, b = blockIdx.z;
   Item it;
   if (!in_order(c, b) || !set_sequence<2 * 8, TILE>(p, it, b) || it.rows > p.stride) return;
+  const int64_t first = scores_of(p, b, g);
+  if (first == NOT_KEPT) return;
   const int per = p.rep * p.maps;
   __shared__ float lse[KEEP];
   if (threadIdx.x < KEEP) {
@@ -733,7 +791,7 @@ __global__ void __launch_bounds__(NK) kept_weights_kernel(const __grid_constant_
     if (pg < 0 || pg >= c.P) continue;                  // recorded where its keys were looked for
     float* to = c.mass + (((int64_t)pg * c.G + g) << c.shift) + (slot & (c.page - 1));
     const float had = *to;
-    const float* s = p.scores + (((int64_t)b * c.G + g) * p.cap + slot) * p.stride;
+    const float* s = p.scores + (first + slot) * p.stride;
     float sum = 0.f;
     if (p.stride % 4 == 0) {
       for (int row = 0; row < it.rows; row += 4) {
@@ -832,15 +890,26 @@ at::Tensor paged4_attention(at::Tensor q1, c10::optional<at::Tensor> q2, c10::op
   p.chunked = most_rows > FEW && p.c.B > 0;
   const bool alone = p.chunked && T == p.c.B * max_new;
   p.few = alone ? 0 : (int)std::min<int64_t>(most_rows, FEW);
-  at::Tensor sums, kept;
+  at::Tensor sums, kept, places;
   if (mass.has_value() && p.c.B > 0) {
     TORCH_CHECK(p.c.B < 65536, "paged_attention: received weights of at most 65535 sequences");
     sums = at::empty({T, H, p.maps}, q1.options().dtype(at::kFloat));
     p.lse = sums.data_ptr<float>();
     if (!alone) {
       p.stride = (int)((std::min<int64_t>(p.few, KEEP) + 1) / 2 * 2);
-      kept = at::empty({p.c.B * (int64_t)p.c.G * p.cap * p.stride}, q1.options().dtype(at::kFloat));
+      // A place for each slot that the block table has room for, or, where that is far more than the pool has, for each
+      // of the pool's: one launch more.
+      const int64_t pool = (int64_t)p.c.P * p.c.page, room = p.c.B * p.cap;
+      const bool dense = 2 * pool < room;
+      kept = at::empty({(dense ? pool : room) * p.c.G * p.stride}, q1.options().dtype(at::kFloat));
       p.scores = kept.data_ptr<float>();
+      if (dense) {
+        places = at::empty({(int64_t)p.c.B * (int64_t)sizeof(Place)}, q1.options().dtype(at::kByte));
+        Place* to = reinterpret_cast<Place*>(places.data_ptr<uint8_t>());
+        p.places = to;
+        places_kernel<<<1, NPL, 0, stream()>>>(p, to, pool);
+        MAMF_LAUNCH_CHECK();
+      }
     }
   }
   const bool bf16 = q1.scalar_type() == at::kBFloat16;

@@ -185,3 +185,66 @@ def test_offsets_out_of_order_give_zeros(bits, hd, diff, wide, off, T, max_new):
             held_by = torch.zeros(cache.mass.shape[0], dtype=torch.bool, device="cuda")
             held_by[table[table >= 0].long()] = True
             assert ((cache.mass[held_by] == 0) | (cache.mass[held_by] == 3)).all()
+
+
+# ---- tables wider than the pool ------------------------------------------------------------------------
+def widened(table, slots, page):
+    """The same sequences in a table with room for `slots` tokens each."""
+    more = max(0, slots // page - table.shape[1])
+    return torch.cat([table, torch.full((table.shape[0], more), -1, dtype=torch.int32, device=table.device)], 1)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("new,lens", CASES)
+@pytest.mark.parametrize("hd,page,G,rep,diff,window,dtype", [(64, 16, 2, 1, True, 0, torch.float16), (128, 16, 1, 3, False, 29, torch.bfloat16),
+                                                             (128, 64, 2, 4, False, 0, torch.bfloat16), (128, 128, 1, 8, True, 64, torch.bfloat16)])
+def test_short_sequences_on_a_wide_table(dev, new, lens, hd, page, G, rep, diff, window, dtype):
+    """What a cache made for long sequences asks of short ones."""
+    cache, table = filled([max(n, 1) for n in lens], page, G, hd, dev)
+    q = rand((sum(new), G * rep, hd), dtype, dev, 3)
+    check(q, cache, widened(table, 20000, page), new, lens, **pair(q, diff), window=window)
+
+
+@pytest.mark.gpu
+def test_received_weights_take_no_more_memory_than_the_pool_has_slots():
+    """64 sequences of a few tokens in a table for 2^17 each: by the table's width the scores alone would take 2 GB."""
+    lens, G, hd, page = [5 + 3 * b for b in range(64)], 8, 64, 64
+    cache, table = filled(lens, page, G, hd, "cuda")
+    table = widened(table, 1 << 17, page)
+    for new, H in (([1] * 64, 32), ([1] * 63 + [100], 32)):
+        q = rand((sum(new), H, hd), torch.bfloat16, "cuda", 3)
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        torch.cuda.reset_peak_memory_stats()
+        had = torch.cuda.memory_allocated()
+        ops.paged_attention(q, cache, table, offsets(new, "cuda"), i32(lens, "cuda"), max(new))
+        assert torch.cuda.max_memory_allocated() - had < 1 << 28
+        check(q, cache, table, new, lens)
+
+
+@pytest.mark.gpu
+def test_lengths_beyond_the_pool_on_a_wide_table():
+    """A length whose pages are not there: reported, the other sequences as without it, weights too."""
+    from mamformer_b200.fault import PagedCacheError, check_device_status
+    lens, G, hd, page = [300, 90, 200], 2, 64, 16
+    cache, table = filled(lens, page, G, hd, "cuda")
+    table = widened(table, 1 << 15, page)
+    q = rand((3, 4, hd), torch.bfloat16, "cuda", 3)
+    check_device_status()
+    for b in range(3):
+        results = []
+        for long_one in (lens[b], 20000):
+            cache.mass.fill_(1.0)
+            got = ops.paged_attention(q, cache, table, offsets([1] * 3, "cuda"), i32([long_one if i == b else n for i, n in enumerate(lens)], "cuda"), 1)
+            results.append((got, cache.mass.clone()))
+            if long_one == 20000:
+                with pytest.raises(PagedCacheError):
+                    check_device_status()
+        (a, am), (c, cm) = results
+        others = [i for i in range(3) if i != b]
+        # its own row and weights are those of whatever is behind its end in its last page
+        assert torch.equal(a[others], c[others])
+        for i in others:
+            pages = table[i, :-(-lens[i] // page)].long()
+            # what does not fit is left out of the weights, never added to others'
+            assert torch.equal(am[pages], cm[pages]) or (cm[pages] == 1.0).all()
