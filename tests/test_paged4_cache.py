@@ -67,3 +67,30 @@ def test_rollouts_of_a_policy_without_a_budget():
     trainer = GRPOTrainer.__new__(GRPOTrainer)
     trainer.cfg, trainer.policy = GRPOConfig(group_size=2), Policy()
     assert len(trainer.rollouts(torch.zeros(1, 3, dtype=torch.long))) == 2
+
+
+def test_decodes_as_the_dense_cache_does_on_the_values_that_it_holds(monkeypatch):
+    """Greedy tokens and every step's logits, against the dense cache with keys and values rounded to the 4-bit levels.  In fp32 both differ in the
+    order of sums of up to 60 terms alone: far less than 2^-10 of the logits' size."""
+    from mamformer_b200 import ops
+    from mamformer_b200.models.model import MamformerForCausalLM
+    from mamformer_b200.ops import reference as ref
+    from test_paged_generate import small_config
+    torch.manual_seed(3)
+    model = MamformerForCausalLM(small_config()).eval()
+    ids = torch.randint(0, 259, (2, 50), generator=torch.Generator().manual_seed(2))
+    seen, calls = [], []
+    sample = model._sample_from_logits
+    monkeypatch.setattr(model, "_sample_from_logits", lambda logits, *a: (seen.append(logits), sample(logits, *a))[1])
+    out = model.generate(ids, max_new_tokens=8, temperature=0.0, kv_cache="paged4")
+    paged = seen[:]
+    del seen[:]
+    levels = lambda x: ref.kv4_values(*ref.kv4_levels(x.float())).to(x.dtype)  # noqa: E731
+    for name, at in (("diff_attention", 2), ("attention", 1)):
+        plain_form = getattr(ops, name)
+        monkeypatch.setattr(ops, name, lambda *a, f=plain_form, at=at, **kw: (calls.append(1), f(*a[:at], levels(a[at]), levels(a[at + 1]), *a[at + 2:], **kw))[1])
+    dense = model.generate(ids, max_new_tokens=8, temperature=0.0)
+    assert calls and len(seen) == len(paged) == 8
+    assert torch.equal(out, dense)
+    for a, b in zip(paged, seen):
+        assert (a - b).abs().max() <= 2.0 ** -10 * b.abs().max()
