@@ -48,6 +48,7 @@ struct Params : Rows {
 };
 struct Params4 : Rows {
   paged4::Cache4 c;
+  int max_new;
 };
 
 // 8 consecutive values of a token's head as floats
@@ -442,7 +443,7 @@ __global__ void __launch_bounds__(NT, 3) append4_kernel(const __grid_constant__ 
   if (ok) {
     const int t0 = c.cu[b], n = c.cu[b + 1] - t0, end = c.lens[b];
     slot = end - n + (t - t0);
-    ok = in_order(c, b) && t >= t0 && t - t0 < n && end - n >= 0;
+    ok = in_order(c, b) && t >= t0 && t - t0 < n && end - n >= 0 && n <= p.max_new;
     if (!ok && sub == 0) record(ERR_LENGTH);
   }
   if (ok) {
@@ -531,6 +532,7 @@ std::vector<at::Tensor> kv4_append(at::Tensor k, at::Tensor v, at::Tensor blocks
   TORCH_CHECK(max_new >= 0, "kv_append: max_new must not be negative");
   std::vector<at::Tensor> outs = take_rows(p, k, v, cos, sin, pos, queries);
   if (T == 0 || p.c.B == 0) return outs;
+  p.max_new = (int)std::min<int64_t>(std::max<int64_t>(max_new, 1), T);      // one token is taken whatever was said, as by the 8-bit kernel
   TORCH_CHECK(T * (hd / 16) < (1LL << 31), "kv_append: sizes");
   MAMF_DISPATCH_FLOAT_BF16(k.scalar_type(), "kv_append", [&] {
     if (hd == 128) launch4<scalar_t, 128>(p); else launch4<scalar_t, 64>(p);

@@ -248,3 +248,34 @@ def test_lengths_beyond_the_pool_on_a_wide_table():
             pages = table[i, :-(-lens[i] // page)].long()
             # what does not fit is left out of the weights, never added to others'
             assert torch.equal(am[pages], cm[pages]) or (cm[pages] == 1.0).all()
+
+
+# ---- append --------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("new,max_new", [([1, 5, 2], 4), ([1, 2, 1], 1), ([40, 3, 90], 64)])
+def test_runs_of_more_tokens_than_were_said_are_reported(bits, new, max_new):
+    """They are not appended, the other sequences' are, by either cache."""
+    from mamformer_b200.fault import PagedCacheError, check_device_status
+    lens, G, hd, page = [50, 70, 130], 2, 64, 16
+    cache, table = cache_of(bits, lens, page, G, hd)
+    tensors = [x for x in cache if x is not None]
+    k, v = rand((sum(new), G, hd), torch.bfloat16, "cuda", 7), rand((sum(new), G, hd), torch.bfloat16, "cuda", 8)
+    cu, ln = offsets(new, "cuda"), i32(lens, "cuda")
+    start = [x.clone() for x in tensors]
+    check_device_status()
+    ops.kv_append(k, v, cache, table, cu, ln, max_new)
+    with pytest.raises(PagedCacheError, match="length"):
+        check_device_status()
+    got = [x.clone() for x in tensors]
+    for x, was in zip(tensors, start):
+        x.copy_(was)
+    at = 0
+    for b, n in enumerate(new):                                       # one by one, as they were to go in
+        if n <= max_new:
+            ops.kv_append(k[at:at + n], v[at:at + n], cache, table[b:b + 1], offsets([n], "cuda"), ln[b:b + 1], max_new)
+        at += n
+    check_device_status()
+    assert any(n > max_new for n in new)
+    for x, y in zip(got, tensors):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
