@@ -107,7 +107,7 @@ struct Evict {
   int out_W, budget, recent;
 };
 
-// The order of floats as that of whole numbers, -0 as 0
+// The order of floats as that of whole numbers, -0 as 0, and any NaN above infinity: the sum makes the positive one of it
 __device__ __forceinline__ uint32_t order_of(float x) {
   const uint32_t u = __float_as_uint(x + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;

@@ -382,7 +382,7 @@ def kv_evict(cache: PagedKV4, block_table: torch.Tensor, kv_lens: torch.Tensor, 
     instance.  Returns the kept slots (B, G, budget) int32, -1 past a shorter sequence's end, and the new lengths (B,)
     int32.  Keys stay rotated as they were appended.  Sliding windows count slots, so they do not go with a cache that
     has been evicted from.  On the GPU, a token of a page out of range is not moved, what is in its new slot stays, and
-    ``fault.check_device_status`` raises afterwards.  A positive NaN counts as heavier than infinity."""
+    ``fault.check_device_status`` raises afterwards.  NaN counts as heavier than infinity."""
     if not isinstance(cache, PagedKV4):
         raise TypeError(f"kv_evict: a PagedKV4 (the 8-bit cache's pages share a scale), got {type(cache).__name__}")
     if cache.mass is None:

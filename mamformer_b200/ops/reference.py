@@ -591,6 +591,7 @@ def kv_evict(cache, block_table, kv_lens, budget, recent, out_table):
                 at = _slots(block_table[b], page, slots[:L - recent])
                 bits = (cache.mass[at[0], g, 16 * at[1] + at[2]] + 0.0).view(torch.int32).long()
                 order = torch.where(bits < 0, -(bits & 0x7FFFFFFF), bits)
+                order = torch.where((bits & 0x7FFFFFFF) > 0x7F800000, 0x7FFFFFFF, order)          # NaN of either sign
                 first = torch.sort(order, descending=True, stable=True).indices[:budget - recent]
                 keep = torch.cat([first.sort().values, slots[L - recent:]])
             kept[b, g, :len(keep)] = keep.to(torch.int32)

@@ -279,3 +279,15 @@ def test_runs_of_more_tokens_than_were_said_are_reported(bits, new, max_new):
     assert any(n > max_new for n in new)
     for x, y in zip(got, tensors):
         assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_weights_that_are_no_numbers_come_first_whatever_their_sign(dev):
+    """An x86 host makes negative NaN of infinity less infinity, a GPU positive: the choice is the same."""
+    cache, table = filled([8], 16, 1, 64, dev)
+    bits = [0x7FC00000, 0xFFC00000, 0xFF800001, 0x7FFFFFFF, 0x7F800000, 0x3F800000, 0x40000000, 0xFFFFFFFF]
+    cache.mass[table[0, 0].long(), 0, :8] = torch.tensor([b - (1 << 32) if b >> 31 else b for b in bits], dtype=torch.int32, device=dev).view(torch.float32)
+    for budget, want in ((1, [0]), (2, [0, 1]), (4, [0, 1, 2, 3]), (5, [0, 1, 2, 3, 7]), (6, [0, 1, 2, 3, 4, 7]), (7, [0, 1, 2, 3, 4, 6, 7])):
+        c = ops.PagedKV4(cache.blocks.clone(), cache.mass.clone())
+        kept, _ = ops.kv_evict(c, table, i32([8], dev), budget, 0)
+        assert kept[0, 0].tolist() == want
