@@ -105,6 +105,7 @@ struct Evict {
   int* lens_out;                                      // (B)
   uint8_t* packed;                                    // in place: the kept tokens on their way
   int out_W, budget, recent;
+  int most;                                           // tokens that a sequence can keep: budget, or what the table has room for
 };
 
 // The order of floats as that of whole numbers, -0 as 0, and any NaN above infinity: the sum makes the positive one of it
@@ -313,7 +314,7 @@ template <int HD, int MODE>
 __global__ void __launch_bounds__(NM) move_kernel(const __grid_constant__ Evict p) {
   const Cache4& c = p.c;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, g = blockIdx.y, b = blockIdx.z, q = lane & 3;
-  const int blocks = (p.budget + 15) >> 4;
+  const int blocks = (p.most + 15) >> 4;
   const int first = (blockIdx.x * (NM / 32) + w) * PAIR;
   if (first >= blocks) return;
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -401,7 +402,7 @@ __global__ void __launch_bounds__(NM) move_kernel(const __grid_constant__ Evict 
 template <int HD, int MODE> void launch_move(const Evict& p) {
   const int per = NM / 32 * PAIR * 16;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((p.budget + per - 1) / per), (unsigned)p.c.G, (unsigned)p.c.B);
+  cfg.gridDim = dim3((unsigned)((p.most + per - 1) / per), (unsigned)p.c.G, (unsigned)p.c.B);
   cfg.blockDim = dim3(NM);
   cfg.stream = stream();
   cudaLaunchAttribute at[1];
@@ -413,7 +414,7 @@ template <int HD, int MODE> void launch_move(const Evict& p) {
 }
 template <int HD> void move_kept(Evict& p, bool in_place) {
   if (!in_place) { launch_move<HD, DIRECT>(p); return; }
-  const int64_t blocks = (int64_t)p.c.B * p.c.G * ((p.budget + 15) / 16);
+  const int64_t blocks = (int64_t)p.c.B * p.c.G * ((p.most + 15) / 16);
   const at::Tensor ws = at::empty({blocks * PACKED<HD>}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA));
   p.packed = ws.data_ptr<uint8_t>();
   launch_move<HD, PACK>(p);
@@ -474,6 +475,7 @@ std::vector<at::Tensor> kv4_evict(at::Tensor blocks, at::Tensor mass, at::Tensor
   p.lens_out = lens_out.data_ptr<int>();
   p.budget = (int)budget;
   p.recent = (int)recent;
+  p.most = (int)std::max<int64_t>(1, most);
   // As many threads and CTAs per (sequence, head) as the table's longest sequence has blocks for.
   const int64_t threads = (int64_t)p.c.W * p.c.page / KPT;
   if (threads <= 256) launch_select<256, 1>(p);

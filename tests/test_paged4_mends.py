@@ -291,3 +291,21 @@ def test_weights_that_are_no_numbers_come_first_whatever_their_sign(dev):
         c = ops.PagedKV4(cache.blocks.clone(), cache.mass.clone())
         kept, _ = ops.kv_evict(c, table, i32([8], dev), budget, 0)
         assert kept[0, 0].tolist() == want
+
+
+@pytest.mark.gpu
+def test_a_budget_beyond_the_table_takes_no_memory_for_it():
+    """Nothing is cut: the workspace is of what the table has room for, and only the kept slots are as many as was asked for."""
+    lens, G, hd, page, budget = [300, 90], 2, 128, 16, 1 << 22
+    cache, table = filled(lens, page, G, hd, "cuda")
+    before = cache.blocks.clone()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    had = torch.cuda.memory_allocated()
+    kept, left = ops.kv_evict(cache, table, i32(lens, "cuda"), budget, 5)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - had < 2 * G * budget * 4 + (1 << 24)
+    assert left.tolist() == lens and torch.equal(cache.blocks, before)
+    for b, n in enumerate(lens):
+        assert torch.equal(kept[b, 0, :n], torch.arange(n, device="cuda", dtype=torch.int32)) and (kept[b, :, n:] == -1).all()
