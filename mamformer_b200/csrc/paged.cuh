@@ -37,7 +37,8 @@ inline Table check_table(const char* what, const at::Tensor& table, const at::Te
     TORCH_CHECK(!t || t->scalar_type() == at::kInt, what, ": int32 block table, offsets and lengths");
   const int64_t B = lens.numel();
   TORCH_CHECK(table.dim() == 2 && table.size(0) == B && (!cu || cu->numel() == B + 1), what, ": a block table row and an offset for each of ", B, " sequences");
-  TORCH_CHECK(P < (1LL << 31) && G <= 65535 && table.size(1) * page < (1LL << 31) && T < (1LL << 31) && B < (1 << 24), what, ": sizes");
+  // slots are counted in 32 bits, and tiles ahead of a sequence's last one too
+  TORCH_CHECK(P < (1LL << 31) && G <= 65535 && table.size(1) * page <= (1LL << 31) - (1 << 20) && T < (1LL << 31) && B < (1 << 24), what, ": sizes");
   return Table{table.data_ptr<int>(), cu ? cu->data_ptr<int>() : nullptr, lens.data_ptr<int>(), (int)P, (int)G, (int)page,
                page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7, (int)table.size(1), (int)B, (int)T};
 }

@@ -309,3 +309,15 @@ def test_a_budget_beyond_the_table_takes_no_memory_for_it():
     assert left.tolist() == lens and torch.equal(cache.blocks, before)
     for b, n in enumerate(lens):
         assert torch.equal(kept[b, 0, :n], torch.arange(n, device="cuda", dtype=torch.int32)) and (kept[b, :, n:] == -1).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+def test_tables_of_more_slots_than_32_bits_count_are_refused(bits):
+    cache, _ = cache_of(bits, [20], 128, 1, 64)
+    table = torch.zeros(1, (1 << 31) // 128 - 8000, dtype=torch.int32, device="cuda")
+    q = rand((1, 1, 64), torch.bfloat16, "cuda", 1)
+    with pytest.raises(RuntimeError, match="sizes"):
+        ops.paged_attention(q, cache, table, offsets([1], "cuda"), i32([20], "cuda"), 1)
+    with pytest.raises(RuntimeError, match="sizes"):
+        ops.kv_append(q, q, cache, table, offsets([1], "cuda"), i32([20], "cuda"), 1)
