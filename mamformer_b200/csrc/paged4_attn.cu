@@ -4,23 +4,27 @@
 //   S = scale q . k,  P = 2^(S log2 e - r),  O = sum P v / sum P,   causal, optional window;
 //   differential: (O1 - lam O2) / (1 - lam + 1e-8);   mass[slot] += sum over rows and maps of P / sum P
 //
-// The work is the list of (sequence, KV head, row tile) items, each a run of 64-token tiles; the grid's CTAs take equal
+// The work is the list of (sequence, KV head, row tile) items, each a run of 128-token tiles; the grid's CTAs take equal
 // contiguous shares of that list, so one long sequence fills the GPU as well as many short ones.  An item that ends in
 // another CTA than it began in leaves partial (r, l, O) in a workspace and a second small kernel joins them in order
 // (results do not depend on timing).
 //
-// A CTA is 4 warps; warp w takes tokens 16 w .. 16 w + 15 of each tile, which is one block of the cache, through a ring
-// of its own: one bulk copy a block, issued by one lane.  It never waits for the other warps inside an item.  The 16
-// tokens are the M rows of mma.m16n8k16 (f16 operands, fp32 sums): S^T = K Q^T and O^T = V^T P^T with up to 8 query rows
+// A CTA is 4 warps; warp w takes tokens 32 w .. 32 w + 31 of each tile, which are two blocks of the cache, through a ring
+// of its own: one bulk copy for both, or one a block where a page is one block, issued by one lane.  It never waits for the
+// other warps inside an item.  A block's 16 tokens are the M rows of mma.m16n8k16 (f16 operands, fp32 sums): S^T = K Q^T and O^T = V^T P^T with up to 8 query rows
 // as N; 16 rows take two.  A code becomes its f16 value in three instructions for two dims, exactly, so the products are
 // those of the stored values; the rows of q are scaled by a power of two to [1, 2) first, which f16 holds exactly down to
 // 2^-14 of a row's largest value.  P is rounded to f16 (11 bits; bf16 would keep 8) at up to 2^15, so that weights down to
-// 2^-21 of a row's largest keep all of their bits, whatever values they are given to.  The order of the head's dims in the
+// 2^-21 of a row's largest keep all of their bits, whatever values they are given to; f16 results of short runs are 2.7e-4 from
+// 64 bits, 2.1e-4 with fp32 weights, and in bf16 the result's own rounding hides it.  The order of the head's dims in the
 // products is free as long as both sides agree: a lane takes 16 adjacent bytes of a key's codes and 8 of a value's.
 //
 // Received weights: the scores of up to 16 rows are left in a workspace, 4 bytes a row and slot, for at most twice
 // the slots of the pool (a slot of the cache has 76 or 148 bytes), and a last kernel turns them into weights with each row's
 // joined sum; longer runs of tokens have them computed from the keys once more (paged4_attn_tc.cu).
+//
+// What bounds it: instructions.  64 sequences of 4096 slots, 32 / 8 heads of 128, two maps (302 MB): 97 us, where reading
+// takes 46; 65% of the issue slots, half of the ALU's (decoding), DRAM 39%, tensor 17%, 14 warps an SM on average.
 #include "paged4.cuh"
 #include "paged_split.cuh"
 
@@ -34,18 +38,23 @@ namespace cg = cooperative_groups;
 using namespace split;
 using namespace paged4;
 
-// Rows of a sequence and KV head above which the chunk kernel takes over.
+// Rows of a sequence and KV head above which the chunk kernel takes over.  us on this kernel and on that one, 8 sequences of
+// 8000 slots: one map of 16 / 4 heads, 48 rows 58 and 72, 64 rows 77 and 87, 80 rows 125 and 87; two maps of 32 / 8, 64 rows
+// 128 and 194, 96 rows 185 and 195, 128 rows 239 and 196.
 constexpr int FEW = 64;
 constexpr int NB = 2, STEP = 16 * NB;          // blocks and tokens of a warp per tile
 constexpr int TILE = STEP * NW;                // tokens per tile
 constexpr float LIFT = 7.f, LAZY = 8.f;        // a row's largest weight is 2^LIFT when its reference is set, and may outgrow it
 constexpr int MOST = 8;                        // CTAs of a cluster
 // Each item gets a cluster of its own where all of these fit on the GPU at once and a CTA has at most SHORT tiles, of the
-// longest sequence that the table has room for: no list to be shared, no second kernel.  Clusters and list, one map of 16 / 4
-// heads, us: 1 sequence of 700 slots 8.0 and 10.8, of 4000 12.4 and 12.4, of 8000 18.2 and 13.9; 16 of 700 10.9 and 13.4, of
-// 4000 19.3 and 23.0, of 8000 30.3 and 31.8; 64 of 700, with clusters of 8 in four waves, 38.2 and 20.2.
+// longest sequence that the table has room for (the host does not know the lengths): no list to be shared, no second
+// kernel.  Clusters and list, one map of 16 / 4 heads, us a call: 1 sequence of 700 slots 10.7 and 12.8, of 4000 14.7 and
+// 14.8, of 8000 20.9 and 16.8; 16 of 700 13.8 and 16.5, of 4000 22.3 and 25.1, of 8000 33.3 and 35.0; 64 of 700 20.6 and
+// 22.9, of 8000 103 and 99.  At 8000 slots it takes the list, which is right for few sequences and for very many.
 constexpr int SHORT = 4;
-constexpr int KEEP = 16;                       // rows whose scores are left for the received weights, at most
+// Rows whose scores are left for the received weights, at most: 4 rows 36 us and, computed from the keys once more, 88, 16 rows
+// 45 and 131 (8 sequences of 8000 slots); 16 rows, two maps, 64 of 4000, 190 and 957.  More would take more than the cache.
+constexpr int KEEP = 16;
 
 // A sequence's scores: [G][n][stride] from slot `lo` on, behind those of `start` slots; start < 0: not kept.
 struct Place { int64_t start; int lo, n; };

@@ -15,6 +15,10 @@
 //
 // P is rounded to f16 (11 bits of a weight) at up to 2^15, so that weights down to 2^-21 of a row's largest keep them; its
 // sum is fp32.
+//
+// 4 x 1024 tokens on 7168 cached, 32 / 8 heads of 128: two maps 1.37 ms, 752 TFLOP/s, one 0.78 ms, 665 TFLOP/s.  Bound by the
+// hand-offs of the 64-key tiles between its roles, as the 8-bit kernel of the same shape (1.22 ms, 0.68): tensor pipe 35%,
+// exponentials 36%, 39% of the issue slots.  Decoding 4 bits takes the two converting warps more instructions than e4m3 does.
 #include "f32x2.cuh"
 #include "paged4.cuh"
 #include "tc5.cuh"
@@ -40,7 +44,8 @@ struct Params : Attn4 {
   float* part;         // [unit * G + head][split][stream][BM][HD + 2]: O (not divided), m, l
 };
 
-// As tc5::bar_wait, without its suspend-time hint: the hand-offs of a tile are short (1.72 ms against 1.77).  The error
+// As tc5::bar_wait, without its suspend-time hint: the hand-offs of a tile are short (on the 8-bit kernel, 1.72 ms against
+// 1.77).  The error
 // word is only written here: a wait that ran out in another CTA, or in an earlier call, ends no wait of this one.  After
 // one that ran out a role waits for nothing more, so a CTA ends within a few limits.
 __device__ __forceinline__ bool try_once(uint64_t* b, uint32_t parity) {
@@ -565,8 +570,11 @@ void launch(const Attn4& attn) {
 //                   weight, two at a time
 //   warp 8          one lane copies tiles into a ring of three
 //   warp 9          TMEM allocation, MMA issue; two accumulators for each half, so that the sums do not wait for a product
-// Bound by the exponentials: 16 a cycle and SM, 2,048 cycles for 256 slots and 128 rows.  256 slots rather than 128: each
-// tile of rows is read from the L2 half as often.
+// 256 slots rather than 128: each tile of rows is read from the L2 half as often.  The exponentials alone, 16 a cycle and SM,
+// are 2,048 cycles for 256 slots and 128 rows; it takes twice that (4 x 1024 tokens on 7168 cached, one map of 32 / 8 heads:
+// 560 us, exponentials 49%, tensor pipe 23%, 31% of the issue slots).  Probably the two summing warps a scheduler are too few to
+// hide a load from tensor memory, fused multiply-adds and exponentials one after another; and the keys are decoded before
+// the first product.
 constexpr int WR = 128, WK = 256, WQ = 3, NTW = 320;       // rows of a tile, slots of a CTA, ring
 template <int HD> constexpr int TILE_BYTES = WR * HD * 2 + WR * 8;
 template <int HD> constexpr int weights_smem() { return 1024 + WK * HD * 2 + WQ * ((TILE_BYTES<HD> + 1023) / 1024 * 1024); }

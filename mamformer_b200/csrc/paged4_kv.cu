@@ -5,9 +5,16 @@
 //
 // select: a cluster of CTAs per (sequence, head) finds the least kept mass by radix: four times 8 bits of the weights' order
 // as whole numbers, each pass a histogram in shared memory that the cluster's CTAs add up through distributed shared
-// memory.  Weights lie in few bins of their leading bits, so the lanes of a warp count apart.  A thread holds the 16 slots of a block, in order, so a scan of the threads' counts gives each kept slot its place.
+// memory.  Weights lie in few bins of their leading bits, so the lanes of a warp count
+// apart.  A thread holds the 16 slots of a block, in order, so a scan of the threads' counts gives each kept slot its place.
 // move: a warp gathers the tokens of two blocks and writes them whole.  To other pages in one pass; in place through a
 // packed copy, since the kept tokens' places overlap.
+//
+// 64 sequences of 4096 slots cut to 2048, 8 heads of 128: 82 us to other pages, 132 in place (every byte twice).  The choice is
+// 18 us (bound by instructions and the four passes' barriers: 59% of the issue slots, 8 MB read), the move 63 (DRAM 69%:
+// 243 MB read for 155, a token's parameters and weight are parts of a 32-byte sector).  One sequence of 131,000 slots, cut to
+// 32,000: 41 us and 52, of which the choice is 22, on 64 CTAs.  300,000 slots, whose weights no longer fit in registers and
+// are read in every pass: 79 us.
 #include "paged4.cuh"
 
 #include <cooperative_groups.h>
@@ -476,7 +483,11 @@ std::vector<at::Tensor> kv4_evict(at::Tensor blocks, at::Tensor mass, at::Tensor
   p.budget = (int)budget;
   p.recent = (int)recent;
   p.most = (int)std::max<int64_t>(1, most);
-  // As many threads and CTAs per (sequence, head) as the table's longest sequence has blocks for.
+  // As many threads and CTAs per (sequence, head) as the longest sequence that the table has room for has blocks (the host does
+  // not know the lengths).  us to cut one sequence of 8 heads to half: 4096 slots on 256 threads 13.6, on 512 14.7; 8192 on
+  // 256 22.9, on 512 16.7, on two CTAs 18.8; 16384 on one CTA 27.4, on two 19.2, on four 20.8; 32768 on two 37.4, on four 22.9;
+  // 65536 on four 47.5, on eight 31.9; 131072 on eight 68.8, with 1024 threads each 58.6.  Sequences far shorter than the table
+  // pay for its width: 64 of 4096 slots take 22 us on 256 threads, 52 on two CTAs, 204 on eight.
   const int64_t threads = (int64_t)p.c.W * p.c.page / KPT;
   if (threads <= 256) launch_select<256, 1>(p);
   else if (threads <= 512) launch_select<512, 1>(p);

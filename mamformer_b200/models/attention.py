@@ -10,8 +10,8 @@ Window semantics: the reference's sliding-window mask keeps keys with
 (``attention.py:157-166, 193-216``), i.e. each query sees itself and the following W-1 keys.
 ``window_mode='reference'`` (default) reproduces that; ``'causal'`` uses ``0 <= q - k < W``.
 
-A ``cache`` of the form ``{"paged": PagedLayer}`` (:mod:`mamformer_b200.paged_cache`) keeps K / V in 8-bit pages and
-attends to all of them causally.
+A ``cache`` of the form ``{"paged": PagedLayer}`` (:mod:`mamformer_b200.paged_cache`) keeps K / V in 8-bit or
+4-bit pages and attends to all of them causally.
 """
 
 from __future__ import annotations

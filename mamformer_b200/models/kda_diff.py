@@ -10,7 +10,7 @@ Reference: ``mamformer/layers/kda_diff.py``.
   Decode keeps the O(1) state ``S (B,H,K,hd)``, ``z (B,H,K,1)``.
 * ``FullDiffAttention`` (``kda_diff.py:639-898``): MLA-style ``k = k_expand(k_compress(x))``,
   same for v, injection, RoPE, two softmaxes with a causal (finfo.min) mask, differential
-  combine, GroupNorm, o_proj.  The KV cache holds the expanded k, v: bf16 tensors, or 8-bit pages
+  combine, GroupNorm, o_proj.  The KV cache holds the expanded k, v: bf16 tensors, or 8-bit or 4-bit pages
   (``{"attn_type": "full", "paged": PagedLayer}``, :mod:`mamformer_b200.paged_cache`).
 * ``DynamicInterleaveGate`` (``kda_diff.py:905-958``): ``sigmoid(MLP(h_states))``.
 * ``KDADiffAttention`` (``kda_diff.py:965-1170``): full attention iff the mean gate > 0.5 when

@@ -411,7 +411,8 @@ class MamformerForCausalLM(GenerationMixin, nn.Module):
         8-bit pages (:class:`mamformer_b200.paged_cache.PagedKVCache`) instead of growing tensors, and attends with
         the paged kernels; ``"paged4"`` does so in 4 bits.  With the latter, ``kv_budget`` bounds what a sequence keeps:
         whenever it holds a page more than that, it is cut to the budget, of which a quarter are its last tokens and the
-        rest those that received the most attention weight."""
+        rest those that received the most attention weight.  Sliding windows count slots, so a model with layers that
+        have one is refused with a budget (``use_sliding_window`` of its config)."""
         if kv_cache not in ("dense", "paged", "paged4"):
             raise ValueError(f"kv_cache must be 'dense', 'paged' or 'paged4', got {kv_cache!r}")
         if kv_budget is not None and (kv_cache != "paged4" or kv_budget < 1):

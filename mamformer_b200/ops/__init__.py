@@ -377,10 +377,10 @@ def kv_evict(cache: PagedKV4, block_table: torch.Tensor, kv_lens: torch.Tensor, 
     of the others those of the largest ``cache.mass`` (ties to the earlier slot).
 
     The kept tokens move, in order, with their mass, to slots 0 .. budget - 1; sequences of up to ``budget`` tokens keep
-    all of theirs.  Without ``out_table`` that is in place.  With it (B, W') int32 they go to its pages, which must be no
-    page of ``block_table``'s, and what block_table names stays as it is: a prompt that other sequences share, for
-    instance.  Returns the kept slots (B, G, budget) int32, -1 past a shorter sequence's end, and the new lengths (B,)
-    int32.  Keys stay rotated as they were appended.  Sliding windows count slots, so they do not go with a cache that
+    all of theirs.  Without ``out_table`` that is in place, and a page must belong to one sequence only.  With it
+    (B, W') int32 they go to its pages, which must be no page of ``block_table``'s, and what block_table names stays as it
+    is: a prompt that other sequences share, for instance.  Returns the kept slots (B, G, budget) int32, -1 past a shorter
+    sequence's end, and the new lengths (B,) int32.  Keys stay rotated as they were appended.  Sliding windows count slots, so they do not go with a cache that
     has been evicted from.  On the GPU, a token of a page out of range is not moved, what is in its new slot stays, and
     ``fault.check_device_status`` raises afterwards.  NaN counts as heavier than infinity."""
     if not isinstance(cache, PagedKV4):

@@ -9,8 +9,8 @@ power-of-two scale per page and KV head (:class:`mamformer_b200.ops.PagedKV`), o
     out = cache.layer(i).attend(q, k, v, cos, sin)   # per attention layer: append, then attend
 
 A layer's pages are allocated when it first attends.  Sequences may differ in length and in the number of new
-tokens; :meth:`release` gives a finished sequence's pages back; :meth:`check` raises what the kernels recorded.  What a page holds is rounded to 4 significant
-bits, so decoded logits differ from an unquantised cache's by that rounding.
+tokens; :meth:`release` gives a finished sequence's pages back; :meth:`check` raises what the kernels recorded.  What
+an 8-bit page holds is rounded to 4 significant bits, so decoded logits differ from an unquantised cache's by that rounding.
 
 ``bits=4`` takes 9 bytes for 16 dims instead of 16: sixteen even levels for each 32 dims of a token's head
 (:class:`mamformer_b200.ops.PagedKV4`).  With ``weights=True`` such a cache adds up the attention weight that each slot
@@ -18,6 +18,8 @@ receives, and :meth:`evict` cuts the sequences to a budget by it, every layer an
 
     cache = PagedKVCache(..., bits=4, weights=True)
     cache.evict(budget=2048, recent=512)             # between steps: the last 512 tokens and the heaviest others stay
+
+Layers with sliding windows are refused while a sequence is there that was evicted from: windows count slots.
 """
 
 from __future__ import annotations

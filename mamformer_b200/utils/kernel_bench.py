@@ -284,6 +284,68 @@ def case_kv_append(B=16, new=1024, H=32, G=8, hd=128, page=64):
             2 * k.numel() * 3 + 4 * q.numel() * 2)
 
 
+def _paged4(B, new, lens, G, hd, page, room=0):
+    """A 4-bit cache full of B equal sequences, in a table with room for that many slots: (blocks, mass, table, cu, lens)."""
+    from mamformer_b200 import ops
+    W = -(-lens // page)
+    P = B * W
+    table = torch.full((B, max(W, room // page)), -1, device="cuda", dtype=torch.int32)
+    table[:, :W] = torch.randperm(P, device="cuda").to(torch.int32).view(B, W)
+    blocks = torch.zeros(P, G, page // 16, 18 * hd, device="cuda", dtype=torch.uint8)
+    ln = torch.full((B,), lens, device="cuda", dtype=torch.int32)
+    step = max(1, 4096 // B)                             # tokens of a sequence that are appended at once
+    for at in range(0, lens, step):
+        n = min(step, lens - at)
+        k, v = (torch.randn(B * n, G, hd, device="cuda").bfloat16() for _ in range(2))
+        ops.kv_append(k, v, ops.PagedKV4(blocks), table, torch.arange(B + 1, device="cuda", dtype=torch.int32) * n, ln - lens + at + n, n)
+    return blocks, torch.zeros(P, G, page, device="cuda"), table, torch.arange(B + 1, device="cuda", dtype=torch.int32) * new, ln
+
+
+def case_paged4_attention(B=64, new=1, lens=4096, H=32, G=8, hd=128, page=64, diff=True, weights=False, room=0):
+    """Attention over the paged 4-bit cache, with or without the weights that its slots receive."""
+    from mamformer_b200 import ops
+    blocks, mass, table, cu, ln = _paged4(B, new, lens, G, hd, page, room)
+    q, q2 = (torch.randn(B * new, H, hd, device="cuda").bfloat16() for _ in range(2))
+    kw = {"q2": q2, "lam": torch.full((H,), 0.5, device="cuda")} if diff else {}
+    cache = ops.PagedKV4(blocks, mass if weights else None)
+    pairs, maps = B * sum(lens - new + i + 1 for i in range(new)), 2 if diff else 1
+    return ((lambda: ops.paged_attention(q, cache, table, cu, ln, new, **kw)), 4.0 * maps * pairs * H * hd,
+            B * lens * G * (hd * 9 // 8 + (8 if weights else 0)) + (maps + 1) * q.numel() * 2)
+
+
+def case_paged4_append(B=16, new=1024, H=32, G=8, hd=128, page=64, read=False):
+    """Appending prompts to the 4-bit cache, with the rotation of K and two query tensors; or reading them back."""
+    from mamformer_b200 import ops
+    blocks, mass, table, cu, ln = _paged4(B, new, new, G, hd, page)
+    cache = ops.PagedKV4(blocks, mass)
+    if read:
+        return (lambda: ops.kv_read(cache, table, cu, ln, B * new, torch.bfloat16)), 0.0, B * new * G * hd * (4 + 9 / 8)
+    k, v = (torch.randn(B * new, G, hd, device="cuda").bfloat16() for _ in range(2))
+    q, q2 = (torch.randn(B * new, H, hd, device="cuda").bfloat16() for _ in range(2))
+    ang = torch.arange(new, device="cuda")[:, None] * torch.rand(hd // 2, device="cuda")[None]
+    cos, sin, pos = ang.cos(), ang.sin(), torch.arange(new, device="cuda").repeat(B)
+    return ((lambda: ops.kv_append(k, v, cache, table, cu, ln, new, cos, sin, pos, [q, q2])), 0.0,
+            k.numel() * (4 + 9 / 8) + 4 * q.numel() * 2)
+
+
+def case_paged4_evict(B=64, lens=4096, budget=2048, recent=256, G=8, hd=128, page=64, in_place=True, room=0):
+    """Eviction to a budget, in place as PagedKVCache does it, or to other pages.  Other weights every time: in place, tokens that
+    have moved once stay where they are."""
+    import itertools
+    from mamformer_b200 import ops
+    blocks, mass, table, _, ln = _paged4(B, 1, lens, G, hd, page, room)
+    to = None
+    if not in_place:
+        n = -(-budget // page)
+        to = (torch.arange(B * n, device="cuda", dtype=torch.int32) + blocks.shape[0]).view(B, n)
+        blocks = torch.cat([blocks, torch.zeros(B * n, *blocks.shape[1:], device="cuda", dtype=torch.uint8)])
+        mass = torch.zeros(blocks.shape[0], G, page, device="cuda")
+    weights = itertools.cycle([torch.randn_like(mass).mul_(2).exp_() for _ in range(24)])
+    kept = B * G * budget
+    return ((lambda: ops.kv_evict(ops.PagedKV4(blocks, next(weights)), table, ln, budget, recent, out_table=to)), 0.0,
+            4 * B * G * lens + kept * 2 * (9 * hd // 8 + 4) + 4 * kept)
+
+
 def case_token_scores(R=4096, V=128000, k=0, backward=False):
     """Log probability and entropy of given tokens; backward: their gradient."""
     from mamformer_b200.ops.native import _C
@@ -334,6 +396,24 @@ CASES = {"gemm": case_gemm, "grouped": case_grouped, "wgrad": case_wgrad, "scan"
          "paged_64_rows": lambda: case_paged_attention(8, 16, 8000, 16, 4, diff=False),
          "paged_80_rows": lambda: case_paged_attention(8, 20, 8000, 16, 4, diff=False),
          "paged_tail": lambda: case_paged_attention(1, 100, 14100),
+         "paged4_append": case_paged4_append, "paged4_read": lambda: case_paged4_append(read=True),
+         "paged4_decode": case_paged4_attention, "paged4_decode_weights": lambda: case_paged4_attention(weights=True),
+         "paged4_one": lambda: case_paged4_attention(1, 1, 700, 16, 4, diff=False),
+         "paged4_one_wide": lambda: case_paged4_attention(1, 1, 700, 16, 4, diff=False, room=8192),
+         "paged4_chunk": lambda: case_paged4_attention(4, 1024, 8192),
+         "paged4_chunk_single": lambda: case_paged4_attention(4, 1024, 8192, diff=False),
+         "paged4_chunk_weights": lambda: case_paged4_attention(4, 1024, 8192, weights=True),
+         "paged4_chunk_single_weights": lambda: case_paged4_attention(4, 1024, 8192, diff=False, weights=True),
+         "paged4_64_rows": lambda: case_paged4_attention(8, 16, 8000, 16, 4, diff=False),
+         "paged4_80_rows": lambda: case_paged4_attention(8, 20, 8000, 16, 4, diff=False),
+         "paged4_16_rows_weights": lambda: case_paged4_attention(8, 4, 8000, 16, 4, diff=False, weights=True),
+         "paged4_20_rows_weights": lambda: case_paged4_attention(8, 5, 8000, 16, 4, diff=False, weights=True),
+         "paged4_evict": case_paged4_evict, "paged4_evict_out": lambda: case_paged4_evict(in_place=False),
+         "paged4_evict_one": lambda: case_paged4_evict(1, 700, 512, 64, 4),
+         "paged4_evict_one_out": lambda: case_paged4_evict(1, 700, 512, 64, 4, in_place=False),
+         "paged4_evict_long": lambda: case_paged4_evict(1, 131000, 32000, 1000, page=128),
+         "paged4_evict_long_out": lambda: case_paged4_evict(1, 131000, 32000, 1000, page=128, in_place=False),
+         "paged4_evict_longer_out": lambda: case_paged4_evict(1, 300000, 32000, 1000, page=128, in_place=False),
          "scores_small": case_scores_small, "scores_constrained": case_scores_constrained,
          "token_scores": case_token_scores, "token_scores_top": lambda: case_token_scores(k=20),
          "token_scores_bwd": lambda: case_token_scores(backward=True)}
