@@ -99,9 +99,10 @@ def check_paged_status(clear: bool = True) -> None:
     C = ext()
     if C is None or not torch.cuda.is_available():
         return
-    seen = 0
-    for word in (C.kv_append_error, C.paged_attention_error, C.kv4_error, C.paged4_attention_error):
-        seen |= int(word(clear))
+    seen = int(C.kv_append_error(clear)) | int(C.paged_attention_error(clear))
+    for name in ("kv4_error", "paged4_attention_error"):
+        if hasattr(C, name):                             # an extension without the 4-bit cache has nothing to record
+            seen |= int(getattr(C, name)(clear))
     codes = [c for c in range(1, 32) if seen >> c & 1]
     if not codes:
         return

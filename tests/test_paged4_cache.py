@@ -94,3 +94,26 @@ def test_decodes_as_the_dense_cache_does_on_the_values_that_it_holds(monkeypatch
     assert torch.equal(out, dense)
     for a, b in zip(paged, seen):
         assert (a - b).abs().max() <= 2.0 ** -10 * b.abs().max()
+
+
+@pytest.mark.parametrize("word", ["kv_append_error", "paged_attention_error", "kv4_error", "paged4_attention_error", None])
+def test_every_word_of_the_paged_kernels_is_read(monkeypatch, word):
+    """Of an extension with the 4-bit cache's words; one without them is checked for those that it has.  (The words are fakes.)"""
+    from mamformer_b200 import fault
+    from mamformer_b200.ops import _ext
+    words = {n: 0 for n in ("kv_append_error", "paged_attention_error", "kv4_error", "paged4_attention_error")}
+    if word:
+        words[word] = 1 << 2
+
+    class Fake:
+        pass
+
+    for n in words if word else ("kv_append_error", "paged_attention_error"):
+        setattr(Fake, n, staticmethod(lambda clear=True, n=n: words.update({n: 0}) or 1 << 2 if words[n] and clear else words[n]))
+    monkeypatch.setattr(_ext, "ext", lambda: Fake)
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    if word:
+        for clear in (False, True):
+            with pytest.raises(fault.PagedCacheError, match="length"):
+                fault.check_paged_status(clear)
+    fault.check_paged_status()
