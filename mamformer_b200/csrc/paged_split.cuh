@@ -217,8 +217,8 @@ __global__ void __launch_bounds__(NJ, 2) join_kernel(const __grid_constant__ P p
     if (lane == 0) sums[w] = make_float2(M, least < 0.f ? -1.f : L);
   }
   __syncthreads();
-  float lse = 0.f;
-  auto value = [&](int row, int d) {
+  // a row's value of dim d, and log2 of its sum of weights where `sum` asks for it
+  auto value = [&](int row, int d, float* sum) {
     float M = NONE, L = 0.f, x = 0.f;
     float least = 0.f;
     for (int i = row; i < groups * n_rows; i += n_rows) {
@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(NJ, 2) join_kernel(const __grid_constant__ P p
       L = fmaf(sums[i].y, e, L);
     }
     const bool none = least < 0.f || L == 0.f;
-    lse = none ? INFINITY : M + log2f(L);
+    if (sum) *sum = none ? INFINITY : M + log2f(L);
     return none ? 0.f : x / L;
   };
   for (int i = threadIdx.x; i < ROWS / p.maps * HD; i += NJ) {
@@ -239,12 +239,8 @@ __global__ void __launch_bounds__(NJ, 2) join_kernel(const __grid_constant__ P p
     if (rr >= n_rows) continue;
     const int row = row0 + rr, tok = t0 + row / per, h = g * p.rep + row % per / p.maps;
     float* sums_at = p.lse && d == 0 ? p.lse + (int64_t)tok * p.H * p.maps + g * per + row % per : nullptr;
-    float x = value(rr, d);
-    if (sums_at) sums_at[0] = lse;
-    if (p.maps == 2) {
-      x = (x - p.lam[h] * value(rr + 1, d)) / (1.f - p.lam[h] + 1e-8f);
-      if (sums_at) sums_at[1] = lse;
-    }
+    float x = value(rr, d, sums_at);
+    if (p.maps == 2) x = (x - p.lam[h] * value(rr + 1, d, sums_at ? sums_at + 1 : nullptr)) / (1.f - p.lam[h] + 1e-8f);
     ((T*)p.out)[((int64_t)tok * p.H + h) * HD + d] = from_f<T>(x);
   }
 }
