@@ -60,6 +60,7 @@ constexpr int KEEP = 16;
 struct Place { int64_t start; int lo, n; };
 
 struct Params : Attn4 {
+  static constexpr bool SUMS = true;      // the rows' sums may be asked for
   int ctas;
   float* part;        // [ctas][2][rows][HD + 2]: O (not divided), r, l
   int4* joins;        // [ctas]: {t0, rows, g | rt << 16, 2 c0 + place} of the item that ends in this CTA after it

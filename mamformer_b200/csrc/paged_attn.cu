@@ -38,6 +38,7 @@ constexpr float LAZY = 8.f;                    // log2 by which a row may outgro
 constexpr float SLACK = 64.f;                  // value scales of up to this times O's unit are not looked at
 
 struct Params : Attn {
+  static constexpr bool SUMS = false;     // nobody asks for the rows' sums
   int ctas;
   float* part;        // [ctas][2][rows][HD + 2]: O (not divided), m, l
   int4* joins;        // [ctas]: {t0, rows, g | rt << 16, 2 c0 + place} of the item that ends in this CTA after it

@@ -157,7 +157,7 @@ __device__ __noinline__ void left_out(const P& p, int hd) {
     const int b = broken ? -1 : sequence_of(c.cu, c.B, t);
     if (broken || (b >= 0 && too_many(b))) {
       for (int i = threadIdx.x; i < p.H * hd; i += NJ) ((T*)p.out)[(int64_t)t * p.H * hd + i] = from_f<T>(0.f);
-      if (p.lse)
+      if (P::SUMS && p.lse)
         for (int i = threadIdx.x; i < p.H * p.maps; i += NJ) p.lse[(int64_t)t * p.H * p.maps + i] = INFINITY;
     }
   }
@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(NJ, 2) join_kernel(const __grid_constant__ P p
     const int rr = i / HD * p.maps, d = i % HD;
     if (rr >= n_rows) continue;
     const int row = row0 + rr, tok = t0 + row / per, h = g * p.rep + row % per / p.maps;
-    float* sums_at = p.lse && d == 0 ? p.lse + (int64_t)tok * p.H * p.maps + g * per + row % per : nullptr;
+    float* sums_at = P::SUMS && p.lse && d == 0 ? p.lse + (int64_t)tok * p.H * p.maps + g * per + row % per : nullptr;
     float x = value(rr, d, sums_at);
     if (p.maps == 2) x = (x - p.lam[h] * value(rr + 1, d, sums_at ? sums_at + 1 : nullptr)) / (1.f - p.lam[h] + 1e-8f);
     ((T*)p.out)[((int64_t)tok * p.H + h) * HD + d] = from_f<T>(x);
